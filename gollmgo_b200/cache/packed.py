@@ -1,0 +1,101 @@
+"""Keys and values held in 4 or 8 bits.
+
+``PackedKV`` is one layer's packed pages (csrc/packed_kv.cuh has the format) and what is done with them: tokens are rotated
+and quantised as they are written, read back as plain keys and values, and attended to where they lie.  Pages, slots and
+block tables are the cache manager's, as of an unpacked layer.  The reference engine has no counterpart.
+"""
+from __future__ import annotations
+
+from typing import Optional, Sequence
+
+import numpy as np
+import torch
+
+from ..csrc import ops
+
+GENERAL_TILE = 16
+
+
+class PackedKV:
+    """``pages``: uint8 [pages, kv heads, bytes of a page and head] (``PackedKV.empty`` makes them).
+
+    All calls run on the current stream of the device that holds the pages, which must be the current one.  Activations are
+    bfloat16 or float32; with float32 ones the whole path computes in 32 bits or more."""
+
+    def __init__(self, pages: torch.Tensor, head_dim: int, page_size: int, bits: int):
+        need = ops.packed_page_bytes(bits, head_dim, page_size)
+        if pages.dtype != torch.uint8 or pages.dim() != 3 or pages.shape[2] != need or not pages.is_contiguous() or not pages.is_cuda:
+            raise ops.KernelError(f"packed pages are contiguous uint8 [pages, kv heads, {need}] on a CUDA device, "
+                                  f"got {pages.dtype} {tuple(pages.shape)} on {pages.device}")
+        self.pages, self.head_dim, self.page_size, self.bits = pages, head_dim, page_size, bits
+        self.kv_heads = pages.shape[1]
+
+    @classmethod
+    def empty(cls, num_pages: int, kv_heads: int, head_dim: int, page_size: int, bits: int, device="cuda") -> "PackedKV":
+        size = ops.packed_page_bytes(bits, head_dim, page_size)
+        return cls(torch.zeros(num_pages, kv_heads, size, dtype=torch.uint8, device=device), head_dim, page_size, bits)
+
+    # ------------------------------------------------------------------ store and read back
+    def write(self, qkv: torch.Tensor, positions: Optional[torch.Tensor], slots: Optional[torch.Tensor], num_heads: int,
+              inv_freq: Optional[torch.Tensor] = None, interleaved: bool = False, magnitude: float = 1.0,
+              q_out: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """Rows of qkv [T, (num_heads + 2 kv heads) * head size]: q and k are rotated by ``positions`` (``inv_freq`` float64
+        [width / 2]; None: they are not), k and v quantised into their pages at ``slots`` (page * page_size + place; below
+        0: not stored; none twice; None: nothing is stored).  Returns the rotated q [T, num_heads, head size], in ``q_out``
+        where given (which may be the q columns of qkv)."""
+        if q_out is None:
+            q_out = torch.empty(qkv.shape[0], num_heads, self.head_dim, dtype=qkv.dtype, device=qkv.device)
+        ops.packed_write(qkv, positions, slots, inv_freq, magnitude, self.pages, q_out, num_heads, self.kv_heads, self.head_dim,
+                         self.page_size, self.bits, interleaved)
+        return q_out
+
+    def read(self, tables: torch.Tensor, lens: torch.Tensor, first_page: torch.Tensor, num_pages: int, dtype=torch.bfloat16,
+             out=None):
+        """Plain keys and values of whole sequences: page j of sequence b (``tables`` [B, width]) becomes page
+        first_page[b] + j of the two results [num_pages, kv heads, page_size, head size], for the pages of its first
+        lens[b] tokens; what lies behind the last token is zero.  Other pages of the results are not written."""
+        if out is None:
+            shape = (num_pages, self.kv_heads, self.page_size, self.head_dim)
+            out = (torch.empty(shape, dtype=dtype, device=self.pages.device), torch.empty(shape, dtype=dtype, device=self.pages.device))
+        ops.packed_read(self.pages, tables, lens, first_page, out[0], out[1], tables.shape[1], self.kv_heads, self.head_dim,
+                        self.page_size, self.bits)
+        return out
+
+    # ------------------------------------------------------------------ attention
+    def decode(self, q: torch.Tensor, tables: torch.Tensor, context_lens: torch.Tensor, max_context: int, scale: float, *,
+               window: int = 0, softcap: float = 0.0, sink=None, slopes=None, temperature=None, cu_q_lens=None, seqs=None,
+               out: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """Attention of single tokens, each the last of its sequence's context_lens[b] stored ones: q [n, heads, head size]
+        (row i of sequence i; with ``seqs`` token i belongs to sequence seqs[i], below 0: padding, and with ``cu_q_lens``
+        its row is cu_q_lens[sequence]).  ``max_context``: none of the contexts is longer (what the split of the work is
+        chosen from).  The options are those of the attention layer; a token with no key in sight gives zeros."""
+        nh, d = q.shape[1], self.head_dim
+        if q.dim() != 3 or q.shape[2] != d or nh % self.kv_heads:
+            raise ops.KernelError(f"decode: q is [tokens, heads in multiples of {self.kv_heads}, {d}], got {tuple(q.shape)}")
+        n = seqs.numel() if seqs is not None else q.shape[0]
+        if out is None:
+            out = torch.empty(q.shape[0], nh, d, dtype=q.dtype, device=q.device)
+        reach = min(max_context, window) if window else max_context
+        splits = max(1, min(64, -(-reach // 64), 592 // max(1, n * self.kv_heads)))
+        part = torch.empty(n * nh * splits * (d + 2), dtype=torch.float32, device=q.device)
+        ops.packed_decode(q, self.pages, tables, cu_q_lens, context_lens, seqs, n, splits, part[:n * nh * splits * d],
+                          part[n * nh * splits * d:], out, nh, self.kv_heads, d, self.page_size, self.bits, window, scale, softcap,
+                          sink, slopes, temperature)
+        return out
+
+    def prefill(self, q: torch.Tensor, tables: torch.Tensor, cu_q_lens: torch.Tensor, context_lens: torch.Tensor,
+                q_lens: Sequence[int], contexts: Sequence[int], scale: float, *, window: int = 0, softcap: float = 0.0, sink=None,
+                slopes=None, temperature=None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """Causal attention of prompt portions: sequence b brings rows cu_q_lens[b] .. cu_q_lens[b + 1] of q [T, heads, head
+        size], the last q_lens[b] of its context_lens[b] stored tokens.  ``q_lens`` and ``contexts`` say on the host what
+        the two device lists hold."""
+        nh, d = q.shape[1], self.head_dim
+        if q.dim() != 3 or q.shape[2] != d or nh % self.kv_heads:
+            raise ops.KernelError(f"prefill: q is [tokens, heads in multiples of {self.kv_heads}, {d}], got {tuple(q.shape)}")
+        if out is None:
+            out = torch.empty(q.shape[0], nh, d, dtype=q.dtype, device=q.device)
+        tiles = [(b, r) for b, n in enumerate(q_lens) for r in range(0, n, GENERAL_TILE)]
+        lists = torch.from_numpy(np.array(tiles, dtype=np.int32).reshape(-1, 2).T.copy()).to(q.device, non_blocking=True)
+        ops.packed_prefill(q, self.pages, tables, cu_q_lens, context_lens, lists[0], lists[1], len(tiles), out, nh, self.kv_heads, d,
+                           self.page_size, self.bits, window, scale, softcap, sink, slopes, temperature)
+        return out

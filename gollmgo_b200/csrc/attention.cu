@@ -16,13 +16,15 @@
 // current call's keys and masks by position alone; this one does not share those
 // two properties.
 #include "attention_common.cuh"
+#include "packed_kv.cuh"
 #include <stdlib.h>
 
 #define ATT_BQ 16
 #define ATT_BK 64
 #define ATT_THREADS 128
 
-template <typename TA, int DMAX>
+// PACKED: the cache holds codes of 4 or 8 bits (packed_kv.cuh), which become float32 as they are staged.
+template <typename TA, int DMAX, bool PACKED>
 __device__ __forceinline__ void attn_tile(const AttnArgs& a, int nrows, const TA* const* qptr_s,
                                           const int* pos_s, const int* head_s, const float* scale_s, int kvh, const int* bt, int lo_main,
                                           int hi_main, int first_hi, float* smem, float* acc) {
@@ -60,7 +62,15 @@ __device__ __forceinline__ void attn_tile(const AttnArgs& a, int nrows, const TA
       const int tok = kb + j;
       int page = -1;
       if (tok >= lo && tok < hi) page = bt[tok / ps];
-      if (page >= 0) {
+      if (PACKED) {
+        const PackedRows r(a.packed_bits, d, ps);
+        const bool there = page >= 0 && page < a.num_pages;
+        const unsigned char* block = (const unsigned char*)a.kcache + ((size_t)(there ? page : 0) * a.nkv + kvh) * r.page_bytes();
+        for (int c = lane; c < d; c += 32) {
+          Ks[j * (d + 1) + c] = there ? r.value(block, 0, tok % ps, c) : 0.f;
+          Vs[j * dv + c] = there ? r.value(block, 1, tok % ps, c) : 0.f;
+        }
+      } else if (page >= 0) {
         const size_t base = (((size_t)page * a.nkv + kvh) * ps + (tok % ps)) * d;
         const size_t vbase = (((size_t)page * nv + vh) * ps + (tok % ps)) * dv;
         for (int c = lane; c < d; c += 32) Ks[j * (d + 1) + c] = to_f32(kc[base + c]);
@@ -154,7 +164,7 @@ __device__ __forceinline__ const float* attn_tile_max(const AttnArgs& a, const f
 }
 
 // ---------------------------------------------------------------- prompt portions
-template <typename TA, int DMAX>
+template <typename TA, int DMAX, bool PACKED>
 __global__ void __launch_bounds__(ATT_THREADS) attn_prefill_kernel(AttnArgs a) {
   constexpr int NACC = ATT_BQ * DMAX / ATT_THREADS;
   extern __shared__ float smem[];
@@ -181,7 +191,7 @@ __global__ void __launch_bounds__(ATT_THREADS) attn_prefill_kernel(AttnArgs a) {
   int lo = a.window > 0 ? max(0, first - a.window + 1) : 0;
   if (a.chunk > 0) lo = max(lo, (first / a.chunk) * a.chunk);       // the chunk of the tile's first row starts earliest
   float acc[NACC];
-  attn_tile<TA, DMAX>(a, nrows, qptr_s, pos_s, head_s, scale_s, kvh, a.block_tables + (size_t)b * a.bt_stride, lo, last + 1,
+  attn_tile<TA, DMAX, PACKED>(a, nrows, qptr_s, pos_s, head_s, scale_s, kvh, a.block_tables + (size_t)b * a.bt_stride, lo, last + 1,
                       min(a.keep_first, lo), smem, acc);
   pdl_trigger();
   float* m_s = const_cast<float*>(attn_tile_max(a, smem));
@@ -221,7 +231,7 @@ __global__ void __launch_bounds__(ATT_THREADS) attn_prefill_kernel(AttnArgs a) {
 // grid (n_dec, nkv * ceil(G/16), num_splits).  Slice s of a context of n visible
 // keys covers ceil(n/S) keys rounded up to 64.  Writes un-normalised partial
 // outputs with their (max, sum); a slice without keys writes (-inf, 0).
-template <typename TA, int DMAX>
+template <typename TA, int DMAX, bool PACKED>
 __global__ void __launch_bounds__(ATT_THREADS) attn_decode_kernel(AttnArgs a) {
   constexpr int NACC = ATT_BQ * DMAX / ATT_THREADS;
   extern __shared__ float smem[];
@@ -231,12 +241,12 @@ __global__ void __launch_bounds__(ATT_THREADS) attn_decode_kernel(AttnArgs a) {
   __shared__ float scale_s[ATT_BQ];
   pdl_wait();
   const int G = a.nh / a.nkv, gchunks = (G + ATT_BQ - 1) / ATT_BQ;
-  const int b = a.dec_seqs[blockIdx.x];
+  const int b = a.dec_seqs ? a.dec_seqs[blockIdx.x] : (int)blockIdx.x;
   const int kvh = blockIdx.y / gchunks, g0 = (blockIdx.y % gchunks) * ATT_BQ;
   const int split = blockIdx.z, S = a.num_splits;
   const int nrows = min(ATT_BQ, G - g0);
   const int ctx = b >= 0 ? a.context_lens[b] : 0;      // b < 0: padding of a captured batch
-  const int t = b >= 0 ? a.cu_q_lens[b] : 0;
+  const int t = b >= 0 ? (a.cu_q_lens ? a.cu_q_lens[b] : b) : 0;
   int lo0 = a.window > 0 ? max(0, ctx - a.window) : 0;
   if (a.chunk > 0 && ctx > 0) lo0 = max(lo0, ((ctx - 1) / a.chunk) * a.chunk);
   const int n = ctx - lo0;
@@ -254,7 +264,7 @@ __global__ void __launch_bounds__(ATT_THREADS) attn_decode_kernel(AttnArgs a) {
   float acc[NACC];
   if (lo < hi) {
     // the first slice also takes the first tokens that stay visible behind the window
-    attn_tile<TA, DMAX>(a, nrows, qptr_s, pos_s, head_s, scale_s, kvh, a.block_tables + (size_t)b * a.bt_stride, lo, hi,
+    attn_tile<TA, DMAX, PACKED>(a, nrows, qptr_s, pos_s, head_s, scale_s, kvh, a.block_tables + (size_t)b * a.bt_stride, lo, hi,
                         split == 0 ? min(a.keep_first, lo0) : 0, smem, acc);
   } else {
 #pragma unroll
@@ -287,10 +297,10 @@ template <typename TA>
 __global__ void attn_merge_kernel(AttnArgs a) {
   pdl_trigger();
   pdl_wait();
-  const int b = a.dec_seqs[blockIdx.x];
+  const int b = a.dec_seqs ? a.dec_seqs[blockIdx.x] : (int)blockIdx.x;
   if (b < 0) return;
   const int h = blockIdx.y, S = a.num_splits, d = a.dv > 0 ? a.dv : a.d;
-  const int t = a.cu_q_lens[b];
+  const int t = a.cu_q_lens ? a.cu_q_lens[b] : b;
   const size_t row0 = ((size_t)blockIdx.x * a.nh + h) * S;
   float M = -INFINITY;
   for (int s = 0; s < S; ++s) M = fmaxf(M, a.part_ml[(row0 + s) * 2]);
@@ -341,22 +351,27 @@ template <typename K> static int set_smem(K kernel, size_t bytes, const char* wh
   return GG_OK;
 }
 
+#define ATT_LAUNCH(KERNEL, TA, DMAX, PACKED, grid, who)                                        \
+  do {                                                                                         \
+    const int rc = set_smem(KERNEL<TA, DMAX, PACKED>, smem, who);                              \
+    if (rc) return rc;                                                                         \
+    gg_launch(KERNEL<TA, DMAX, PACKED>, dim3(grid), dim3(ATT_THREADS), smem, stream, a);       \
+  } while (0)
+#define ATT_SIZES(KERNEL, TA, PACKED, grid, who)                                               \
+  do {                                                                                         \
+    if (dvv <= 64) ATT_LAUNCH(KERNEL, TA, 64, PACKED, grid, who);                              \
+    else if (dvv <= 128) ATT_LAUNCH(KERNEL, TA, 128, PACKED, grid, who);                       \
+    else ATT_LAUNCH(KERNEL, TA, 256, PACKED, grid, who);                                       \
+  } while (0)
 #define ATT_DISPATCH(KERNEL, grid, who)                                                        \
   do {                                                                                         \
     const int dvv = a.dv > 0 ? a.dv : a.d;                                                     \
     const size_t smem = (size_t)attn_smem_floats(a.d, dvv) * sizeof(float);                    \
-    int rc = GG_OK;                                                                            \
-    if (dtype == GG_F32) {                                                                     \
-      if (dvv <= 64) { rc = set_smem(KERNEL<float, 64>, smem, who); if (rc) return rc; gg_launch(KERNEL<float, 64>, dim3(grid), dim3(ATT_THREADS), smem, stream, a); } \
-      else if (dvv <= 128) { rc = set_smem(KERNEL<float, 128>, smem, who); if (rc) return rc; gg_launch(KERNEL<float, 128>, dim3(grid), dim3(ATT_THREADS), smem, stream, a); } \
-      else { rc = set_smem(KERNEL<float, 256>, smem, who); if (rc) return rc; gg_launch(KERNEL<float, 256>, dim3(grid), dim3(ATT_THREADS), smem, stream, a); } \
-    } else if (dtype == GG_BF16) {                                                             \
-      if (dvv <= 64) { rc = set_smem(KERNEL<__nv_bfloat16, 64>, smem, who); if (rc) return rc; gg_launch(KERNEL<__nv_bfloat16, 64>, dim3(grid), dim3(ATT_THREADS), smem, stream, a); } \
-      else if (dvv <= 128) { rc = set_smem(KERNEL<__nv_bfloat16, 128>, smem, who); if (rc) return rc; gg_launch(KERNEL<__nv_bfloat16, 128>, dim3(grid), dim3(ATT_THREADS), smem, stream, a); } \
-      else { rc = set_smem(KERNEL<__nv_bfloat16, 256>, smem, who); if (rc) return rc; gg_launch(KERNEL<__nv_bfloat16, 256>, dim3(grid), dim3(ATT_THREADS), smem, stream, a); } \
-    } else {                                                                                   \
-      return gg_fail(GG_ERR_INVALID, "%s: unknown dtype %d", who, dtype);                      \
-    }                                                                                          \
+    if (dtype == GG_F32 && a.packed_bits) ATT_SIZES(KERNEL, float, true, grid, who);           \
+    else if (dtype == GG_F32) ATT_SIZES(KERNEL, float, false, grid, who);                      \
+    else if (dtype == GG_BF16 && a.packed_bits) ATT_SIZES(KERNEL, __nv_bfloat16, true, grid, who); \
+    else if (dtype == GG_BF16) ATT_SIZES(KERNEL, __nv_bfloat16, false, grid, who);             \
+    else return gg_fail(GG_ERR_INVALID, "%s: unknown dtype %d", who, dtype);                   \
   } while (0)
 
 int attn_prefill_general(const AttnArgs& a, int dtype, int num_tiles, cudaStream_t stream) {

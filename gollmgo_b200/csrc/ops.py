@@ -1517,3 +1517,126 @@ def streams_join(streams: torch.Tensor, count: int, *, start: Optional[torch.Ten
     _check(lib().gg_streams_join(_p(streams), _p(start), _p(dense), _p(y), _p(place), _p(wgt), int(top), _p(same), _p(mix), _p(w_out),
                                  _p(w_in), _p(norm_weight), ctypes.c_float(eps), _p(normed), _p(total), T, count, D, dtype_code(dt),
                                  _stream()))
+
+
+# ---------------------------------------------------------------- the packed cache (csrc/packed_kv.cuh)
+def packed_group(d: int) -> int:
+    """Channels that share a scale and an offset in a packed cache."""
+    return 64 if d % 64 == 0 else 32 if d % 32 == 0 else 16
+
+
+def packed_page_bytes(bits: int, d: int, page_size: int) -> int:
+    """Bytes of one page and kv head of a packed cache; raises where the sizes are not taken."""
+    if bits not in (4, 8) or d % 16 or not 16 <= d <= 256 or not 4 <= page_size <= 256 or page_size & (page_size - 1):
+        raise KernelError(f"a packed cache has 4 or 8 bits, heads of 16 to 256 channels in sixteens and pages of a power of two of 4 to 256 "
+                          f"tokens (got {bits} bits, head size {d}, pages of {page_size})")
+    return 2 * page_size * (d * bits // 8 + 4 * (d // packed_group(d)))
+
+
+def _here(*tensors):
+    """The tensors live on the current device (the launch goes to its stream)."""
+    cur = _current_device()
+    for t in tensors:
+        if t is not None and t.get_device() != cur:
+            raise KernelError(f"kernel arguments must be on the current device {cur} (one is on {t.device})")
+
+
+def _rows_of(t: torch.Tensor, width: int, what: str) -> int:
+    """Row stride of rows [T, ...] of ``width`` values that are contiguous in themselves."""
+    if t.dim() == 2:
+        ok = t.shape[1] == width and (t.stride(1) == 1 or width == 1)
+    else:
+        ok = t.dim() == 3 and t.shape[1] * t.shape[2] == width and t.stride(2) == 1 and (t.shape[1] == 1 or t.stride(1) == t.shape[2])
+    if not ok or (t.shape[0] > 1 and t.stride(0) < width):
+        raise KernelError(f"{what} must be rows of {width} neighbouring values, got shape {tuple(t.shape)} with strides {t.stride()}")
+    return t.stride(0)
+
+
+def _ints(what: str, n: int, *tensors):
+    for t in tensors:
+        if t is not None and (t.dtype != torch.int32 or not t.is_contiguous() or t.numel() < n):
+            raise KernelError(f"{what}: index lists are contiguous int32 of at least {n} entries")
+
+
+def packed_write(qkv: torch.Tensor, positions: Optional[torch.Tensor], slots: Optional[torch.Tensor], inv_freq: Optional[torch.Tensor],
+                 magnitude: float, pages: torch.Tensor, q_out: Optional[torch.Tensor], nh: int, nkv: int, d: int, page_size: int,
+                 bits: int, interleaved: bool = False) -> None:
+    """Rotate the q heads of qkv [T, (nh + 2 nkv) d] into ``q_out`` [T, nh d] (None: they are left alone; it may be the
+    columns of qkv itself), rotate the k heads, and quantise k and v into ``pages`` at slots[t] = page * page_size + place.
+    A slot below 0 or outside the pool is not written; no slot may be given twice.  ``inv_freq`` None: no rotation.
+    ``positions``, ``slots`` and ``inv_freq`` are read before the kernel ahead of this one has finished."""
+    T = qkv.shape[0]
+    _here(qkv, positions, slots, inv_freq, pages, q_out)
+    stride = _rows_of(qkv, (nh + 2 * nkv) * d, "packed_write: qkv")
+    q_stride = 0
+    if q_out is not None:
+        if q_out.dtype != qkv.dtype or q_out.shape[0] != T:
+            raise KernelError("packed_write: q_out has one row per token in the type of qkv")
+        q_stride = _rows_of(q_out, nh * d, "packed_write: q_out")
+    _ints("packed_write", T, positions, slots)
+    rot = 0
+    if inv_freq is not None:
+        if inv_freq.dtype != torch.float64 or not inv_freq.is_contiguous():
+            raise KernelError("packed_write: inverse frequencies must be contiguous float64")
+        rot = 2 * inv_freq.numel()
+    _check(lib().gg_packed_write(_p(qkv), ctypes.c_longlong(stride), dtype_code(qkv.dtype), _p(positions), _p(slots), _p(inv_freq),
+                                 ctypes.c_float(magnitude), _p(pages), pages.shape[0], _p(q_out), ctypes.c_longlong(q_stride), T, nh, nkv,
+                                 d, rot, page_size, bits, int(interleaved), _stream()))
+
+
+def packed_read(pages: torch.Tensor, tables: torch.Tensor, lens: torch.Tensor, first_page: torch.Tensor, k_out: torch.Tensor,
+                v_out: torch.Tensor, most_pages: int, nkv: int, d: int, page_size: int, bits: int) -> None:
+    """Keys and values that the pages of each sequence stand for: page j of sequence b (``tables`` [B, width] of page ids)
+    becomes k_out, v_out [first_page[b] + j] ([pages, nkv, page_size, d]), for the pages that hold its first lens[b] tokens.
+    What lies behind a sequence's last token, and a page id outside the pool, reads as zero."""
+    B = tables.shape[0]
+    _here(pages, tables, lens, first_page, k_out, v_out)
+    if tables.dim() != 2:
+        raise KernelError("packed_read: the block tables are [sequences, pages]")
+    _ints("packed_read", B, tables, lens, first_page)
+    shape = (k_out.shape[0], nkv, page_size, d)
+    if k_out.shape != shape or v_out.shape != shape or k_out.dtype != v_out.dtype or not (k_out.is_contiguous() and v_out.is_contiguous()):
+        raise KernelError(f"packed_read: the outputs are contiguous [pages, {nkv}, {page_size}, {d}] of one type")
+    _check(lib().gg_packed_read(_p(pages), pages.shape[0], _p(tables), tables.shape[1], _p(lens), _p(first_page), _p(k_out), _p(v_out),
+                                dtype_code(k_out.dtype), shape[0], B, most_pages, nkv, d, page_size, bits, _stream()))
+
+
+def _packed_q(what, q, pages, tables, out, nh, d):
+    _here(q, pages, tables, out)
+    stride = _rows_of(q, nh * d, what + ": q")
+    if out.dtype != q.dtype or not out.is_contiguous() or out.numel() != q.shape[0] * nh * d:
+        raise KernelError(f"{what}: out is contiguous [T, {nh}, {d}] in the type of q")
+    if tables.dim() != 2 or tables.dtype != torch.int32 or not tables.is_contiguous():
+        raise KernelError(f"{what}: the block tables are contiguous int32 [sequences, pages]")
+    return stride
+
+
+def packed_prefill(q: torch.Tensor, pages: torch.Tensor, tables: torch.Tensor, cu_q_lens: torch.Tensor, context_lens: torch.Tensor,
+                   tile_seq: torch.Tensor, tile_q0: torch.Tensor, num_tiles: int, out: torch.Tensor, nh: int, nkv: int, d: int,
+                   page_size: int, bits: int, window: int, scale: float, softcap: float = 0.0, sink: Optional[torch.Tensor] = None,
+                   slopes: Optional[torch.Tensor] = None, temperature=None) -> None:
+    """attn_prefill_x over a packed cache on the general kernel (float32 arithmetic); ``tile_*`` list tiles of 16 queries."""
+    stride = _packed_q("packed_prefill", q, pages, tables, out, nh, d)
+    _attn_extras(nh, None, None, None, sink, slopes)
+    _ints("packed_prefill", num_tiles, tile_seq, tile_q0)
+    _check(lib().gg_packed_prefill(_p(q), ctypes.c_longlong(stride), dtype_code(q.dtype), _p(pages), pages.shape[0], _p(tables),
+                                   tables.shape[1], _p(cu_q_lens), _p(context_lens), _p(tile_seq), _p(tile_q0), num_tiles, _p(out), nh, nkv,
+                                   d, page_size, bits, window, ctypes.c_float(scale), ctypes.c_float(softcap), _p(sink), _p(slopes),
+                                   *_temperature(temperature), _stream()))
+
+
+def packed_decode(q: torch.Tensor, pages: torch.Tensor, tables: torch.Tensor, cu_q_lens: Optional[torch.Tensor], context_lens: torch.Tensor,
+                  seqs: Optional[torch.Tensor], n: int, splits: int, part_o: torch.Tensor, part_ml: torch.Tensor, out: torch.Tensor, nh: int,
+                  nkv: int, d: int, page_size: int, bits: int, window: int, scale: float, softcap: float = 0.0,
+                  sink: Optional[torch.Tensor] = None, slopes: Optional[torch.Tensor] = None, temperature=None) -> None:
+    """attn_decode_x over a packed cache on the general kernel (float32 arithmetic).  ``seqs`` None: token i belongs to
+    sequence i; ``cu_q_lens`` None: sequence b's token is row b."""
+    stride = _packed_q("packed_decode", q, pages, tables, out, nh, d)
+    _attn_extras(nh, None, None, None, sink, slopes)
+    _ints("packed_decode", n, context_lens if seqs is None else None, seqs)
+    if part_o.numel() < n * nh * splits * d or part_ml.numel() < n * nh * splits * 2:
+        raise KernelError("packed_decode: scratch too small")
+    _check(lib().gg_packed_decode(_p(q), ctypes.c_longlong(stride), dtype_code(q.dtype), _p(pages), pages.shape[0], _p(tables),
+                                  tables.shape[1], _p(cu_q_lens), _p(context_lens), _p(seqs), n, splits, _p(part_o), _p(part_ml), _p(out),
+                                  nh, nkv, d, page_size, bits, window, ctypes.c_float(scale), ctypes.c_float(softcap), _p(sink), _p(slopes),
+                                  *_temperature(temperature), _stream()), 2)

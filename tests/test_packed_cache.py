@@ -1,0 +1,307 @@
+"""The packed cache on the device against its plain 64-bit implementation (tests/plain_packed.py): what a write leaves in the
+pages, what reads back, and attention over them, with the sizes, masks and layouts where it can go wrong."""
+import math
+
+import pytest
+import torch
+
+import plain_packed as plain
+
+pytestmark = pytest.mark.gpu
+
+BF16, F32, F64 = torch.bfloat16, torch.float32, torch.float64
+
+
+def kit():
+    from gollmgo_b200.cache import PackedKV
+    from gollmgo_b200.csrc import ops
+    return PackedKV, ops
+
+
+def freqs(rot, theta=500000.0):
+    return theta ** (-torch.arange(0, rot, 2, dtype=F64) / rot)
+
+
+class Pool:
+    """Packed pages of several sequences in a shuffled pool, with random codes where nothing was written, and the float64
+    keys and values that the pages stand for (host)."""
+
+    def __init__(self, lens, nkv, d, page, bits, seed, dtype=BF16, spare=3):
+        PackedKV, _ = kit()
+        g = torch.Generator().manual_seed(seed)
+        self.lens, self.nkv, self.d, self.page, self.bits = list(lens), nkv, d, page, bits
+        counts = [-(-n // page) for n in lens]
+        total = sum(counts) + spare
+        order = torch.randperm(total, generator=g).tolist()
+        self.width = max(counts + [1]) + 1
+        self.tables = torch.full((len(lens), self.width), -1, dtype=torch.int32)
+        host = torch.randint(0, 256, (total, nkv, plain.page_bytes(bits, d, page)), dtype=torch.uint8, generator=g)
+        # whatever was there before: every pair a NaN, so that a key that is not in sight shows where it is used
+        pairs = 2 * page * (d * bits // 8)
+        host[..., pairs:] = 0xff
+        self.keys, self.values = [], []
+        at = 0
+        for b, (n, c) in enumerate(zip(lens, counts)):
+            self.tables[b, :c] = torch.tensor(order[at:at + c], dtype=torch.int32)
+            at += c
+            x = torch.randn(2, n, nkv, d, generator=g).to(dtype).double()
+            code, scale, off = plain.quantise(x, bits)
+            y = plain.dequantise(code, scale, off)
+            self.keys.append(y[0])
+            self.values.append(y[1])
+            if n == 0:
+                continue
+            row, par = d * bits // 8, 4 * (d // plain.group_of(d))
+            c8 = code.to(torch.int64)
+            if bits == 4:
+                c8 = c8[..., 0::2] + 16 * c8[..., 1::2]
+            c8 = c8.to(torch.uint8)
+            pr = torch.stack([scale, off], -1).flatten(-2).float().to(BF16).contiguous().view(torch.uint8)
+            tok = torch.arange(n)
+            pg, pl = self.tables[b][tok // page].long(), tok % page
+            for which in (0, 1):
+                for h in range(nkv):
+                    cols = which * page * row + pl[:, None] * row + torch.arange(row)
+                    host[pg[:, None], h, cols] = c8[which, :, h]
+                    cols = 2 * page * row + which * page * par + pl[:, None] * par + torch.arange(par)
+                    host[pg[:, None], h, cols] = pr[which, :, h]
+        self.host = host
+        self.kv = PackedKV(host.cuda(), d, page, bits)
+
+    def slots(self, b, lo, hi):
+        t = torch.arange(lo, hi)
+        return (self.tables[b][t // self.page].long() * self.page + t % self.page).to(torch.int32)
+
+
+# ---------------------------------------------------------------- the write
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("nh,nkv,d,rot,interleaved,page", [
+    (4, 2, 64, 64, False, 16), (32, 8, 128, 128, False, 16), (5, 5, 96, 64, False, 8), (3, 1, 256, 256, True, 32),
+    (2, 2, 16, 8, True, 4), (6, 3, 80, 0, False, 16), (8, 1, 128, 128, False, 64), (16, 4, 128, 64, False, 16)])
+def test_write_leaves_the_codes_of_the_formula(bits, dtype, nh, nkv, d, rot, interleaved, page):
+    PackedKV, _ = kit()
+    T, pages_n = 21, 7
+    g = torch.Generator().manual_seed(bits * 1000 + d + nh)
+    qkv = (torch.randn(T, (nh + 2 * nkv) * d, generator=g) * torch.exp(torch.randn(T, 1, generator=g))).to(dtype)
+    pos = torch.randint(0, 100000, (T,), generator=g, dtype=torch.int32)
+    slots = torch.randperm(pages_n * page, generator=g)[:T].to(torch.int32)
+    slots[3], slots[7], slots[8] = -1, pages_n * page, 2 ** 31 - 1          # not stored
+    before = torch.randint(0, 256, (pages_n, nkv, plain.page_bytes(bits, d, page)), dtype=torch.uint8, generator=g)
+    kv = PackedKV(before.clone().cuda(), d, page, bits)
+    inv = freqs(rot) if rot else None
+    q = kv.write(qkv.cuda(), pos.cuda(), slots.cuda(), nh, inv.cuda() if rot else None, interleaved, 1.25 if rot else 1.0)
+    want, stored = before.clone(), 0
+    eps = torch.finfo(dtype).eps / 2
+    wrong = 0
+    for t in range(T):
+        x = qkv[t].double().view(nh + 2 * nkv, d)
+        y = plain.rotate(x[:nh + nkv], float(pos[t]), inv, interleaved, 1.25) if rot else x[:nh + nkv]
+        # one rounding of the result, and (bfloat16 mode) a float32 rotation: a few float32 steps of the two products
+        big = torch.maximum(x[:nh].abs().amax(-1, keepdim=True), y[:nh].abs())
+        assert ((q[t].cpu().double() - y[:nh]).abs() <= eps * y[:nh].abs() + (8 * 2.0 ** -24 if dtype == BF16 else 2.0 ** -50) * 2 * big).all()
+        s = int(slots[t])
+        if s < 0 or s >= pages_n * page:
+            continue
+        for h in range(nkv):
+            plain.put(want, s, h, y[nh + h], x[nh + nkv + h], bits, page)
+            stored += 2 * d
+    got = kv.pages.cpu()
+    if dtype == F32 or not rot:
+        assert torch.equal(got, want)
+        return
+    # float32 rotation: a key within a few float32 steps of a border may take the neighbouring code, or its group's pair the
+    # neighbouring bfloat16; what it stands for stays within a step of the formula's
+    same = (got == want).float().mean().item()
+    assert same > 0.995
+    for t in range(T):
+        s = int(slots[t])
+        if s < 0 or s >= pages_n * page:
+            continue
+        for h in range(nkv):
+            k1, v1 = plain.get(got, s, h, d, bits, page)
+            k2, v2 = plain.get(want, s, h, d, bits, page)
+            assert torch.equal(v1, v2)
+            span = (k2.max() - k2.min())
+            assert ((k1 - k2).abs() <= span / (2 ** bits - 1) * 1.02).all()
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_write_of_hard_rows(bits, dtype):
+    """Constant rows, zeros, one huge value, the largest range, subnormals, exact ties, infinities and NaN."""
+    PackedKV, _ = kit()
+    d, page = 64, 16
+    big = torch.finfo(BF16).max
+    rows = [torch.zeros(d), torch.full((d,), -3.0), torch.full((d,), 0.1), torch.arange(d).float(), torch.arange(d) * 0.5 - 7,
+            torch.cat([torch.tensor([1e4]), torch.linspace(-1, 1, d - 1)]), torch.linspace(-big, big, d), torch.full((d,), 2.0 ** -130),
+            torch.linspace(-2.0 ** -120, 2.0 ** -121, d), torch.cat([torch.tensor([math.inf]), torch.ones(d - 1)]),
+            torch.cat([torch.ones(d - 1), torch.tensor([math.nan])]), torch.cat([torch.tensor([-math.inf]), torch.zeros(d - 1)]),
+            torch.cat([torch.tensor([0.0, 15.0]), torch.arange(d - 2) % 30 * 0.5]), torch.cat([torch.tensor([0.0, 255.0]), torch.arange(d - 2) % 510 * 0.5])]
+    T = len(rows)
+    v = torch.stack(rows).to(dtype)
+    qkv = torch.cat([v.flip(0), v], 1)                        # no q heads: keys and values alone
+    kv = PackedKV.empty(2, 1, d, page, bits)
+    slots = torch.arange(T, dtype=torch.int32)
+    q = kv.write(qkv.cuda(), None, slots.cuda(), 0)
+    assert q.shape == (T, 0, d)
+    got = kv.pages.cpu()
+    for t in range(T):
+        k1, v1 = plain.get(got, t, 0, d, bits, page)
+        for y, x in ((k1, v.flip(0)[t].double()), (v1, v[t].double())):
+            if not torch.isfinite(x).all():
+                assert torch.isnan(y).all()
+                continue
+            code, scale, off = plain.quantise(x, bits)
+            tiny = 2.0 ** -132                                 # a scale below the smallest normal bfloat16 is one of the subnormal ones
+            assert ((y - x).abs() <= scale.max() * 0.5 + tiny).all()
+            if scale.max() > 2.0 ** -126 or scale.max() == 0:
+                assert torch.equal(y, plain.dequantise(code, scale, off))
+
+
+def test_write_takes_strided_rows_and_rotates_in_place():
+    PackedKV, _ = kit()
+    nh, nkv, d, T = 4, 2, 64, 9
+    g = torch.Generator().manual_seed(3)
+    wide = torch.randn(T, (nh + 2 * nkv) * d + 40, generator=g).to(BF16).cuda()
+    pos, slots, inv = torch.arange(T, dtype=torch.int32).cuda() + 50, torch.arange(T, dtype=torch.int32).cuda(), freqs(d).cuda()
+    a, b = PackedKV.empty(1, nkv, d, 16, 4), PackedKV.empty(1, nkv, d, 16, 4)
+    q1 = a.write(wide[:, :(nh + 2 * nkv) * d].contiguous(), pos, slots, nh, inv)
+    rest = wide[:, nh * d:].clone()
+    view = wide[:, :nh * d].unflatten(1, (nh, d))
+    q2 = b.write(wide[:, :(nh + 2 * nkv) * d], pos, slots, nh, inv, q_out=view)
+    assert torch.equal(q1, q2) and q2.data_ptr() == wide.data_ptr()
+    assert torch.equal(a.pages, b.pages)
+    assert torch.equal(wide[:, nh * d:], rest)               # only the q columns were written
+
+
+# ---------------------------------------------------------------- reading back
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("nkv,d,page", [(2, 64, 16), (8, 128, 16), (1, 96, 8), (3, 256, 4), (2, 16, 32), (5, 80, 16)])
+def test_read_gives_what_the_pages_stand_for(bits, dtype, nkv, d, page):
+    lens = [1, page, page + 1, 3 * page - 1, 0, 2 * page]
+    pool = Pool(lens, nkv, d, page, bits, seed=d + bits)
+    pool.tables[5, 0] = -1                                    # given back: reads as zero
+    counts = [-(-n // page) for n in lens]
+    first, at = [], 2
+    for c in counts:
+        first.append(at)
+        at += c
+    mark = 7.0
+    out = tuple(torch.full((at + 1, nkv, page, d), mark, dtype=dtype, device="cuda") for _ in range(2))
+    k, v = pool.kv.read(pool.tables.cuda(), torch.tensor(lens, dtype=torch.int32).cuda(), torch.tensor(first, dtype=torch.int32).cuda(),
+                        at + 1, dtype, out)
+    eps = torch.finfo(dtype).eps / 2
+    for got, held in ((k, pool.keys), (v, pool.values)):
+        got = got.cpu().double()
+        assert (got[:2] == mark).all() and (got[at:] == mark).all()
+        for b, n in enumerate(lens):
+            rows = got[first[b]:first[b] + counts[b]].transpose(1, 2).reshape(-1, nkv, d)
+            want = held[b].clone()
+            if b == 5:
+                want[:page] = 0
+            # the result rounds once; scale * code + offset in float32 before that is off by its own rounding
+            assert ((rows[:n] - want).abs() <= (eps + 2.0 ** -23) * want.abs() + 1e-30).all()
+            assert (rows[n:] == 0).all()
+
+
+# ---------------------------------------------------------------- attention
+def bound(ref, values, dtype, score_err, weight_err):
+    """|out - ref| at most: the result's own rounding, and weights off by score_err (relative, twice: numerator and sum) and weight_err."""
+    top = max(float(v.abs().max()) if v.numel() else 0.0 for v in values)
+    return torch.finfo(dtype).eps / 2 * ref.abs() + (2 * score_err + weight_err) * top + 1e-30
+
+
+OPTIONS = [dict(), dict(window=20), dict(softcap=5.0), dict(sink=True), dict(slopes=True, window=33, sink=True, temperature=(0.1, 16))]
+
+
+def options_of(o, nh, seed):
+    g = torch.Generator().manual_seed(seed)
+    o = dict(o)
+    if o.get("sink"):
+        o["sink"] = torch.randn(nh, generator=g)
+    if o.get("slopes"):
+        o["slopes"] = torch.tensor([2.0 ** (-8.0 * (h + 1) / nh) for h in range(nh)])
+    return o, {k: v.cuda() if torch.is_tensor(v) else v for k, v in o.items()}
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("option", range(len(OPTIONS)))
+@pytest.mark.parametrize("nh,nkv,d,page", [(8, 2, 64, 16), (32, 8, 128, 16), (5, 5, 128, 32), (16, 1, 128, 16), (40, 2, 64, 64), (6, 2, 96, 16),
+                                           (4, 1, 256, 16), (4, 2, 128, 8), (3, 1, 16, 4)])
+def test_decode(bits, dtype, option, nh, nkv, d, page):
+    lens = [1, 15, 16, 17, 64, 65, 200, 0, 131]
+    pool = Pool(lens, nkv, d, page, bits, seed=d + option, dtype=dtype)
+    o, oc = options_of(OPTIONS[option], nh, 5)
+    g = torch.Generator().manual_seed(9)
+    q = torch.randn(len(lens), nh, d, generator=g).to(dtype)
+    scale = d ** -0.5
+    out = pool.kv.decode(q.cuda(), pool.tables.cuda(), torch.tensor(lens, dtype=torch.int32).cuda(), max(lens), scale, **oc).cpu().double()
+    for b, n in enumerate(lens):
+        if n == 0:
+            assert (out[b] == 0).all()
+            continue
+        ref = plain.attend(q[b:b + 1].double(), pool.keys[b], pool.values[b], n, scale, **o)[0]
+        assert ((out[b] - ref).abs() <= bound(ref, [pool.values[b]], dtype, *errors_of(dtype, q[b], pool.keys[b], scale))).all(), (b, n)
+
+
+def errors_of(dtype, q, keys, scale):
+    """Scores: d products summed in float32, relative to sum |q k| <= |q| |k|: a few steps of 2^-24 of it (the sum may be
+    truncated where a tensor core adds: 2^-21).  Weights: 2^-11 in bfloat16 mode (they are rounded to half precision), 2^-20 in float32."""
+    size = float(q.double().norm(dim=-1).max() * keys.norm(dim=-1).max()) * scale * 1.2
+    return size * 2.0 ** -20 + 2.0 ** -20, 2.0 ** -11 if dtype == BF16 else 2.0 ** -20
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+def test_decode_of_listed_sequences(bits):
+    """Tokens of some of a step's sequences: seqs with padding, rows through cu_q_lens, the other rows left as they were."""
+    nh, nkv, d, page = 8, 2, 128, 16
+    lens = [40, 7, 90, 33]
+    pool = Pool(lens, nkv, d, page, bits, seed=1)
+    g = torch.Generator().manual_seed(2)
+    cu = torch.tensor([0, 3, 4, 9, 10], dtype=torch.int32)                 # sequences 1 and 3 bring one token
+    wide = torch.randn(10, (nh + 2 * nkv) * d, generator=g).to(BF16).cuda()
+    q = wide[:, :nh * d].unflatten(1, (nh, d))
+    out = torch.full((10, nh, d), 3.0, dtype=BF16, device="cuda")
+    seqs = torch.tensor([3, -1, 1], dtype=torch.int32).cuda()
+    pool.kv.decode(q, pool.tables.cuda(), torch.tensor(lens, dtype=torch.int32).cuda(), 90, d ** -0.5, cu_q_lens=cu.cuda(), seqs=seqs, out=out)
+    for b in (1, 3):
+        row = int(cu[b])
+        ref = plain.attend(q[row:row + 1].cpu().double(), pool.keys[b], pool.values[b], lens[b], d ** -0.5)[0]
+        e = errors_of(BF16, q[row].cpu(), pool.keys[b], d ** -0.5)
+        assert ((out[row].cpu().double() - ref).abs() <= bound(ref, [pool.values[b]], BF16, *e)).all()
+    others = [r for r in range(10) if r not in (3, 9)]
+    assert (out[others] == 3.0).all()
+
+
+def prompt_errors(dtype, q, keys, scale):
+    """Prompt portions may read the cache back in the type of the activations: keys, values and weights round once each."""
+    s, w = errors_of(dtype, q, keys, scale)
+    if dtype == BF16:
+        s += float(q.double().norm(dim=-1).max() * keys.norm(dim=-1).max()) * scale * 2.0 ** -8
+        w += 2 * 2.0 ** -8
+    return s, w
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("option", range(len(OPTIONS)))
+@pytest.mark.parametrize("nh,nkv,d,page", [(8, 2, 64, 16), (8, 4, 128, 16), (5, 5, 128, 32), (6, 2, 96, 16), (2, 1, 256, 8), (3, 1, 16, 4)])
+def test_prefill(bits, dtype, option, nh, nkv, d, page):
+    q_lens, lens = [5, 1, 33, 16, 2, 70], [5, 40, 90, 16, 65, 140]
+    pool = Pool(lens, nkv, d, page, bits, seed=d + option, dtype=dtype)
+    o, oc = options_of(OPTIONS[option], nh, 5)
+    cu = [0]
+    for a in q_lens:
+        cu.append(cu[-1] + a)
+    g = torch.Generator().manual_seed(9)
+    q = torch.randn(cu[-1], nh, d, generator=g).to(dtype)
+    dev = lambda x: torch.tensor(x, dtype=torch.int32).cuda()
+    out = pool.kv.prefill(q.cuda(), pool.tables.cuda(), dev(cu), dev(lens), q_lens, lens, d ** -0.5, **oc).cpu().double()
+    for b, (a, n) in enumerate(zip(q_lens, lens)):
+        x = q[cu[b]:cu[b + 1]]
+        ref = plain.attend(x.double(), pool.keys[b], pool.values[b], n, d ** -0.5, **o)
+        e = prompt_errors(dtype, x, pool.keys[b], d ** -0.5)
+        assert ((out[cu[b]:cu[b + 1]] - ref).abs() <= bound(ref, [pool.values[b]], dtype, *e)).all(), (b, a, n)
