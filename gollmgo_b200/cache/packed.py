@@ -75,12 +75,19 @@ class PackedKV:
         n = seqs.numel() if seqs is not None else q.shape[0]
         if out is None:
             out = torch.empty(q.shape[0], nh, d, dtype=q.dtype, device=q.device)
+        more = (window, scale, softcap, sink, slopes, temperature)
+        if ops.packed_decode_mma_ok(q.dtype, d, self.page_size) and q.data_ptr() % 16 == 0 and q.stride(0) % 8 == 0 \
+                and n <= ops.PACKED_DECODE_TOKENS:
+            size = ops.packed_decode_scratch(n, nh, self.kv_heads, d, self.bits, max_context, window)
+            scratch = torch.empty(size, dtype=torch.float32, device=q.device)
+            ops.packed_decode_mma(q, self.pages, tables, cu_q_lens, context_lens, seqs, n, max_context, scratch, out, nh, self.kv_heads,
+                                  d, self.page_size, self.bits, *more)
+            return out
         reach = min(max_context, window) if window else max_context
         splits = max(1, min(64, -(-reach // 64), 592 // max(1, n * self.kv_heads)))
         part = torch.empty(n * nh * splits * (d + 2), dtype=torch.float32, device=q.device)
         ops.packed_decode(q, self.pages, tables, cu_q_lens, context_lens, seqs, n, splits, part[:n * nh * splits * d],
-                          part[n * nh * splits * d:], out, nh, self.kv_heads, d, self.page_size, self.bits, window, scale, softcap,
-                          sink, slopes, temperature)
+                          part[n * nh * splits * d:], out, nh, self.kv_heads, d, self.page_size, self.bits, *more)
         return out
 
     def prefill(self, q: torch.Tensor, tables: torch.Tensor, cu_q_lens: torch.Tensor, context_lens: torch.Tensor,

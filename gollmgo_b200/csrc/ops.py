@@ -1640,3 +1640,39 @@ def packed_decode(q: torch.Tensor, pages: torch.Tensor, tables: torch.Tensor, cu
                                   tables.shape[1], _p(cu_q_lens), _p(context_lens), _p(seqs), n, splits, _p(part_o), _p(part_ml), _p(out),
                                   nh, nkv, d, page_size, bits, window, ctypes.c_float(scale), ctypes.c_float(softcap), _p(sink), _p(slopes),
                                   *_temperature(temperature), _stream()), 2)
+
+
+PACKED_DECODE_TOKENS = 1024      # tokens that packed_decode_mma takes in one launch
+
+
+def packed_decode_mma_ok(dtype: torch.dtype, d: int, page_size: int) -> bool:
+    """Whether packed_decode_mma takes these sizes: bfloat16, heads of 64 or 128, pages of 16 tokens or more."""
+    return dtype == torch.bfloat16 and d in (64, 128) and page_size >= 16
+
+
+def packed_decode_scratch(n: int, nh: int, nkv: int, d: int, bits: int, max_context: int, window: int) -> int:
+    """float32 scratch of packed_decode_mma."""
+    f = lib().gg_packed_decode_scratch
+    f.restype = ctypes.c_longlong
+    return int(f(n, nh, nkv, d, bits, max_context, window))
+
+
+def packed_decode_mma(q: torch.Tensor, pages: torch.Tensor, tables: torch.Tensor, cu_q_lens: Optional[torch.Tensor],
+                      context_lens: torch.Tensor, seqs: Optional[torch.Tensor], n: int, max_context: int, scratch: torch.Tensor,
+                      out: torch.Tensor, nh: int, nkv: int, d: int, page_size: int, bits: int, window: int, scale: float,
+                      softcap: float = 0.0, sink: Optional[torch.Tensor] = None, slopes: Optional[torch.Tensor] = None,
+                      temperature=None) -> None:
+    """packed_decode on the tensor cores (packed_decode_mma_ok).  ``scratch`` float32 of packed_decode_scratch for the same
+    sizes; contexts longer than ``max_context`` are right too, only the work was split for shorter ones."""
+    global tc_launched
+    stride = _packed_q("packed_decode", q, pages, tables, out, nh, d)
+    _attn_extras(nh, None, None, None, sink, slopes)
+    _ints("packed_decode", n, context_lens if seqs is None else None, seqs)
+    if scratch.dtype != torch.float32 or not scratch.is_contiguous():
+        raise KernelError("packed_decode: the scratch is contiguous float32")
+    tc_launched = True
+    _check(lib().gg_packed_decode_mma(_p(q), ctypes.c_longlong(stride), _p(pages), pages.shape[0], _p(tables), tables.shape[1],
+                                      _p(cu_q_lens), _p(context_lens), _p(seqs), n, max_context, _p(scratch),
+                                      ctypes.c_longlong(scratch.numel()), _p(out), nh, nkv, d, page_size, bits, window,
+                                      ctypes.c_float(scale), ctypes.c_float(softcap), _p(sink), _p(slopes), *_temperature(temperature),
+                                      _p(tc_status(q.device)), _stream()), 2)
