@@ -13,7 +13,7 @@ import torch
 
 from ..csrc import ops
 
-GENERAL_TILE = 16
+SHORT_PROMPT_KEYS = 256
 
 
 class PackedKV:
@@ -29,6 +29,7 @@ class PackedKV:
                                   f"got {pages.dtype} {tuple(pages.shape)} on {pages.device}")
         self.pages, self.head_dim, self.page_size, self.bits = pages, head_dim, page_size, bits
         self.kv_heads = pages.shape[1]
+        self._sms = 148
 
     @classmethod
     def empty(cls, num_pages: int, kv_heads: int, head_dim: int, page_size: int, bits: int, device="cuda") -> "PackedKV":
@@ -92,17 +93,54 @@ class PackedKV:
 
     def prefill(self, q: torch.Tensor, tables: torch.Tensor, cu_q_lens: torch.Tensor, context_lens: torch.Tensor,
                 q_lens: Sequence[int], contexts: Sequence[int], scale: float, *, window: int = 0, softcap: float = 0.0, sink=None,
-                slopes=None, temperature=None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+                slopes=None, temperature=None, least: int = 1, out: Optional[torch.Tensor] = None) -> torch.Tensor:
         """Causal attention of prompt portions: sequence b brings rows cu_q_lens[b] .. cu_q_lens[b + 1] of q [T, heads, head
         size], the last q_lens[b] of its context_lens[b] stored tokens.  ``q_lens`` and ``contexts`` say on the host what
-        the two device lists hold."""
+        the two device lists hold.  Sequences of fewer than ``least`` rows are left out (their rows of ``out`` stay as they are)."""
         nh, d = q.shape[1], self.head_dim
         if q.dim() != 3 or q.shape[2] != d or nh % self.kv_heads:
             raise ops.KernelError(f"prefill: q is [tokens, heads in multiples of {self.kv_heads}, {d}], got {tuple(q.shape)}")
         if out is None:
             out = torch.empty(q.shape[0], nh, d, dtype=q.dtype, device=q.device)
-        tiles = [(b, r) for b, n in enumerate(q_lens) for r in range(0, n, GENERAL_TILE)]
-        lists = torch.from_numpy(np.array(tiles, dtype=np.int32).reshape(-1, 2).T.copy()).to(q.device, non_blocking=True)
-        ops.packed_prefill(q, self.pages, tables, cu_q_lens, context_lens, lists[0], lists[1], len(tiles), out, nh, self.kv_heads, d,
-                           self.page_size, self.bits, window, scale, softcap, sink, slopes, temperature)
+        P, dev, i32 = self.page_size, q.device, torch.int32
+        pages = most = tiles16 = tiles64 = tiles128 = 0
+        long = 0
+        for a, c in zip(q_lens, contexts):
+            if a >= least:
+                n = -(-c // P)
+                most = max(most, n)
+                pages += n - (max(0, c - a - window + 1) // P if window else 0)
+                tiles16 += -(-a // 16)
+                tiles64 += -(-a // 64)
+                tiles128 += -(-a // 128)
+                long = max(long, c)
+        if not pages:
+            return out
+        B, width = tables.shape
+        fast = q.dtype == torch.bfloat16 and d in (64, 128) and q.stride(0) % 8 == 0 and q.data_ptr() % 16 == 0
+        keep = torch.empty(2, pages, self.kv_heads, P, d, dtype=q.dtype, device=dev)
+        lists = [(64, tiles64)] if fast else [(16, tiles16)]
+        if fast and (tiles128 * ((nh + 1) // 2) * 2 > self._sms or min(long, window or long) > SHORT_PROMPT_KEYS):
+            lists.append((128, tiles128))
+        ints = torch.empty(B * width + 2 * sum(n for _, n in lists), dtype=i32, device=dev)
+        at, full = B * width, []
+        for h, n in lists:
+            full.append((h, n, ints[at:at + n], ints[at + n:at + 2 * n]))
+            at += 2 * n
+        plain_tables = ints[:B * width].view(B, width)
+        ops.packed_unfold(self.pages, tables, cu_q_lens, context_lens, keep[0], keep[1], most, plain_tables, full, self.kv_heads, d, P,
+                          self.bits, window, least)
+        t = {h: dict(seq=s, q0=r, n=n) for h, n, s, r in full}
+        t16, t64, t128 = (t.get(h) or dict(seq=None, q0=None, n=0) for h in (16, 64, 128))
+        more = {}
+        if t128["n"]:
+            more = dict(tile128_seq=t128["seq"], tile128_q0=t128["q0"], num_tiles128=t128["n"])
+        if softcap > 0 or sink is not None or slopes is not None or temperature is not None:
+            ops.attn_prefill_x(q, q.stride(0), keep[0], keep[1], plain_tables, width, cu_q_lens, context_lens, t16["seq"], t16["q0"], t16["n"],
+                               out, nh, self.kv_heads, d, d, 1, P, window, scale, softcap, t64["seq"], t64["q0"], t64["n"],
+                               allow_mma=fast, sink=sink, slopes=slopes, temperature=temperature, **more)
+        else:
+            ops.attn_prefill(q, q.stride(0), keep[0], keep[1], plain_tables, width, cu_q_lens, context_lens, t16["seq"], t16["q0"], t16["n"],
+                             out, nh, self.kv_heads, d, P, window, scale, t64["seq"], t64["q0"], t64["n"], allow_mma=fast,
+                             allow_tc=bool(more), **more)
         return out

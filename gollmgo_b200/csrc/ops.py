@@ -1676,3 +1676,23 @@ def packed_decode_mma(q: torch.Tensor, pages: torch.Tensor, tables: torch.Tensor
                                       ctypes.c_longlong(scratch.numel()), _p(out), nh, nkv, d, page_size, bits, window,
                                       ctypes.c_float(scale), ctypes.c_float(softcap), _p(sink), _p(slopes), *_temperature(temperature),
                                       _p(tc_status(q.device)), _stream()), 2)
+
+
+def packed_unfold(pages: torch.Tensor, tables: torch.Tensor, cu_q_lens: torch.Tensor, context_lens: torch.Tensor, k_out: torch.Tensor,
+                  v_out: torch.Tensor, most_pages: int, out_tables: torch.Tensor, lists, nkv: int, d: int, page_size: int, bits: int,
+                  window: int, least: int = 1) -> None:
+    """What the prompt kernels need of the portions of a step (sequences with ``least`` rows or more in cu_q_lens): their pages as
+    plain keys and values behind one another in k_out, v_out [pages, nkv, page_size, d], block tables of those pages in
+    ``out_tables`` (shape of ``tables``), and one or two tile lists: ``lists`` of (height, count, seq, q0) with the number of
+    tiles that the portions cut into rows of that height make.  Pages that the window hides are left out."""
+    B = tables.shape[0]
+    _here(pages, tables, cu_q_lens, context_lens, k_out, v_out, out_tables)
+    _ints("packed_unfold", B, tables, context_lens, out_tables)
+    _ints("packed_unfold", B + 1, cu_q_lens)
+    flat = []
+    for height, count, seq, q0 in list(lists) + [(0, 0, None, None)] * (2 - len(lists)):
+        _ints("packed_unfold", count, seq, q0)
+        flat += [height, count, _p(seq), _p(q0)]
+    _check(lib().gg_packed_unfold(_p(pages), pages.shape[0], _p(tables), tables.shape[1], _p(cu_q_lens), _p(context_lens), B, _p(k_out),
+                                  _p(v_out), dtype_code(k_out.dtype), k_out.shape[0], most_pages, _p(out_tables), *flat, least, nkv, d, page_size,
+                                  bits, window, _stream()))

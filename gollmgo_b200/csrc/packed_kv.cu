@@ -131,33 +131,166 @@ packed_write_kernel(const TA* __restrict__ qkv, long long row_stride, const int*
 }
 
 // ---------------------------------------------------------------- read
-// grid (pages of the longest sequence, B): a block turns one page of a sequence, all its kv heads, into keys and values
-// [pages, nkv, P, d].  Rows behind the sequence's last token, and pages that were given back, read as zero.
-template <typename TO>
+// Eight neighbouring channels (of one group) of a token.
+template <int BITS>
+__device__ __forceinline__ void unpack8(const unsigned char* codes, unsigned pair, float* y) {
+  const float s = __uint_as_float(pair << 16), o = __uint_as_float(pair & 0xffff0000u);
+  if (BITS == 4) {
+    const unsigned w = *reinterpret_cast<const unsigned*>(codes);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) y[i] = fmaf(s, (float)((w >> (4 * i)) & 15u), o);
+  } else {
+    const uint2 w = *reinterpret_cast<const uint2*>(codes);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      y[i] = fmaf(s, (float)((w.x >> (8 * i)) & 255u), o);
+      y[4 + i] = fmaf(s, (float)((w.y >> (8 * i)) & 255u), o);
+    }
+  }
+}
+__device__ __forceinline__ void store8(float* p, const float* y) {
+  reinterpret_cast<float4*>(p)[0] = make_float4(y[0], y[1], y[2], y[3]);
+  reinterpret_cast<float4*>(p)[1] = make_float4(y[4], y[5], y[6], y[7]);
+}
+__device__ __forceinline__ void store8(__nv_bfloat16* p, const float* y) {
+  *reinterpret_cast<uint4*>(p) = make_uint4(pack_bf16(y[0], y[1]), pack_bf16(y[2], y[3]), pack_bf16(y[4], y[5]), pack_bf16(y[6], y[7]));
+}
+
+// One page of one sequence: the codes of kv heads z, z + nz, ... become keys and values; the tokens from `real` on, and all
+// of a page that was given back, become zeros.
+template <typename TO, int BITS>
+__device__ __forceinline__ void unpack_page(const unsigned char* pages, int page, int num_pages, int real, TO* k_out, TO* v_out, int nkv, int d,
+                                            int page_size) {
+  const PackedRows r(BITS, d, page_size);
+  const int per_row = d >> 3, units = 2 * page_size * per_row;
+  if (page < 0 || page >= num_pages) { page = 0; real = 0; }
+  for (int u = threadIdx.x; u < units; u += blockDim.x) {
+    const int row = u / per_row, c = (u - row * per_row) << 3, which = row >= page_size, place = row - which * page_size;
+    const unsigned char* block = pages + ((size_t)page * nkv + blockIdx.z) * r.page_bytes();
+    const int codes = row * r.row() + c * BITS / 8, pair = r.pairs(which, place) + (c / r.group) * 4;
+    TO* o = (which ? v_out : k_out) + ((size_t)blockIdx.z * page_size + place) * d + c;
+#pragma unroll 4
+    for (int h = blockIdx.z; h < nkv; h += gridDim.z) {
+      float y[8];
+      unpack8<BITS>(block + codes, *reinterpret_cast<const unsigned*>(block + pair), y);
+      if (place >= real) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) y[i] = 0.f;
+      }
+      store8(o, y);
+      block += (size_t)gridDim.z * r.page_bytes();
+      o += (size_t)gridDim.z * page_size * d;
+    }
+  }
+}
+
+// grid (pages of the longest sequence, B, nz): page j of sequence b becomes page first_page[b] + j of the results.
+template <typename TO, int BITS>
 __global__ void __launch_bounds__(256)
 packed_read_kernel(const unsigned char* __restrict__ pages, int num_pages, const int* __restrict__ tables, int bt_stride,
                    const int* __restrict__ lens, const int* __restrict__ first_page, TO* __restrict__ k_out, TO* __restrict__ v_out,
-                   int out_pages, int nkv, int d, int page_size, int bits) {
+                   int out_pages, int nkv, int d, int page_size) {
   pdl_trigger();
   pdl_wait();
   const int b = blockIdx.y, j = blockIdx.x, len = lens[b];
   if (j * page_size >= len) return;
   const int to = first_page[b] + j;
   if (to < 0 || to >= out_pages) return;
-  const int page = tables[(size_t)b * bt_stride + j];
-  const bool there = page >= 0 && page < num_pages;
-  const PackedRows r(bits, d, page_size);
-  const int per_row = d / 8, units = 2 * nkv * page_size * per_row;
-  for (int u = threadIdx.x; u < units; u += blockDim.x) {
-    const int c = (u % per_row) * 8, place = (u / per_row) % page_size, hw = u / (per_row * page_size), kvh = hw >> 1, which = hw & 1;
-    const unsigned char* block = pages + ((size_t)(there ? page : 0) * nkv + kvh) * r.page_bytes();
-    TO* o = (which ? v_out : k_out) + (((size_t)to * nkv + kvh) * page_size + place) * d + c;
-    const bool real = there && j * page_size + place < len;
-    float y[8];
+  const size_t at = (size_t)to * nkv * page_size * d;
+  unpack_page<TO, BITS>(pages, tables[(size_t)b * bt_stride + j], num_pages, len - j * page_size, k_out + at, v_out + at, nkv, d, page_size);
+}
+
+// What the prompt kernels need of a packed layer's portions (sequences that bring `least` tokens or more), in one launch: their
+// pages as plain keys and values, one sequence behind the other; block tables of those pages; and the portions cut into tiles
+// of query rows, those that attend to most keys first (up to UNFOLD_SORTED tiles; more stay in the order of the sequences).
+// Pages behind the window of a portion's first token are left out (-1 in the table).
+#define UNFOLD_SORTED 1024
+struct UnfoldTiles { int height, count; int *seq, *q0; };
+struct UnfoldArgs {
+  const unsigned char* pages;
+  int num_pages;
+  const int *tables, *cu_q_lens, *context_lens;
+  int bt_stride, B, least, nkv, d, page_size, window, out_pages;
+  int* out_tables;                 // [B, bt_stride]
+  UnfoldTiles tiles[2];            // height 0: none
+};
+__device__ __forceinline__ int unfold_keys(const UnfoldArgs& a, int b, int* q_len) {
+  *q_len = a.cu_q_lens[b + 1] - a.cu_q_lens[b];
+  if (*q_len < a.least) *q_len = 0;
+  return *q_len ? (int)min((long long)a.context_lens[b], (long long)a.bt_stride * a.page_size) : 0;
+}
+__device__ __forceinline__ int unfold_skip(const UnfoldArgs& a, int ctx, int q_len) {          // pages nobody sees
+  return a.window > 0 ? max(0, ctx - q_len - a.window + 1) / a.page_size : 0;
+}
+
+template <typename TO, int BITS>
+__global__ void __launch_bounds__(256) packed_unfold_kernel(UnfoldArgs a, TO* __restrict__ k_out, TO* __restrict__ v_out) {
+  __shared__ int red[8];
+  pdl_trigger();
+  pdl_wait();
+  const int b = blockIdx.y, j = blockIdx.x, lane = threadIdx.x & 31;
+  int q_len;
+  const int ctx = unfold_keys(a, b, &q_len);
+  const int skip = unfold_skip(a, ctx, q_len), P = a.page_size;
+  // pages of the sequences before this one
+  int before = 0;
+  for (int i = threadIdx.x; i < b; i += blockDim.x) {
+    int n;
+    const int c = unfold_keys(a, i, &n);
+    before += (c + P - 1) / P - unfold_skip(a, c, n);
+  }
 #pragma unroll
-    for (int i = 0; i < 8; ++i) y[i] = real ? r.value(block, which, place, c + i) : 0.f;
-    store4(o, make_float4(y[0], y[1], y[2], y[3]));
-    store4(o + 4, make_float4(y[4], y[5], y[6], y[7]));
+  for (int o = 16; o > 0; o >>= 1) before += __shfl_xor_sync(0xffffffffu, before, o);
+  if (lane == 0) red[threadIdx.x >> 5] = before;
+  __syncthreads();
+  before = 0;
+#pragma unroll
+  for (int w = 0; w < 8; ++w) before += red[w];
+  if (j * P < ctx) {
+    const int to = before + j - skip;
+    const bool seen = j >= skip && to < a.out_pages;
+    if (threadIdx.x == 0 && blockIdx.z == 0) a.out_tables[(size_t)b * a.bt_stride + j] = seen ? to : -1;
+    if (seen) {
+      const size_t at = (size_t)to * a.nkv * P * a.d;
+      unpack_page<TO, BITS>(a.pages, a.tables[(size_t)b * a.bt_stride + j], a.num_pages, ctx - j * P, k_out + at, v_out + at, a.nkv, a.d, P);
+    }
+  }
+  if (j != gridDim.x - 1 || b != 0 || blockIdx.z != 0) return;
+  // ---- one block lists the tiles: each thread takes sequences, then tiles
+  __shared__ int seq_s[UNFOLD_SORTED], q0_s[UNFOLD_SORTED], keys_s[UNFOLD_SORTED];
+  for (int l = 0; l < 2; ++l) {
+    const UnfoldTiles t = a.tiles[l];
+    if (!t.height) continue;
+    __syncthreads();
+    const bool sorted = t.count <= UNFOLD_SORTED;
+    for (int i = threadIdx.x; i < t.count; i += blockDim.x) {   // (a count beyond what the portions make repeats a tile)
+      if (sorted) { seq_s[i] = -1; keys_s[i] = -1; }
+      else { t.seq[i] = 0; t.q0[i] = 0; }
+    }
+    __syncthreads();
+    for (int s = threadIdx.x; s < a.B; s += blockDim.x) {
+      int n, at = 0;
+      for (int i = 0; i < s; ++i) {
+        const int m = a.cu_q_lens[i + 1] - a.cu_q_lens[i];
+        at += m >= a.least ? (m + t.height - 1) / t.height : 0;
+      }
+      const int c = unfold_keys(a, s, &n);
+      for (int r = 0; r < n; r += t.height, ++at) {
+        if (at >= t.count) break;
+        if (sorted) { seq_s[at] = s; q0_s[at] = r; keys_s[at] = c - n + min(n, r + t.height); }
+        else { t.seq[at] = s; t.q0[at] = r; }
+      }
+    }
+    if (!sorted) continue;
+    __syncthreads();
+    for (int i = threadIdx.x; i < t.count; i += blockDim.x) {
+      int rank = 0;
+      const int mine = keys_s[i];
+      for (int k = 0; k < t.count; ++k) rank += keys_s[k] > mine || (keys_s[k] == mine && k < i);
+      const int k = seq_s[i] < 0 ? 0 : i;
+      t.seq[rank] = max(seq_s[k], 0);
+      t.q0[rank] = seq_s[k] < 0 ? 0 : q0_s[k];
+    }
   }
 }
 
@@ -194,6 +327,13 @@ extern "C" int gg_packed_write(const void* qkv, long long row_stride, int act_dt
   return gg_check_launch("packed_write");
 }
 
+// Blocks of a page: its kv heads are spread until the launch has a few blocks for every multiprocessor.
+static int head_blocks(long long pages, int nkv) {
+  int z = 1;
+  while (z < nkv && z < 64 && pages * z < 1200) z *= 2;
+  return z < nkv ? z : nkv;
+}
+
 extern "C" int gg_packed_read(const void* pages, int num_pages, const int* tables, int bt_stride, const int* lens, const int* first_page,
                               void* k_out, void* v_out, int out_dtype, int out_pages, int B, int most_pages, int nkv, int d, int page_size,
                               int bits, cudaStream_t stream) {
@@ -201,17 +341,37 @@ extern "C" int gg_packed_read(const void* pages, int num_pages, const int* table
   if (rc) return rc;
   GG_REQUIRE(B >= 0 && B <= 65535 && most_pages >= 0 && most_pages <= bt_stride, "packed_read: bad sizes B=%d pages=%d of %d", B, most_pages, bt_stride);
   GG_REQUIRE(((size_t)k_out % 16) == 0 && ((size_t)v_out % 16) == 0, "packed_read: the outputs must start on 16 bytes");
+  GG_REQUIRE(out_dtype == GG_F32 || out_dtype == GG_BF16, "packed_read: unknown dtype %d", out_dtype);
   if (B == 0 || most_pages == 0) return GG_OK;
-  const dim3 grid(most_pages, B), block(256);
-  if (out_dtype == GG_F32)
-    gg_launch(packed_read_kernel<float>, grid, block, 0, stream, (const unsigned char*)pages, num_pages, tables, bt_stride, lens, first_page,
-              (float*)k_out, (float*)v_out, out_pages, nkv, d, page_size, bits);
-  else if (out_dtype == GG_BF16)
-    gg_launch(packed_read_kernel<__nv_bfloat16>, grid, block, 0, stream, (const unsigned char*)pages, num_pages, tables, bt_stride, lens,
-              first_page, (__nv_bfloat16*)k_out, (__nv_bfloat16*)v_out, out_pages, nkv, d, page_size, bits);
-  else
-    return gg_fail(GG_ERR_INVALID, "packed_read: unknown dtype %d", out_dtype);
+  const dim3 grid(most_pages, B, head_blocks(out_pages, nkv)), block(256);
+#define READ_LAUNCH(TO, BITS) gg_launch(packed_read_kernel<TO, BITS>, grid, block, 0, stream, (const unsigned char*)pages, num_pages, tables, \
+                                        bt_stride, lens, first_page, (TO*)k_out, (TO*)v_out, out_pages, nkv, d, page_size)
+  if (out_dtype == GG_F32) { if (bits == 4) READ_LAUNCH(float, 4); else READ_LAUNCH(float, 8); }
+  else { if (bits == 4) READ_LAUNCH(__nv_bfloat16, 4); else READ_LAUNCH(__nv_bfloat16, 8); }
   return gg_check_launch("packed_read");
+}
+
+extern "C" int gg_packed_unfold(const void* pages, int num_pages, const int* tables, int bt_stride, const int* cu_q_lens,
+                                const int* context_lens, int B, void* k_out, void* v_out, int out_dtype, int out_pages, int most_pages,
+                                int* out_tables, int height0, int count0, int* seq0, int* q00, int height1, int count1, int* seq1, int* q01,
+                                int least, int nkv, int d, int page_size, int bits, int window, cudaStream_t stream) {
+  int rc = check_packed("packed_unfold", pages, num_pages, nkv, d, page_size, bits);
+  if (rc) return rc;
+  GG_REQUIRE(B > 0 && B <= 65535 && most_pages > 0 && most_pages <= bt_stride && window >= 0 && height0 >= 0 && height1 >= 0,
+             "packed_unfold: bad sizes B=%d pages=%d of %d window=%d", B, most_pages, bt_stride, window);
+  GG_REQUIRE(((size_t)k_out % 16) == 0 && ((size_t)v_out % 16) == 0, "packed_unfold: the outputs must start on 16 bytes");
+  GG_REQUIRE(out_dtype == GG_F32 || out_dtype == GG_BF16, "packed_unfold: unknown dtype %d", out_dtype);
+  UnfoldArgs a = {};
+  a.pages = (const unsigned char*)pages; a.num_pages = num_pages; a.tables = tables; a.cu_q_lens = cu_q_lens; a.context_lens = context_lens;
+  a.bt_stride = bt_stride; a.B = B; a.least = least > 1 ? least : 1; a.nkv = nkv; a.d = d; a.page_size = page_size; a.window = window; a.out_pages = out_pages;
+  a.out_tables = out_tables;
+  a.tiles[0] = {height0, count0, seq0, q00};
+  a.tiles[1] = {height1, count1, seq1, q01};
+  const dim3 grid(most_pages, B, head_blocks(out_pages, nkv)), block(256);
+#define UNFOLD_LAUNCH(TO, BITS) gg_launch(packed_unfold_kernel<TO, BITS>, grid, block, 0, stream, a, (TO*)k_out, (TO*)v_out)
+  if (out_dtype == GG_F32) { if (bits == 4) UNFOLD_LAUNCH(float, 4); else UNFOLD_LAUNCH(float, 8); }
+  else { if (bits == 4) UNFOLD_LAUNCH(__nv_bfloat16, 4); else UNFOLD_LAUNCH(__nv_bfloat16, 8); }
+  return gg_check_launch("packed_unfold");
 }
 
 // ---------------------------------------------------------------- attention
