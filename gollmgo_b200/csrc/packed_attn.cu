@@ -16,19 +16,17 @@
 // channels of four keys for the output, whose pairs (key, key) are put together by byte permutation.  The weights pass from the
 // score layout to the B operand by a register transpose of 8 x 8.
 //
-// Bytes are what bounds it (4.5 or 8.5 bits a channel; two products on 16 keys cost ~170 instructions a warp), so the work is cut
-// into equal ranges of tiles of 32 keys over all (token, kv head) pairs: one range a block, tile after tile to the block's
-// warps.  A warp brings its tiles by bulk copies (one per page and kv head) into a ring of its own, ahead of the pair it works
-// on, and shares nothing with the others until the block's part of a pair is merged.  Pairs that were cut between blocks are
-// joined by a second kernel.
+// Bytes are what bounds it (4.5 or 8.5 bits a channel), closely followed by the masks that make operands of codes.  The work is
+// cut into equal ranges of tiles over all (token, kv head) pairs, a range for each warp.  A warp brings its tiles by bulk copies
+// (one per page and kv head) into a ring of its own, the pages of its next 16 or 32 tiles found by one lane each, and shares
+// nothing until it is done: a pair that lies inside its range is written out, parts of pairs are joined inside the block and
+// then, by a second kernel, between blocks.
 #include "attention_common.cuh"
 #include "packed_kv.cuh"
 #include "tc_common.cuh"
 
 #include <cuda_fp16.h>
 
-#define PD_TILE 32                 // keys of a tile
-#define PD_WARPS 8
 #define PD_MAX_TOKENS 1024         // tokens of one launch
 #define PD_STATUS 71               // reported where a copy did not arrive
 #define PD_LOG2E 1.4426950408889634f
@@ -53,8 +51,9 @@ struct PackedDecode {
   const float* sink;
   const float* slopes;
   float temp_coef, temp_every;
-  float* part;                     // [2 * blocks][8 NT * D + 2 * 8 NT]: outputs, then (max, sum) pairs
-  int* prefix;                     // [n + 1]
+  float* part;                     // parts of pairs, [8 NT * D + 2 * 8 NT] each (outputs, then max and sum of each head): two of every block,
+                                   // then one of every warp
+  int4* cut;                       // of each block: what the second kernel joins (see there)
   int blocks, stages;
   int* status;
 };
@@ -85,30 +84,29 @@ __device__ __forceinline__ uint4 lds128(unsigned a) {
 }
 __device__ __forceinline__ float power_of_two(int e) { return __uint_as_float((unsigned)(e + 127) << 23); }   // -126 <= e <= 127
 
-// The keys in sight of token i: [lo, context), counted in tiles from the tile of lo.  A context that its block table
-// cannot hold is cut there.
-__device__ __forceinline__ void token_keys(const PackedDecode& a, int i, int* seq, int* context, int* lo) {
-  const int b = a.seqs ? a.seqs[i] : i;
-  long long most = (long long)a.bt_stride << a.page_log2;
-  const int c = b >= 0 ? (int)min((long long)a.context_lens[b], most) : 0;
-  *seq = b;
-  *context = max(c, 0);
-  *lo = a.window > 0 ? max(0, c - a.window) : 0;
+// Tokens of sequence b that can be in sight: a context that its block table cannot hold is cut there.
+__device__ __forceinline__ int context_of(const PackedDecode& a, int b) {
+  const long long most = (long long)a.bt_stride << a.page_log2;
+  return b >= 0 ? max(0, (int)min((long long)a.context_lens[b], most)) : 0;
 }
-__device__ __forceinline__ int token_tiles(const PackedDecode& a, int i) {
-  int b, c, lo;
-  token_keys(a, i, &b, &c, &lo);
-  return c > lo ? (c + PD_TILE - 1) / PD_TILE - lo / PD_TILE : 0;
-}
+// Its keys in sight are [first_key, context), counted in tiles from the tile of the first.
+__device__ __forceinline__ int first_key(const PackedDecode& a, int context) { return a.window > 0 ? max(0, context - a.window) : 0; }
+// Pairs of a token are (kv head, chunk of its query heads), chunk by chunk.
+__device__ __forceinline__ int kv_head(const PackedDecode& a, int pair) { return a.chunks == 1 ? pair : pair / a.chunks; }
 
-// prefix[i] = tiles of the tokens before i (of all their pairs), for every block alike
-template <int THREADS>
-__device__ __forceinline__ void scan_tiles(const PackedDecode& a, int pairs, int* prefix, int* wsum) {
+// prefix[i] = tiles of the tokens before i (of all their pairs), contexts[i] = context of token i, for every block alike
+template <int TILE, int THREADS>
+__device__ __forceinline__ void scan_tiles(const PackedDecode& a, int pairs, int* prefix, int* contexts, int* wsum) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   int base = 0;
   for (int i0 = 0; i0 < a.n; i0 += THREADS) {
     const int i = i0 + threadIdx.x;
-    const int mine = i < a.n ? token_tiles(a, i) * pairs : 0;
+    int mine = 0;
+    if (i < a.n) {
+      const int c = context_of(a, a.seqs ? a.seqs[i] : i), lo = first_key(a, c);
+      contexts[i] = c;
+      mine = c > lo ? ((c + TILE - 1) / TILE - lo / TILE) * pairs : 0;
+    }
     int v = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -133,136 +131,169 @@ __device__ __forceinline__ void scan_tiles(const PackedDecode& a, int pairs, int
 __device__ __forceinline__ int range_start(int block, int blocks, int total) { return (int)((long long)total * block / blocks); }
 
 // A place in the sequence of all tiles: tile f lies in pair `pair` of token i, whose tiles are [base, base + tiles).
-struct TileCursor {
+template <int TILE> struct TileCursor {
   int i, pair, base, tiles;
-  __device__ __forceinline__ void settle(const int* prefix, int pairs) {   // tiles of token i
-    tiles = (prefix[i + 1] - prefix[i]) / pairs;
+  __device__ __forceinline__ void settle(const PackedDecode& a, const int* contexts) {   // tiles of token i
+    tiles = (int)((unsigned)(contexts[i] + TILE - 1) / TILE - (unsigned)first_key(a, contexts[i]) / TILE);
   }
-  __device__ __forceinline__ void start(const int* prefix, int n, int pairs, int f) {
-    int lo = 0, hi = n - 1;                       // the last token whose tiles start at f or before and that has any
+  __device__ __forceinline__ void start(const PackedDecode& a, const int* prefix, const int* contexts, int f) {
+    int lo = 0, hi = a.n - 1;                     // the last token whose tiles start at f or before and that has any
     while (lo < hi) {
       const int m = (lo + hi + 1) >> 1;
       if (prefix[m] <= f) lo = m; else hi = m - 1;
     }
     i = lo;
-    settle(prefix, pairs);
-    pair = (f - prefix[i]) / tiles;
+    settle(a, contexts);
+    const int rest = f - prefix[i];
+    pair = (int)__fdividef((float)rest, (float)tiles);      // a small number: off by one at most
+    if (pair * tiles > rest) --pair;
+    if ((pair + 1) * tiles <= rest) ++pair;
     base = prefix[i] + pair * tiles;
   }
-  __device__ __forceinline__ void advance(const int* prefix, int pairs, int f) {   // f < prefix[n]
+  __device__ __forceinline__ void advance(const PackedDecode& a, const int* contexts, int pairs, int f) {   // f < prefix[n]
     while (f >= base + tiles) {
       base += tiles;
       if (++pair == pairs) {
         pair = 0;
-        do { ++i; settle(prefix, pairs); } while (tiles == 0);
+        do { ++i; settle(a, contexts); } while (tiles <= 0);
       }
     }
   }
 };
 
-template <int D, int BITS, int NT, bool OPT>
-__global__ void __launch_bounds__(PD_WARPS * 32, (D == 128 && NT == 1 && BITS == 4) || (D == 64 && NT == 1) ? 2 : 1)
-packed_decode_kernel(PackedDecode a) {
-  constexpr int GR = D / 64, ROW = D * BITS / 8, HEADS = 8 * NT;
-  constexpr int STAGE = 2 * PD_TILE * (ROW + 4 * GR);
-  extern __shared__ __align__(128) unsigned char smem[];
-  __shared__ int wsum[PD_WARPS];
-  __shared__ float top_s[PD_WARPS][HEADS], sum_s[PD_WARPS][HEADS];
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
-  const int pairs = a.nkv * a.chunks;
-  // shared memory: rings, merge buffer [WARPS / 2][HEADS * D], barriers, which chunks of a stage are there, prefix
-  unsigned char* ring_p = smem + (size_t)warp * a.stages * STAGE;
-  float* merge = reinterpret_cast<float*>(smem + (size_t)PD_WARPS * a.stages * STAGE);
-  unsigned long long* bars = reinterpret_cast<unsigned long long*>(merge + PD_WARPS / 2 * HEADS * D);
-  unsigned* there = reinterpret_cast<unsigned*>(bars + PD_WARPS * a.stages);
-  int* prefix = reinterpret_cast<int*>(there + PD_WARPS * a.stages);
-  const unsigned ring = tc_smem(ring_p), bar0 = tc_smem(bars + warp * a.stages);
-  there += warp * a.stages;
-  if (lane == 0) {
-    for (int s = 0; s < a.stages; ++s) mbar_init(bar0 + 8 * s, 1);
-    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+// Shapes of the kernel: warps of a block (16 at 128 registers a thread, or 8), keys of a tile.  Twice the heads take twice the
+// registers, so half the warps; a
+// tile is about the same bytes in 4 and in 8 bits.
+template <int D, int BITS, int NT> struct PdSizes {
+  static constexpr int WARPS = NT == 1 ? 16 : 8, TILE = BITS == 4 ? 32 : 16, THREADS = WARPS * 32;
+  static constexpr int GR = D / 64, ROW = D * BITS / 8, HEADS = 8 * NT, PART = HEADS * D + 2 * HEADS;      // PART in floats
+  static constexpr int STAGE = 2 * TILE * (ROW + 4 * GR);
+  static constexpr int smem(int stages, int n) {
+    return WARPS * stages * (STAGE + 8 + 4) + (2 * n + 1) * 4;
   }
+};
+
+template <int D, int BITS, int NT, bool OPT>
+__global__ void __launch_bounds__(PdSizes<D, BITS, NT>::THREADS, 1) packed_decode_kernel(PackedDecode a) {
+  typedef PdSizes<D, BITS, NT> Z;
+  constexpr int GR = Z::GR, ROW = Z::ROW, HEADS = Z::HEADS, STAGE = Z::STAGE, TILE = Z::TILE, WARPS = Z::WARPS, KB = TILE / 16;
+  extern __shared__ __align__(128) unsigned char smem[];
+  __shared__ int wsum[WARPS];
+  // a warp's two parts: which pair (its first tile) they belong to, or -1; maximum and sum of each head; weight in the joined pair
+  __shared__ int part_base[2 * WARPS];
+  __shared__ int4 part_pair[2 * WARPS];            // tiles and heads of that pair, its first row of the result
+  __shared__ float part_top[2 * WARPS][HEADS], part_sum[2 * WARPS][HEADS], part_weight[2 * WARPS][HEADS];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
+  const int pairs = a.nkv * a.chunks, S = a.stages;
+  // shared memory: a ring per warp, its barriers, the chunks of a stage that are there, prefix, contexts
+  unsigned long long* bars = reinterpret_cast<unsigned long long*>(smem + (size_t)WARPS * S * STAGE);
+  unsigned* here = reinterpret_cast<unsigned*>(bars + WARPS * S) + warp * S;
+  int* prefix = reinterpret_cast<int*>(bars + WARPS * S) + WARPS * S;
+  int* contexts = prefix + a.n + 1;
+  float* parts = a.part + ((size_t)2 * a.blocks + (size_t)blockIdx.x * WARPS) * Z::PART;
+  const unsigned ring = tc_smem(smem) + warp * S * STAGE, full = tc_smem(bars + warp * S);
+  if (lane < S) mbar_init(full + 8 * lane, 1);
+  if (tid < 2 * WARPS) part_base[tid] = -1;
+  asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   pdl_trigger();
   pdl_wait();
-  scan_tiles<PD_WARPS * 32>(a, pairs, prefix, wsum);
+  scan_tiles<TILE, Z::THREADS>(a, pairs, prefix, contexts, wsum);
   const int total = prefix[a.n];
-  if (blockIdx.x == 0)
-    for (int i = tid; i <= a.n; i += PD_WARPS * 32) a.prefix[i] = prefix[i];
-  const int f_lo = range_start(blockIdx.x, a.blocks, total), f_hi = range_start(blockIdx.x + 1, a.blocks, total);
-  if (f_lo >= f_hi) return;
-  if (lane == 0) asm volatile("fence.proxy.async;" ::: "memory");    // pages that the kernel ahead wrote, read by bulk copies
+  for (int i = blockIdx.x; i < a.n; i += a.blocks) {          // a token without a key in sight gets zeros
+    const int b = a.seqs ? a.seqs[i] : i;
+    if (contexts[i] > 0 || b < 0) continue;
+    __nv_bfloat162* o = reinterpret_cast<__nv_bfloat162*>(a.out + (size_t)(a.cu_q_lens ? a.cu_q_lens[b] : b) * a.nh * D);
+    for (int e = tid; e < a.nh * D / 2; e += Z::THREADS) o[e] = __floats2bfloat162_rn(0.f, 0.f);
+  }
+  if (tid == 0) a.cut[blockIdx.x] = make_int4(-1, 0, 0, 0);
+  const int blocks = min(a.blocks, total);         // each has a tile at least
+  if ((int)blockIdx.x >= blocks) return;
+  const int b_lo = range_start(blockIdx.x, blocks, total), b_hi = range_start(blockIdx.x + 1, blocks, total);
+  asm volatile("fence.proxy.async;" ::: "memory");            // pages that the kernel ahead wrote, read by bulk copies
 
-  // chunks: the tokens of a tile that lie in one page, 16 or 32
-  const int chunk = a.page_log2 == 4 ? 16 : 32, chunks = PD_TILE / chunk;
+  // chunks: the tokens of a tile that lie in one page
+  const int chunk = a.page_log2 == 4 ? 16 : TILE, chunks = TILE / chunk, two = chunks >> 1;      // two: log2 of chunks
   const int chunk_bytes = 2 * chunk * (ROW + 4 * GR);
-  const int page_mask = (1 << a.page_log2) - 1;
+  const int w_lo = b_lo + (b_hi - b_lo) * warp / WARPS, w_hi = b_lo + (b_hi - b_lo) * (warp + 1) / WARPS;
 
-  // ---- the ring: tile f = f_lo + warp + PD_WARPS * k of this warp goes to stage k % stages
-  TileCursor ahead;
-  int f_ahead = f_lo + warp, ahead_id = -1;       // the next tile to be asked for, and (lane < chunks) its page
-  int ahead_seq = -1, ahead_token = -1, ahead_first = 0, ahead_ctx = 0;
-  if (f_ahead < f_hi) ahead.start(prefix, a.n, pairs, f_ahead);
-  const int* ahead_row = nullptr;
-  auto look_up = [&]() {                          // load the page id of the tile at f_ahead
-    if (f_ahead >= f_hi) return;
-    ahead.advance(prefix, pairs, f_ahead);
-    if (ahead.i != ahead_token) {
-      int lo;
-      token_keys(a, ahead.i, &ahead_seq, &ahead_ctx, &lo);
-      ahead_token = ahead.i;
-      ahead_first = lo / PD_TILE * PD_TILE;
-      ahead_row = a.tables + (size_t)ahead_seq * a.bt_stride;
-    }
-    const int key = ahead_first + (f_ahead - ahead.base) * PD_TILE + lane * chunk;
-    ahead_id = lane < chunks && key < ahead_ctx ? ahead_row[key >> a.page_log2] : -1;
+  // ---- the ring.  Lane j knows chunk j of the tiles [batch, batch + 32 / chunks): its page, kv head and place in the page;
+  // the ones of the batch that follows are being looked up.
+  int batch = w_lo, f_ask = w_lo, id = -1, id_next = -1, spot = 0, spot_next = 0;
+  unsigned there = 0;
+  TileCursor<TILE> mine;
+  auto look_up = [&](int from) {
+    const int f = from + (lane >> two);
+    id_next = -1;
+    if (f >= w_hi) return;
+    TileCursor<TILE>& at = mine;
+    at.start(a, prefix, contexts, f);
+    const int ctx = contexts[at.i], b = a.seqs ? a.seqs[at.i] : at.i;
+    const int key = first_key(a, ctx) / TILE * TILE + (f - at.base) * TILE + (lane & (chunks - 1)) * chunk;
+    if (key < ctx) id_next = a.tables[(size_t)b * a.bt_stride + (key >> a.page_log2)];
+    spot_next = kv_head(a, at.pair) << 8 | (key & ((1 << a.page_log2) - 1));
   };
-  auto ask = [&](int stage) {                     // start the copies of the tile at f_ahead
-    if (f_ahead >= f_hi) return;
-    const bool ok = ahead_id >= 0 && ahead_id < a.num_pages;
-    const unsigned mask = __ballot_sync(0xffffffffu, ok);
-    const unsigned bar = bar0 + 8 * stage;
+  auto ask = [&](int stage) {                      // start the copies of tile f_ask
+    if (f_ask >= w_hi) return;
+    if (f_ask == batch + (32 >> two) || f_ask == w_lo) {
+      batch = f_ask;
+      id = id_next;
+      spot = spot_next;
+      there = __ballot_sync(0xffffffffu, id >= 0 && id < a.num_pages);
+      look_up(batch + (32 >> two));
+    }
+    const int k = f_ask - batch;
+    const unsigned mask = (there >> (k << two)) & ((1u << chunks) - 1), bar = full + 8 * stage;
     if (lane == 0) {
-      there[stage] = mask;
+      here[stage] = mask;
       mbar_expect_tx(bar, __popc(mask) * chunk_bytes);
     }
     __syncwarp();
-    if (ok) {
-      const int key = ahead_first + (f_ahead - ahead.base) * PD_TILE + lane * chunk;
-      const unsigned char* block = a.pages + ((size_t)ahead_id * a.nkv + ahead.pair / a.chunks) * a.page_bytes;
-      const unsigned dst = ring + stage * STAGE + lane * chunk_bytes;
+    if ((lane >> two) == k && ((there >> lane) & 1)) {
+      const unsigned char* block = a.pages + ((size_t)id * a.nkv + (spot >> 8)) * a.page_bytes;
+      const unsigned dst = ring + stage * STAGE + (lane & (chunks - 1)) * chunk_bytes;
       if (a.page_log2 == 4) {
         bulk_load(dst, block, chunk_bytes, bar);
       } else {
-        const int place = key & page_mask, P = page_mask + 1;
+        const int place = spot & 255, P = 1 << a.page_log2;
         bulk_load(dst, block + place * ROW, chunk * ROW, bar);
         bulk_load(dst + chunk * ROW, block + (P + place) * ROW, chunk * ROW, bar);
         bulk_load(dst + 2 * chunk * ROW, block + 2 * P * ROW + place * GR * 4, chunk * GR * 4, bar);
         bulk_load(dst + 2 * chunk * ROW + chunk * GR * 4, block + 2 * P * ROW + (P + place) * GR * 4, chunk * GR * 4, bar);
       }
     }
-    f_ahead += PD_WARPS;
+    ++f_ask;
   };
-  look_up();
-  for (int s = 0; s < a.stages; ++s) { ask(s); look_up(); }
+  look_up(w_lo);
+  TileCursor<TILE> at;                             // the first pair of the range, which lane 0 has just found
+  at.i = __shfl_sync(0xffffffffu, mine.i, 0);
+  at.pair = __shfl_sync(0xffffffffu, mine.pair, 0);
+  at.base = __shfl_sync(0xffffffffu, mine.base, 0);
+  at.tiles = __shfl_sync(0xffffffffu, mine.tiles, 0);
+  if (w_lo < w_hi) {
+    const int b = a.seqs ? a.seqs[at.i] : at.i, row = a.cu_q_lens ? a.cu_q_lens[b] : b;
+    const int kvh = kv_head(a, at.pair), head = kvh * a.group + (at.pair - kvh * a.chunks) * HEADS;
+    // the queries are on their way while the first pages are looked up: 64 bytes a lane
+    if (lane < min(HEADS, a.nh - head) * D / 32)
+      asm volatile("prefetch.global.L1 [%0];" ::"l"(a.q + (size_t)row * a.q_stride + (size_t)head * D + lane * 32));
+  }
+#pragma unroll 1
+  for (int s = 0; s < S; ++s) ask(s);
 
-  // ---- the pairs of this block's range, one after the other
+  // ---- the pairs of the warp's range, one after the other
   const int key_g = (g >> 1) + 4 * (g & 1);       // the key (of 16) in row g of the scores; row g + 8 has key_g + 8
   const int step_c = chunk == 16 ? chunk_bytes : 16 * ROW, step_p = chunk == 16 ? chunk_bytes : 16 * GR * 4;   // from 16 keys to the next
   const unsigned off_k = key_g * ROW + t * (2 * BITS);                     // a lane's 16 channels of its key
   const unsigned off_v = chunk * ROW + t * ROW + g * BITS;                 // its 8 channels of keys t, t + 4, t + 8, t + 12
   const unsigned off_kp = 2 * chunk * ROW + key_g * GR * 4, off_vp = off_kp + chunk * GR * 4;
-  int stage = 0, f = f_lo + warp;
+  int stage = 0, f = w_lo;
   unsigned phase = 0;
   bool broken = false;
-  TileCursor at;
-  at.start(prefix, a.n, pairs, f_lo);
-  for (int seg = f_lo; seg < f_hi;) {
-    at.advance(prefix, pairs, seg);
-    const int seg_end = min(at.base + at.tiles, f_hi);
-    int b, ctx, lo;
-    token_keys(a, at.i, &b, &ctx, &lo);
-    const int first_key = lo / PD_TILE * PD_TILE;
-    const int kvh = at.pair / a.chunks, head0 = (at.pair % a.chunks) * HEADS;
+  while (f < w_hi) {
+    at.advance(a, contexts, pairs, f);
+    const int seg = f, seg_end = min(at.base + at.tiles, w_hi);
+    const int b = a.seqs ? a.seqs[at.i] : at.i, ctx = contexts[at.i], lo = first_key(a, ctx);
+    const int tile0 = lo / TILE * TILE;
+    const int kvh = kv_head(a, at.pair), head0 = (at.pair - kvh * a.chunks) * HEADS;
     const int heads = min(HEADS, a.group - head0);
     const int row = a.cu_q_lens ? a.cu_q_lens[b] : b;
 
@@ -280,7 +311,7 @@ packed_decode_kernel(PackedDecode a) {
     }
     int vexp = -120;                               // weights are held times 2^(6 - vexp)
 
-    if (f < seg_end) {
+    {
       // ---- q of this pair: B operands, and its sums over each group
       unsigned qf[GR][4][NT][2];
       float qsum[GR][NT][2], qfac;
@@ -351,19 +382,19 @@ packed_decode_kernel(PackedDecode a) {
           }
       }
 
-      for (; f < seg_end; f += PD_WARPS) {
-        if (!broken) broken = __any_sync(0xffffffffu, !mbar_wait(bar0 + 8 * stage, phase));
+      for (; f < seg_end; ++f) {
+        if (!broken) broken = __any_sync(0xffffffffu, !mbar_wait(full + 8 * stage, phase));
         if (broken) {
           if (lane == 0 && a.status) *a.status = PD_STATUS;
         } else {
           const unsigned base = ring + stage * STAGE;
-          const int key0 = first_key + (f - at.base) * PD_TILE;
-          const unsigned mask = there[stage];
-          const bool whole = key0 >= lo && key0 + PD_TILE <= ctx && mask == (1u << chunks) - 1;
-          // ---- scores of 32 keys
-          float s[2][NT][4];
+          const int key0 = tile0 + (f - at.base) * TILE;
+          const unsigned mask = here[stage];
+          const bool whole = key0 >= lo && key0 + TILE <= ctx && mask == (1u << chunks) - 1;
+          // ---- scores
+          float s[KB][NT][4];
 #pragma unroll
-          for (int kb = 0; kb < 2; ++kb) {
+          for (int kb = 0; kb < KB; ++kb) {
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) s[kb][nt][0] = s[kb][nt][1] = s[kb][nt][2] = s[kb][nt][3] = 0.f;
             unsigned kp[2][GR];
@@ -418,7 +449,7 @@ packed_decode_kernel(PackedDecode a) {
           }
           if (OPT) {
 #pragma unroll
-            for (int kb = 0; kb < 2; ++kb)
+            for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
               for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -430,9 +461,9 @@ packed_decode_kernel(PackedDecode a) {
                 }
           }
           // pairs of the values, and what is out of sight
-          float sv[2][2][GR], ov[2][2][GR];
+          float sv[KB][2][GR], ov[KB][2][GR];
 #pragma unroll
-          for (int kb = 0; kb < 2; ++kb)
+          for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
               unsigned u[GR];
@@ -452,7 +483,7 @@ packed_decode_kernel(PackedDecode a) {
             }
           if (!whole) {
 #pragma unroll
-            for (int kb = 0; kb < 2; ++kb)
+            for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
               for (int half = 0; half < 2; ++half) {
                 const int key = key0 + 16 * kb + 8 * half + key_g;
@@ -471,7 +502,8 @@ packed_decode_kernel(PackedDecode a) {
           for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
-              mx[nt][j] = fmaxf(fmaxf(s[0][nt][j], s[0][nt][2 + j]), fmaxf(s[1][nt][j], s[1][nt][2 + j]));
+              mx[nt][j] = fmaxf(s[0][nt][j], s[0][nt][2 + j]);
+              if (KB == 2) mx[nt][j] = fmaxf(mx[nt][j], fmaxf(s[KB - 1][nt][j], s[KB - 1][nt][2 + j]));
               over = over || mx[nt][j] > ref[nt][j] + 8.f;
             }
           if (__any_sync(0xffffffffu, over)) {
@@ -493,9 +525,9 @@ packed_decode_kernel(PackedDecode a) {
                 for (int i = 0; i < GR * 4; ++i) { o[i][nt][j] *= al; o[i][nt][2 + j] *= al; }
               }
           }
-          float pmax = 0.f, smax = 0.f;
+          float smax = 0.f;
 #pragma unroll
-          for (int kb = 0; kb < 2; ++kb)
+          for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
 #pragma unroll
@@ -507,16 +539,15 @@ packed_decode_kernel(PackedDecode a) {
                   const float p = fast_exp2(s[kb][nt][2 * half + j] - ref[nt][j]);
                   s[kb][nt][2 * half + j] = p;
                   l[nt][j] += p;
-                  pmax = fmaxf(pmax, p);
 #pragma unroll
                   for (int gr = 0; gr < GR; ++gr) r[gr][nt][j] = fmaf(p, ov[kb][half][gr], r[gr][nt][j]);
                 }
             }
-          // ---- the weights' power of two: p s' stays below 2^9 times it
-          if (__any_sync(0xffffffffu, pmax * smax > power_of_two(vexp) * 512.f)) {
+          // ---- the weights' power of two: p s' stays below 2^9 times it (p is below 2^8)
+          if (__any_sync(0xffffffffu, smax > power_of_two(vexp + 1))) {
             float w = 0.f;
 #pragma unroll
-            for (int kb = 0; kb < 2; ++kb)
+            for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
               for (int half = 0; half < 2; ++half) {
                 float p = 0.f, z = 0.f;
@@ -527,7 +558,7 @@ packed_decode_kernel(PackedDecode a) {
                 w = fmaxf(w, p * z);
               }
             w = warp_max(w);
-            const int e = max(vexp, min(100, (int)(__float_as_uint(w) >> 23) - 127));
+            const int e = w > power_of_two(vexp) * 512.f ? min(100, (int)(__float_as_uint(w) >> 23) - 127) : vexp;
             const float down = vexp - e < -126 ? 0.f : power_of_two(vexp - e);
             vexp = e;
 #pragma unroll
@@ -540,7 +571,7 @@ packed_decode_kernel(PackedDecode a) {
           const float inv = power_of_two(6 - vexp);
           // ---- output: channels x heads
 #pragma unroll
-          for (int kb = 0; kb < 2; ++kb)
+          for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
             for (int gr = 0; gr < GR; ++gr) {
               unsigned pb[NT][2];
@@ -580,12 +611,12 @@ packed_decode_kernel(PackedDecode a) {
             }
         }
         __syncwarp();                              // every lane has read the stage
-        if (!broken) { ask(stage); look_up(); }
-        if (++stage == a.stages) { stage = 0; phase ^= 1; }
+        if (!broken) ask(stage);
+        if (++stage == S) { stage = 0; phase ^= 1; }
       }
     }
 
-    // ---- the warps' parts of the pair become one
+    // ---- the pair's result, or this warp's part of it
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -596,155 +627,168 @@ packed_decode_kernel(PackedDecode a) {
 #pragma unroll
           for (int gr = 0; gr < GR; ++gr) r[gr][nt][j] += __shfl_xor_sync(0xffffffffu, r[gr][nt][j], m);
         }
-    if (g == 0) {
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          top_s[warp][nt * 8 + 2 * t + j] = ref[nt][j];
-          sum_s[warp][nt * 8 + 2 * t + j] = l[nt][j];
-        }
+    const bool complete = seg == at.base && seg_end == at.base + at.tiles;
+    // the last part of the range goes where the ring was (all its copies have arrived and been read), the first to the scratch
+    const bool last = seg_end == w_hi;
+    float* part = last ? reinterpret_cast<float*>(smem + (size_t)warp * S * STAGE) : parts + warp * Z::PART;
+    if (!complete && lane == 0) {
+      part_base[2 * warp + last] = at.base;
+      part_pair[2 * warp + last] = make_int4(at.tiles, heads, row * a.nh + kvh * a.group + head0, 0);
     }
-    __syncthreads();
-    float M[NT][2], L[NT][2];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
         const int h = nt * 8 + 2 * t + j;
-        M[nt][j] = PD_NO_KEY;
-        L[nt][j] = 0.f;
-        for (int w = 0; w < PD_WARPS; ++w) M[nt][j] = fmaxf(M[nt][j], top_s[w][h]);
-        for (int w = 0; w < PD_WARPS; ++w) L[nt][j] += sum_s[w][h] * fast_exp2(top_s[w][h] - M[nt][j]);
-        const float fc = fast_exp2(ref[nt][j] - M[nt][j]);
+        float fac = 1.f;
+        if (complete) {
+          float sum = l[nt][j];
+          if (OPT && a.sink && h < heads) {
+            const float sk = a.sink[kvh * a.group + head0 + h] * PD_LOG2E, top = fmaxf(ref[nt][j], sk);
+            fac = fast_exp2(ref[nt][j] - top);
+            sum = sum * fac + fast_exp2(sk - top);
+          }
+          fac = sum != 0.f ? fac / sum : 0.f;
+        } else if (g == 0) {
+          part_top[2 * warp + last][h] = ref[nt][j];
+          part_sum[2 * warp + last][h] = l[nt][j];
+        }
+        const float even = power_of_two(18 + vexp) * fac, odd = BITS == 4 ? even * 0.0625f : even;
 #pragma unroll
-        for (int i = 0; i < GR * 4; ++i) {
-          const float off = r[i / 4][nt][j];
-          o[i][nt][j] = (scalbnf(o[i][nt][j], 18 + vexp) + off) * fc;
-          o[i][nt][2 + j] = (scalbnf(o[i][nt][2 + j], (BITS == 4 ? 14 : 18) + vexp) + off) * fc;
+        for (int gr = 0; gr < GR; ++gr) {
+          const float off = r[gr][nt][j] * fac;
+          float y[8];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            y[2 * i] = fmaf(o[gr * 4 + i][nt][j], even, off);
+            y[2 * i + 1] = fmaf(o[gr * 4 + i][nt][2 + j], odd, off);
+          }
+          const int c = gr * 64 + g * 8;
+          if (!complete) {
+            float4* p = reinterpret_cast<float4*>(part + h * D + c);
+            p[0] = make_float4(y[0], y[1], y[2], y[3]);
+            p[1] = make_float4(y[4], y[5], y[6], y[7]);
+          } else if (h < heads) {
+            const uint4 u = make_uint4(pack_bf16(y[0], y[1]), pack_bf16(y[2], y[3]), pack_bf16(y[4], y[5]), pack_bf16(y[6], y[7]));
+            *reinterpret_cast<uint4*>(a.out + ((size_t)row * a.nh + kvh * a.group + head0 + h) * D + c) = u;
+          }
         }
       }
-    // float4 slots [half of the warps][i, nt][lane]
-    float4* slot = reinterpret_cast<float4*>(merge);
-    constexpr int REGS = GR * 4 * NT;
-#pragma unroll
-    for (int w = PD_WARPS / 2; w >= 1; w >>= 1) {
-      if (warp >= w && warp < 2 * w) {
-#pragma unroll
-        for (int i = 0; i < GR * 4; ++i)
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
-            slot[((warp - w) * REGS + i * NT + nt) * 32 + lane] = make_float4(o[i][nt][0], o[i][nt][1], o[i][nt][2], o[i][nt][3]);
-      }
-      __syncthreads();
-      if (warp < w) {
-#pragma unroll
-        for (int i = 0; i < GR * 4; ++i)
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt) {
-            const float4 v = slot[(warp * REGS + i * NT + nt) * 32 + lane];
-            o[i][nt][0] += v.x; o[i][nt][1] += v.y; o[i][nt][2] += v.z; o[i][nt][3] += v.w;
-          }
-      }
-      __syncthreads();
-    }
-    if (warp == 0) {
-      const bool complete = seg == at.base && seg_end == at.base + at.tiles;
-      // a part that is not the whole pair is the block's first (slot 0) or its last
-      float* part = a.part + (size_t)(2 * blockIdx.x + (seg == f_lo ? 0 : 1)) * (HEADS * D + 2 * HEADS);
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const int h = nt * 8 + 2 * t + j;
-          if (h >= heads) continue;
-          float fac = 1.f;
-          if (complete) {
-            float sum = L[nt][j];
-            if (OPT && a.sink) {
-              const float sk = a.sink[kvh * a.group + head0 + h] * PD_LOG2E, top = fmaxf(M[nt][j], sk);
-              fac = fast_exp2(M[nt][j] - top);
-              sum = sum * fac + fast_exp2(sk - top);
-            }
-            fac = sum != 0.f ? fac / sum : 0.f;
-          } else if (g == 0) {
-            part[HEADS * D + 2 * h] = M[nt][j];
-            part[HEADS * D + 2 * h + 1] = L[nt][j];
-          }
-#pragma unroll
-          for (int gr = 0; gr < GR; ++gr) {
-            float y[8];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) { y[2 * i] = o[gr * 4 + i][nt][j] * fac; y[2 * i + 1] = o[gr * 4 + i][nt][2 + j] * fac; }
-            const int c = gr * 64 + g * 8;
-            if (complete) {
-              const uint4 u = make_uint4(pack_bf16(y[0], y[1]), pack_bf16(y[2], y[3]), pack_bf16(y[4], y[5]), pack_bf16(y[6], y[7]));
-              *reinterpret_cast<uint4*>(a.out + ((size_t)row * a.nh + kvh * a.group + head0 + h) * D + c) = u;
-            } else {
-              float4* p = reinterpret_cast<float4*>(part + h * D + c);
-              p[0] = make_float4(y[0], y[1], y[2], y[3]);
-              p[1] = make_float4(y[4], y[5], y[6], y[7]);
-            }
-          }
-        }
-    }
-    seg = seg_end;
   }
   if (broken) {                                    // leave no copy in flight behind
-    for (int s = 0; s < a.stages; ++s) mbar_wait(bar0 + 8 * ((stage + s) % a.stages), stage + s >= a.stages ? phase ^ 1 : phase);
+    if (lane == 0 && a.status) *a.status = PD_STATUS;
+    for (int s = 0; s < S; ++s) mbar_wait(full + 8 * ((stage + s) % S), stage + s >= S ? phase ^ 1 : phase);
+  }
+
+  // ---- the parts of one pair become the result, or this block's part of the pair
+  __syncthreads();
+  const int lane_base = lane < 2 * WARPS ? part_base[lane] : -1;
+  const unsigned same = __match_any_sync(0xffffffffu, lane_base);           // the parts of the same pair
+  unsigned leaders = __ballot_sync(0xffffffffu, lane_base >= 0 && (same & ((1u << lane) - 1)) == 0);
+  if (!leaders) return;
+  for (int e = tid; e < 2 * WARPS * HEADS; e += Z::THREADS) {               // (all threads, or whole warps of them)
+    const int i = e / HEADS, h = e % HEADS;
+    const unsigned members = __shfl_sync(0xffffffffu, same, i);
+    if (part_base[i] < 0) continue;
+    float M = PD_NO_KEY, L = 0.f;
+    for (unsigned m = members; m; m &= m - 1) M = fmaxf(M, part_top[__ffs(m) - 1][h]);
+    float w = fast_exp2(part_top[i][h] - M);
+    const int4 pair = part_pair[i];
+    const bool lead = i == __ffs(members) - 1, whole = part_base[i] >= b_lo && part_base[i] + pair.x <= b_hi;
+    if (lead || whole)
+      for (unsigned m = members; m; m &= m - 1) L += part_sum[__ffs(m) - 1][h] * fast_exp2(part_top[__ffs(m) - 1][h] - M);
+    if (whole) {                                   // the weight in the result
+      if (OPT && a.sink && h < pair.y) {
+        const float sk = a.sink[pair.z % a.nh + h] * PD_LOG2E, top = fmaxf(M, sk), u = fast_exp2(M - top);
+        w *= u;
+        L = L * u + fast_exp2(sk - top);
+      }
+      w = L != 0.f ? w / L : 0.f;
+    } else if (lead) {
+      float* to = a.part + (size_t)(2 * blockIdx.x + (part_base[i] < b_lo ? 0 : 1)) * Z::PART;
+      to[HEADS * D + 2 * h] = M;
+      to[HEADS * D + 2 * h + 1] = L;
+      // a pair that began in an earlier block and ends here is joined from there to here
+      if (h == 0 && part_base[i] < b_lo && part_base[i] + pair.x <= b_hi) {
+        int c = (int)(((long long)part_base[i] * blocks) / total);        // the block that holds its first tile
+        while (range_start(c + 1, blocks, total) <= part_base[i]) ++c;
+        while (range_start(c, blocks, total) > part_base[i]) --c;
+        a.cut[blockIdx.x] = make_int4(c, pair.y, pair.z, 0);
+      }
+    }
+    part_weight[i][h] = w;
+  }
+  __syncthreads();
+  // four values a thread: pairs side by side, PART / 4 threads each
+  constexpr int QUADS = HEADS * D / 4;
+  const int runs = __popc(leaders);
+  for (int e = tid; e < runs * QUADS; e += Z::THREADS) {                    // (whole warps: QUADS is a multiple of 32)
+    const int run = e / QUADS, x = (e % QUADS) * 4, h = x / D;
+    unsigned rest = leaders;
+    for (int i = 0; i < run; ++i) rest &= rest - 1;
+    const int k = __ffs(rest) - 1;
+    unsigned members = __shfl_sync(0xffffffffu, same, k);
+    const int4 pair = part_pair[k];
+    float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+    for (; members; members &= members - 1) {
+      const int i = __ffs(members) - 1;
+      const float* p = i & 1 ? reinterpret_cast<const float*>(smem + (size_t)(i >> 1) * S * STAGE) : parts + (i >> 1) * Z::PART;
+      const float4 v = *reinterpret_cast<const float4*>(p + x);
+      const float w = part_weight[i][h];
+      y.x = fmaf(w, v.x, y.x); y.y = fmaf(w, v.y, y.y); y.z = fmaf(w, v.z, y.z); y.w = fmaf(w, v.w, y.w);
+    }
+    if (part_base[k] >= b_lo && part_base[k] + pair.x <= b_hi) {
+      if (h < pair.y) *reinterpret_cast<uint2*>(a.out + (size_t)pair.z * D + x) = make_uint2(pack_bf16(y.x, y.y), pack_bf16(y.z, y.w));
+    } else {
+      *reinterpret_cast<float4*>(a.part + (size_t)(2 * blockIdx.x + (part_base[k] < b_lo ? 0 : 1)) * Z::PART + x) = y;
+    }
   }
 }
 
-// One block per (token, kv head, chunk of heads): joins the parts of a pair that was cut between blocks; a token without a
-// key in sight gets zeros.
+// Joins the pairs that were cut between blocks.  One block of threads for each block of the first kernel and head: where a pair
+// from an earlier block ends in it, cut[c] = (block of the pair's first tile, heads, first row of the result); that block has
+// its part second, the ones after it first.  Every 32 or 16 threads take some of the parts.
 template <int D, int NT>
-__global__ void __launch_bounds__(256) packed_join_kernel(PackedDecode a) {
-  constexpr int HEADS = 8 * NT, PART = HEADS * D + 2 * HEADS;
+__global__ void __launch_bounds__(128) packed_join_kernel(PackedDecode a) {
+  constexpr int HEADS = 8 * NT, PART = HEADS * D + 2 * HEADS, LANES = D / 4, SETS = 128 / LANES;
+  __shared__ float ml_s[SETS][2];
+  __shared__ float4 y_s[SETS][LANES];
   pdl_trigger();
   pdl_wait();
-  const int pairs = a.nkv * a.chunks, i = blockIdx.x / pairs, pair = blockIdx.x % pairs;
-  const int b = a.seqs ? a.seqs[i] : i;
-  if (b < 0) return;
-  const int lo = a.prefix[i], total = a.prefix[a.n], tiles = (a.prefix[i + 1] - lo) / pairs;
-  const int kvh = pair / a.chunks, head0 = (pair % a.chunks) * HEADS, heads = min(HEADS, a.group - head0);
-  const int row = a.cu_q_lens ? a.cu_q_lens[b] : b;
-  const int f0 = lo + pair * tiles, f1 = f0 + tiles;
-  int first = 0, last = -1;
-  if (tiles) {
-    // the block that holds tile f: the largest c with total * c / blocks <= f
-    auto holder = [&](int f) {
-      int c = (int)(((long long)f * a.blocks) / total);
-      while (c + 1 < a.blocks && range_start(c + 1, a.blocks, total) <= f) ++c;
-      while (c > 0 && range_start(c, a.blocks, total) > f) --c;
-      return c;
-    };
-    first = holder(f0);
-    last = holder(f1 - 1);
-    if (first == last) return;                     // whole in one block, which wrote the result
+  const int last = blockIdx.x, h = blockIdx.y, set = threadIdx.x / LANES, e = threadIdx.x % LANES;
+  const int4 cut = a.cut[last];
+  const int first = cut.x;
+  if (first < 0 || h >= cut.y) return;
+  float M = PD_NO_KEY, L = 0.f;
+  float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+  for (int c = first + set; c <= last; c += SETS) {
+    const float* p = a.part + (size_t)(2 * c + (c == first ? 1 : 0)) * PART;
+    const float m = p[HEADS * D + 2 * h], l = p[HEADS * D + 2 * h + 1];
+    const float4 v = reinterpret_cast<const float4*>(p + h * D)[e];
+    const float top = fmaxf(M, m), u = fast_exp2(M - top), w = fast_exp2(m - top);
+    L = L * u + w * l;
+    y.x = fmaf(w, v.x, u * y.x); y.y = fmaf(w, v.y, u * y.y); y.z = fmaf(w, v.z, u * y.z); y.w = fmaf(w, v.w, u * y.w);
+    M = top;
   }
-  for (int e = threadIdx.x * 4; e < heads * D; e += blockDim.x * 4) {
-    const int h = e / D;
-    float M = PD_NO_KEY, L = 0.f;
-    float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
-    auto part_of = [&](int c) { return a.part + (size_t)(2 * c + (c == first && range_start(c, a.blocks, total) != f0 ? 1 : 0)) * PART; };
-    for (int c = first; c <= last; ++c) M = fmaxf(M, part_of(c)[HEADS * D + 2 * h]);
-    for (int c = first; c <= last; ++c) {
-      const float* p = part_of(c);
-      const float w = fast_exp2(p[HEADS * D + 2 * h] - M);
-      const float4 v = *reinterpret_cast<const float4*>(p + e);
-      L = fmaf(w, p[HEADS * D + 2 * h + 1], L);
-      y.x = fmaf(w, v.x, y.x); y.y = fmaf(w, v.y, y.y); y.z = fmaf(w, v.z, y.z); y.w = fmaf(w, v.w, y.w);
-    }
-    float fac = 1.f;
-    if (a.sink) {
-      const float sk = a.sink[kvh * a.group + head0 + h] * PD_LOG2E, top = fmaxf(M, sk);
-      fac = fast_exp2(M - top);
-      L = L * fac + fast_exp2(sk - top);
-    }
-    fac = L != 0.f ? fac / L : 0.f;
-    const uint2 u = make_uint2(pack_bf16(y.x * fac, y.y * fac), pack_bf16(y.z * fac, y.w * fac));
-    *reinterpret_cast<uint2*>(a.out + ((size_t)row * a.nh + kvh * a.group + head0) * D + e) = u;
+  if (e == 0) { ml_s[set][0] = M; ml_s[set][1] = L; }
+  y_s[set][e] = y;
+  __syncthreads();
+  if (set) return;
+  const float sk = a.sink ? a.sink[cut.z % a.nh + h] * PD_LOG2E : PD_NO_KEY;
+  float top = sk;
+  for (int k = 0; k < SETS; ++k) top = fmaxf(top, ml_s[k][0]);
+  float sum = a.sink ? fast_exp2(sk - top) : 0.f;
+  y = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int k = 0; k < SETS; ++k) {
+    const float w = fast_exp2(ml_s[k][0] - top);
+    const float4 v = y_s[k][e];
+    sum = fmaf(w, ml_s[k][1], sum);
+    y.x = fmaf(w, v.x, y.x); y.y = fmaf(w, v.y, y.y); y.z = fmaf(w, v.z, y.z); y.w = fmaf(w, v.w, y.w);
   }
+  const float fac = sum != 0.f ? 1.f / sum : 0.f;
+  reinterpret_cast<uint2*>(a.out + ((size_t)cut.z + h) * D)[e] = make_uint2(pack_bf16(y.x * fac, y.y * fac), pack_bf16(y.z * fac, y.w * fac));
 }
 
 // ---------------------------------------------------------------- launchers
@@ -761,42 +805,50 @@ static int pd_sms() {
   return n > 0 ? n : 148;
 }
 
-struct PdShape { int nt, chunks, blocks, stages; size_t smem; long long part_floats; };
-static size_t pd_smem(int d, int bits, int nt, int n, int stages) {
-  const size_t stage = 2 * PD_TILE * (d * bits / 8 + 4 * (d / 64));
-  return PD_WARPS * (stages * (stage + 12)) + PD_WARPS / 2 * 8 * nt * d * 4 + (n + 1) * 4;
+struct PdShape { int nt, chunks, blocks, stages, smem; long long part_floats; };
+template <int D, int BITS, int NT> static void pd_fill(PdShape* s, int n, int nkv, int max_context, int window) {
+  typedef PdSizes<D, BITS, NT> Z;
+  s->stages = 8;
+  while (s->stages > 2 && Z::smem(s->stages, n) > 222 * 1024) --s->stages;      // of 227 KB, with what a block has besides
+  s->smem = Z::smem(s->stages, n);
+  const long long reach = window > 0 && window < max_context ? (long long)window + Z::TILE - 1 : max_context;
+  const long long tiles = (long long)n * nkv * s->chunks * ((reach + Z::TILE - 1) / Z::TILE);
+  // few tiles go to as many multiprocessors as there are: a block's warps share its instruction slots
+  s->blocks = (int)(tiles < 1 ? 1 : tiles < pd_sms() ? tiles : pd_sms());
+  s->part_floats = (long long)s->blocks * (2 + Z::WARPS) * Z::PART;
 }
+#define PD_SIZES(CALL)                                                                   \
+  do {                                                                                   \
+    if (d == 64 && bits == 4) { if (nt == 1) CALL(64, 4, 1); else CALL(64, 4, 2); }      \
+    else if (d == 64) { if (nt == 1) CALL(64, 8, 1); else CALL(64, 8, 2); }              \
+    else if (bits == 4) { if (nt == 1) CALL(128, 4, 1); else CALL(128, 4, 2); }          \
+    else { if (nt == 1) CALL(128, 8, 1); else CALL(128, 8, 2); }                         \
+  } while (0)
 static PdShape pd_shape(int n, int nh, int nkv, int d, int bits, int max_context, int window) {
   PdShape s;
-  const int group = nh / nkv;
-  s.nt = group > 8 ? 2 : 1;
-  s.chunks = (group + 8 * s.nt - 1) / (8 * s.nt);
-  const bool two = (d == 128 && s.nt == 1 && bits == 4) || (d == 64 && s.nt == 1);
-  const size_t most = two ? 111 * 1024 : 225 * 1024;      // of 228 KB, with what a block has besides
-  s.stages = 6;
-  while (s.stages > 2 && pd_smem(d, bits, s.nt, n, s.stages) > most) --s.stages;
-  s.smem = pd_smem(d, bits, s.nt, n, s.stages);
-  const long long reach = window > 0 && window < max_context ? (long long)window + PD_TILE - 1 : max_context;
-  const long long tiles = (long long)n * nkv * s.chunks * ((reach + PD_TILE - 1) / PD_TILE);
-  const long long want = (tiles + PD_WARPS - 1) / PD_WARPS, fit = (long long)pd_sms() * (two ? 2 : 1);
-  s.blocks = (int)(want < 1 ? 1 : want < fit ? want : fit);
-  s.part_floats = 2LL * s.blocks * (8 * s.nt * d + 16 * s.nt);
+  const int group = nh / nkv, nt = group > 8 ? 2 : 1;
+  s.nt = nt;
+  s.chunks = (group + 8 * nt - 1) / (8 * nt);
+#define PD_FILL(D, BITS, NT) pd_fill<D, BITS, NT>(&s, n, nkv, max_context, window)
+  PD_SIZES(PD_FILL);
   return s;
 }
 
-// Scratch of gg_packed_decode_mma, in floats (the prefix lies behind the parts).
+// Scratch of gg_packed_decode_mma, in floats (what is to be joined lies behind the parts).
 extern "C" long long gg_packed_decode_scratch(int n, int nh, int nkv, int d, int bits, int max_context, int window) {
-  return pd_shape(n, nh, nkv, d, bits, max_context, window).part_floats + n + 1;
+  const PdShape s = pd_shape(n, nh, nkv, d, bits, max_context, window);
+  return s.part_floats + 4LL * s.blocks;
 }
 
 template <int D, int BITS, int NT, bool OPT>
-static int pd_launch(const PackedDecode& a, size_t smem, cudaStream_t stream) {
-  cudaError_t e = cudaFuncSetAttribute(packed_decode_kernel<D, BITS, NT, OPT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+static int pd_launch(const PackedDecode& a, int smem, cudaStream_t stream) {
+  cudaError_t e = cudaFuncSetAttribute(packed_decode_kernel<D, BITS, NT, OPT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) return gg_fail(GG_ERR_CUDA, "packed_decode: %s", cudaGetErrorString(e));
-  gg_launch(packed_decode_kernel<D, BITS, NT, OPT>, dim3(a.blocks), dim3(PD_WARPS * 32), smem, stream, a);
+  gg_launch(packed_decode_kernel<D, BITS, NT, OPT>, dim3(a.blocks), dim3(PdSizes<D, BITS, NT>::THREADS), smem, stream, a);
   int rc = gg_check_launch("packed_decode");
   if (rc) return rc;
-  gg_launch(packed_join_kernel<D, NT>, dim3(a.n * a.nkv * a.chunks), dim3(256), 0, stream, a);
+  if (a.blocks == 1) return GG_OK;
+  gg_launch(packed_join_kernel<D, NT>, dim3(a.blocks, a.group < 8 * NT ? a.group : 8 * NT), dim3(128), 0, stream, a);
   return gg_check_launch("packed_join");
 }
 
@@ -813,7 +865,7 @@ extern "C" int gg_packed_decode_mma(const void* q, long long q_stride, const voi
              "packed_decode: q, its rows, the output and the pages must start on 16 bytes");
   if (n == 0) return GG_OK;
   const PdShape s = pd_shape(n, nh, nkv, d, bits, max_context, window);
-  GG_REQUIRE(scratch && ((size_t)scratch % 16) == 0 && scratch_floats >= s.part_floats + n + 1, "packed_decode: scratch too small");
+  GG_REQUIRE(scratch && ((size_t)scratch % 16) == 0 && scratch_floats >= s.part_floats + 4LL * s.blocks, "packed_decode: scratch too small");
   PackedDecode a = {};
   a.q = (const __nv_bfloat16*)q; a.q_stride = q_stride; a.pages = (const unsigned char*)pages; a.num_pages = num_pages;
   a.tables = tables; a.bt_stride = bt_stride; a.cu_q_lens = cu_q_lens; a.context_lens = context_lens; a.seqs = seqs; a.n = n;
@@ -821,12 +873,9 @@ extern "C" int gg_packed_decode_mma(const void* q, long long q_stride, const voi
   a.page_log2 = 31 - __builtin_clz(page_size);
   a.page_bytes = PackedRows(bits, d, page_size).page_bytes();
   a.window = window; a.scale = scale; a.softcap = softcap; a.sink = sink; a.slopes = slopes; a.temp_coef = temp_coef; a.temp_every = temp_every;
-  a.part = scratch; a.prefix = reinterpret_cast<int*>(scratch + s.part_floats); a.blocks = s.blocks; a.stages = s.stages; a.status = status;
+  a.part = scratch; a.cut = reinterpret_cast<int4*>(scratch + s.part_floats); a.blocks = s.blocks; a.stages = s.stages; a.status = status;
   const bool opt = softcap > 0.f || sink || slopes || temp_every > 0.f;
-#define PD_OPT(D, BITS, NT) return opt ? pd_launch<D, BITS, NT, true>(a, s.smem, stream) : pd_launch<D, BITS, NT, false>(a, s.smem, stream)
-#define PD_NT(D, BITS) do { if (s.nt == 1) PD_OPT(D, BITS, 1); else PD_OPT(D, BITS, 2); } while (0)
-  if (d == 64 && bits == 4) PD_NT(64, 4);
-  if (d == 64) PD_NT(64, 8);
-  if (bits == 4) PD_NT(128, 4);
-  PD_NT(128, 8);
+  const int nt = s.nt;
+#define PD_RUN(D, BITS, NT) return opt ? pd_launch<D, BITS, NT, true>(a, s.smem, stream) : pd_launch<D, BITS, NT, false>(a, s.smem, stream)
+  PD_SIZES(PD_RUN);
 }
