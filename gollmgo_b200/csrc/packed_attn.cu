@@ -29,6 +29,7 @@
 
 #define PD_MAX_TOKENS 1024         // tokens of one launch
 #define PD_STATUS 71               // reported where a copy did not arrive
+#define PD_STAGES 8                // most stages of a ring
 #define PD_LOG2E 1.4426950408889634f
 #define PD_NO_KEY (-3.0e38f)       // the running maximum before the first key: below every finite score
 
@@ -75,13 +76,7 @@ __device__ __forceinline__ void bulk_load(unsigned dst, const void* src, unsigne
   asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
                ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
 }
-__device__ __forceinline__ unsigned lds32(unsigned a) { unsigned v; asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(a)); return v; }
-__device__ __forceinline__ uint2 lds64(unsigned a) { uint2 v; asm volatile("ld.shared.v2.b32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a)); return v; }
-__device__ __forceinline__ uint4 lds128(unsigned a) {
-  uint4 v;
-  asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a));
-  return v;
-}
+template <typename T> __device__ __forceinline__ T ld(const unsigned char* p) { return *reinterpret_cast<const T*>(p); }
 __device__ __forceinline__ float power_of_two(int e) { return __uint_as_float((unsigned)(e + 127) << 23); }   // -126 <= e <= 127
 
 // Tokens of sequence b that can be in sight: a context that its block table cannot hold is cut there.
@@ -128,7 +123,16 @@ __device__ __forceinline__ void scan_tiles(const PackedDecode& a, int pairs, int
   if (threadIdx.x == 0) prefix[a.n] = base;
   __syncthreads();
 }
-__device__ __forceinline__ int range_start(int block, int blocks, int total) { return (int)((long long)total * block / blocks); }
+// `total` tiles over `blocks` blocks: the first total % blocks have one more than the others.
+struct BlockRanges {
+  int each, more;
+  __device__ __forceinline__ BlockRanges(int total, int blocks) : each((unsigned)total / (unsigned)blocks), more(total - each * blocks) {}
+  __device__ __forceinline__ int start(int block) const { return block * each + min(block, more); }
+  __device__ __forceinline__ int holder(int f) const {                // the block that has tile f
+    const int edge = more * (each + 1);
+    return f < edge ? (unsigned)f / (unsigned)(each + 1) : more + (unsigned)(f - edge) / (unsigned)each;
+  }
+};
 
 // A place in the sequence of all tiles: tile f lies in pair `pair` of token i, whose tiles are [base, base + tiles).
 template <int TILE> struct TileCursor {
@@ -136,11 +140,17 @@ template <int TILE> struct TileCursor {
   __device__ __forceinline__ void settle(const PackedDecode& a, const int* contexts) {   // tiles of token i
     tiles = (int)((unsigned)(contexts[i] + TILE - 1) / TILE - (unsigned)first_key(a, contexts[i]) / TILE);
   }
+  // from all lanes of a warp, the same f
   __device__ __forceinline__ void start(const PackedDecode& a, const int* prefix, const int* contexts, int f) {
     int lo = 0, hi = a.n - 1;                     // the last token whose tiles start at f or before and that has any
-    while (lo < hi) {
-      const int m = (lo + hi + 1) >> 1;
-      if (prefix[m] <= f) lo = m; else hi = m - 1;
+    if (hi < 32) {
+      const int lane = threadIdx.x & 31;
+      lo = 31 - __clz(__ballot_sync(0xffffffffu, lane <= hi && prefix[min(lane, hi)] <= f));
+    } else {
+      while (lo < hi) {
+        const int m = (lo + hi + 1) >> 1;
+        if (prefix[m] <= f) lo = m; else hi = m - 1;
+      }
     }
     i = lo;
     settle(a, contexts);
@@ -208,7 +218,8 @@ __global__ void __launch_bounds__(PdSizes<D, BITS, NT>::THREADS, 1) packed_decod
   if (tid == 0) a.cut[blockIdx.x] = make_int4(-1, 0, 0, 0);
   const int blocks = min(a.blocks, total);         // each has a tile at least
   if ((int)blockIdx.x >= blocks) return;
-  const int b_lo = range_start(blockIdx.x, blocks, total), b_hi = range_start(blockIdx.x + 1, blocks, total);
+  const BlockRanges ranges(total, blocks);
+  const int b_lo = ranges.start(blockIdx.x), b_hi = ranges.start(blockIdx.x + 1);
   asm volatile("fence.proxy.async;" ::: "memory");            // pages that the kernel ahead wrote, read by bulk copies
 
   // chunks: the tokens of a tile that lie in one page
@@ -220,17 +231,19 @@ __global__ void __launch_bounds__(PdSizes<D, BITS, NT>::THREADS, 1) packed_decod
   // the ones of the batch that follows are being looked up.
   int batch = w_lo, f_ask = w_lo, id = -1, id_next = -1, spot = 0, spot_next = 0;
   unsigned there = 0;
-  TileCursor<TILE> mine;
+  TileCursor<TILE> at;                             // of the first tile that was looked up last
   auto look_up = [&](int from) {
-    const int f = from + (lane >> two);
     id_next = -1;
+    if (from >= w_hi) return;
+    at.start(a, prefix, contexts, from);
+    const int f = from + (lane >> two);
     if (f >= w_hi) return;
-    TileCursor<TILE>& at = mine;
-    at.start(a, prefix, contexts, f);
-    const int ctx = contexts[at.i], b = a.seqs ? a.seqs[at.i] : at.i;
-    const int key = first_key(a, ctx) / TILE * TILE + (f - at.base) * TILE + (lane & (chunks - 1)) * chunk;
+    TileCursor<TILE> mine = at;
+    mine.advance(a, contexts, pairs, f);
+    const int ctx = contexts[mine.i], b = a.seqs ? a.seqs[mine.i] : mine.i;
+    const int key = first_key(a, ctx) / TILE * TILE + (f - mine.base) * TILE + (lane & (chunks - 1)) * chunk;
     if (key < ctx) id_next = a.tables[(size_t)b * a.bt_stride + (key >> a.page_log2)];
-    spot_next = kv_head(a, at.pair) << 8 | (key & ((1 << a.page_log2) - 1));
+    spot_next = kv_head(a, mine.pair) << 8 | (key & ((1 << a.page_log2) - 1));
   };
   auto ask = [&](int stage) {                      // start the copies of tile f_ask
     if (f_ask >= w_hi) return;
@@ -239,9 +252,9 @@ __global__ void __launch_bounds__(PdSizes<D, BITS, NT>::THREADS, 1) packed_decod
       id = id_next;
       spot = spot_next;
       there = __ballot_sync(0xffffffffu, id >= 0 && id < a.num_pages);
-      look_up(batch + (32 >> two));
     }
     const int k = f_ask - batch;
+    if (k == PD_STAGES) look_up(batch + (32 >> two));         // not before the first stages are on their way
     const unsigned mask = (there >> (k << two)) & ((1u << chunks) - 1), bar = full + 8 * stage;
     if (lane == 0) {
       here[stage] = mask;
@@ -264,11 +277,6 @@ __global__ void __launch_bounds__(PdSizes<D, BITS, NT>::THREADS, 1) packed_decod
     ++f_ask;
   };
   look_up(w_lo);
-  TileCursor<TILE> at;                             // the first pair of the range, which lane 0 has just found
-  at.i = __shfl_sync(0xffffffffu, mine.i, 0);
-  at.pair = __shfl_sync(0xffffffffu, mine.pair, 0);
-  at.base = __shfl_sync(0xffffffffu, mine.base, 0);
-  at.tiles = __shfl_sync(0xffffffffu, mine.tiles, 0);
   if (w_lo < w_hi) {
     const int b = a.seqs ? a.seqs[at.i] : at.i, row = a.cu_q_lens ? a.cu_q_lens[b] : b;
     const int kvh = kv_head(a, at.pair), head = kvh * a.group + (at.pair - kvh * a.chunks) * HEADS;
@@ -276,6 +284,7 @@ __global__ void __launch_bounds__(PdSizes<D, BITS, NT>::THREADS, 1) packed_decod
     if (lane < min(HEADS, a.nh - head) * D / 32)
       asm volatile("prefetch.global.L1 [%0];" ::"l"(a.q + (size_t)row * a.q_stride + (size_t)head * D + lane * 32));
   }
+  TileCursor<TILE> now = at;                       // the pair the warp is at
 #pragma unroll 1
   for (int s = 0; s < S; ++s) ask(s);
 
@@ -289,11 +298,11 @@ __global__ void __launch_bounds__(PdSizes<D, BITS, NT>::THREADS, 1) packed_decod
   unsigned phase = 0;
   bool broken = false;
   while (f < w_hi) {
-    at.advance(a, contexts, pairs, f);
-    const int seg = f, seg_end = min(at.base + at.tiles, w_hi);
-    const int b = a.seqs ? a.seqs[at.i] : at.i, ctx = contexts[at.i], lo = first_key(a, ctx);
+    now.advance(a, contexts, pairs, f);
+    const int seg = f, seg_end = min(now.base + now.tiles, w_hi);
+    const int b = a.seqs ? a.seqs[now.i] : now.i, ctx = contexts[now.i], lo = first_key(a, ctx);
     const int tile0 = lo / TILE * TILE;
-    const int kvh = kv_head(a, at.pair), head0 = (at.pair - kvh * a.chunks) * HEADS;
+    const int kvh = kv_head(a, now.pair), head0 = (now.pair - kvh * a.chunks) * HEADS;
     const int heads = min(HEADS, a.group - head0);
     const int row = a.cu_q_lens ? a.cu_q_lens[b] : b;
 
@@ -387,8 +396,8 @@ __global__ void __launch_bounds__(PdSizes<D, BITS, NT>::THREADS, 1) packed_decod
         if (broken) {
           if (lane == 0 && a.status) *a.status = PD_STATUS;
         } else {
-          const unsigned base = ring + stage * STAGE;
-          const int key0 = tile0 + (f - at.base) * TILE;
+          const unsigned char* base = smem + (size_t)(warp * S + stage) * STAGE;
+          const int key0 = tile0 + (f - now.base) * TILE;
           const unsigned mask = here[stage];
           const bool whole = key0 >= lo && key0 + TILE <= ctx && mask == (1u << chunks) - 1;
           // ---- scores
@@ -400,13 +409,13 @@ __global__ void __launch_bounds__(PdSizes<D, BITS, NT>::THREADS, 1) packed_decod
             unsigned kp[2][GR];
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
-              const unsigned p = base + off_kp + kb * step_p + half * 8 * GR * 4;
+              const unsigned char* p = base + off_kp + kb * step_p + half * 8 * GR * 4;
               if (GR == 2) {
-                const uint2 u = lds64(p);
+                const uint2 u = ld<uint2>(p);
                 kp[half][0] = u.x;
                 kp[half][GR - 1] = u.y;
               } else {
-                kp[half][0] = lds32(p);
+                kp[half][0] = ld<unsigned>(p);
               }
             }
 #pragma unroll
@@ -414,9 +423,9 @@ __global__ void __launch_bounds__(PdSizes<D, BITS, NT>::THREADS, 1) packed_decod
               float acc[NT][4];
 #pragma unroll
               for (int nt = 0; nt < NT; ++nt) acc[nt][0] = acc[nt][1] = acc[nt][2] = acc[nt][3] = 0.f;
-              const unsigned kc = base + off_k + kb * step_c + gr * (8 * BITS);
+              const unsigned char* kc = base + off_k + kb * step_c + gr * (8 * BITS);
               if (BITS == 4) {
-                const uint2 ua = lds64(kc), ub = lds64(kc + 8 * ROW);
+                const uint2 ua = ld<uint2>(kc), ub = ld<uint2>(kc + 8 * ROW);
 #pragma unroll
                 for (int w = 0; w < 2; ++w) {
                   const unsigned wa = w ? ua.y : ua.x, wb = w ? ub.y : ub.x, xa = wa >> 8, xb = wb >> 8;
@@ -427,7 +436,7 @@ __global__ void __launch_bounds__(PdSizes<D, BITS, NT>::THREADS, 1) packed_decod
                   }
                 }
               } else {
-                const uint4 ua = lds128(kc), ub = lds128(kc + 8 * ROW);
+                const uint4 ua = ld<uint4>(kc), ub = ld<uint4>(kc + 8 * ROW);
                 const unsigned wa[4] = {ua.x, ua.y, ua.z, ua.w}, wb[4] = {ub.x, ub.y, ub.z, ub.w};
 #pragma unroll
                 for (int w = 0; w < 4; ++w)
@@ -467,13 +476,13 @@ __global__ void __launch_bounds__(PdSizes<D, BITS, NT>::THREADS, 1) packed_decod
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
               unsigned u[GR];
-              const unsigned p = base + off_vp + kb * step_p + half * 8 * GR * 4;
+              const unsigned char* p = base + off_vp + kb * step_p + half * 8 * GR * 4;
               if (GR == 2) {
-                const uint2 w = lds64(p);
+                const uint2 w = ld<uint2>(p);
                 u[0] = w.x;
                 u[GR - 1] = w.y;
               } else {
-                u[0] = lds32(p);
+                u[0] = ld<unsigned>(p);
               }
 #pragma unroll
               for (int gr = 0; gr < GR; ++gr) {
@@ -581,9 +590,9 @@ __global__ void __launch_bounds__(PdSizes<D, BITS, NT>::THREADS, 1) packed_decod
                 pb[nt][0] = transpose8(half_pair(s[kb][nt][0] * w0, s[kb][nt][1] * w0));
                 pb[nt][1] = transpose8(half_pair(s[kb][nt][2] * w1, s[kb][nt][3] * w1));
               }
-              const unsigned vc = base + off_v + kb * step_c + gr * (8 * BITS);
+              const unsigned char* vc = base + off_v + kb * step_c + gr * (8 * BITS);
               if (BITS == 4) {
-                const unsigned w0 = lds32(vc), w1 = lds32(vc + 4 * ROW), w2 = lds32(vc + 8 * ROW), w3 = lds32(vc + 12 * ROW);
+                const unsigned w0 = ld<unsigned>(vc), w1 = ld<unsigned>(vc + 4 * ROW), w2 = ld<unsigned>(vc + 8 * ROW), w3 = ld<unsigned>(vc + 12 * ROW);
 #pragma unroll
                 for (int v = 0; v < 2; ++v) {
                   unsigned x = __byte_perm(w0, w1, v ? 0x7632 : 0x5410), y = __byte_perm(w2, w3, v ? 0x7632 : 0x5410);
@@ -597,7 +606,7 @@ __global__ void __launch_bounds__(PdSizes<D, BITS, NT>::THREADS, 1) packed_decod
                   }
                 }
               } else {
-                const uint2 w0 = lds64(vc), w1 = lds64(vc + 4 * ROW), w2 = lds64(vc + 8 * ROW), w3 = lds64(vc + 12 * ROW);
+                const uint2 w0 = ld<uint2>(vc), w1 = ld<uint2>(vc + 4 * ROW), w2 = ld<uint2>(vc + 8 * ROW), w3 = ld<uint2>(vc + 12 * ROW);
 #pragma unroll
                 for (int v = 0; v < 4; ++v) {
                   const unsigned sel = v & 1 ? 0x7632 : 0x5410;
@@ -627,13 +636,13 @@ __global__ void __launch_bounds__(PdSizes<D, BITS, NT>::THREADS, 1) packed_decod
 #pragma unroll
           for (int gr = 0; gr < GR; ++gr) r[gr][nt][j] += __shfl_xor_sync(0xffffffffu, r[gr][nt][j], m);
         }
-    const bool complete = seg == at.base && seg_end == at.base + at.tiles;
+    const bool complete = seg == now.base && seg_end == now.base + now.tiles;
     // the last part of the range goes where the ring was (all its copies have arrived and been read), the first to the scratch
     const bool last = seg_end == w_hi;
     float* part = last ? reinterpret_cast<float*>(smem + (size_t)warp * S * STAGE) : parts + warp * Z::PART;
     if (!complete && lane == 0) {
-      part_base[2 * warp + last] = at.base;
-      part_pair[2 * warp + last] = make_int4(at.tiles, heads, row * a.nh + kvh * a.group + head0, 0);
+      part_base[2 * warp + last] = now.base;
+      part_pair[2 * warp + last] = make_int4(now.tiles, heads, row * a.nh + kvh * a.group + head0, 0);
     }
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
@@ -686,37 +695,45 @@ __global__ void __launch_bounds__(PdSizes<D, BITS, NT>::THREADS, 1) packed_decod
   const unsigned same = __match_any_sync(0xffffffffu, lane_base);           // the parts of the same pair
   unsigned leaders = __ballot_sync(0xffffffffu, lane_base >= 0 && (same & ((1u << lane) - 1)) == 0);
   if (!leaders) return;
-  for (int e = tid; e < 2 * WARPS * HEADS; e += Z::THREADS) {               // (all threads, or whole warps of them)
-    const int i = e / HEADS, h = e % HEADS;
-    const unsigned members = __shfl_sync(0xffffffffu, same, i);
-    if (part_base[i] < 0) continue;
-    float M = PD_NO_KEY, L = 0.f;
-    for (unsigned m = members; m; m &= m - 1) M = fmaxf(M, part_top[__ffs(m) - 1][h]);
-    float w = fast_exp2(part_top[i][h] - M);
-    const int4 pair = part_pair[i];
-    const bool lead = i == __ffs(members) - 1, whole = part_base[i] >= b_lo && part_base[i] + pair.x <= b_hi;
-    if (lead || whole)
-      for (unsigned m = members; m; m &= m - 1) L += part_sum[__ffs(m) - 1][h] * fast_exp2(part_top[__ffs(m) - 1][h] - M);
-    if (whole) {                                   // the weight in the result
+  // lane i of the warps takes part i; a pair's parts lie between its first one and the next pair's
+  const int from = max(0, 31 - __clz(leaders & ((2u << lane) - 1)));
+  const unsigned beyond = lane == 31 ? 0u : leaders >> (lane + 1);
+  const int to = beyond ? lane + __ffs(beyond) - 1 : 31;
+  for (int h = warp; h < HEADS; h += WARPS) {
+    const bool real = lane_base >= 0;
+    float top = real ? part_top[lane][h] : PD_NO_KEY;
+    const float mine = top;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const float v = __shfl_up_sync(0xffffffffu, top, o);
+      if (lane - o >= from) top = fmaxf(top, v);
+    }
+    const float M = __shfl_sync(0xffffffffu, top, to);
+    float w = real ? fast_exp2(mine - M) : 0.f, L = real ? part_sum[lane][h] * w : 0.f;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const float v = __shfl_up_sync(0xffffffffu, L, o);
+      if (lane - o >= from) L += v;
+    }
+    L = __shfl_sync(0xffffffffu, L, to);
+    if (!real) continue;
+    const int4 pair = part_pair[lane];
+    if (lane_base >= b_lo && lane_base + pair.x <= b_hi) {        // the weight in the result
       if (OPT && a.sink && h < pair.y) {
-        const float sk = a.sink[pair.z % a.nh + h] * PD_LOG2E, top = fmaxf(M, sk), u = fast_exp2(M - top);
+        const float sk = a.sink[pair.z % a.nh + h] * PD_LOG2E, all = fmaxf(M, sk), u = fast_exp2(M - all);
         w *= u;
-        L = L * u + fast_exp2(sk - top);
+        L = L * u + fast_exp2(sk - all);
       }
       w = L != 0.f ? w / L : 0.f;
-    } else if (lead) {
-      float* to = a.part + (size_t)(2 * blockIdx.x + (part_base[i] < b_lo ? 0 : 1)) * Z::PART;
-      to[HEADS * D + 2 * h] = M;
-      to[HEADS * D + 2 * h + 1] = L;
+    } else if (lane == from) {
+      float* out = a.part + (size_t)(2 * blockIdx.x + (lane_base < b_lo ? 0 : 1)) * Z::PART;
+      out[HEADS * D + 2 * h] = M;
+      out[HEADS * D + 2 * h + 1] = L;
       // a pair that began in an earlier block and ends here is joined from there to here
-      if (h == 0 && part_base[i] < b_lo && part_base[i] + pair.x <= b_hi) {
-        int c = (int)(((long long)part_base[i] * blocks) / total);        // the block that holds its first tile
-        while (range_start(c + 1, blocks, total) <= part_base[i]) ++c;
-        while (range_start(c, blocks, total) > part_base[i]) --c;
-        a.cut[blockIdx.x] = make_int4(c, pair.y, pair.z, 0);
-      }
+      if (h == 0 && lane_base < b_lo && lane_base + pair.x <= b_hi)
+        a.cut[blockIdx.x] = make_int4(ranges.holder(lane_base), pair.y, pair.z, 0);
     }
-    part_weight[i][h] = w;
+    part_weight[lane][h] = w;
   }
   __syncthreads();
   // four values a thread: pairs side by side, PART / 4 threads each
@@ -727,14 +744,20 @@ __global__ void __launch_bounds__(PdSizes<D, BITS, NT>::THREADS, 1) packed_decod
     unsigned rest = leaders;
     for (int i = 0; i < run; ++i) rest &= rest - 1;
     const int k = __ffs(rest) - 1;
-    unsigned members = __shfl_sync(0xffffffffu, same, k);
+    const unsigned members = __shfl_sync(0xffffffffu, same, k);
     const int4 pair = part_pair[k];
     float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+    const int end = 32 - __clz(members);
 #pragma unroll 4
-    for (; members; members &= members - 1) {
-      const int i = __ffs(members) - 1;
-      const float* p = i & 1 ? reinterpret_cast<const float*>(smem + (size_t)(i >> 1) * S * STAGE) : parts + (i >> 1) * Z::PART;
-      const float4 v = *reinterpret_cast<const float4*>(p + x);
+    for (int i = k | 1; i < end; i += 2) {         // last parts, in shared memory
+      const bool in = (members >> i) & 1;
+      const float4 v = in ? *reinterpret_cast<const float4*>(smem + (size_t)(i >> 1) * S * STAGE + x * 4) : make_float4(0.f, 0.f, 0.f, 0.f);
+      const float w = in ? part_weight[i][h] : 0.f;
+      y.x = fmaf(w, v.x, y.x); y.y = fmaf(w, v.y, y.y); y.z = fmaf(w, v.z, y.z); y.w = fmaf(w, v.w, y.w);
+    }
+    for (unsigned m = members & 0x55555555u; m; m &= m - 1) {               // first parts (a pair has one in the block, or two)
+      const int i = __ffs(m) - 1;
+      const float4 v = *reinterpret_cast<const float4*>(parts + (i >> 1) * Z::PART + x);
       const float w = part_weight[i][h];
       y.x = fmaf(w, v.x, y.x); y.y = fmaf(w, v.y, y.y); y.z = fmaf(w, v.z, y.z); y.w = fmaf(w, v.w, y.w);
     }
@@ -808,7 +831,7 @@ static int pd_sms() {
 struct PdShape { int nt, chunks, blocks, stages, smem; long long part_floats; };
 template <int D, int BITS, int NT> static void pd_fill(PdShape* s, int n, int nkv, int max_context, int window) {
   typedef PdSizes<D, BITS, NT> Z;
-  s->stages = 8;
+  s->stages = PD_STAGES;
   while (s->stages > 2 && Z::smem(s->stages, n) > 222 * 1024) --s->stages;      // of 227 KB, with what a block has besides
   s->smem = Z::smem(s->stages, n);
   const long long reach = window > 0 && window < max_context ? (long long)window + Z::TILE - 1 : max_context;
