@@ -39,15 +39,16 @@ class PackedKV:
     # ------------------------------------------------------------------ store and read back
     def write(self, qkv: torch.Tensor, positions: Optional[torch.Tensor], slots: Optional[torch.Tensor], num_heads: int,
               inv_freq: Optional[torch.Tensor] = None, interleaved: bool = False, magnitude: float = 1.0,
-              q_out: Optional[torch.Tensor] = None) -> torch.Tensor:
+              q_out: Optional[torch.Tensor] = None, early: bool = False) -> torch.Tensor:
         """Rows of qkv [T, (num_heads + 2 kv heads) * head size]: q and k are rotated by ``positions`` (``inv_freq`` float64
         [width / 2]; None: they are not), k and v quantised into their pages at ``slots`` (page * page_size + place; below
         0: not stored; none twice; None: nothing is stored).  Returns the rotated q [T, num_heads, head size], in ``q_out``
-        where given (which may be the q columns of qkv)."""
+        where given (which may be the q columns of qkv).  ``early``: positions, slots and inv_freq are not the output of the kernel
+        ahead on the stream, and may be read while it runs."""
         if q_out is None:
             q_out = torch.empty(qkv.shape[0], num_heads, self.head_dim, dtype=qkv.dtype, device=qkv.device)
         ops.packed_write(qkv, positions, slots, inv_freq, magnitude, self.pages, q_out, num_heads, self.kv_heads, self.head_dim,
-                         self.page_size, self.bits, interleaved)
+                         self.page_size, self.bits, interleaved, early)
         return q_out
 
     def read(self, tables: torch.Tensor, lens: torch.Tensor, first_page: torch.Tensor, num_pages: int, dtype=torch.bfloat16,

@@ -1560,11 +1560,12 @@ def _ints(what: str, n: int, *tensors):
 
 def packed_write(qkv: torch.Tensor, positions: Optional[torch.Tensor], slots: Optional[torch.Tensor], inv_freq: Optional[torch.Tensor],
                  magnitude: float, pages: torch.Tensor, q_out: Optional[torch.Tensor], nh: int, nkv: int, d: int, page_size: int,
-                 bits: int, interleaved: bool = False) -> None:
+                 bits: int, interleaved: bool = False, early: bool = False) -> None:
     """Rotate the q heads of qkv [T, (nh + 2 nkv) d] into ``q_out`` [T, nh d] (None: they are left alone; it may be the
     columns of qkv itself), rotate the k heads, and quantise k and v into ``pages`` at slots[t] = page * page_size + place.
     A slot below 0 or outside the pool is not written; no slot may be given twice.  ``inv_freq`` None: no rotation.
-    ``positions``, ``slots`` and ``inv_freq`` are read before the kernel ahead of this one has finished."""
+    ``early``: ``positions``, ``slots`` and ``inv_freq`` may be read before the kernel ahead of this one has finished (they are
+    not its output)."""
     T = qkv.shape[0]
     _here(qkv, positions, slots, inv_freq, pages, q_out)
     stride = _rows_of(qkv, (nh + 2 * nkv) * d, "packed_write: qkv")
@@ -1581,7 +1582,7 @@ def packed_write(qkv: torch.Tensor, positions: Optional[torch.Tensor], slots: Op
         rot = 2 * inv_freq.numel()
     _check(lib().gg_packed_write(_p(qkv), ctypes.c_longlong(stride), dtype_code(qkv.dtype), _p(positions), _p(slots), _p(inv_freq),
                                  ctypes.c_float(magnitude), _p(pages), pages.shape[0], _p(q_out), ctypes.c_longlong(q_stride), T, nh, nkv,
-                                 d, rot, page_size, bits, int(interleaved), _stream()))
+                                 d, rot, page_size, bits, int(interleaved), int(early), _stream()))
 
 
 def packed_read(pages: torch.Tensor, tables: torch.Tensor, lens: torch.Tensor, first_page: torch.Tensor, k_out: torch.Tensor,

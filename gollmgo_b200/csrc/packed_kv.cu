@@ -69,11 +69,12 @@ template <typename TA>
 __global__ void __launch_bounds__(PACK_WARPS * 32)
 packed_write_kernel(const TA* __restrict__ qkv, long long row_stride, const int* __restrict__ positions, const int* __restrict__ slots,
                     const double* __restrict__ inv_freq, float mag, unsigned char* __restrict__ pages, int num_pages, TA* __restrict__ q_out,
-                    long long q_stride, int nh, int nkv, int d, int rot, int page_size, int bits, int interleaved) {
+                    long long q_stride, int nh, int nkv, int d, int rot, int page_size, int bits, int interleaved, int early) {
   typedef typename PackMath<TA>::T TC;
   extern __shared__ double smem_d[];
   TC* cs = reinterpret_cast<TC*>(smem_d);             // cos[rot / 2], sin[rot / 2], then a row of each warp
   pdl_trigger();
+  if (!early) pdl_wait();
   const int t = blockIdx.x, half = rot >> 1, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   TC* row = cs + 2 * half + warp * d;
   if (half > 0) {
@@ -82,7 +83,7 @@ packed_write_kernel(const TA* __restrict__ qkv, long long row_stride, const int*
   }
   const int slot = slots ? slots[t] : -1;
   __syncthreads();
-  pdl_wait();
+  if (early) pdl_wait();
   const int h = blockIdx.y * PACK_WARPS + warp;
   if (h >= nh + 2 * nkv) return;
   if (h < nh ? q_out == nullptr : (slot < 0 || slot / page_size >= num_pages)) return;
@@ -127,6 +128,149 @@ packed_write_kernel(const TA* __restrict__ qkv, long long row_stride, const int*
       else *reinterpret_cast<unsigned short*>(block + r.codes(which, place) + c) = (unsigned short)(qa | (qb << 8));
     }
     if (lane == 0) *reinterpret_cast<unsigned*>(block + r.pairs(which, place) + g * 4) = coder.pair;
+  }
+}
+
+// The codes of eight values, 4 or 8 bits each, as one or two words.  A quotient by the reciprocal is off by less than 2^-21
+// of the largest code; where one lies that near to a border (half between two codes: with bfloat16 values and scales many lie
+// on it) the remainder decides, which one multiply-add gives to the last bit.  Halves keep a wide group's differences finite,
+// and a group of tiny values is brought up by 2^64 so that its scale has a reciprocal.
+template <int BITS>
+__device__ __forceinline__ uint2 codes8(const PackCoder& k, const float* x) {
+  constexpr float MOST = (1 << BITS) - 1, NEAR = 0.5f - MOST * 0x1p-21f;
+  constexpr float MAGIC = 12582912.f;                  // 1.5 * 2^23: added, the whole number stands in the low bits
+  const float up = k.half_scale < 0x1p-60f ? 0x1p64f : 1.f, scale = k.half_scale * up, offset = k.half_offset * up, half = 0.5f * up;
+  const float inv = scale > 0.f ? 1.f / scale : 0.f;
+  unsigned q[8];
+  float far = 0.f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float t = fmaf(half, x[i], -offset) * inv, m = t + MAGIC;
+    far = fmaxf(far, fabsf(t - (m - MAGIC)));
+    q[i] = __float_as_uint(m);
+  }
+  if (far >= NEAR) {
+    const float border = 0.5f * scale;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float c = __uint_as_float(q[i]) - MAGIC, rest = fmaf(-c, scale, fmaf(half, x[i], -offset));
+      const bool odd = q[i] & 1u;
+      q[i] += (rest > border || (rest == border && odd)) ? 1u : (rest < -border || (rest == -border && odd)) ? ~0u : 0u;
+    }
+  }
+  unsigned w[2] = {0u, 0u};
+#pragma unroll
+  for (int i = 0; i < 8; ++i) w[i * BITS / 32] |= (q[i] & ((1u << BITS) - 1)) << (i * BITS & 31);
+  return k.pair == 0x7fff7fffu ? make_uint2(0u, 0u) : make_uint2(w[0], w[1]);
+}
+
+// The common case: bfloat16, heads of 64 or 128, half-split pairs over the whole head or no rotation, rows in 16-byte steps.
+// Blocks of y = 0 take the k and v heads of TOK tokens, blocks of y = 1 their q heads (a tenth of the work a row: apart, so that
+// all warps of a block are busy as long).  A thread takes channels p .. p + 7 and D / 2 + p .. of one head (two 16-byte loads,
+// those of its next row under way while it works), so that a head's extremes are found by 4 or 8 neighbouring lanes.
+#define WRITE_THREADS 256
+template <int D, int BITS, int TOK>
+__global__ void __launch_bounds__(WRITE_THREADS)
+packed_write_vec_kernel(const __nv_bfloat16* __restrict__ qkv, long long row_stride, const int* __restrict__ positions,
+                        const int* __restrict__ slots, const double* __restrict__ inv_freq, float mag, unsigned char* __restrict__ pages,
+                        int num_pages, __nv_bfloat16* __restrict__ q_out, long long q_stride, int T, int nh, int nkv, int page_log2, int early) {
+  constexpr int HALF = D / 2, LANES = D / 16;         // lanes of a head
+  __shared__ float cs[TOK][2][HALF];
+  pdl_trigger();
+  if (!early) pdl_wait();
+  const int t0 = blockIdx.x * TOK, tokens = min(TOK, T - t0);
+  const bool queries = blockIdx.y == 1;
+  const int first = queries ? 0 : nh, per = (queries ? nh : 2 * nkv) * LANES;
+  if (inv_freq) {
+    for (int e = threadIdx.x; e < tokens * HALF; e += WRITE_THREADS) {
+      const int p = e % HALF, i = e / HALF;
+      turn_of((double)positions[t0 + i], inv_freq[p], mag, &cs[i][0][p], &cs[i][1][p]);
+    }
+  }
+  if (early) pdl_wait();
+  const int P = 1 << page_log2;
+  const PackedRows r(BITS, D, P);
+  int w = threadIdx.x, i = 0;                         // item w of token i
+  auto settle = [&]() { while (w >= per) { w -= per; ++i; } };
+  auto row_at = [&]() { return qkv + (size_t)(t0 + i) * row_stride + (size_t)(first + w / LANES) * D + (w % LANES) * 8; };
+  uint4 lo, hi;
+  settle();
+  if (i < tokens) {
+    lo = *reinterpret_cast<const uint4*>(row_at());
+    hi = *reinterpret_cast<const uint4*>(row_at() + HALF);
+  }
+  __syncthreads();                                    // the angles are there
+  // (every lane of a head is in the same round: LANES divides the items of a token and 32)
+  while (i < tokens) {
+    const int h = first + w / LANES, p = (w % LANES) * 8, n = i;
+    const unsigned wl[4] = {lo.x, lo.y, lo.z, lo.w}, wh[4] = {hi.x, hi.y, hi.z, hi.w};
+    w += WRITE_THREADS;
+    settle();
+    if (i < tokens) {
+      lo = *reinterpret_cast<const uint4*>(row_at());
+      hi = *reinterpret_cast<const uint4*>(row_at() + HALF);
+    }
+    float a[8], c[8];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      a[2 * j] = __uint_as_float(wl[j] << 16);
+      a[2 * j + 1] = __uint_as_float(wl[j] & 0xffff0000u);
+      c[2 * j] = __uint_as_float(wh[j] << 16);
+      c[2 * j + 1] = __uint_as_float(wh[j] & 0xffff0000u);
+    }
+    if (inv_freq && h < nh + nkv) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float u = a[j], v = c[j], co = cs[n][0][p + j], si = cs[n][1][p + j];
+        a[j] = u * co - v * si;
+        c[j] = u * si + v * co;
+      }
+    }
+    if (queries) {
+      __nv_bfloat16* o = q_out + (size_t)(t0 + n) * q_stride + (size_t)h * D + p;
+      *reinterpret_cast<uint4*>(o) = make_uint4(pack_bf16(a[0], a[1]), pack_bf16(a[2], a[3]), pack_bf16(a[4], a[5]), pack_bf16(a[6], a[7]));
+      *reinterpret_cast<uint4*>(o + HALF) = make_uint4(pack_bf16(c[0], c[1]), pack_bf16(c[2], c[3]), pack_bf16(c[4], c[5]), pack_bf16(c[6], c[7]));
+      continue;
+    }
+    const int slot = slots ? slots[t0 + n] : -1;
+    if (slot < 0 || (slot >> page_log2) >= num_pages) continue;
+    // extremes of either half's group (heads of 64: one group); a NaN shows in the sum of x * 0, an infinity as an extreme
+    float mn[2] = {a[0], c[0]}, mx[2] = {a[0], c[0]}, nan[2] = {0.f, 0.f};
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      mn[0] = fminf(mn[0], a[j]); mx[0] = fmaxf(mx[0], a[j]); nan[0] = fmaf(a[j], 0.f, nan[0]);
+      mn[1] = fminf(mn[1], c[j]); mx[1] = fmaxf(mx[1], c[j]); nan[1] = fmaf(c[j], 0.f, nan[1]);
+    }
+    if (D == 64) { mn[0] = fminf(mn[0], mn[1]); mx[0] = fmaxf(mx[0], mx[1]); nan[0] += nan[1]; }
+    const unsigned mates = ((1u << LANES) - 1) << ((threadIdx.x & 31) & ~(LANES - 1));
+    PackCoder k[2];
+#pragma unroll
+    for (int g = 0; g < D / 64; ++g) {
+#pragma unroll
+      for (int o = 1; o < LANES; o <<= 1) {
+        mn[g] = fminf(mn[g], __shfl_xor_sync(mates, mn[g], o));
+        mx[g] = fmaxf(mx[g], __shfl_xor_sync(mates, mx[g], o));
+      }
+      const bool bad = __any_sync(mates, nan[g] != 0.f) || !(mx[g] - mx[g] == 0.f) || !(mn[g] - mn[g] == 0.f);
+      k[g].set(mn[g], mx[g], bad, BITS);
+    }
+    if (D == 64) k[1] = k[0];
+    const int which = h >= nh + nkv, kvh = h - nh - which * nkv, place = slot & (P - 1);
+    unsigned char* block = pages + ((size_t)(slot >> page_log2) * nkv + kvh) * r.page_bytes();
+    unsigned char* o = block + r.codes(which, place) + p * BITS / 8;
+    const uint2 c0 = codes8<BITS>(k[0], a), c1 = codes8<BITS>(k[1], c);
+    if (BITS == 4) {
+      *reinterpret_cast<unsigned*>(o) = c0.x;
+      *reinterpret_cast<unsigned*>(o + HALF * BITS / 8) = c1.x;
+    } else {
+      *reinterpret_cast<uint2*>(o) = c0;
+      *reinterpret_cast<uint2*>(o + HALF * BITS / 8) = c1;
+    }
+    if (p == 0) {
+      unsigned* q = reinterpret_cast<unsigned*>(block + r.pairs(which, place));
+      if (D == 128) *reinterpret_cast<uint2*>(q) = make_uint2(k[0].pair, k[1].pair);
+      else *q = k[0].pair;
+    }
   }
 }
 
@@ -205,6 +349,7 @@ packed_read_kernel(const unsigned char* __restrict__ pages, int num_pages, const
 // of query rows, those that attend to most keys first (up to UNFOLD_SORTED tiles; more stay in the order of the sequences).
 // Pages behind the window of a portion's first token are left out (-1 in the table).
 #define UNFOLD_SORTED 1024
+#define UNFOLD_SEQS 1024          // most sequences of a step
 struct UnfoldTiles { int height, count; int *seq, *q0; };
 struct UnfoldArgs {
   const unsigned char* pages;
@@ -223,6 +368,68 @@ __device__ __forceinline__ int unfold_skip(const UnfoldArgs& a, int ctx, int q_l
   return a.window > 0 ? max(0, ctx - q_len - a.window + 1) / a.page_size : 0;
 }
 
+// By one block.  first[b] = tiles before sequence b; a tile finds its sequence by search and its place by counting the tiles
+// that attend to more keys.
+__device__ __noinline__ void list_tiles(const UnfoldArgs& a) {
+  __shared__ int keys_s[UNFOLD_SORTED], first_s[UNFOLD_SEQS + 1], ctx_s[UNFOLD_SEQS], len_s[UNFOLD_SEQS];
+  for (int b = threadIdx.x; b < a.B; b += blockDim.x) {
+    int n;
+    ctx_s[b] = unfold_keys(a, b, &n);
+    len_s[b] = n;
+  }
+  for (int l = 0; l < 2; ++l) {
+    const UnfoldTiles t = a.tiles[l];
+    if (!t.height) continue;
+    __syncthreads();
+    if (threadIdx.x < 32) {                            // tiles before each sequence: a warp's scan, 32 at a time
+      int base = 0;
+      for (int b0 = 0; b0 < a.B; b0 += 32) {
+        const int b = b0 + threadIdx.x, n = b < a.B ? (len_s[b] + t.height - 1) / t.height : 0;
+        int v = n;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const int u = __shfl_up_sync(0xffffffffu, v, o);
+          if ((int)threadIdx.x >= o) v += u;
+        }
+        if (b < a.B) first_s[b] = base + v - n;
+        base += __shfl_sync(0xffffffffu, v, 31);
+      }
+      if (threadIdx.x == 0) first_s[a.B] = base;
+    }
+    __syncthreads();
+    const int made = first_s[a.B];
+    auto tile = [&](int i, int* seq, int* q0) {        // (a count beyond what the portions make repeats the first tile)
+      if (i >= made) i = 0;
+      int lo = 0, hi = a.B - 1;                        // the last sequence whose tiles start at i or before
+      while (lo < hi) {
+        const int m = (lo + hi + 1) >> 1;
+        if (first_s[m] <= i) lo = m; else hi = m - 1;
+      }
+      *seq = lo;
+      *q0 = (i - first_s[lo]) * t.height;
+      return ctx_s[lo] - len_s[lo] + min(len_s[lo], *q0 + t.height);
+    };
+    const bool sorted = t.count <= UNFOLD_SORTED;
+    int seq, q0;
+    for (int i = threadIdx.x; i < t.count; i += blockDim.x) {
+      const int keys = tile(i, &seq, &q0);
+      if (sorted) keys_s[i] = keys;
+      else { t.seq[i] = seq; t.q0[i] = q0; }
+    }
+    if (!sorted) continue;
+    __syncthreads();
+    for (int i = threadIdx.x; i < t.count; i += blockDim.x) {
+      const int mine = keys_s[i];
+      int rank = 0;
+#pragma unroll 8
+      for (int k = 0; k < t.count; ++k) rank += keys_s[k] > mine || (keys_s[k] == mine && k < i);
+      tile(i, &seq, &q0);
+      t.seq[rank] = seq;
+      t.q0[rank] = q0;
+    }
+  }
+}
+
 template <typename TO, int BITS>
 __global__ void __launch_bounds__(256) packed_unfold_kernel(UnfoldArgs a, TO* __restrict__ k_out, TO* __restrict__ v_out) {
   __shared__ int red[8];
@@ -232,6 +439,7 @@ __global__ void __launch_bounds__(256) packed_unfold_kernel(UnfoldArgs a, TO* __
   int q_len;
   const int ctx = unfold_keys(a, b, &q_len);
   const int skip = unfold_skip(a, ctx, q_len), P = a.page_size;
+  if (j == 0 && b == 0 && blockIdx.z == 0) list_tiles(a);
   // pages of the sequences before this one
   int before = 0;
   for (int i = threadIdx.x; i < b; i += blockDim.x) {
@@ -255,43 +463,6 @@ __global__ void __launch_bounds__(256) packed_unfold_kernel(UnfoldArgs a, TO* __
       unpack_page<TO, BITS>(a.pages, a.tables[(size_t)b * a.bt_stride + j], a.num_pages, ctx - j * P, k_out + at, v_out + at, a.nkv, a.d, P);
     }
   }
-  if (j != gridDim.x - 1 || b != 0 || blockIdx.z != 0) return;
-  // ---- one block lists the tiles: each thread takes sequences, then tiles
-  __shared__ int seq_s[UNFOLD_SORTED], q0_s[UNFOLD_SORTED], keys_s[UNFOLD_SORTED];
-  for (int l = 0; l < 2; ++l) {
-    const UnfoldTiles t = a.tiles[l];
-    if (!t.height) continue;
-    __syncthreads();
-    const bool sorted = t.count <= UNFOLD_SORTED;
-    for (int i = threadIdx.x; i < t.count; i += blockDim.x) {   // (a count beyond what the portions make repeats a tile)
-      if (sorted) { seq_s[i] = -1; keys_s[i] = -1; }
-      else { t.seq[i] = 0; t.q0[i] = 0; }
-    }
-    __syncthreads();
-    for (int s = threadIdx.x; s < a.B; s += blockDim.x) {
-      int n, at = 0;
-      for (int i = 0; i < s; ++i) {
-        const int m = a.cu_q_lens[i + 1] - a.cu_q_lens[i];
-        at += m >= a.least ? (m + t.height - 1) / t.height : 0;
-      }
-      const int c = unfold_keys(a, s, &n);
-      for (int r = 0; r < n; r += t.height, ++at) {
-        if (at >= t.count) break;
-        if (sorted) { seq_s[at] = s; q0_s[at] = r; keys_s[at] = c - n + min(n, r + t.height); }
-        else { t.seq[at] = s; t.q0[at] = r; }
-      }
-    }
-    if (!sorted) continue;
-    __syncthreads();
-    for (int i = threadIdx.x; i < t.count; i += blockDim.x) {
-      int rank = 0;
-      const int mine = keys_s[i];
-      for (int k = 0; k < t.count; ++k) rank += keys_s[k] > mine || (keys_s[k] == mine && k < i);
-      const int k = seq_s[i] < 0 ? 0 : i;
-      t.seq[rank] = max(seq_s[k], 0);
-      t.q0[rank] = seq_s[k] < 0 ? 0 : q0_s[k];
-    }
-  }
 }
 
 static int check_packed(const char* who, const void* pages, int num_pages, int nkv, int d, int page_size, int bits) {
@@ -302,26 +473,37 @@ static int check_packed(const char* who, const void* pages, int num_pages, int n
   return GG_OK;
 }
 
-// positions, slots and inv_freq are read before the kernel ahead has finished
+// early: positions, slots and inv_freq are read before the kernel ahead has finished
 extern "C" int gg_packed_write(const void* qkv, long long row_stride, int act_dtype, const int* positions, const int* slots,
                                const double* inv_freq, float mag, void* pages, int num_pages, void* q_out, long long q_stride, int T,
-                               int nh, int nkv, int d, int rot, int page_size, int bits, int interleaved, cudaStream_t stream) {
+                               int nh, int nkv, int d, int rot, int page_size, int bits, int interleaved, int early, cudaStream_t stream) {
   int rc = check_packed("packed_write", pages, num_pages, nkv, d, page_size, bits);
   if (rc) return rc;
   GG_REQUIRE(T >= 0 && nh >= 0, "packed_write: bad sizes T=%d nh=%d", T, nh);
   GG_REQUIRE(rot >= 0 && rot <= d && rot % 2 == 0, "packed_write: rotary width %d must be even and <= head size %d", rot, d);
   GG_REQUIRE(rot == 0 || (inv_freq && positions), "packed_write: a rotation without frequencies or positions");
   if (T == 0) return GG_OK;
+  if (act_dtype == GG_BF16 && (d == 64 || d == 128) && (rot == 0 || (rot == d && !interleaved)) && ((size_t)qkv % 16) == 0 &&
+      row_stride % 8 == 0 && ((size_t)q_out % 16) == 0 && q_stride % 8 == 0) {
+#define WRITE_VEC_T(D, BITS, TOK) gg_launch(packed_write_vec_kernel<D, BITS, TOK>, dim3((T + TOK - 1) / TOK, q_out ? 2 : 1), dim3(WRITE_THREADS), 0, \
+                                            stream, (const __nv_bfloat16*)qkv, row_stride, positions, slots, rot ? inv_freq : nullptr, mag, \
+                                            (unsigned char*)pages, num_pages, (__nv_bfloat16*)q_out, q_stride, T, nh, nkv, \
+                                            31 - __builtin_clz(page_size), early)
+#define WRITE_VEC(D, BITS) do { if (T >= 1024) WRITE_VEC_T(D, BITS, 4); else WRITE_VEC_T(D, BITS, 1); } while (0)
+    if (d == 64) { if (bits == 4) WRITE_VEC(64, 4); else WRITE_VEC(64, 8); }
+    else { if (bits == 4) WRITE_VEC(128, 4); else WRITE_VEC(128, 8); }
+    return gg_check_launch("packed_write");
+  }
   const dim3 grid(T, (nh + 2 * nkv + PACK_WARPS - 1) / PACK_WARPS), block(PACK_WARPS * 32);
   GG_REQUIRE(grid.y <= 65535, "packed_write: too many heads");
   const int esize = act_dtype == GG_F32 ? 8 : 4;
   const size_t smem = (size_t)(rot + PACK_WARPS * d) * esize;
   if (act_dtype == GG_F32)
     gg_launch(packed_write_kernel<float>, grid, block, smem, stream, (const float*)qkv, row_stride, positions, slots, inv_freq, mag,
-              (unsigned char*)pages, num_pages, (float*)q_out, q_stride, nh, nkv, d, rot, page_size, bits, interleaved);
+              (unsigned char*)pages, num_pages, (float*)q_out, q_stride, nh, nkv, d, rot, page_size, bits, interleaved, early);
   else if (act_dtype == GG_BF16)
     gg_launch(packed_write_kernel<__nv_bfloat16>, grid, block, smem, stream, (const __nv_bfloat16*)qkv, row_stride, positions, slots,
-              inv_freq, mag, (unsigned char*)pages, num_pages, (__nv_bfloat16*)q_out, q_stride, nh, nkv, d, rot, page_size, bits, interleaved);
+              inv_freq, mag, (unsigned char*)pages, num_pages, (__nv_bfloat16*)q_out, q_stride, nh, nkv, d, rot, page_size, bits, interleaved, early);
   else
     return gg_fail(GG_ERR_INVALID, "packed_write: unknown dtype %d", act_dtype);
   return gg_check_launch("packed_write");
@@ -357,7 +539,7 @@ extern "C" int gg_packed_unfold(const void* pages, int num_pages, const int* tab
                                 int least, int nkv, int d, int page_size, int bits, int window, cudaStream_t stream) {
   int rc = check_packed("packed_unfold", pages, num_pages, nkv, d, page_size, bits);
   if (rc) return rc;
-  GG_REQUIRE(B > 0 && B <= 65535 && most_pages > 0 && most_pages <= bt_stride && window >= 0 && height0 >= 0 && height1 >= 0,
+  GG_REQUIRE(B > 0 && B <= UNFOLD_SEQS && most_pages > 0 && most_pages <= bt_stride && window >= 0 && height0 >= 0 && height1 >= 0,
              "packed_unfold: bad sizes B=%d pages=%d of %d window=%d", B, most_pages, bt_stride, window);
   GG_REQUIRE(((size_t)k_out % 16) == 0 && ((size_t)v_out % 16) == 0, "packed_unfold: the outputs must start on 16 bytes");
   GG_REQUIRE(out_dtype == GG_F32 || out_dtype == GG_BF16, "packed_unfold: unknown dtype %d", out_dtype);
