@@ -21,7 +21,7 @@ import time
 def _engine_flags(ap: argparse.ArgumentParser) -> None:
     ap.add_argument("--model", default="", help="local model folder (config.json + *.safetensors)")
     ap.add_argument("--config", default="", help="JSON file with engine keys: max_batch_size, "
-                    "max_token_budget, max_queue_depth, prefill_chunk_size, block_size, max_memory_fraction")
+                    "max_token_budget, max_queue_depth, prefill_chunk_size, block_size, max_memory_fraction, cache_bits")
     ap.add_argument("--device", type=int, default=0, help="CUDA device index")
     ap.add_argument("--log-level", default="info", choices=["debug", "info", "warn", "error"])
     ap.add_argument("--dtype", default="bfloat16", choices=["bfloat16", "float32"])
@@ -36,6 +36,7 @@ def _engine_flags(ap: argparse.ArgumentParser) -> None:
     ap.add_argument("--num-blocks", type=int, help="cache pages (default: from --max-memory-fraction)")
     ap.add_argument("--max-memory-fraction", type=float)
     ap.add_argument("--max-model-len", type=int)
+    ap.add_argument("--cache-bits", type=int, choices=[4, 8], help="hold keys and values in so many bits (default: in --dtype)")
     ap.add_argument("--no-cuda-graphs", action="store_true")
 
 
@@ -56,11 +57,11 @@ def _make_engine(args):
             data = json.load(f)
         data = {**data, **data.get("server", {})}       # reference: internal/config/load.go:21-30
         for k in ("max_batch_size", "max_token_budget", "max_queue_depth", "prefill_chunk_size",
-                  "block_size", "max_memory_fraction"):
+                  "block_size", "max_memory_fraction", "cache_bits"):
             if k in data:
                 setattr(ecfg, k, data[k])
     for k in ("max_batch_size", "max_token_budget", "max_queue_depth", "prefill_chunk_size",
-              "block_size", "num_blocks", "max_memory_fraction", "max_model_len"):
+              "block_size", "num_blocks", "max_memory_fraction", "max_model_len", "cache_bits"):
         v = getattr(args, k)
         if v is not None:
             setattr(ecfg, k, v)

@@ -4,7 +4,8 @@ group, and state slots.
 Layers are grouped by what they need of the cache.  A *paged* need is
 (kv heads, head size, window); layers with equal needs share one group: one page
 pool, one block table per request, one device tensor of shape
-``[layers of the group, 2 (k, v), pages, kv heads, page size, head size]`` (one
+``[layers of the group, 2 (k, v), pages, kv heads, page size, head size]`` (packed needs:
+``[layers, pages, kv heads, bytes]``, see packed.py; one
 instead of 2 where keys and values are the same rows: ``shared_kv``; two tensors
 where values have a head count or size of their own: ``v_heads``, ``v_head_dim``),
 so one page id addresses every layer of the group.  A group with a window gives a
@@ -40,6 +41,7 @@ class PagedKVNeed:
     v_head_dim: Optional[int] = None  # (None: as the keys); values then live in a tensor of their own
     keep_first: int = 0               # with a window: the first tokens of a sequence stay visible behind it,
                                       # so the pages that hold them are never given back
+    bits: Optional[int] = None        # 4 or 8: keys and values are packed (packed.py), a page and head in one block of bytes
 
     @property
     def split_kv(self) -> bool:
@@ -57,7 +59,7 @@ class PagedGroup:
     need: PagedKVNeed
     cache_ids: List[int]              # which cache entries (run-order caches) live here
     pool: PagePool
-    kv: object = None                 # device tensor [n, 2, pages, nkv, page, d] or None on the host
+    kv: object = None                 # device tensor [n, 2, pages, nkv, page, d] or None on the host; packed: uint8 [n, pages, nkv, bytes]
     v: object = None                  # values [n, 1, pages, v heads, page, dv] where their shape differs (kv then holds keys only)
 
 
@@ -124,6 +126,11 @@ class CacheManager:
         if device is not None:
             import torch
             for g in self.groups:
+                if g.need.bits:
+                    from ..csrc.ops import packed_page_bytes
+                    g.kv = torch.zeros(len(g.cache_ids), num_pages, g.need.n_kv_heads,
+                                       packed_page_bytes(g.need.bits, g.need.head_dim, page_size), dtype=torch.uint8, device=device)
+                    continue
                 split = g.need.split_kv
                 g.kv = torch.zeros(len(g.cache_ids), 1 if (g.need.shared_kv or split) else 2, num_pages,
                                    g.need.n_kv_heads, page_size, g.need.head_dim, dtype=dtype, device=device)
@@ -150,7 +157,10 @@ class CacheManager:
                 flat.append(need)
         spread(list(needs))
         for need in flat:
-            if isinstance(need, PagedKVNeed) and need.split_kv:
+            if isinstance(need, PagedKVNeed) and need.bits:
+                from ..csrc.ops import packed_page_bytes
+                total += need.n_kv_heads * packed_page_bytes(need.bits, need.head_dim, page_size)
+            elif isinstance(need, PagedKVNeed) and need.split_kv:
                 total += (need.n_kv_heads * need.head_dim + (need.v_heads or need.n_kv_heads)
                           * (need.v_head_dim or need.head_dim)) * page_size * element_size
             elif isinstance(need, PagedKVNeed):
@@ -160,9 +170,14 @@ class CacheManager:
     def layer_cache(self, cache_id):
         """(k, v) tensors [pages, nkv, page, d] of one cache entry (or part of one: ``(entry, part)``),
         and its group index.  A group whose keys and values are one tensor gives that tensor twice;
-        one whose values have a shape of their own gives v as [pages, v heads, page, dv]."""
+        one whose values have a shape of their own gives v as [pages, v heads, page, dv]; a packed one gives
+        its ``PackedKV`` twice."""
         gi, idx = self.group_of[cache_id]
         g = self.groups[gi]
+        if g.need.bits:
+            from .packed import PackedKV
+            kv = PackedKV(g.kv[idx], g.need.head_dim, self.page_size, g.need.bits)
+            return kv, kv, gi
         if g.v is not None:
             return g.kv[idx, 0], g.v[idx, 0], gi
         return g.kv[idx, 0], g.kv[idx, 0 if g.need.shared_kv else 1], gi
@@ -184,7 +199,9 @@ class CacheManager:
         step launched so far): a kernel that read a page its request no longer holds would
         then show up as NaN logits."""
         g = self.groups[gi]
-        if self.poison_freed and g.kv is not None:
+        if self.poison_freed and g.kv is not None and g.need.bits:
+            g.kv[:, page] = 255                   # (scales and offsets of all ones are NaN)
+        elif self.poison_freed and g.kv is not None:
             g.kv[:, :, page] = float("nan")
             if g.v is not None:
                 g.v[:, :, page] = float("nan")

@@ -8,12 +8,13 @@ from __future__ import annotations
 
 from typing import Optional, Sequence
 
-import numpy as np
 import torch
 
 from ..csrc import ops
 
-SHORT_PROMPT_KEYS = 256
+SHORT_PROMPT_KEYS = 256        # as in parts/attention.py
+SCRATCH_TOKENS = 65536         # tokens that prefill() reads back at a time (one sequence may be longer)
+MOST_SEQUENCES = 1024          # ... of so many sequences
 
 
 class PackedKV:
@@ -64,32 +65,48 @@ class PackedKV:
         return out
 
     # ------------------------------------------------------------------ attention
+    def _out(self, what: str, q: torch.Tensor, out: Optional[torch.Tensor]) -> torch.Tensor:
+        if q.dim() != 3 or q.shape[2] != self.head_dim or q.shape[1] == 0 or q.shape[1] % self.kv_heads:
+            raise ops.KernelError(f"{what}: q is [tokens, heads in multiples of {self.kv_heads}, {self.head_dim}], got {tuple(q.shape)}")
+        return torch.empty(q.shape, dtype=q.dtype, device=q.device) if out is None else out
+
     def decode(self, q: torch.Tensor, tables: torch.Tensor, context_lens: torch.Tensor, max_context: int, scale: float, *,
                window: int = 0, softcap: float = 0.0, sink=None, slopes=None, temperature=None, cu_q_lens=None, seqs=None,
                out: Optional[torch.Tensor] = None) -> torch.Tensor:
         """Attention of single tokens, each the last of its sequence's context_lens[b] stored ones: q [n, heads, head size]
         (row i of sequence i; with ``seqs`` token i belongs to sequence seqs[i], below 0: padding, and with ``cu_q_lens``
-        its row is cu_q_lens[sequence]).  ``max_context``: none of the contexts is longer (what the split of the work is
-        chosen from).  The options are those of the attention layer; a token with no key in sight gives zeros."""
+        its row is cu_q_lens[sequence]).  ``max_context``: no context is expected to be longer (the work is spread by it).
+        The options are those of the attention layer; a token with no key in sight gives zeros."""
+        out = self._out("decode", q, out)
         nh, d = q.shape[1], self.head_dim
-        if q.dim() != 3 or q.shape[2] != d or nh % self.kv_heads:
-            raise ops.KernelError(f"decode: q is [tokens, heads in multiples of {self.kv_heads}, {d}], got {tuple(q.shape)}")
         n = seqs.numel() if seqs is not None else q.shape[0]
-        if out is None:
-            out = torch.empty(q.shape[0], nh, d, dtype=q.dtype, device=q.device)
         more = (window, scale, softcap, sink, slopes, temperature)
         if ops.packed_decode_mma_ok(q.dtype, d, self.page_size) and q.data_ptr() % 16 == 0 and q.stride(0) % 8 == 0 \
-                and n <= ops.PACKED_DECODE_TOKENS:
-            size = ops.packed_decode_scratch(n, nh, self.kv_heads, d, self.bits, max_context, window)
-            scratch = torch.empty(size, dtype=torch.float32, device=q.device)
-            ops.packed_decode_mma(q, self.pages, tables, cu_q_lens, context_lens, seqs, n, max_context, scratch, out, nh, self.kv_heads,
-                                  d, self.page_size, self.bits, *more)
+                and out.data_ptr() % 16 == 0:
+            # (a launch takes so many tokens: more go in several)
+            for lo in range(0, n, ops.PACKED_DECODE_TOKENS):
+                m = min(n - lo, ops.PACKED_DECODE_TOKENS)
+                size = ops.packed_decode_scratch(m, nh, self.kv_heads, d, self.bits, max_context, window)
+                scratch = torch.empty(size, dtype=torch.float32, device=q.device)
+                if m == n:
+                    part = (q, tables, cu_q_lens, context_lens, seqs, out)
+                elif seqs is not None:
+                    part = (q, tables, cu_q_lens, context_lens, seqs[lo:lo + m], out)
+                else:
+                    part = (q if cu_q_lens is not None else q[lo:lo + m], tables[lo:lo + m],
+                            None if cu_q_lens is None else cu_q_lens[lo:lo + m + 1], context_lens[lo:lo + m], None,
+                            out if cu_q_lens is not None else out[lo:lo + m])
+                x, tb, cu, ctx, sq, o = part
+                ops.packed_decode_mma(x, self.pages, tb, cu, ctx, sq, m, max_context, scratch, o, nh, self.kv_heads, d, self.page_size,
+                                      self.bits, *more)
             return out
+        # the general kernel: slices of the context until every multiprocessor has four blocks
         reach = min(max_context, window) if window else max_context
         splits = max(1, min(64, -(-reach // 64), 592 // max(1, n * self.kv_heads)))
-        part = torch.empty(n * nh * splits * (d + 2), dtype=torch.float32, device=q.device)
-        ops.packed_decode(q, self.pages, tables, cu_q_lens, context_lens, seqs, n, splits, part[:n * nh * splits * d],
-                          part[n * nh * splits * d:], out, nh, self.kv_heads, d, self.page_size, self.bits, *more)
+        rows = n * nh * splits
+        part = torch.empty(rows * (d + 2), dtype=torch.float32, device=q.device)
+        ops.packed_decode(q, self.pages, tables, cu_q_lens, context_lens, seqs, n, splits, part[:rows * d], part[rows * d:], out, nh,
+                          self.kv_heads, d, self.page_size, self.bits, *more)
         return out
 
     def prefill(self, q: torch.Tensor, tables: torch.Tensor, cu_q_lens: torch.Tensor, context_lens: torch.Tensor,
@@ -97,51 +114,76 @@ class PackedKV:
                 slopes=None, temperature=None, least: int = 1, out: Optional[torch.Tensor] = None) -> torch.Tensor:
         """Causal attention of prompt portions: sequence b brings rows cu_q_lens[b] .. cu_q_lens[b + 1] of q [T, heads, head
         size], the last q_lens[b] of its context_lens[b] stored tokens.  ``q_lens`` and ``contexts`` say on the host what
-        the two device lists hold.  Sequences of fewer than ``least`` rows are left out (their rows of ``out`` stay as they are)."""
-        nh, d = q.shape[1], self.head_dim
-        if q.dim() != 3 or q.shape[2] != d or nh % self.kv_heads:
-            raise ops.KernelError(f"prefill: q is [tokens, heads in multiples of {self.kv_heads}, {d}], got {tuple(q.shape)}")
-        if out is None:
-            out = torch.empty(q.shape[0], nh, d, dtype=q.dtype, device=q.device)
-        P, dev, i32 = self.page_size, q.device, torch.int32
-        pages = most = tiles16 = tiles64 = tiles128 = 0
-        long = 0
-        for a, c in zip(q_lens, contexts):
-            if a >= least:
-                n = -(-c // P)
-                most = max(most, n)
-                pages += n - (max(0, c - a - window + 1) // P if window else 0)
-                tiles16 += -(-a // 16)
-                tiles64 += -(-a // 64)
-                tiles128 += -(-a // 128)
-                long = max(long, c)
-        if not pages:
-            return out
+        the two device lists hold.  Sequences of fewer than ``least`` rows are left out (their rows of ``out`` stay as they are).
+
+        The pages of the portions are read back once, in the type of the activations, and the prompt kernels run on them;
+        steps of many long portions go in runs of sequences, so that what is read back at a time stays within
+        ``SCRATCH_TOKENS`` (or the longest sequence)."""
+        out = self._out("prefill", q, out)
+        B, P = len(q_lens), self.page_size
+        if len(contexts) != B or tables.shape[0] < B:
+            raise ops.KernelError(f"prefill: {B} portions, {len(contexts)} contexts and block tables of {tables.shape[0]} sequences")
+        lo = pages = most = longest = 0
+        counts = [0, 0, 0]
+
+        def run(hi):
+            self._portions(q, out, tables, cu_q_lens, context_lens, lo, hi, pages, most, counts, longest, scale, window, softcap, sink, slopes,
+                           temperature, least)
+        for b in range(B):
+            a, c = q_lens[b], contexts[b]
+            if a < least or a <= 0:
+                continue
+            if a > c or c > tables.shape[1] * P:
+                raise ops.KernelError(f"prefill: sequence {b} brings {a} of {c} tokens, its block table holds {tables.shape[1] * P}")
+            n = -(-c // P)
+            seen = n - (max(0, c - a - window + 1) // P if window else 0)
+            if pages and ((pages + seen) * P > SCRATCH_TOKENS or b - lo >= MOST_SEQUENCES):
+                run(b)
+                lo, pages, most, longest, counts = b, 0, 0, 0, [0, 0, 0]
+            pages += seen
+            most = max(most, n)
+            longest = max(longest, c)
+            for i, h in enumerate((16, 64, 128)):
+                counts[i] += -(-a // h)
+        if pages:
+            run(B if B - lo <= MOST_SEQUENCES else lo + MOST_SEQUENCES)
+        return out
+
+    def _portions(self, q, out, tables, cu_q_lens, context_lens, lo, hi, pages, most, counts, longest, scale, window, softcap, sink, slopes,
+                  temperature, least):
+        """prefill() of sequences lo .. hi, whose portions see ``pages`` pages and make counts[i] tiles of 16, 64 and 128 rows."""
+        nh, d, P = q.shape[1], self.head_dim, self.page_size
+        if hi - lo != tables.shape[0]:
+            tables, context_lens, cu_q_lens = tables[lo:hi], context_lens[lo:hi], cu_q_lens[lo:hi + 1]
         B, width = tables.shape
         fast = q.dtype == torch.bfloat16 and d in (64, 128) and q.stride(0) % 8 == 0 and q.data_ptr() % 16 == 0
-        keep = torch.empty(2, pages, self.kv_heads, P, d, dtype=q.dtype, device=dev)
-        lists = [(64, tiles64)] if fast else [(16, tiles16)]
-        if fast and (tiles128 * ((nh + 1) // 2) * 2 > self._sms or min(long, window or long) > SHORT_PROMPT_KEYS):
-            lists.append((128, tiles128))
-        ints = torch.empty(B * width + 2 * sum(n for _, n in lists), dtype=i32, device=dev)
+        lists = [(64, counts[1])] if fast else [(16, counts[0])]
+        # the line between the tcgen05 and the mma.sync prompt kernels is the attention layer's: few tiles of few keys
+        if fast and (counts[2] * ((nh + 1) // 2) * 2 > self._sms or min(longest, window or longest) > SHORT_PROMPT_KEYS):
+            lists.append((128, counts[2]))
+        k, v = torch.empty(2, pages, self.kv_heads, P, d, dtype=q.dtype, device=q.device).unbind(0)
+        ints = torch.empty(B * width + 2 * sum(n for _, n in lists), dtype=torch.int32, device=q.device)
         at, full = B * width, []
         for h, n in lists:
             full.append((h, n, ints[at:at + n], ints[at + n:at + 2 * n]))
             at += 2 * n
-        plain_tables = ints[:B * width].view(B, width)
-        ops.packed_unfold(self.pages, tables, cu_q_lens, context_lens, keep[0], keep[1], most, plain_tables, full, self.kv_heads, d, P,
-                          self.bits, window, least)
-        t = {h: dict(seq=s, q0=r, n=n) for h, n, s, r in full}
-        t16, t64, t128 = (t.get(h) or dict(seq=None, q0=None, n=0) for h in (16, 64, 128))
-        more = {}
-        if t128["n"]:
-            more = dict(tile128_seq=t128["seq"], tile128_q0=t128["q0"], num_tiles128=t128["n"])
-        if softcap > 0 or sink is not None or slopes is not None or temperature is not None:
-            ops.attn_prefill_x(q, q.stride(0), keep[0], keep[1], plain_tables, width, cu_q_lens, context_lens, t16["seq"], t16["q0"], t16["n"],
-                               out, nh, self.kv_heads, d, d, 1, P, window, scale, softcap, t64["seq"], t64["q0"], t64["n"],
-                               allow_mma=fast, sink=sink, slopes=slopes, temperature=temperature, **more)
-        else:
-            ops.attn_prefill(q, q.stride(0), keep[0], keep[1], plain_tables, width, cu_q_lens, context_lens, t16["seq"], t16["q0"], t16["n"],
-                             out, nh, self.kv_heads, d, P, window, scale, t64["seq"], t64["q0"], t64["n"], allow_mma=fast,
-                             allow_tc=bool(more), **more)
-        return out
+        plain = ints[:B * width]
+        ops.packed_unfold(self.pages, tables, cu_q_lens, context_lens, k, v, most, plain, full, self.kv_heads, d, P, self.bits, window, least)
+        _, n0, seq0, q00 = full[0]
+        t16, t64 = ((None, None, 0), (seq0, q00, n0)) if fast else ((seq0, q00, n0), (None, None, 0))
+        long = dict(tile128_seq=full[1][2], tile128_q0=full[1][3], num_tiles128=full[1][1]) if len(full) > 1 else {}
+        with ops.after_everything():               # the prompt kernels read early what packed_unfold has just written
+            if softcap > 0 or sink is not None or slopes is not None or temperature is not None:
+                ops.attn_prefill_x(q, q.stride(0), k, v, plain, width, cu_q_lens, context_lens, *t16, out, nh, self.kv_heads, d, d, 1, P,
+                                   window, scale, softcap, *t64, allow_mma=fast, sink=sink, slopes=slopes, temperature=temperature, **long)
+            else:
+                ops.attn_prefill(q, q.stride(0), k, v, plain, width, cu_q_lens, context_lens, *t16, out, nh, self.kv_heads, d, P, window,
+                                 scale, *t64, allow_mma=fast, allow_tc=bool(long), **long)
+
+    @staticmethod
+    def scratch_bytes(needs, max_context: int, dtype) -> int:
+        """Most bytes that prefill() reads back at a time for any packed need among ``needs``."""
+        def flat(need):
+            return [n for sub in need for n in flat(sub)] if isinstance(need, (tuple, list)) else [need]
+        width = max((n.n_kv_heads * n.head_dim for n in flat(list(needs)) if getattr(n, "bits", None)), default=0)
+        return max(max_context, SCRATCH_TOKENS) * width * 2 * torch.empty((), dtype=dtype).element_size()

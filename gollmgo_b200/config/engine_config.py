@@ -21,6 +21,8 @@ class EngineConfig:
     strict_fcfs: bool = True               # the head of the queue blocks those behind it; False: a
                                            # request that does not fit is passed over, as in the
                                            # reference (internal/scheduler/fcfs.go:130-161)
+    cache_bits: Optional[int] = None       # 4 or 8: keys and values are held in so many bits (gollmgo_b200/cache/packed.py);
+                                           # None: in dtype
     cuda_graphs: bool = True               # capture decode-only steps
     capture_at_start: bool = True          # capture every batch bucket when the engine is built, not at first use
     state_slots: Optional[int] = None      # requests that can be admitted at once (each holds a state slot);
@@ -32,6 +34,10 @@ class EngineConfig:
             raise ValueError(f"dtype must be bfloat16 or float32, got {self.dtype!r}")
         if self.block_size <= 0 or self.block_size & (self.block_size - 1):
             raise ValueError(f"block_size must be a power of two, got {self.block_size}")
+        if self.cache_bits not in (None, 4, 8):
+            raise ValueError(f"cache_bits must be 4, 8 or None, got {self.cache_bits!r}")
+        if self.cache_bits and not 4 <= self.block_size <= 256:
+            raise ValueError(f"a packed cache has pages of 4 to 256 tokens, got block_size {self.block_size}")
         if self.max_batch_size <= 0:
             raise ValueError("max_batch_size must be positive")
         if self.max_token_budget <= 0:

@@ -164,7 +164,7 @@ __device__ __forceinline__ const float* attn_tile_max(const AttnArgs& a, const f
 }
 
 // ---------------------------------------------------------------- prompt portions
-template <typename TA, int DMAX, bool PACKED>
+template <typename TA, int DMAX>
 __global__ void __launch_bounds__(ATT_THREADS) attn_prefill_kernel(AttnArgs a) {
   constexpr int NACC = ATT_BQ * DMAX / ATT_THREADS;
   extern __shared__ float smem[];
@@ -191,7 +191,7 @@ __global__ void __launch_bounds__(ATT_THREADS) attn_prefill_kernel(AttnArgs a) {
   int lo = a.window > 0 ? max(0, first - a.window + 1) : 0;
   if (a.chunk > 0) lo = max(lo, (first / a.chunk) * a.chunk);       // the chunk of the tile's first row starts earliest
   float acc[NACC];
-  attn_tile<TA, DMAX, PACKED>(a, nrows, qptr_s, pos_s, head_s, scale_s, kvh, a.block_tables + (size_t)b * a.bt_stride, lo, last + 1,
+  attn_tile<TA, DMAX, false>(a, nrows, qptr_s, pos_s, head_s, scale_s, kvh, a.block_tables + (size_t)b * a.bt_stride, lo, last + 1,
                       min(a.keep_first, lo), smem, acc);
   pdl_trigger();
   float* m_s = const_cast<float*>(attn_tile_max(a, smem));
@@ -351,34 +351,29 @@ template <typename K> static int set_smem(K kernel, size_t bytes, const char* wh
   return GG_OK;
 }
 
-#define ATT_LAUNCH(KERNEL, TA, DMAX, PACKED, grid, who)                                        \
+#define ATT_LAUNCH(KERNEL, grid, who)                                                         \
   do {                                                                                         \
-    const int rc = set_smem(KERNEL<TA, DMAX, PACKED>, smem, who);                              \
+    const int rc = set_smem(KERNEL, smem, who);                                                \
     if (rc) return rc;                                                                         \
-    gg_launch(KERNEL<TA, DMAX, PACKED>, dim3(grid), dim3(ATT_THREADS), smem, stream, a);       \
+    gg_launch(KERNEL, dim3(grid), dim3(ATT_THREADS), smem, stream, a);                         \
   } while (0)
-#define ATT_SIZES(KERNEL, TA, PACKED, grid, who)                                               \
-  do {                                                                                         \
-    if (dvv <= 64) ATT_LAUNCH(KERNEL, TA, 64, PACKED, grid, who);                              \
-    else if (dvv <= 128) ATT_LAUNCH(KERNEL, TA, 128, PACKED, grid, who);                       \
-    else ATT_LAUNCH(KERNEL, TA, 256, PACKED, grid, who);                                       \
-  } while (0)
-#define ATT_DISPATCH(KERNEL, grid, who)                                                        \
+// KERNEL<type, largest head size[, PACKED]>
+#define ATT_SIZES(KERNEL, TA, grid, who, ...)                                                  \
   do {                                                                                         \
     const int dvv = a.dv > 0 ? a.dv : a.d;                                                     \
     const size_t smem = (size_t)attn_smem_floats(a.d, dvv) * sizeof(float);                    \
-    if (dtype == GG_F32 && a.packed_bits) ATT_SIZES(KERNEL, float, true, grid, who);           \
-    else if (dtype == GG_F32) ATT_SIZES(KERNEL, float, false, grid, who);                      \
-    else if (dtype == GG_BF16 && a.packed_bits) ATT_SIZES(KERNEL, __nv_bfloat16, true, grid, who); \
-    else if (dtype == GG_BF16) ATT_SIZES(KERNEL, __nv_bfloat16, false, grid, who);             \
-    else return gg_fail(GG_ERR_INVALID, "%s: unknown dtype %d", who, dtype);                   \
+    if (dvv <= 64) ATT_LAUNCH((KERNEL<TA, 64, ##__VA_ARGS__>), grid, who);                     \
+    else if (dvv <= 128) ATT_LAUNCH((KERNEL<TA, 128, ##__VA_ARGS__>), grid, who);              \
+    else ATT_LAUNCH((KERNEL<TA, 256, ##__VA_ARGS__>), grid, who);                              \
   } while (0)
 
 int attn_prefill_general(const AttnArgs& a, int dtype, int num_tiles, cudaStream_t stream) {
   GG_REQUIRE(num_tiles >= 0 && a.nh <= 65535, "attn_prefill: bad grid %d x %d", num_tiles, a.nh);
   if (num_tiles == 0) return GG_OK;
   dim3 grid(num_tiles, a.nh);
-  ATT_DISPATCH(attn_prefill_kernel, grid, "attn_prefill");
+  if (dtype == GG_F32) ATT_SIZES(attn_prefill_kernel, float, grid, "attn_prefill");
+  else if (dtype == GG_BF16) ATT_SIZES(attn_prefill_kernel, __nv_bfloat16, grid, "attn_prefill");
+  else return gg_fail(GG_ERR_INVALID, "attn_prefill: unknown dtype %d", dtype);
   return gg_check_launch("attn_prefill");
 }
 
@@ -386,7 +381,11 @@ int attn_decode_general(const AttnArgs& a, int dtype, int n_dec, cudaStream_t st
   const int G = a.nh / a.nkv, gchunks = (G + ATT_BQ - 1) / ATT_BQ;
   GG_REQUIRE(a.nkv * gchunks <= 65535 && a.nh <= 65535, "attn_decode: too many heads");
   dim3 grid(n_dec, a.nkv * gchunks, a.num_splits);
-  ATT_DISPATCH(attn_decode_kernel, grid, "attn_decode");
+  if (dtype == GG_F32 && a.packed_bits) ATT_SIZES(attn_decode_kernel, float, grid, "attn_decode", true);
+  else if (dtype == GG_F32) ATT_SIZES(attn_decode_kernel, float, grid, "attn_decode", false);
+  else if (dtype == GG_BF16 && a.packed_bits) ATT_SIZES(attn_decode_kernel, __nv_bfloat16, grid, "attn_decode", true);
+  else if (dtype == GG_BF16) ATT_SIZES(attn_decode_kernel, __nv_bfloat16, grid, "attn_decode", false);
+  else return gg_fail(GG_ERR_INVALID, "attn_decode: unknown dtype %d", dtype);
   return gg_check_launch("attn_decode");
 }
 

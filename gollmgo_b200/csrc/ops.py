@@ -6,6 +6,7 @@ launches go to torch's current CUDA stream, so they can be captured in a graph.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 from typing import Optional
 
@@ -1533,29 +1534,67 @@ def packed_page_bytes(bits: int, d: int, page_size: int) -> int:
     return 2 * page_size * (d * bits // 8 + 4 * (d // packed_group(d)))
 
 
-def _here(*tensors):
-    """The tensors live on the current device (the launch goes to its stream)."""
+_I, _L, _F, _P = ctypes.c_int, ctypes.c_longlong, ctypes.c_float, ctypes.c_void_p
+# These calls are made once or twice a layer and step and are short on the device, so their arguments go to the library as they
+# are (addresses as whole numbers), converted by the signatures below: half the host time of building a ctypes object for each.
+_PACKED_TYPES = {
+    "gg_packed_write": [_P, _L, _I, _P, _P, _P, _F, _P, _I, _P, _L, _I, _I, _I, _I, _I, _I, _I, _I, _I, _P],
+    "gg_packed_read": [_P, _I, _P, _I, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _P],
+    "gg_packed_decode": [_P, _L, _I, _P, _I, _P, _I, _P, _P, _P, _I, _I, _P, _P, _P, _I, _I, _I, _I, _I, _I, _F, _F, _P, _P, _F, _F, _P],
+    "gg_packed_decode_mma": [_P, _L, _P, _I, _P, _I, _P, _P, _P, _I, _I, _P, _L, _P, _I, _I, _I, _I, _I, _I, _F, _F, _P, _P, _F, _F, _P, _P],
+    "gg_packed_decode_scratch": [_I, _I, _I, _I, _I, _I, _I],
+    "gg_packed_unfold": [_P, _I, _P, _I, _P, _P, _I, _P, _P, _I, _I, _I, _P, _I, _I, _P, _P, _I, _I, _P, _P, _I, _I, _I, _I, _I, _I, _P],
+}
+_PACKED = {}
+
+
+def _packed(name: str):
+    f = _PACKED.get(name)
+    if f is None:
+        f = getattr(lib(), name)
+        f.argtypes = _PACKED_TYPES[name]
+        if name == "gg_packed_decode_scratch":
+            f.restype = ctypes.c_longlong
+        _PACKED[name] = f
+    return f
+
+
+def _at(t):
+    return t.data_ptr() if t is not None else None
+
+
+def _stream_of(what: str, *tensors) -> int:
+    """The current stream of the current device, which must be the one that holds the tensors."""
     cur = _current_device()
     for t in tensors:
         if t is not None and t.get_device() != cur:
-            raise KernelError(f"kernel arguments must be on the current device {cur} (one is on {t.device})")
+            raise KernelError(f"{what}: kernel arguments must be on the current device {cur} (one is on {t.device})")
+    return _raw_stream(cur) if _raw_stream is not None else torch.cuda.current_stream().cuda_stream
 
 
 def _rows_of(t: torch.Tensor, width: int, what: str) -> int:
     """Row stride of rows [T, ...] of ``width`` values that are contiguous in themselves."""
-    if t.dim() == 2:
-        ok = t.shape[1] == width and (t.stride(1) == 1 or width == 1)
+    shape, strides = t.shape, t.stride()
+    if len(shape) == 3:
+        ok = shape[1] * shape[2] == width and (width == 0 or (strides[2] == 1 and (shape[1] == 1 or strides[1] == shape[2])))
     else:
-        ok = t.dim() == 3 and t.shape[1] * t.shape[2] == width and t.stride(2) == 1 and (t.shape[1] == 1 or t.stride(1) == t.shape[2])
-    if not ok or (t.shape[0] > 1 and t.stride(0) < width):
-        raise KernelError(f"{what} must be rows of {width} neighbouring values, got shape {tuple(t.shape)} with strides {t.stride()}")
-    return t.stride(0)
+        ok = len(shape) == 2 and shape[1] == width and (strides[1] == 1 or width <= 1)
+    if not ok or (shape[0] > 1 and strides[0] < width):
+        raise KernelError(f"{what} must be rows of {width} neighbouring values, got shape {tuple(shape)} with strides {strides}")
+    return strides[0]
 
 
 def _ints(what: str, n: int, *tensors):
     for t in tensors:
-        if t is not None and (t.dtype != torch.int32 or not t.is_contiguous() or t.numel() < n):
+        if t is not None and (t.dtype != torch.int32 or t.numel() < n or not t.is_contiguous()):
             raise KernelError(f"{what}: index lists are contiguous int32 of at least {n} entries")
+
+
+def _tables(what: str, tables: torch.Tensor):
+    """(sequences, width) of block tables."""
+    if tables.dtype != torch.int32 or tables.dim() != 2 or not tables.is_contiguous():
+        raise KernelError(f"{what}: the block tables are contiguous int32 [sequences, pages]")
+    return tables.shape
 
 
 def packed_write(qkv: torch.Tensor, positions: Optional[torch.Tensor], slots: Optional[torch.Tensor], inv_freq: Optional[torch.Tensor],
@@ -1567,7 +1606,7 @@ def packed_write(qkv: torch.Tensor, positions: Optional[torch.Tensor], slots: Op
     ``early``: ``positions``, ``slots`` and ``inv_freq`` may be read before the kernel ahead of this one has finished (they are
     not its output)."""
     T = qkv.shape[0]
-    _here(qkv, positions, slots, inv_freq, pages, q_out)
+    stream = _stream_of("packed_write", qkv, positions, slots, inv_freq, pages, q_out)
     stride = _rows_of(qkv, (nh + 2 * nkv) * d, "packed_write: qkv")
     q_stride = 0
     if q_out is not None:
@@ -1580,9 +1619,9 @@ def packed_write(qkv: torch.Tensor, positions: Optional[torch.Tensor], slots: Op
         if inv_freq.dtype != torch.float64 or not inv_freq.is_contiguous():
             raise KernelError("packed_write: inverse frequencies must be contiguous float64")
         rot = 2 * inv_freq.numel()
-    _check(lib().gg_packed_write(_p(qkv), ctypes.c_longlong(stride), dtype_code(qkv.dtype), _p(positions), _p(slots), _p(inv_freq),
-                                 ctypes.c_float(magnitude), _p(pages), pages.shape[0], _p(q_out), ctypes.c_longlong(q_stride), T, nh, nkv,
-                                 d, rot, page_size, bits, int(interleaved), int(early), _stream()))
+    _check(_packed("gg_packed_write")(qkv.data_ptr(), stride, dtype_code(qkv.dtype), _at(positions), _at(slots), _at(inv_freq), magnitude,
+                                      pages.data_ptr(), pages.shape[0], _at(q_out) if nh else None, q_stride, T, nh, nkv, d, rot, page_size,
+                                      bits, interleaved, early, stream))
 
 
 def packed_read(pages: torch.Tensor, tables: torch.Tensor, lens: torch.Tensor, first_page: torch.Tensor, k_out: torch.Tensor,
@@ -1590,40 +1629,35 @@ def packed_read(pages: torch.Tensor, tables: torch.Tensor, lens: torch.Tensor, f
     """Keys and values that the pages of each sequence stand for: page j of sequence b (``tables`` [B, width] of page ids)
     becomes k_out, v_out [first_page[b] + j] ([pages, nkv, page_size, d]), for the pages that hold its first lens[b] tokens.
     What lies behind a sequence's last token, and a page id outside the pool, reads as zero."""
-    B = tables.shape[0]
-    _here(pages, tables, lens, first_page, k_out, v_out)
-    if tables.dim() != 2:
-        raise KernelError("packed_read: the block tables are [sequences, pages]")
-    _ints("packed_read", B, tables, lens, first_page)
+    stream = _stream_of("packed_read", pages, tables, lens, first_page, k_out, v_out)
+    B, width = _tables("packed_read", tables)
+    _ints("packed_read", B, lens, first_page)
     shape = (k_out.shape[0], nkv, page_size, d)
     if k_out.shape != shape or v_out.shape != shape or k_out.dtype != v_out.dtype or not (k_out.is_contiguous() and v_out.is_contiguous()):
         raise KernelError(f"packed_read: the outputs are contiguous [pages, {nkv}, {page_size}, {d}] of one type")
-    _check(lib().gg_packed_read(_p(pages), pages.shape[0], _p(tables), tables.shape[1], _p(lens), _p(first_page), _p(k_out), _p(v_out),
-                                dtype_code(k_out.dtype), shape[0], B, most_pages, nkv, d, page_size, bits, _stream()))
+    _check(_packed("gg_packed_read")(pages.data_ptr(), pages.shape[0], tables.data_ptr(), width, lens.data_ptr(), first_page.data_ptr(),
+                                     k_out.data_ptr(), v_out.data_ptr(), dtype_code(k_out.dtype), shape[0], B, most_pages, nkv, d,
+                                     page_size, bits, stream))
 
 
-def _packed_q(what, q, pages, tables, out, nh, d):
-    _here(q, pages, tables, out)
+def _packed_q(what, q, out, nh, d):
     stride = _rows_of(q, nh * d, what + ": q")
     if out.dtype != q.dtype or not out.is_contiguous() or out.numel() != q.shape[0] * nh * d:
         raise KernelError(f"{what}: out is contiguous [T, {nh}, {d}] in the type of q")
-    if tables.dim() != 2 or tables.dtype != torch.int32 or not tables.is_contiguous():
-        raise KernelError(f"{what}: the block tables are contiguous int32 [sequences, pages]")
     return stride
 
 
-def packed_prefill(q: torch.Tensor, pages: torch.Tensor, tables: torch.Tensor, cu_q_lens: torch.Tensor, context_lens: torch.Tensor,
-                   tile_seq: torch.Tensor, tile_q0: torch.Tensor, num_tiles: int, out: torch.Tensor, nh: int, nkv: int, d: int,
-                   page_size: int, bits: int, window: int, scale: float, softcap: float = 0.0, sink: Optional[torch.Tensor] = None,
-                   slopes: Optional[torch.Tensor] = None, temperature=None) -> None:
-    """attn_prefill_x over a packed cache on the general kernel (float32 arithmetic); ``tile_*`` list tiles of 16 queries."""
-    stride = _packed_q("packed_prefill", q, pages, tables, out, nh, d)
-    _attn_extras(nh, None, None, None, sink, slopes)
-    _ints("packed_prefill", num_tiles, tile_seq, tile_q0)
-    _check(lib().gg_packed_prefill(_p(q), ctypes.c_longlong(stride), dtype_code(q.dtype), _p(pages), pages.shape[0], _p(tables),
-                                   tables.shape[1], _p(cu_q_lens), _p(context_lens), _p(tile_seq), _p(tile_q0), num_tiles, _p(out), nh, nkv,
-                                   d, page_size, bits, window, ctypes.c_float(scale), ctypes.c_float(softcap), _p(sink), _p(slopes),
-                                   *_temperature(temperature), _stream()))
+def _packed_tokens(what, q, cu_q_lens, context_lens, seqs, n, B):
+    """The index lists of n single tokens fit each other and q."""
+    _ints(what, B, context_lens)
+    if seqs is not None:
+        _ints(what, n, seqs)
+    elif n > B:
+        raise KernelError(f"{what}: {n} tokens of {B} sequences")
+    if cu_q_lens is not None:
+        _ints(what, B + 1, cu_q_lens)
+    elif q.shape[0] < (B if seqs is not None else n):
+        raise KernelError(f"{what}: q has {q.shape[0]} rows for {B} sequences")
 
 
 def packed_decode(q: torch.Tensor, pages: torch.Tensor, tables: torch.Tensor, cu_q_lens: Optional[torch.Tensor], context_lens: torch.Tensor,
@@ -1632,15 +1666,18 @@ def packed_decode(q: torch.Tensor, pages: torch.Tensor, tables: torch.Tensor, cu
                   sink: Optional[torch.Tensor] = None, slopes: Optional[torch.Tensor] = None, temperature=None) -> None:
     """attn_decode_x over a packed cache on the general kernel (float32 arithmetic).  ``seqs`` None: token i belongs to
     sequence i; ``cu_q_lens`` None: sequence b's token is row b."""
-    stride = _packed_q("packed_decode", q, pages, tables, out, nh, d)
+    stream = _stream_of("packed_decode", q, pages, tables, cu_q_lens, context_lens, seqs, part_o, part_ml, out, sink, slopes)
+    stride = _packed_q("packed_decode", q, out, nh, d)
     _attn_extras(nh, None, None, None, sink, slopes)
-    _ints("packed_decode", n, context_lens if seqs is None else None, seqs)
+    B, width = _tables("packed_decode", tables)
+    _packed_tokens("packed_decode", q, cu_q_lens, context_lens, seqs, n, B)
     if part_o.numel() < n * nh * splits * d or part_ml.numel() < n * nh * splits * 2:
         raise KernelError("packed_decode: scratch too small")
-    _check(lib().gg_packed_decode(_p(q), ctypes.c_longlong(stride), dtype_code(q.dtype), _p(pages), pages.shape[0], _p(tables),
-                                  tables.shape[1], _p(cu_q_lens), _p(context_lens), _p(seqs), n, splits, _p(part_o), _p(part_ml), _p(out),
-                                  nh, nkv, d, page_size, bits, window, ctypes.c_float(scale), ctypes.c_float(softcap), _p(sink), _p(slopes),
-                                  *_temperature(temperature), _stream()), 2)
+    coef, every = temperature or (0.0, 0.0)
+    _check(_packed("gg_packed_decode")(q.data_ptr(), stride, dtype_code(q.dtype), pages.data_ptr(), pages.shape[0], tables.data_ptr(), width,
+                                       _at(cu_q_lens), context_lens.data_ptr(), _at(seqs), n, splits, part_o.data_ptr(), part_ml.data_ptr(),
+                                       out.data_ptr(), nh, nkv, d, page_size, bits, window, scale, softcap, _at(sink), _at(slopes), coef,
+                                       every, stream), 2)
 
 
 PACKED_DECODE_TOKENS = 1024      # tokens that packed_decode_mma takes in one launch
@@ -1653,9 +1690,7 @@ def packed_decode_mma_ok(dtype: torch.dtype, d: int, page_size: int) -> bool:
 
 def packed_decode_scratch(n: int, nh: int, nkv: int, d: int, bits: int, max_context: int, window: int) -> int:
     """float32 scratch of packed_decode_mma."""
-    f = lib().gg_packed_decode_scratch
-    f.restype = ctypes.c_longlong
-    return int(f(n, nh, nkv, d, bits, max_context, window))
+    return _packed("gg_packed_decode_scratch")(n, nh, nkv, d, bits, max_context, window)
 
 
 def packed_decode_mma(q: torch.Tensor, pages: torch.Tensor, tables: torch.Tensor, cu_q_lens: Optional[torch.Tensor],
@@ -1666,17 +1701,32 @@ def packed_decode_mma(q: torch.Tensor, pages: torch.Tensor, tables: torch.Tensor
     """packed_decode on the tensor cores (packed_decode_mma_ok).  ``scratch`` float32 of packed_decode_scratch for the same
     sizes; contexts longer than ``max_context`` are right too, only the work was split for shorter ones."""
     global tc_launched
-    stride = _packed_q("packed_decode", q, pages, tables, out, nh, d)
-    _attn_extras(nh, None, None, None, sink, slopes)
-    _ints("packed_decode", n, context_lens if seqs is None else None, seqs)
+    stream = _stream_of("packed_decode", q, pages, tables, cu_q_lens, context_lens, seqs, scratch, out, sink, slopes)
+    stride = _packed_q("packed_decode", q, out, nh, d)
+    if sink is not None or slopes is not None:
+        _attn_extras(nh, None, None, None, sink, slopes)
+    B, width = _tables("packed_decode", tables)
+    _packed_tokens("packed_decode", q, cu_q_lens, context_lens, seqs, n, B)
     if scratch.dtype != torch.float32 or not scratch.is_contiguous():
         raise KernelError("packed_decode: the scratch is contiguous float32")
+    coef, every = temperature or (0.0, 0.0)
     tc_launched = True
-    _check(lib().gg_packed_decode_mma(_p(q), ctypes.c_longlong(stride), _p(pages), pages.shape[0], _p(tables), tables.shape[1],
-                                      _p(cu_q_lens), _p(context_lens), _p(seqs), n, max_context, _p(scratch),
-                                      ctypes.c_longlong(scratch.numel()), _p(out), nh, nkv, d, page_size, bits, window,
-                                      ctypes.c_float(scale), ctypes.c_float(softcap), _p(sink), _p(slopes), *_temperature(temperature),
-                                      _p(tc_status(q.device)), _stream()), 2)
+    _check(_packed("gg_packed_decode_mma")(q.data_ptr(), stride, pages.data_ptr(), pages.shape[0], tables.data_ptr(), width, _at(cu_q_lens),
+                                           context_lens.data_ptr(), _at(seqs), n, max_context, scratch.data_ptr(), scratch.numel(),
+                                           out.data_ptr(), nh, nkv, d, page_size, bits, window, scale, softcap, _at(sink), _at(slopes),
+                                           coef, every, tc_status(q.device).data_ptr(), stream), 2)
+
+
+@contextlib.contextmanager
+def after_everything():
+    """Launches in this block start when the kernels ahead of them have completed, also those that read their lists early:
+    for kernels whose tile lists or block tables the kernel directly ahead writes."""
+    pause = lib().gg_pause_pdl
+    pause(1)
+    try:
+        yield
+    finally:
+        pause(0)
 
 
 def packed_unfold(pages: torch.Tensor, tables: torch.Tensor, cu_q_lens: torch.Tensor, context_lens: torch.Tensor, k_out: torch.Tensor,
@@ -1686,14 +1736,18 @@ def packed_unfold(pages: torch.Tensor, tables: torch.Tensor, cu_q_lens: torch.Te
     plain keys and values behind one another in k_out, v_out [pages, nkv, page_size, d], block tables of those pages in
     ``out_tables`` (shape of ``tables``), and one or two tile lists: ``lists`` of (height, count, seq, q0) with the number of
     tiles that the portions cut into rows of that height make.  Pages that the window hides are left out."""
-    B = tables.shape[0]
-    _here(pages, tables, cu_q_lens, context_lens, k_out, v_out, out_tables)
-    _ints("packed_unfold", B, tables, context_lens, out_tables)
+    stream = _stream_of("packed_unfold", pages, tables, cu_q_lens, context_lens, k_out, v_out, out_tables)
+    B, width = _tables("packed_unfold", tables)
+    _ints("packed_unfold", B, context_lens)
+    _ints("packed_unfold", B * width, out_tables)
     _ints("packed_unfold", B + 1, cu_q_lens)
     flat = []
-    for height, count, seq, q0 in list(lists) + [(0, 0, None, None)] * (2 - len(lists)):
+    for height, count, seq, q0 in lists:
         _ints("packed_unfold", count, seq, q0)
-        flat += [height, count, _p(seq), _p(q0)]
-    _check(lib().gg_packed_unfold(_p(pages), pages.shape[0], _p(tables), tables.shape[1], _p(cu_q_lens), _p(context_lens), B, _p(k_out),
-                                  _p(v_out), dtype_code(k_out.dtype), k_out.shape[0], most_pages, _p(out_tables), *flat, least, nkv, d, page_size,
-                                  bits, window, _stream()))
+        flat += [height, count, seq.data_ptr(), q0.data_ptr()]
+    if len(lists) == 1:
+        flat += [0, 0, None, None]
+    _check(_packed("gg_packed_unfold")(pages.data_ptr(), pages.shape[0], tables.data_ptr(), width, cu_q_lens.data_ptr(),
+                                       context_lens.data_ptr(), B, k_out.data_ptr(), v_out.data_ptr(), dtype_code(k_out.dtype),
+                                       k_out.shape[0], most_pages, out_tables.data_ptr(), *flat, least, nkv, d, page_size, bits, window,
+                                       stream))

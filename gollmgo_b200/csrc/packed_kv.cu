@@ -433,13 +433,15 @@ __device__ __noinline__ void list_tiles(const UnfoldArgs& a) {
 template <typename TO, int BITS>
 __global__ void __launch_bounds__(256) packed_unfold_kernel(UnfoldArgs a, TO* __restrict__ k_out, TO* __restrict__ v_out) {
   __shared__ int red[8];
-  pdl_trigger();
-  pdl_wait();
-  const int b = blockIdx.y, j = blockIdx.x, lane = threadIdx.x & 31;
+  pdl_wait();                                        // (no early start for what follows: it reads tables and lists at once)
+  if (blockIdx.x == 0) {                             // a block of its own, among the first
+    if (blockIdx.y == 0 && blockIdx.z == 0) list_tiles(a);
+    return;
+  }
+  const int b = blockIdx.y, j = blockIdx.x - 1, lane = threadIdx.x & 31;
   int q_len;
   const int ctx = unfold_keys(a, b, &q_len);
   const int skip = unfold_skip(a, ctx, q_len), P = a.page_size;
-  if (j == 0 && b == 0 && blockIdx.z == 0) list_tiles(a);
   // pages of the sequences before this one
   int before = 0;
   for (int i = threadIdx.x; i < b; i += blockDim.x) {
@@ -549,7 +551,7 @@ extern "C" int gg_packed_unfold(const void* pages, int num_pages, const int* tab
   a.out_tables = out_tables;
   a.tiles[0] = {height0, count0, seq0, q00};
   a.tiles[1] = {height1, count1, seq1, q01};
-  const dim3 grid(most_pages, B, head_blocks(out_pages, nkv)), block(256);
+  const dim3 grid(most_pages + 1, B, head_blocks(out_pages, nkv)), block(256);
 #define UNFOLD_LAUNCH(TO, BITS) gg_launch(packed_unfold_kernel<TO, BITS>, grid, block, 0, stream, a, (TO*)k_out, (TO*)v_out)
   if (out_dtype == GG_F32) { if (bits == 4) UNFOLD_LAUNCH(float, 4); else UNFOLD_LAUNCH(float, 8); }
   else { if (bits == 4) UNFOLD_LAUNCH(__nv_bfloat16, 4); else UNFOLD_LAUNCH(__nv_bfloat16, 8); }
@@ -571,20 +573,6 @@ static int check_heads(const char* who, int nh, int nkv, int bt_stride, int wind
   GG_REQUIRE(nh > 0 && nh <= 65535 && nh % nkv == 0, "%s: %d heads are not a multiple of %d kv heads", who, nh, nkv);
   GG_REQUIRE(bt_stride > 0 && window >= 0, "%s: bad block table width %d or window %d", who, bt_stride, window);
   return GG_OK;
-}
-
-// Prompt portions on the general kernel: tiles of 16 query rows.
-extern "C" int gg_packed_prefill(const void* q, long long q_stride, int act_dtype, const void* pages, int num_pages, const int* tables,
-                                 int bt_stride, const int* cu_q_lens, const int* context_lens, const int* tile_seq, const int* tile_q0,
-                                 int num_tiles, void* out, int nh, int nkv, int d, int page_size, int bits, int window, float scale,
-                                 float softcap, const float* sink, const float* slopes, float temp_coef, float temp_every, cudaStream_t stream) {
-  int rc = check_packed("packed_prefill", pages, num_pages, nkv, d, page_size, bits);
-  if (!rc) rc = check_heads("packed_prefill", nh, nkv, bt_stride, window);
-  if (rc) return rc;
-  AttnArgs a = packed_args(q, q_stride, pages, num_pages, tables, bt_stride, cu_q_lens, context_lens, out, nh, nkv, d, page_size, bits, window,
-                           scale, softcap, sink, slopes, temp_coef, temp_every);
-  a.tile_seq = tile_seq; a.tile_q0 = tile_q0;
-  return attn_prefill_general(a, act_dtype, num_tiles, stream);
 }
 
 // Single tokens on the general kernel.  part_o float[n * nh * splits * d], part_ml float[n * nh * splits * 2].

@@ -21,7 +21,7 @@ from typing import Dict, List, Optional, Sequence
 import torch
 
 from .. import architectures  # noqa: F401  (registers the architectures)
-from ..cache import CacheManager, OutOfPages, PagedKVNeed
+from ..cache import CacheManager, OutOfPages, PackedKV, PagedKVNeed
 from ..config import EngineConfig, read_config_json
 from ..csrc import ops
 from ..parts import BuildContext, StepFacts, build_model, set_matmul_precision
@@ -49,7 +49,7 @@ class ModelRunner:
         self.dtype = _DTYPES[engine_config.dtype]
         max_tokens = engine_config.max_token_budget
         ctx = BuildContext(self.dtype, self.device, max_tokens, engine_config.max_batch_size,
-                           engine_config.block_size)
+                           engine_config.block_size, cache_bits=engine_config.cache_bits)
         self.ctx = ctx
         self.config, self.spec, self.model = build_model(config_dict, ctx)
         manifest = self.model.manifest()
@@ -92,7 +92,7 @@ class ModelRunner:
         # every layer of a group shares the page id, so one page id costs per_page per layer;
         # bytes_per_page already sums over cache entries
         free, _ = torch.cuda.mem_get_info(self.device)
-        reserve = self.ctx.workspace.nbytes() + (512 << 20)
+        reserve = self.ctx.workspace.nbytes() + (512 << 20) + PackedKV.scratch_bytes(needs, self.max_model_len, self.dtype)
         avail = int((free - reserve) * self.ecfg.max_memory_fraction)
         if per_page <= 0:
             return 64

@@ -173,6 +173,13 @@ class Attention:
                         or self.has_sink or self.slopes is not None or self.temperature is not None
                         or float(getattr(self.position, "magnitude", 1.0)) != 1.0)
         self.qkv_width = (self.nh + self.nkv) * self.d + self.nv * self.dv
+        # keys and values in 4 or 8 bits: whatever the options, on the kernels of the packed cache
+        self.packed = int(ctx.cache_bits or 0)
+        if self.packed:
+            if self.dv != self.d or self.v_share > 1 or self.bias or self.extras or self.row_norm is not None:
+                raise ValueError("a cache in 4 or 8 bits takes attention without values of another size or shared, biases on q, k and v, or "
+                                 "norms over whole projections: leave cache_bits unset for this model")
+            ops.packed_page_bytes(self.packed, self.d, ctx.page_size)          # refuses sizes it does not take
         self.qkv_bias = None
         self.o_bias = None
         # the general path on mma.sync: bfloat16, keys and values of 64 or 128
@@ -216,12 +223,16 @@ class Attention:
         self.w_o = None
 
     def cache_need(self):
+        if self.packed:
+            return PagedKVNeed(self.nkv, self.d, self.window, bits=self.packed)
         if self.nv != self.nkv or self.dv != self.d:
             return PagedKVNeed(self.nkv, self.d, self.window, v_heads=self.nv, v_head_dim=self.dv)
         return PagedKVNeed(self.nkv, self.d, self.window)
 
     def query_tiles(self):
         """The tile lists of the prompt kernels this mixer can end up using."""
+        if self.packed:
+            return []                # (PackedKV.prefill makes its own)
         need = [TILES_GENERAL]
         if self.general:
             if self._mma_x:
@@ -280,6 +291,9 @@ class Attention:
         """The count of slices this step's decoded tokens would be cut into: a step that is
         captured with one count is replayed only for steps that choose the same."""
         n = facts.num_seqs if facts.decode_only else 0
+        if self.packed:              # the blocks a step is spread over: more contexts change nothing once the device is full
+            tiles = context_tiles(facts.max_context, self.window)
+            return (f"packed_tiles={min(tiles, -(-self.num_sms // max(1, n * self.nkv)))}",) if n else ()
         if n == 0 or self._flat_step(n):
             return ()
         return (f"kv_slices={self._splits(n, facts.max_context)}",)
@@ -309,7 +323,7 @@ class Attention:
 
     # the optional protocol of parts/linear.py
     def takes_normed_rows(self, num_tokens):
-        return not self.general and fuses_norms(num_tokens, self.w_qkv, self.ctx.act_dtype)
+        return (self.packed or not self.general) and fuses_norms(num_tokens, self.w_qkv, self.ctx.act_dtype)
 
     def fuses_next_norm(self, num_tokens):
         return fuses_norms(num_tokens, self.w_o, self.ctx.act_dtype)
@@ -403,9 +417,40 @@ class Attention:
                               allow_mma=self._mma_x, **more)
         return out
 
+    def _attend_packed(self, x, batch, cache, writes_cache, out):
+        """q, k, v projections, rotation, write and attention over a packed cache; fills ``out`` [T, nh * d]."""
+        T, d = x.shape[0], self.d
+        kv, _, group = cache
+        qkv = self.ctx.workspace.get("qkv", T, self.qkv_width)
+        linear(x, self.w_qkv, qkv)
+        table = self.position.rope_table()
+        if hasattr(self.position, "apply"):
+            self.position.apply(qkv, batch, self.nh, self.nkv, d)
+            table = None
+        q = qkv[:, :self.nh * d].unflatten(1, (self.nh, d))
+        if table is not None or writes_cache:
+            kv.write(qkv, batch.positions, batch.slot_mapping[group] if writes_cache else None, self.nh, table, self.position.interleaved,
+                     float(getattr(self.position, "magnitude", 1.0)), q_out=q, early=True)
+        rows = out.view(T, self.nh, d)
+        tables = batch.block_tables[group].view(-1, batch.bt_stride)
+        more = dict(window=int(self.window or 0), softcap=self.softcap, sink=self.sink, slopes=self.slopes, temperature=self.temperature,
+                    out=rows)
+        if batch.num_portions:
+            kv.prefill(q, tables, batch.cu_q_lens, batch.context_lens, batch.q_lens, [s + n for s, n in zip(batch.q_starts, batch.q_lens)],
+                       self.scale, least=2, **more)
+        if batch.num_decode:
+            facts = getattr(batch, "facts", None)
+            longest = facts.max_context if facts is not None else max(s + q for s, q in zip(batch.q_starts, batch.q_lens))
+            kv.decode(q, tables, batch.context_lens, context_tiles(longest) * TILE_KEYS, self.scale, cu_q_lens=batch.cu_q_lens,
+                      seqs=batch.dec_seqs[:batch.num_decode], **more)
+        return out
+
     def forward(self, x, batch, cache, writes_cache=True, then=None):
         T = x.shape[0]
         ws = self.ctx.workspace
+        if self.packed:
+            out = self._attend_packed(x, batch, cache, writes_cache, ws.get("attn_out", T, self.nh * self.d))
+            return linear(out, self.w_o, ws.get(self.out_buffer, T, self.hidden), then)
         if self.general:
             out = self.attend_general(x, batch, cache, writes_cache, ws.get("attn_out", T, self.nh * self.dv))
             return linear(out, self.w_o, ws.get(self.out_buffer, T, self.hidden), then)

@@ -91,10 +91,11 @@ class Workspace:
 
 class BuildContext:
     def __init__(self, act_dtype: torch.dtype, device, max_tokens: int, max_seqs: int,
-                 page_size: int, workspace: Optional[Workspace] = None):
+                 page_size: int, workspace: Optional[Workspace] = None, cache_bits: Optional[int] = None):
         self.act_dtype = act_dtype
         self.device = torch.device(device)
         self.max_tokens = max_tokens          # most tokens in one step
         self.max_seqs = max_seqs              # most sequences in one step
         self.page_size = page_size
+        self.cache_bits = cache_bits          # keys and values are held in 4 or 8 bits (None: in act_dtype)
         self.workspace = workspace or Workspace(self.device)

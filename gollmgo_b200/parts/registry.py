@@ -66,9 +66,20 @@ def register_feed_forward(name, cls): _register("feed_forward", name, cls)
 def register_block(name, cls): _register("block", name, cls)
 
 
+def _needs(need):
+    return [n for sub in need for n in _needs(sub)] if isinstance(need, (tuple, list)) else [need]
+
+
 def build_norm(spec, ctx): return _build("norm", spec, ctx)
 def build_position(spec, ctx): return _build("position", spec, ctx)
-def build_mixer(spec, ctx): return _build("mixer", spec, ctx)
+def build_mixer(spec, ctx):
+    mixer = _build("mixer", spec, ctx)
+    if getattr(ctx, "cache_bits", None):
+        for need in _needs(mixer.cache_need()):
+            if hasattr(need, "head_dim") and not need.bits:
+                raise ValueError(f"mixer {spec.kind!r} ({type(mixer).__name__}) keeps pages that cannot be held in {ctx.cache_bits} bits: "
+                                 f"leave cache_bits unset for this model")
+    return mixer
 def build_feed_forward(spec, ctx): return _build("feed_forward", spec, ctx)
 
 
