@@ -47,7 +47,7 @@ class PackedKV:
         where given (which may be the q columns of qkv).  ``early``: positions, slots and inv_freq are not the output of the kernel
         ahead on the stream, and may be read while it runs."""
         if q_out is None:
-            q_out = torch.empty(qkv.shape[0], num_heads, self.head_dim, dtype=qkv.dtype, device=qkv.device)
+            q_out = qkv.new_empty((qkv.shape[0], num_heads, self.head_dim))
         ops.packed_write(qkv, positions, slots, inv_freq, magnitude, self.pages, q_out, num_heads, self.kv_heads, self.head_dim,
                          self.page_size, self.bits, interleaved, early)
         return q_out
@@ -58,47 +58,50 @@ class PackedKV:
         first_page[b] + j of the two results [num_pages, kv heads, page_size, head size], for the pages of its first
         lens[b] tokens; what lies behind the last token is zero.  Other pages of the results are not written."""
         if out is None:
-            shape = (num_pages, self.kv_heads, self.page_size, self.head_dim)
-            out = (torch.empty(shape, dtype=dtype, device=self.pages.device), torch.empty(shape, dtype=dtype, device=self.pages.device))
+            out = self.pages.new_empty((2, num_pages, self.kv_heads, self.page_size, self.head_dim), dtype=dtype).unbind(0)
         ops.packed_read(self.pages, tables, lens, first_page, out[0], out[1], tables.shape[1], self.kv_heads, self.head_dim,
                         self.page_size, self.bits)
         return out
 
     # ------------------------------------------------------------------ attention
     def _out(self, what: str, q: torch.Tensor, out: Optional[torch.Tensor]) -> torch.Tensor:
-        if q.dim() != 3 or q.shape[2] != self.head_dim or q.shape[1] == 0 or q.shape[1] % self.kv_heads:
-            raise ops.KernelError(f"{what}: q is [tokens, heads in multiples of {self.kv_heads}, {self.head_dim}], got {tuple(q.shape)}")
-        return torch.empty(q.shape, dtype=q.dtype, device=q.device) if out is None else out
+        shape = q.shape
+        if len(shape) != 3 or shape[2] != self.head_dim or shape[1] == 0 or shape[1] % self.kv_heads:
+            raise ops.KernelError(f"{what}: q is [tokens, heads in multiples of {self.kv_heads}, {self.head_dim}], got {tuple(shape)}")
+        return q.new_empty(shape) if out is None else out
 
     def decode(self, q: torch.Tensor, tables: torch.Tensor, context_lens: torch.Tensor, max_context: int, scale: float, *,
                window: int = 0, softcap: float = 0.0, sink=None, slopes=None, temperature=None, cu_q_lens=None, seqs=None,
-               out: Optional[torch.Tensor] = None) -> torch.Tensor:
+               out: Optional[torch.Tensor] = None, early: bool = False) -> torch.Tensor:
         """Attention of single tokens, each the last of its sequence's context_lens[b] stored ones: q [n, heads, head size]
         (row i of sequence i; with ``seqs`` token i belongs to sequence seqs[i], below 0: padding, and with ``cu_q_lens``
         its row is cu_q_lens[sequence]).  ``max_context``: no context is expected to be longer (the work is spread by it).
-        The options are those of the attention layer; a token with no key in sight gives zeros."""
+        The options are those of the attention layer; a token with no key in sight gives zeros.  ``early``: block tables
+        and index lists are not the output of the kernel ahead on the stream, and may be read while it runs."""
         out = self._out("decode", q, out)
         nh, d = q.shape[1], self.head_dim
         n = seqs.numel() if seqs is not None else q.shape[0]
         more = (window, scale, softcap, sink, slopes, temperature)
         if ops.packed_decode_mma_ok(q.dtype, d, self.page_size) and q.data_ptr() % 16 == 0 and q.stride(0) % 8 == 0 \
                 and out.data_ptr() % 16 == 0:
-            # (a launch takes so many tokens: more go in several)
-            for lo in range(0, n, ops.PACKED_DECODE_TOKENS):
-                m = min(n - lo, ops.PACKED_DECODE_TOKENS)
-                size = ops.packed_decode_scratch(m, nh, self.kv_heads, d, self.bits, max_context, window)
-                scratch = torch.empty(size, dtype=torch.float32, device=q.device)
-                if m == n:
-                    part = (q, tables, cu_q_lens, context_lens, seqs, out)
-                elif seqs is not None:
-                    part = (q, tables, cu_q_lens, context_lens, seqs[lo:lo + m], out)
-                else:
-                    part = (q if cu_q_lens is not None else q[lo:lo + m], tables[lo:lo + m],
-                            None if cu_q_lens is None else cu_q_lens[lo:lo + m + 1], context_lens[lo:lo + m], None,
-                            out if cu_q_lens is not None else out[lo:lo + m])
-                x, tb, cu, ctx, sq, o = part
-                ops.packed_decode_mma(x, self.pages, tb, cu, ctx, sq, m, max_context, scratch, o, nh, self.kv_heads, d, self.page_size,
-                                      self.bits, *more)
+            shape = (nh, self.kv_heads, d, self.page_size, self.bits)
+            most = ops.PACKED_DECODE_TOKENS
+            size = ops.packed_decode_scratch(min(n, most), nh, self.kv_heads, d, self.bits, max_context, window)
+            scratch = q.new_empty((size,), dtype=torch.float32)
+            if n <= most:
+                ops.packed_decode_mma(q, self.pages, tables, cu_q_lens, context_lens, seqs, n, max_context, scratch, out, *shape, *more, early)
+                return out
+            if seqs is None and cu_q_lens is None:      # more tokens than a launch takes: rows of q go with their sequences
+                for lo in range(0, n, most):
+                    hi = min(n, lo + most)
+                    ops.packed_decode_mma(q[lo:hi], self.pages, tables[lo:hi], None, context_lens[lo:hi], None, hi - lo, max_context, scratch,
+                                          out[lo:hi], *shape, *more, early)
+                return out
+            if seqs is None:
+                seqs = torch.arange(n, dtype=torch.int32, device=q.device)
+            for lo in range(0, n, most):
+                part = seqs[lo:lo + most]
+                ops.packed_decode_mma(q, self.pages, tables, cu_q_lens, context_lens, part, part.numel(), max_context, scratch, out, *shape, *more, early)
             return out
         # the general kernel: slices of the context until every multiprocessor has four blocks
         reach = min(max_context, window) if window else max_context

@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import contextlib
 import ctypes
+import functools
 from typing import Optional
 
 import torch
@@ -1541,7 +1542,7 @@ _PACKED_TYPES = {
     "gg_packed_write": [_P, _L, _I, _P, _P, _P, _F, _P, _I, _P, _L, _I, _I, _I, _I, _I, _I, _I, _I, _I, _P],
     "gg_packed_read": [_P, _I, _P, _I, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _P],
     "gg_packed_decode": [_P, _L, _I, _P, _I, _P, _I, _P, _P, _P, _I, _I, _P, _P, _P, _I, _I, _I, _I, _I, _I, _F, _F, _P, _P, _F, _F, _P],
-    "gg_packed_decode_mma": [_P, _L, _P, _I, _P, _I, _P, _P, _P, _I, _I, _P, _L, _P, _I, _I, _I, _I, _I, _I, _F, _F, _P, _P, _F, _F, _P, _P],
+    "gg_packed_decode_mma": [_P, _L, _P, _I, _P, _I, _P, _P, _P, _I, _I, _P, _L, _P, _I, _I, _I, _I, _I, _I, _F, _F, _P, _P, _F, _F, _P, _I, _P],
     "gg_packed_decode_scratch": [_I, _I, _I, _I, _I, _I, _I],
     "gg_packed_unfold": [_P, _I, _P, _I, _P, _P, _I, _P, _P, _I, _I, _I, _P, _I, _I, _P, _P, _I, _I, _P, _P, _I, _I, _I, _I, _I, _I, _P],
 }
@@ -1688,6 +1689,7 @@ def packed_decode_mma_ok(dtype: torch.dtype, d: int, page_size: int) -> bool:
     return dtype == torch.bfloat16 and d in (64, 128) and page_size >= 16
 
 
+@functools.lru_cache(maxsize=4096)
 def packed_decode_scratch(n: int, nh: int, nkv: int, d: int, bits: int, max_context: int, window: int) -> int:
     """float32 scratch of packed_decode_mma."""
     return _packed("gg_packed_decode_scratch")(n, nh, nkv, d, bits, max_context, window)
@@ -1697,9 +1699,10 @@ def packed_decode_mma(q: torch.Tensor, pages: torch.Tensor, tables: torch.Tensor
                       context_lens: torch.Tensor, seqs: Optional[torch.Tensor], n: int, max_context: int, scratch: torch.Tensor,
                       out: torch.Tensor, nh: int, nkv: int, d: int, page_size: int, bits: int, window: int, scale: float,
                       softcap: float = 0.0, sink: Optional[torch.Tensor] = None, slopes: Optional[torch.Tensor] = None,
-                      temperature=None) -> None:
+                      temperature=None, early: bool = False) -> None:
     """packed_decode on the tensor cores (packed_decode_mma_ok).  ``scratch`` float32 of packed_decode_scratch for the same
-    sizes; contexts longer than ``max_context`` are right too, only the work was split for shorter ones."""
+    sizes; contexts longer than ``max_context`` are right too, only the work was split for shorter ones.  ``early``: the index
+    lists and block tables may be read before the kernel ahead of this one has finished (they are not its output)."""
     global tc_launched
     stream = _stream_of("packed_decode", q, pages, tables, cu_q_lens, context_lens, seqs, scratch, out, sink, slopes)
     stride = _packed_q("packed_decode", q, out, nh, d)
@@ -1714,7 +1717,7 @@ def packed_decode_mma(q: torch.Tensor, pages: torch.Tensor, tables: torch.Tensor
     _check(_packed("gg_packed_decode_mma")(q.data_ptr(), stride, pages.data_ptr(), pages.shape[0], tables.data_ptr(), width, _at(cu_q_lens),
                                            context_lens.data_ptr(), _at(seqs), n, max_context, scratch.data_ptr(), scratch.numel(),
                                            out.data_ptr(), nh, nkv, d, page_size, bits, window, scale, softcap, _at(sink), _at(slopes),
-                                           coef, every, tc_status(q.device).data_ptr(), stream), 2)
+                                           coef, every, tc_status(q.device).data_ptr(), early, stream), 2)
 
 
 @contextlib.contextmanager

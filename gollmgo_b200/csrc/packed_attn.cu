@@ -25,11 +25,15 @@
 #include "packed_kv.cuh"
 #include "tc_common.cuh"
 
+#include <atomic>
 #include <cuda_fp16.h>
 
 #define PD_MAX_TOKENS 1024         // tokens of one launch
 #define PD_STATUS 71               // reported where a copy did not arrive
 #define PD_STAGES 8                // most stages of a ring
+#define PD_EACH 4                  // tiles of a block below which fewer blocks are launched
+#define PD_ALONE 2                 // tiles a warp up to which a single token's pairs get a block each
+#define PD_SMEM (222 * 1024)       // dynamic shared memory: of 227 KB, with what a block has besides
 #define PD_LOG2E 1.4426950408889634f
 #define PD_NO_KEY (-3.0e38f)       // the running maximum before the first key: below every finite score
 
@@ -55,7 +59,7 @@ struct PackedDecode {
   float* part;                     // parts of pairs, [8 NT * D + 2 * 8 NT] each (outputs, then max and sum of each head): two of every block,
                                    // then one of every warp
   int4* cut;                       // of each block: what the second kernel joins (see there)
-  int blocks, stages;
+  int blocks, stages, early;       // early: the lists are not the output of the kernel ahead
   int* status;
 };
 
@@ -206,21 +210,26 @@ __global__ void __launch_bounds__(PdSizes<D, BITS, NT>::THREADS, 1) packed_decod
   if (tid < 2 * WARPS) part_base[tid] = -1;
   asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   pdl_trigger();
-  pdl_wait();
+  if (!a.early) pdl_wait();
   scan_tiles<TILE, Z::THREADS>(a, pairs, prefix, contexts, wsum);
   const int total = prefix[a.n];
-  for (int i = blockIdx.x; i < a.n; i += a.blocks) {          // a token without a key in sight gets zeros
-    const int b = a.seqs ? a.seqs[i] : i;
-    if (contexts[i] > 0 || b < 0) continue;
-    __nv_bfloat162* o = reinterpret_cast<__nv_bfloat162*>(a.out + (size_t)(a.cu_q_lens ? a.cu_q_lens[b] : b) * a.nh * D);
-    for (int e = tid; e < a.nh * D / 2; e += Z::THREADS) o[e] = __floats2bfloat162_rn(0.f, 0.f);
-  }
-  if (tid == 0) a.cut[blockIdx.x] = make_int4(-1, 0, 0, 0);
+  auto zeros = [&]() {                             // tokens without a key in sight, spread over the blocks
+    for (int i = blockIdx.x; i < a.n; i += a.blocks) {
+      const int b = a.seqs ? a.seqs[i] : i;
+      if (contexts[i] > 0 || b < 0) continue;
+      __nv_bfloat162* o = reinterpret_cast<__nv_bfloat162*>(a.out + (size_t)(a.cu_q_lens ? a.cu_q_lens[b] : b) * a.nh * D);
+      for (int e = tid; e < a.nh * D / 2; e += Z::THREADS) o[e] = __floats2bfloat162_rn(0.f, 0.f);
+    }
+  };
   const int blocks = min(a.blocks, total);         // each has a tile at least
-  if ((int)blockIdx.x >= blocks) return;
+  if ((int)blockIdx.x >= blocks) {
+    if (a.early) pdl_wait();
+    if (tid == 0) a.cut[blockIdx.x] = make_int4(-1, 0, 0, 0);
+    zeros();
+    return;
+  }
   const BlockRanges ranges(total, blocks);
   const int b_lo = ranges.start(blockIdx.x), b_hi = ranges.start(blockIdx.x + 1);
-  asm volatile("fence.proxy.async;" ::: "memory");            // pages that the kernel ahead wrote, read by bulk copies
 
   // chunks: the tokens of a tile that lie in one page
   const int chunk = a.page_log2 == 4 ? 16 : TILE, chunks = TILE / chunk, two = chunks >> 1;      // two: log2 of chunks
@@ -277,6 +286,8 @@ __global__ void __launch_bounds__(PdSizes<D, BITS, NT>::THREADS, 1) packed_decod
     ++f_ask;
   };
   look_up(w_lo);
+  if (a.early) pdl_wait();
+  TileCursor<TILE> now = at;                       // the pair the warp is at
   if (w_lo < w_hi) {
     const int b = a.seqs ? a.seqs[at.i] : at.i, row = a.cu_q_lens ? a.cu_q_lens[b] : b;
     const int kvh = kv_head(a, at.pair), head = kvh * a.group + (at.pair - kvh * a.chunks) * HEADS;
@@ -284,9 +295,10 @@ __global__ void __launch_bounds__(PdSizes<D, BITS, NT>::THREADS, 1) packed_decod
     if (lane < min(HEADS, a.nh - head) * D / 32)
       asm volatile("prefetch.global.L1 [%0];" ::"l"(a.q + (size_t)row * a.q_stride + (size_t)head * D + lane * 32));
   }
-  TileCursor<TILE> now = at;                       // the pair the warp is at
 #pragma unroll 1
   for (int s = 0; s < S; ++s) ask(s);
+  if (tid == 0) a.cut[blockIdx.x] = make_int4(-1, 0, 0, 0);
+  zeros();
 
   // ---- the pairs of the warp's range, one after the other
   const int key_g = (g >> 1) + 4 * (g & 1);       // the key (of 16) in row g of the scores; row g + 8 has key_g + 8
@@ -769,13 +781,13 @@ __global__ void __launch_bounds__(PdSizes<D, BITS, NT>::THREADS, 1) packed_decod
   }
 }
 
-// Joins the pairs that were cut between blocks.  One block of threads for each block of the first kernel and head: where a pair
+// Joins the pairs that were cut between blocks.  A block of threads for each block of the first kernel and head: where a pair
 // from an earlier block ends in it, cut[c] = (block of the pair's first tile, heads, first row of the result); that block has
-// its part second, the ones after it first.  Every 32 or 16 threads take some of the parts.
+// its part second, the ones after it first.  Every 32 or 16 threads take some of the parts, four values each.
 template <int D, int NT>
-__global__ void __launch_bounds__(128) packed_join_kernel(PackedDecode a) {
-  constexpr int HEADS = 8 * NT, PART = HEADS * D + 2 * HEADS, LANES = D / 4, SETS = 128 / LANES;
-  __shared__ float ml_s[SETS][2];
+__global__ void __launch_bounds__(256) packed_join_kernel(PackedDecode a) {
+  constexpr int HEADS = 8 * NT, PART = HEADS * D + 2 * HEADS, LANES = D / 4, SETS = 256 / LANES;
+  __shared__ float2 ml_s[SETS];
   __shared__ float4 y_s[SETS][LANES];
   pdl_trigger();
   pdl_wait();
@@ -788,26 +800,27 @@ __global__ void __launch_bounds__(128) packed_join_kernel(PackedDecode a) {
 #pragma unroll 4
   for (int c = first + set; c <= last; c += SETS) {
     const float* p = a.part + (size_t)(2 * c + (c == first ? 1 : 0)) * PART;
-    const float m = p[HEADS * D + 2 * h], l = p[HEADS * D + 2 * h + 1];
+    const float2 ml = *reinterpret_cast<const float2*>(p + HEADS * D + 2 * h);
     const float4 v = reinterpret_cast<const float4*>(p + h * D)[e];
-    const float top = fmaxf(M, m), u = fast_exp2(M - top), w = fast_exp2(m - top);
-    L = L * u + w * l;
+    const float top = fmaxf(M, ml.x), u = fast_exp2(M - top), w = fast_exp2(ml.x - top);
+    L = L * u + w * ml.y;
     y.x = fmaf(w, v.x, u * y.x); y.y = fmaf(w, v.y, u * y.y); y.z = fmaf(w, v.z, u * y.z); y.w = fmaf(w, v.w, u * y.w);
     M = top;
   }
-  if (e == 0) { ml_s[set][0] = M; ml_s[set][1] = L; }
+  if (e == 0) ml_s[set] = make_float2(M, L);
   y_s[set][e] = y;
   __syncthreads();
   if (set) return;
   const float sk = a.sink ? a.sink[cut.z % a.nh + h] * PD_LOG2E : PD_NO_KEY;
+  const int sets = min(SETS, last - first + 1);
   float top = sk;
-  for (int k = 0; k < SETS; ++k) top = fmaxf(top, ml_s[k][0]);
+  for (int k = 0; k < sets; ++k) top = fmaxf(top, ml_s[k].x);
   float sum = a.sink ? fast_exp2(sk - top) : 0.f;
   y = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int k = 0; k < SETS; ++k) {
-    const float w = fast_exp2(ml_s[k][0] - top);
+  for (int k = 0; k < sets; ++k) {
+    const float w = fast_exp2(ml_s[k].x - top);
     const float4 v = y_s[k][e];
-    sum = fmaf(w, ml_s[k][1], sum);
+    sum = fmaf(w, ml_s[k].y, sum);
     y.x = fmaf(w, v.x, y.x); y.y = fmaf(w, v.y, y.y); y.z = fmaf(w, v.z, y.z); y.w = fmaf(w, v.w, y.w);
   }
   const float fac = sum != 0.f ? 1.f / sum : 0.f;
@@ -828,16 +841,22 @@ static int pd_sms() {
   return n > 0 ? n : 148;
 }
 
-struct PdShape { int nt, chunks, blocks, stages, smem; long long part_floats; };
+struct PdShape { int nt, chunks, blocks, stages, smem; bool join; long long part_floats; };
 template <int D, int BITS, int NT> static void pd_fill(PdShape* s, int n, int nkv, int max_context, int window) {
   typedef PdSizes<D, BITS, NT> Z;
   s->stages = PD_STAGES;
-  while (s->stages > 2 && Z::smem(s->stages, n) > 222 * 1024) --s->stages;      // of 227 KB, with what a block has besides
+  while (s->stages > 2 && Z::smem(s->stages, n) > PD_SMEM) --s->stages;
   s->smem = Z::smem(s->stages, n);
   const long long reach = window > 0 && window < max_context ? (long long)window + Z::TILE - 1 : max_context;
   const long long tiles = (long long)n * nkv * s->chunks * ((reach + Z::TILE - 1) / Z::TILE);
-  // few tiles go to as many multiprocessors as there are: a block's warps share its instruction slots
-  s->blocks = (int)(tiles < 1 ? 1 : tiles < pd_sms() ? tiles : pd_sms());
+  const long long want = (tiles + PD_EACH - 1) / PD_EACH;
+  s->blocks = (int)(want < 1 ? 1 : want < pd_sms() ? want : pd_sms());
+  // one token of a short context: a block for each pair, which then is cut nowhere and needs no second kernel
+  s->join = true;
+  if (n == 1 && nkv * s->chunks <= pd_sms() && (reach + Z::TILE - 1) / Z::TILE <= PD_ALONE * Z::WARPS) {
+    s->blocks = nkv * s->chunks;
+    s->join = false;
+  }
   s->part_floats = (long long)s->blocks * (2 + Z::WARPS) * Z::PART;
 }
 #define PD_SIZES(CALL)                                                                   \
@@ -864,14 +883,21 @@ extern "C" long long gg_packed_decode_scratch(int n, int nh, int nkv, int d, int
 }
 
 template <int D, int BITS, int NT, bool OPT>
-static int pd_launch(const PackedDecode& a, int smem, cudaStream_t stream) {
-  cudaError_t e = cudaFuncSetAttribute(packed_decode_kernel<D, BITS, NT, OPT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+static int pd_launch(const PackedDecode& a, int smem, bool join, cudaStream_t stream) {
+  // the most it may ever ask for, once for each device
+  static std::atomic<unsigned long long> allowed{0};
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e == cudaSuccess && (dev >= 64 || !((allowed.load(std::memory_order_relaxed) >> dev) & 1))) {
+    e = cudaFuncSetAttribute(packed_decode_kernel<D, BITS, NT, OPT>, cudaFuncAttributeMaxDynamicSharedMemorySize, PD_SMEM);
+    if (e == cudaSuccess && dev < 64) allowed.fetch_or(1ull << dev, std::memory_order_relaxed);
+  }
   if (e != cudaSuccess) return gg_fail(GG_ERR_CUDA, "packed_decode: %s", cudaGetErrorString(e));
   gg_launch(packed_decode_kernel<D, BITS, NT, OPT>, dim3(a.blocks), dim3(PdSizes<D, BITS, NT>::THREADS), smem, stream, a);
   int rc = gg_check_launch("packed_decode");
   if (rc) return rc;
-  if (a.blocks == 1) return GG_OK;
-  gg_launch(packed_join_kernel<D, NT>, dim3(a.blocks, a.group < 8 * NT ? a.group : 8 * NT), dim3(128), 0, stream, a);
+  if (!join || a.blocks == 1) return GG_OK;
+  gg_launch(packed_join_kernel<D, NT>, dim3(a.blocks, a.group < 8 * NT ? a.group : 8 * NT), dim3(256), 0, stream, a);
   return gg_check_launch("packed_join");
 }
 
@@ -879,7 +905,7 @@ extern "C" int gg_packed_decode_mma(const void* q, long long q_stride, const voi
                                     const int* cu_q_lens, const int* context_lens, const int* seqs, int n, int max_context, float* scratch,
                                     long long scratch_floats, void* out, int nh, int nkv, int d, int page_size, int bits, int window,
                                     float scale, float softcap, const float* sink, const float* slopes, float temp_coef, float temp_every,
-                                    int* status, cudaStream_t stream) {
+                                    int* status, int early, cudaStream_t stream) {
   GG_REQUIRE(gg_packed_decode_mma_ok(GG_BF16, d, page_size, bits), "packed_decode: head size %d, pages of %d tokens or %d bits are not taken", d, page_size, bits);
   GG_REQUIRE(nkv > 0 && nh > 0 && nh % nkv == 0, "packed_decode: %d heads are not a multiple of %d kv heads", nh, nkv);
   GG_REQUIRE(n >= 0 && n <= PD_MAX_TOKENS && num_pages >= 0 && bt_stride > 0 && window >= 0 && max_context >= 0,
@@ -896,9 +922,9 @@ extern "C" int gg_packed_decode_mma(const void* q, long long q_stride, const voi
   a.page_log2 = 31 - __builtin_clz(page_size);
   a.page_bytes = PackedRows(bits, d, page_size).page_bytes();
   a.window = window; a.scale = scale; a.softcap = softcap; a.sink = sink; a.slopes = slopes; a.temp_coef = temp_coef; a.temp_every = temp_every;
-  a.part = scratch; a.cut = reinterpret_cast<int4*>(scratch + s.part_floats); a.blocks = s.blocks; a.stages = s.stages; a.status = status;
+  a.part = scratch; a.cut = reinterpret_cast<int4*>(scratch + s.part_floats); a.blocks = s.blocks; a.stages = s.stages; a.status = status; a.early = early;
   const bool opt = softcap > 0.f || sink || slopes || temp_every > 0.f;
   const int nt = s.nt;
-#define PD_RUN(D, BITS, NT) return opt ? pd_launch<D, BITS, NT, true>(a, s.smem, stream) : pd_launch<D, BITS, NT, false>(a, s.smem, stream)
+#define PD_RUN(D, BITS, NT) return opt ? pd_launch<D, BITS, NT, true>(a, s.smem, s.join, stream) : pd_launch<D, BITS, NT, false>(a, s.smem, s.join, stream)
   PD_SIZES(PD_RUN);
 }

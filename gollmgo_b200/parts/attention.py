@@ -442,7 +442,7 @@ class Attention:
             facts = getattr(batch, "facts", None)
             longest = facts.max_context if facts is not None else max(s + q for s, q in zip(batch.q_starts, batch.q_lens))
             kv.decode(q, tables, batch.context_lens, context_tiles(longest) * TILE_KEYS, self.scale, cu_q_lens=batch.cu_q_lens,
-                      seqs=batch.dec_seqs[:batch.num_decode], **more)
+                      seqs=batch.dec_seqs[:batch.num_decode], early=True, **more)
         return out
 
     def forward(self, x, batch, cache, writes_cache=True, then=None):
