@@ -327,7 +327,7 @@ __global__ void attn_merge_kernel(AttnArgs a) {
       const float m = a.part_ml[(row0 + s) * 2];
       if (m != -INFINITY) o += expf(m - M) * a.part_o[(row0 + s) * d + c];
     }
-    o = L > 0.f ? o / L : 0.f;
+    o = L > 0.f || (a.packed_bits && L != 0.f) ? o / L : 0.f;        // (a packed cache: a NaN stays one)
     if (a.out_f32) ((float*)a.out)[at + c] = o;
     else ((TA*)a.out)[at + c] = from_f32<TA>(o);
   }

@@ -579,7 +579,7 @@ __global__ void __launch_bounds__(PdSizes<D, BITS, NT>::THREADS, 1) packed_decod
                 w = fmaxf(w, p * z);
               }
             w = warp_max(w);
-            const int e = w > power_of_two(vexp) * 512.f ? min(100, (int)(__float_as_uint(w) >> 23) - 127) : vexp;
+            const int e = w > power_of_two(vexp) * 512.f ? min(127, (int)(__float_as_uint(w) >> 23) - 127) : vexp;
             const float down = vexp - e < -126 ? 0.f : power_of_two(vexp - e);
             vexp = e;
 #pragma unroll
@@ -674,15 +674,16 @@ __global__ void __launch_bounds__(PdSizes<D, BITS, NT>::THREADS, 1) packed_decod
           part_top[2 * warp + last][h] = ref[nt][j];
           part_sum[2 * warp + last][h] = l[nt][j];
         }
-        const float even = power_of_two(18 + vexp) * fac, odd = BITS == 4 ? even * 0.0625f : even;
+        // codes stood at 2^-24 (in 4 bits every second one at 2^-20), weights at 2^(6 - vexp)
+        const float even = power_of_two(vexp) * fac, up = 0x1p18f, odd = BITS == 4 ? 0x1p14f : up;
 #pragma unroll
         for (int gr = 0; gr < GR; ++gr) {
           const float off = r[gr][nt][j] * fac;
           float y[8];
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            y[2 * i] = fmaf(o[gr * 4 + i][nt][j], even, off);
-            y[2 * i + 1] = fmaf(o[gr * 4 + i][nt][2 + j], odd, off);
+            y[2 * i] = fmaf(o[gr * 4 + i][nt][j] * up, even, off);
+            y[2 * i + 1] = fmaf(o[gr * 4 + i][nt][2 + j] * odd, even, off);
           }
           const int c = gr * 64 + g * 8;
           if (!complete) {

@@ -305,3 +305,197 @@ def test_prefill(bits, dtype, option, nh, nkv, d, page):
         ref = plain.attend(x.double(), pool.keys[b], pool.values[b], n, d ** -0.5, **o)
         e = prompt_errors(dtype, x, pool.keys[b], d ** -0.5)
         assert ((out[cu[b]:cu[b + 1]] - ref).abs() <= bound(ref, [pool.values[b]], dtype, *e)).all(), (b, a, n)
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("nh,nkv", [(2, 2), (3, 1), (7, 1), (9, 1), (24, 1), (17, 1), (32, 1), (66, 2)])
+@pytest.mark.parametrize("d", [64, 128])
+def test_decode_groups_of_any_size(bits, nh, nkv, d):
+    lens = [33, 5, 260]
+    pool = Pool(lens, nkv, d, 16, bits, seed=nh)
+    g = torch.Generator().manual_seed(nh)
+    q = torch.randn(3, nh, d, generator=g).to(BF16)
+    out = pool.kv.decode(q.cuda(), pool.tables.cuda(), torch.tensor(lens, dtype=torch.int32).cuda(), 260, d ** -0.5).cpu().double()
+    for b, n in enumerate(lens):
+        ref = plain.attend(q[b:b + 1].double(), pool.keys[b], pool.values[b], n, d ** -0.5)[0]
+        assert ((out[b] - ref).abs() <= bound(ref, [pool.values[b]], BF16, *errors_of(BF16, q[b], pool.keys[b], d ** -0.5))).all()
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("window", [0, 1, 16, 31, 1000])
+def test_decode_of_contexts_longer_than_said_and_of_every_split(bits, window):
+    """max_context only spreads the work: any value gives the same attention.  Long contexts are cut between blocks."""
+    nh, nkv, d, page = 4, 1, 128, 16
+    lens = [900, 1, 31, 2500]
+    pool = Pool(lens, nkv, d, page, bits, seed=window)
+    g = torch.Generator().manual_seed(3)
+    q = torch.randn(4, nh, d, generator=g).to(BF16)
+    args = (q.cuda(), pool.tables.cuda(), torch.tensor(lens, dtype=torch.int32).cuda())
+    for said in (1, 40, 600, 2500, 100000):
+        out = pool.kv.decode(*args, said, d ** -0.5, window=window).cpu().double()
+        for b, n in enumerate(lens):
+            ref = plain.attend(q[b:b + 1].double(), pool.keys[b], pool.values[b], n, d ** -0.5, window=window)[0]
+            assert ((out[b] - ref).abs() <= bound(ref, [pool.values[b]], BF16, *errors_of(BF16, q[b], pool.keys[b], d ** -0.5))).all(), (said, n)
+    alone = pool.kv.decode(args[0][3:], args[1][3:], args[2][3:], 2500, d ** -0.5, window=window).cpu().double()
+    ref = plain.attend(q[3:].double(), pool.keys[3], pool.values[3], 2500, d ** -0.5, window=window)[0]
+    assert ((alone[0] - ref).abs() <= bound(ref, [pool.values[3]], BF16, *errors_of(BF16, q[3], pool.keys[3], d ** -0.5))).all()
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_decode_of_bad_values_and_far_scales(bits, dtype):
+    """Infinities and NaN reach the heads (keys) or channels (values) that see them and nothing else; values of 2^100 beside values of
+    2^-100, and a loud token that is hardly attended to, cost the others nothing."""
+    nh, nkv, d, page, n = 4, 2, 128, 16, 100
+    g = torch.Generator().manual_seed(7)
+    x = torch.randn(4, n, (nh + 2 * nkv) * d, generator=g)
+    k0 = nh * d
+    v0 = k0 + nkv * d
+    x[0, 3, k0 + 5] = math.nan                      # sequence 0: a key of kv head 0, behind the window
+    x[0, 2, v0 + d + 70] = math.inf                 # ... and a value of kv head 1
+    x[1, 90, k0 + 5] = -math.inf                    # sequence 1: a key of kv head 0 in sight
+    x[1, 91, v0 + d + 70] = math.nan                # ... a value of kv head 1, second group of channels
+    x[2, :, v0:v0 + d] *= 2.0 ** 100                # sequence 2: huge and tiny values
+    x[2, :, v0 + d:] *= 2.0 ** -100
+    x[3, 80, v0:] *= 2.0 ** 20                      # sequence 3: one loud value, whose key points away
+    x[3, 80, k0:v0] *= -4.0
+    x = x.to(dtype)
+    kv = PackedKV_of(4 * 8, nkv, d, page, bits)
+    tables = torch.arange(32, dtype=torch.int32).view(4, 8)
+    slots = (tables.repeat_interleave(page, 1)[:, :n] * page + torch.arange(n) % page).to(torch.int32)
+    q = x[:, -1, :k0].view(4, nh, d) * 1.0
+    q[3] = -8 * x[3, 80, k0:v0].view(nkv, 1, d).expand(nkv, nh // nkv, d).reshape(nh, d) / x[3, 80, k0:v0].abs().max()
+    kv.write(x.reshape(4 * n, -1).cuda(), None, slots.reshape(-1).cuda(), nh)
+    out = kv.decode(q.cuda(), tables.cuda(), torch.full((4,), n, dtype=torch.int32).cuda(), n, d ** -0.5, window=90).cpu().double()
+    grp = nh // nkv
+    for b in range(4):
+        held = [torch.stack([torch.stack([plain.get(kv.pages[b * 8:b * 8 + 8].cpu(), t, h, d, bits, page)[w] for h in range(nkv)]) for t in range(n)])
+                for w in (0, 1)]
+        for h in range(nh):
+            kvh = h // grp
+            ref = plain.attend(q[b:b + 1, h:h + 1].double(), held[0][:, kvh:kvh + 1], held[1][:, kvh:kvh + 1], n, d ** -0.5, window=90)[0, 0]
+            if b == 1 and kvh == 0:
+                assert torch.isnan(out[b, h]).all()
+                continue
+            if b == 1:
+                bad = torch.isnan(ref)
+                assert bad[64:].all() and not bad[:64].any()
+                assert torch.equal(torch.isnan(out[b, h]), bad)
+                continue
+            seen = held[1][n - 90:, kvh]
+            p = torch.softmax(held[0][n - 90:, kvh] @ q[b, h].double() * d ** -0.5, 0)
+            size = (p[:, None] * seen.abs()).sum(0).max()          # what the weights' roundings are relative to
+            e, wt = errors_of(dtype, q[b, h:h + 1], held[0][n - 90:, kvh:kvh + 1], d ** -0.5)
+            assert ((out[b, h] - ref).abs() <= torch.finfo(dtype).eps / 2 * ref.abs() + (2 * e + 2 * wt) * size).all(), (b, h)
+
+
+def PackedKV_of(*a):
+    return kit()[0].empty(*a)
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+def test_more_tokens_than_a_launch_takes(bits):
+    PackedKV, ops = kit()
+    n, nh, nkv, d, page = ops.PACKED_DECODE_TOKENS + 77, 2, 1, 64, 16
+    kv = PackedKV.empty(n, nkv, d, page, bits)
+    g = torch.Generator().manual_seed(0)
+    rows = torch.randn(n * page, (nh + 2 * nkv) * d, generator=g).to(BF16).cuda()
+    kv.write(rows, None, torch.arange(n * page, dtype=torch.int32).cuda(), nh)
+    tables = torch.randperm(n, generator=g).to(torch.int32).view(n, 1).cuda()
+    ctx = torch.randint(0, page + 1, (n,), generator=g).to(torch.int32).cuda()
+    q = torch.randn(n, nh, d, generator=g).to(BF16).cuda()
+    out = kv.decode(q, tables, ctx, page, 0.125)
+    k, v = kv.read(tables, torch.full_like(ctx, page), torch.arange(n, dtype=torch.int32).cuda(), n, F32)
+    z = torch.einsum("bhd,bpd->bhp", q.float(), k[:, 0]) * 0.125
+    z = z.masked_fill(torch.arange(page, device="cuda") >= ctx[:, None, None], -math.inf)
+    w = torch.where(ctx[:, None, None] > 0, torch.softmax(z, -1), 0).nan_to_num()
+    ref = torch.einsum("bhp,bpd->bhd", w, v[:, 0])
+    assert ((out.float() - ref).abs() <= 2.0 ** -8 * ref.abs() + 2.0 ** -10 * float(v.abs().max())).all()
+    order = torch.randperm(n, generator=g).to(torch.int32).cuda()
+    cu = torch.arange(n + 1, dtype=torch.int32).cuda()
+    assert torch.equal(kv.decode(q, tables, ctx, page, 0.125, seqs=order, cu_q_lens=cu), out)
+    assert torch.equal(kv.decode(q, tables, ctx, page, 0.125, cu_q_lens=cu), out)
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+def test_offsets_past_32_bits(bits):
+    """Pages that lie more than 2^31 and 2^32 bytes into the pool."""
+    PackedKV, ops = kit()
+    nh, nkv, d, page = 8, 8, 128, 16
+    block = nkv * ops.packed_page_bytes(bits, d, page)
+    pages_n = 2 ** 32 // block + 40
+    kv = PackedKV.empty(pages_n, nkv, d, page, bits)
+    small = PackedKV.empty(8, nkv, d, page, bits)
+    n = 100
+    high = torch.tensor([pages_n - 1, 2 ** 31 // block + 1, 3, pages_n - 7, 2 ** 32 // block + 1, 2 ** 31 // block, 0], dtype=torch.int32)
+    low = torch.tensor([6, 1, 3, 2, 4, 5, 0], dtype=torch.int32)
+    g = torch.Generator().manual_seed(0)
+    rows = torch.randn(n, (nh + 2 * nkv) * d, generator=g).to(BF16).cuda()
+    q = torch.randn(1, nh, d, generator=g).to(BF16).cuda()
+    dev = lambda x: torch.tensor(x, dtype=torch.int32).cuda()
+    got = []
+    for c, table in ((kv, high), (small, low)):
+        t = torch.arange(n)
+        slots = (table[t // page].long() * page + t % page).to(torch.int32).cuda()
+        tables = table.view(1, -1).cuda()
+        c.write(rows, dev(list(range(n))), slots, nh, freqs(d).cuda())
+        got.append((*c.read(tables, dev([n]), dev([0]), 7), c.decode(q, tables, dev([n]), n, 0.1),
+                    c.prefill(rows[:, :nh * d].unflatten(1, (nh, d)), tables, dev([0, n]), dev([n]), [n], [n], 0.1)))
+    assert all(torch.equal(a, b) for a, b in zip(*got))
+
+
+def test_calls_that_are_refused():
+    PackedKV, ops = kit()
+    pool = Pool([20], 2, 64, 16, 4, seed=0)
+    kv, tables, ctx = pool.kv, pool.tables.cuda(), torch.tensor([20], dtype=torch.int32).cuda()
+    q = torch.zeros(1, 4, 64, dtype=BF16, device="cuda")
+    E = ops.KernelError
+    for bad in (dict(tables=tables.cpu()), dict(tables=tables.long()), dict(tables=tables[0]), dict(context_lens=ctx.long()), dict(context_lens=ctx.cpu()),
+                dict(q=q.half()), dict(q=q.cpu()), dict(q=torch.zeros(2, 4, 64, dtype=BF16, device="cuda")), dict(window=-1),
+                dict(sink=torch.zeros(3, device="cuda")), dict(slopes=torch.zeros(4, device="cuda", dtype=BF16)), dict(out=torch.zeros(1, 4, 64, device="cuda")),
+                dict(seqs=torch.zeros(1, device="cuda", dtype=torch.int64)), dict(cu_q_lens=torch.zeros(1, device="cuda", dtype=torch.int32))):
+        args = dict(dict(q=q, tables=tables, context_lens=ctx, max_context=20, scale=0.1), **bad)
+        with pytest.raises(E):
+            kv.decode(**args)
+    row = torch.zeros(1, 8 * 64, dtype=BF16, device="cuda")
+    pos = torch.zeros(1, dtype=torch.int32, device="cuda")
+    for a in ((row[:, :100], pos, pos, 4), (row, pos.long(), pos, 4), (row, pos, pos[:0], 4), (row.half(), pos, pos, 4), (row, pos, pos, 3),
+              (row, pos, pos, 4, torch.ones(32, device="cuda")), (row, None, pos, 4, torch.ones(32, device="cuda", dtype=F64)),
+              (row, pos, pos, 4, torch.ones(33, device="cuda", dtype=F64))):
+        with pytest.raises(E):
+            kv.write(*a)
+    with pytest.raises(E):
+        kv.read(tables, ctx, pos, 2, out=(torch.zeros(2, 2, 16, 64, device="cuda"), torch.zeros(2, 2, 16, 64, device="cuda", dtype=BF16)))
+    with pytest.raises(E):
+        kv.read(tables, ctx.long(), pos, 2)
+    assert kv.decode(q[:0], tables[:0], ctx[:0], 20, 0.1).shape == (0, 4, 64)
+    assert kv.write(row[:0], pos[:0], pos[:0], 4).shape == (0, 4, 64)
+    assert kv.prefill(q[:0], tables, torch.zeros(2, dtype=torch.int32, device="cuda"), ctx, [0], [20], 0.1).shape == (0, 4, 64)
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+def test_prefill_in_several_runs(bits, monkeypatch):
+    """More tokens than are read back at a time: the same result in runs of sequences."""
+    from gollmgo_b200.cache import packed
+    nh, nkv, d, page = 8, 2, 64, 16
+    q_lens, lens = [5, 0, 33, 16, 2, 70], [5, 9, 90, 16, 65, 140]
+    pool = Pool(lens, nkv, d, page, bits, seed=4)
+    cu = [0]
+    for a in q_lens:
+        cu.append(cu[-1] + a)
+    g = torch.Generator().manual_seed(9)
+    q = torch.randn(cu[-1], nh, d, generator=g).to(BF16).cuda()
+    dev = lambda x: torch.tensor(x, dtype=torch.int32).cuda()
+    args = (q, pool.tables.cuda(), dev(cu), dev(lens), q_lens, lens, 0.125)
+    want = pool.kv.prefill(*args)
+    for most in (1, 100, 200):
+        monkeypatch.setattr(packed, "SCRATCH_TOKENS", most)
+        got = pool.kv.prefill(*args)
+        # (runs of few keys may go to another of the prompt kernels)
+        assert float((got.float() - want.float()).abs().max()) <= 2.0 ** -6 * float(want.abs().max())
+    monkeypatch.setattr(packed, "MOST_SEQUENCES", 2)
+    assert float((pool.kv.prefill(*args).float() - want.float()).abs().max()) <= 2.0 ** -6 * float(want.abs().max())
+    mark = torch.full_like(want, 9.0)
+    pool.kv.prefill(*args, least=10, out=mark)
+    kept = [r for b in (0, 4) for r in range(cu[b], cu[b + 1])]
+    assert (mark[kept] == 9.0).all() and (mark != 9.0).any(-1).any(-1).sum() == cu[-1] - len(kept)
