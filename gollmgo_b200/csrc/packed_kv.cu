@@ -4,17 +4,16 @@
 #include "packed_kv.cuh"
 
 // ---------------------------------------------------------------- write
-// Arithmetic: float32 for bfloat16 activations, float64 for float32 ones (whose last bits decide codes next to a border).
-template <typename TA> struct PackMath;
-template <> struct PackMath<__nv_bfloat16> { typedef float T; };
-template <> struct PackMath<float> { typedef double T; };
+// Which code a value gets is decided in exact or float64 arithmetic: a bfloat16 value as it came is decided in float32, where its
+// difference from the offset is exact; a rotated key, and whatever came in float32, in float64, whose last bits lie far below
+// a code's border.
 
 __device__ __forceinline__ unsigned short bf16_down(float x) { return __bfloat16_as_ushort(__float2bfloat16_rd(x)); }
 __device__ __forceinline__ unsigned short bf16_up(float x) { return __bfloat16_as_ushort(__float2bfloat16_ru(x)); }
 __device__ __forceinline__ float bf16_value(unsigned short b) { return __uint_as_float((unsigned)b << 16); }
 
-// (scale, offset) of a group from its smallest and largest value, and a value's code.  Halves keep the range of a group
-// that spans more than the largest float finite; halving is exact.
+// (scale, offset) of a group from its smallest and largest value, and a float64 value's code.  In float32, halves keep the range
+// of a group that spans more than the largest float finite; halving is exact.
 struct PackCoder {
   unsigned pair;
   float half_offset, half_scale;
@@ -37,10 +36,6 @@ struct PackCoder {
     const unsigned short s = bf16_up(__double2float_ru((mx - offset) / most));
     scale = bf16_value(s);
     pair = (unsigned)s | ((unsigned)o << 16);
-  }
-  __device__ __forceinline__ unsigned code(float x) const {
-    if (!(half_scale > 0.f)) return 0u;
-    return (unsigned)fminf(fmaxf(rintf((0.5f * x - half_offset) / half_scale), 0.f), (float)most);
   }
   __device__ __forceinline__ unsigned code(double x) const {
     if (!(scale > 0.0)) return 0u;
@@ -70,7 +65,7 @@ __global__ void __launch_bounds__(PACK_WARPS * 32)
 packed_write_kernel(const TA* __restrict__ qkv, long long row_stride, const int* __restrict__ positions, const int* __restrict__ slots,
                     const double* __restrict__ inv_freq, float mag, unsigned char* __restrict__ pages, int num_pages, TA* __restrict__ q_out,
                     long long q_stride, int nh, int nkv, int d, int rot, int page_size, int bits, int interleaved, int early) {
-  typedef typename PackMath<TA>::T TC;
+  typedef double TC;
   extern __shared__ double smem_d[];
   TC* cs = reinterpret_cast<TC*>(smem_d);             // cos[rot / 2], sin[rot / 2], then a row of each warp
   pdl_trigger();
@@ -164,6 +159,82 @@ __device__ __forceinline__ uint2 codes8(const PackCoder& k, const float* x) {
   return k.pair == 0x7fff7fffu ? make_uint2(0u, 0u) : make_uint2(w[0], w[1]);
 }
 
+// The same for float64 values: the quotient in float32, and near a border the remainder in float64.
+template <int BITS>
+__device__ __forceinline__ uint2 codes8(const PackCoder& k, const double* x) {
+  constexpr float MOST = (1 << BITS) - 1, NEAR = 0.5f - MOST * 0x1p-20f;
+  constexpr float MAGIC = 12582912.f;
+  // (differences of halves stay inside float32's range; a scale whose reciprocal does not is brought up first)
+  const double offset = k.offset, scale = k.scale;
+  const float up = scale < 0x1p-60 ? 0x1p64f : 1.f, inv = scale > 0.0 ? 1.f / ((float)(0.5 * scale) * up) : 0.f;
+  unsigned q[8];
+  float far = 0.f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float t = ((float)(0.5 * (x[i] - offset)) * up) * inv, m = t + MAGIC;
+    far = fmaxf(far, fabsf(t - (m - MAGIC)));
+    q[i] = __float_as_uint(m);
+  }
+  if (far >= NEAR) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const double rest = fma(-(double)(__uint_as_float(q[i]) - MAGIC), scale, x[i] - offset), border = 0.5 * scale;
+      const bool odd = q[i] & 1u;
+      q[i] += (rest > border || (rest == border && odd)) ? 1u : (rest < -border || (rest == -border && odd)) ? ~0u : 0u;
+    }
+  }
+  unsigned w[2] = {0u, 0u};
+#pragma unroll
+  for (int i = 0; i < 8; ++i) w[i * BITS / 32] |= (q[i] & ((1u << BITS) - 1)) << (i * BITS & 31);
+  return k.pair == 0x7fff7fffu ? make_uint2(0u, 0u) : make_uint2(w[0], w[1]);
+}
+
+// One head of one token, channels p .. p + 7 (a) and D / 2 + p .. (c) in each of the head's lanes: the group's extremes, its pair, the codes.
+__device__ __forceinline__ float least(float a, float b) { return fminf(a, b); }
+__device__ __forceinline__ float most(float a, float b) { return fmaxf(a, b); }
+__device__ __forceinline__ double least(double a, double b) { return fmin(a, b); }
+__device__ __forceinline__ double most(double a, double b) { return fmax(a, b); }
+template <int D, int BITS, typename TC>
+__device__ __forceinline__ void store_head(const TC* a, const TC* c, int p, unsigned char* block, const PackedRows& r, int which, int place) {
+  constexpr int HALF = D / 2, LANES = D / 16;
+  // (heads of 64: one group)  A NaN shows in the sum of x * 0, an infinity as an extreme.
+  TC mn[2] = {a[0], c[0]}, mx[2] = {a[0], c[0]};
+  float nan[2] = {0.f, 0.f};
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    mn[0] = least(mn[0], a[j]); mx[0] = most(mx[0], a[j]); nan[0] = fmaf((float)a[j], 0.f, nan[0]);
+    mn[1] = least(mn[1], c[j]); mx[1] = most(mx[1], c[j]); nan[1] = fmaf((float)c[j], 0.f, nan[1]);
+  }
+  if (D == 64) { mn[0] = least(mn[0], mn[1]); mx[0] = most(mx[0], mx[1]); nan[0] += nan[1]; }
+  const unsigned mates = ((1u << LANES) - 1) << ((threadIdx.x & 31) & ~(LANES - 1));
+  PackCoder k[2];
+#pragma unroll
+  for (int g = 0; g < D / 64; ++g) {
+#pragma unroll
+    for (int o = 1; o < LANES; o <<= 1) {
+      mn[g] = least(mn[g], __shfl_xor_sync(mates, mn[g], o));
+      mx[g] = most(mx[g], __shfl_xor_sync(mates, mx[g], o));
+    }
+    const bool bad = __any_sync(mates, nan[g] != 0.f) || !(mx[g] - mx[g] == 0) || !(mn[g] - mn[g] == 0);
+    k[g].set(mn[g], mx[g], bad, BITS);
+  }
+  if (D == 64) k[1] = k[0];
+  unsigned char* o = block + r.codes(which, place) + p * BITS / 8;
+  const uint2 c0 = codes8<BITS>(k[0], a), c1 = codes8<BITS>(k[1], c);
+  if (BITS == 4) {
+    *reinterpret_cast<unsigned*>(o) = c0.x;
+    *reinterpret_cast<unsigned*>(o + HALF * BITS / 8) = c1.x;
+  } else {
+    *reinterpret_cast<uint2*>(o) = c0;
+    *reinterpret_cast<uint2*>(o + HALF * BITS / 8) = c1;
+  }
+  if (p == 0) {
+    unsigned* q = reinterpret_cast<unsigned*>(block + r.pairs(which, place));
+    if (D == 128) *reinterpret_cast<uint2*>(q) = make_uint2(k[0].pair, k[1].pair);
+    else *q = k[0].pair;
+  }
+}
+
 // The common case: bfloat16, heads of 64 or 128, half-split pairs over the whole head or no rotation, rows in 16-byte steps.
 // Blocks of y = 0 take the k and v heads of TOK tokens, blocks of y = 1 their q heads (a tenth of the work a row: apart, so that
 // all warps of a block are busy as long).  A thread takes channels p .. p + 7 and D / 2 + p .. of one head (two 16-byte loads,
@@ -175,16 +246,19 @@ packed_write_vec_kernel(const __nv_bfloat16* __restrict__ qkv, long long row_str
                         const int* __restrict__ slots, const double* __restrict__ inv_freq, float mag, unsigned char* __restrict__ pages,
                         int num_pages, __nv_bfloat16* __restrict__ q_out, long long q_stride, int T, int nh, int nkv, int page_log2, int early) {
   constexpr int HALF = D / 2, LANES = D / 16;         // lanes of a head
-  __shared__ float cs[TOK][2][HALF];
+  __shared__ double cs[TOK][2][HALF];                 // (queries: the same as float32)
   pdl_trigger();
   if (!early) pdl_wait();
   const int t0 = blockIdx.x * TOK, tokens = min(TOK, T - t0);
   const bool queries = blockIdx.y == 1;
   const int first = queries ? 0 : nh, per = (queries ? nh : 2 * nkv) * LANES;
+  float* cf = reinterpret_cast<float*>(cs);
   if (inv_freq) {
     for (int e = threadIdx.x; e < tokens * HALF; e += WRITE_THREADS) {
       const int p = e % HALF, i = e / HALF;
-      turn_of((double)positions[t0 + i], inv_freq[p], mag, &cs[i][0][p], &cs[i][1][p]);
+      const double pos = (double)positions[t0 + i];
+      if (queries) turn_of(pos, inv_freq[p], mag, &cf[(2 * i) * HALF + p], &cf[(2 * i + 1) * HALF + p]);
+      else turn_of(pos, inv_freq[p], mag, &cs[i][0][p], &cs[i][1][p]);
     }
   }
   if (early) pdl_wait();
@@ -218,15 +292,15 @@ packed_write_vec_kernel(const __nv_bfloat16* __restrict__ qkv, long long row_str
       c[2 * j] = __uint_as_float(wh[j] << 16);
       c[2 * j + 1] = __uint_as_float(wh[j] & 0xffff0000u);
     }
-    if (inv_freq && h < nh + nkv) {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const float u = a[j], v = c[j], co = cs[n][0][p + j], si = cs[n][1][p + j];
-        a[j] = u * co - v * si;
-        c[j] = u * si + v * co;
-      }
-    }
     if (queries) {
+      if (inv_freq) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const float u = a[j], v = c[j], co = cf[(2 * n) * HALF + p + j], si = cf[(2 * n + 1) * HALF + p + j];
+          a[j] = u * co - v * si;
+          c[j] = u * si + v * co;
+        }
+      }
       __nv_bfloat16* o = q_out + (size_t)(t0 + n) * q_stride + (size_t)h * D + p;
       *reinterpret_cast<uint4*>(o) = make_uint4(pack_bf16(a[0], a[1]), pack_bf16(a[2], a[3]), pack_bf16(a[4], a[5]), pack_bf16(a[6], a[7]));
       *reinterpret_cast<uint4*>(o + HALF) = make_uint4(pack_bf16(c[0], c[1]), pack_bf16(c[2], c[3]), pack_bf16(c[4], c[5]), pack_bf16(c[6], c[7]));
@@ -234,42 +308,19 @@ packed_write_vec_kernel(const __nv_bfloat16* __restrict__ qkv, long long row_str
     }
     const int slot = slots ? slots[t0 + n] : -1;
     if (slot < 0 || (slot >> page_log2) >= num_pages) continue;
-    // extremes of either half's group (heads of 64: one group); a NaN shows in the sum of x * 0, an infinity as an extreme
-    float mn[2] = {a[0], c[0]}, mx[2] = {a[0], c[0]}, nan[2] = {0.f, 0.f};
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      mn[0] = fminf(mn[0], a[j]); mx[0] = fmaxf(mx[0], a[j]); nan[0] = fmaf(a[j], 0.f, nan[0]);
-      mn[1] = fminf(mn[1], c[j]); mx[1] = fmaxf(mx[1], c[j]); nan[1] = fmaf(c[j], 0.f, nan[1]);
-    }
-    if (D == 64) { mn[0] = fminf(mn[0], mn[1]); mx[0] = fmaxf(mx[0], mx[1]); nan[0] += nan[1]; }
-    const unsigned mates = ((1u << LANES) - 1) << ((threadIdx.x & 31) & ~(LANES - 1));
-    PackCoder k[2];
-#pragma unroll
-    for (int g = 0; g < D / 64; ++g) {
-#pragma unroll
-      for (int o = 1; o < LANES; o <<= 1) {
-        mn[g] = fminf(mn[g], __shfl_xor_sync(mates, mn[g], o));
-        mx[g] = fmaxf(mx[g], __shfl_xor_sync(mates, mx[g], o));
-      }
-      const bool bad = __any_sync(mates, nan[g] != 0.f) || !(mx[g] - mx[g] == 0.f) || !(mn[g] - mn[g] == 0.f);
-      k[g].set(mn[g], mx[g], bad, BITS);
-    }
-    if (D == 64) k[1] = k[0];
     const int which = h >= nh + nkv, kvh = h - nh - which * nkv, place = slot & (P - 1);
     unsigned char* block = pages + ((size_t)(slot >> page_log2) * nkv + kvh) * r.page_bytes();
-    unsigned char* o = block + r.codes(which, place) + p * BITS / 8;
-    const uint2 c0 = codes8<BITS>(k[0], a), c1 = codes8<BITS>(k[1], c);
-    if (BITS == 4) {
-      *reinterpret_cast<unsigned*>(o) = c0.x;
-      *reinterpret_cast<unsigned*>(o + HALF * BITS / 8) = c1.x;
+    if (inv_freq && !which) {
+      double x[8], y[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const double u = a[j], v = c[j], co = cs[n][0][p + j], si = cs[n][1][p + j];
+        x[j] = u * co - v * si;
+        y[j] = u * si + v * co;
+      }
+      store_head<D, BITS, double>(x, y, p, block, r, which, place);
     } else {
-      *reinterpret_cast<uint2*>(o) = c0;
-      *reinterpret_cast<uint2*>(o + HALF * BITS / 8) = c1;
-    }
-    if (p == 0) {
-      unsigned* q = reinterpret_cast<unsigned*>(block + r.pairs(which, place));
-      if (D == 128) *reinterpret_cast<uint2*>(q) = make_uint2(k[0].pair, k[1].pair);
-      else *q = k[0].pair;
+      store_head<D, BITS, float>(a, c, p, block, r, which, place);
     }
   }
 }
@@ -498,8 +549,7 @@ extern "C" int gg_packed_write(const void* qkv, long long row_stride, int act_dt
   }
   const dim3 grid(T, (nh + 2 * nkv + PACK_WARPS - 1) / PACK_WARPS), block(PACK_WARPS * 32);
   GG_REQUIRE(grid.y <= 65535, "packed_write: too many heads");
-  const int esize = act_dtype == GG_F32 ? 8 : 4;
-  const size_t smem = (size_t)(rot + PACK_WARPS * d) * esize;
+  const size_t smem = (size_t)(rot + PACK_WARPS * d) * sizeof(double);
   if (act_dtype == GG_F32)
     gg_launch(packed_write_kernel<float>, grid, block, smem, stream, (const float*)qkv, row_stride, positions, slots, inv_freq, mag,
               (unsigned char*)pages, num_pages, (float*)q_out, q_stride, nh, nkv, d, rot, page_size, bits, interleaved, early);
