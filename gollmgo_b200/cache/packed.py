@@ -74,7 +74,7 @@ class PackedKV:
                window: int = 0, softcap: float = 0.0, sink=None, slopes=None, temperature=None, cu_q_lens=None, seqs=None,
                out: Optional[torch.Tensor] = None, early: bool = False) -> torch.Tensor:
         """Attention of single tokens, each the last of its sequence's context_lens[b] stored ones: q [n, heads, head size]
-        (row i of sequence i; with ``seqs`` token i belongs to sequence seqs[i], below 0: padding, and with ``cu_q_lens``
+        (row i of sequence i; with ``seqs`` token i belongs to sequence seqs[i], none of the tables': padding, and with ``cu_q_lens``
         its row is cu_q_lens[sequence]).  ``max_context``: no context is expected to be longer (the work is spread by it).
         The options are those of the attention layer; a token with no key in sight gives zeros.  ``early``: block tables
         and index lists are not the output of the kernel ahead on the stream, and may be read while it runs."""

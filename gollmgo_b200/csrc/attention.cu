@@ -241,11 +241,13 @@ __global__ void __launch_bounds__(ATT_THREADS) attn_decode_kernel(AttnArgs a) {
   __shared__ float scale_s[ATT_BQ];
   pdl_wait();
   const int G = a.nh / a.nkv, gchunks = (G + ATT_BQ - 1) / ATT_BQ;
-  const int b = a.dec_seqs ? a.dec_seqs[blockIdx.x] : (int)blockIdx.x;
+  int b = a.dec_seqs ? a.dec_seqs[blockIdx.x] : (int)blockIdx.x;
+  if (PACKED && b >= a.num_seqs) b = -1;
   const int kvh = blockIdx.y / gchunks, g0 = (blockIdx.y % gchunks) * ATT_BQ;
   const int split = blockIdx.z, S = a.num_splits;
   const int nrows = min(ATT_BQ, G - g0);
-  const int ctx = b >= 0 ? a.context_lens[b] : 0;      // b < 0: padding of a captured batch
+  int ctx = b >= 0 ? a.context_lens[b] : 0;            // b < 0: padding of a captured batch
+  if (PACKED) ctx = (int)min((long long)ctx, (long long)a.bt_stride * a.page_size);
   const int t = b >= 0 ? (a.cu_q_lens ? a.cu_q_lens[b] : b) : 0;
   int lo0 = a.window > 0 ? max(0, ctx - a.window) : 0;
   if (a.chunk > 0 && ctx > 0) lo0 = max(lo0, ((ctx - 1) / a.chunk) * a.chunk);
@@ -298,7 +300,7 @@ __global__ void attn_merge_kernel(AttnArgs a) {
   pdl_trigger();
   pdl_wait();
   const int b = a.dec_seqs ? a.dec_seqs[blockIdx.x] : (int)blockIdx.x;
-  if (b < 0) return;
+  if (b < 0 || (a.packed_bits && b >= a.num_seqs)) return;
   const int h = blockIdx.y, S = a.num_splits, d = a.dv > 0 ? a.dv : a.d;
   const int t = a.cu_q_lens ? a.cu_q_lens[b] : b;
   const size_t row0 = ((size_t)blockIdx.x * a.nh + h) * S;

@@ -49,6 +49,7 @@ struct AttnArgs {
   // a packed cache (packed_kv.cuh; the general decode kernel with PACKED): kcache is then its pages, vcache unused
   int packed_bits;          // 4 or 8; 0 = keys and values as they are
   int num_pages;            // pages of a packed cache: an id outside reads as a page that was given back
+  int num_seqs;             // rows of its block tables: a dec_seqs entry outside is padding
 };
 
 // the factor on the query at position p (1 where the layer has none)

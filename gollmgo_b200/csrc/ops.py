@@ -1541,8 +1541,8 @@ _I, _L, _F, _P = ctypes.c_int, ctypes.c_longlong, ctypes.c_float, ctypes.c_void_
 _PACKED_TYPES = {
     "gg_packed_write": [_P, _L, _I, _P, _P, _P, _F, _P, _I, _P, _L, _I, _I, _I, _I, _I, _I, _I, _I, _I, _P],
     "gg_packed_read": [_P, _I, _P, _I, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _P],
-    "gg_packed_decode": [_P, _L, _I, _P, _I, _P, _I, _P, _P, _P, _I, _I, _P, _P, _P, _I, _I, _I, _I, _I, _I, _F, _F, _P, _P, _F, _F, _P],
-    "gg_packed_decode_mma": [_P, _L, _P, _I, _P, _I, _P, _P, _P, _I, _I, _P, _L, _P, _I, _I, _I, _I, _I, _I, _F, _F, _P, _P, _F, _F, _P, _I, _P],
+    "gg_packed_decode": [_P, _L, _I, _P, _I, _P, _I, _I, _P, _P, _P, _I, _I, _P, _P, _P, _I, _I, _I, _I, _I, _I, _F, _F, _P, _P, _F, _F, _P],
+    "gg_packed_decode_mma": [_P, _L, _P, _I, _P, _I, _I, _P, _P, _P, _I, _I, _P, _L, _P, _I, _I, _I, _I, _I, _I, _F, _F, _P, _P, _F, _F, _P, _I, _P],
     "gg_packed_decode_scratch": [_I, _I, _I, _I, _I, _I, _I],
     "gg_packed_unfold": [_P, _I, _P, _I, _P, _P, _I, _P, _P, _I, _I, _I, _P, _I, _I, _P, _P, _I, _I, _P, _P, _I, _I, _I, _I, _I, _I, _P],
 }
@@ -1675,7 +1675,7 @@ def packed_decode(q: torch.Tensor, pages: torch.Tensor, tables: torch.Tensor, cu
     if part_o.numel() < n * nh * splits * d or part_ml.numel() < n * nh * splits * 2:
         raise KernelError("packed_decode: scratch too small")
     coef, every = temperature or (0.0, 0.0)
-    _check(_packed("gg_packed_decode")(q.data_ptr(), stride, dtype_code(q.dtype), pages.data_ptr(), pages.shape[0], tables.data_ptr(), width,
+    _check(_packed("gg_packed_decode")(q.data_ptr(), stride, dtype_code(q.dtype), pages.data_ptr(), pages.shape[0], tables.data_ptr(), width, B,
                                        _at(cu_q_lens), context_lens.data_ptr(), _at(seqs), n, splits, part_o.data_ptr(), part_ml.data_ptr(),
                                        out.data_ptr(), nh, nkv, d, page_size, bits, window, scale, softcap, _at(sink), _at(slopes), coef,
                                        every, stream), 2)
@@ -1714,7 +1714,7 @@ def packed_decode_mma(q: torch.Tensor, pages: torch.Tensor, tables: torch.Tensor
         raise KernelError("packed_decode: the scratch is contiguous float32")
     coef, every = temperature or (0.0, 0.0)
     tc_launched = True
-    _check(_packed("gg_packed_decode_mma")(q.data_ptr(), stride, pages.data_ptr(), pages.shape[0], tables.data_ptr(), width, _at(cu_q_lens),
+    _check(_packed("gg_packed_decode_mma")(q.data_ptr(), stride, pages.data_ptr(), pages.shape[0], tables.data_ptr(), width, B, _at(cu_q_lens),
                                            context_lens.data_ptr(), _at(seqs), n, max_context, scratch.data_ptr(), scratch.numel(),
                                            out.data_ptr(), nh, nkv, d, page_size, bits, window, scale, softcap, _at(sink), _at(slopes),
                                            coef, every, tc_status(q.device).data_ptr(), early, stream), 2)

@@ -47,7 +47,7 @@ struct PackedDecode {
   const int* cu_q_lens;
   const int* context_lens;
   const int* seqs;
-  int n;
+  int n, B;                        // tokens; sequences (rows of the tables): a token of none is padding
   __nv_bfloat16* out;
   int nh, nkv, group, chunks;      // heads of a kv head, in chunks of 8 NT
   int page_log2, page_bytes;
@@ -83,6 +83,11 @@ __device__ __forceinline__ void bulk_load(unsigned dst, const void* src, unsigne
 template <typename T> __device__ __forceinline__ T ld(const unsigned char* p) { return *reinterpret_cast<const T*>(p); }
 __device__ __forceinline__ float power_of_two(int e) { return __uint_as_float((unsigned)(e + 127) << 23); }   // -126 <= e <= 127
 
+// The sequence of token i, or -1.
+__device__ __forceinline__ int sequence_of(const PackedDecode& a, int i) {
+  const int b = a.seqs ? a.seqs[i] : i;
+  return b < a.B ? b : -1;
+}
 // Tokens of sequence b that can be in sight: a context that its block table cannot hold is cut there.
 __device__ __forceinline__ int context_of(const PackedDecode& a, int b) {
   const long long most = (long long)a.bt_stride << a.page_log2;
@@ -102,7 +107,7 @@ __device__ __forceinline__ void scan_tiles(const PackedDecode& a, int pairs, int
     const int i = i0 + threadIdx.x;
     int mine = 0;
     if (i < a.n) {
-      const int c = context_of(a, a.seqs ? a.seqs[i] : i), lo = first_key(a, c);
+      const int c = context_of(a, sequence_of(a, i)), lo = first_key(a, c);
       contexts[i] = c;
       mine = c > lo ? ((c + TILE - 1) / TILE - lo / TILE) * pairs : 0;
     }
@@ -215,7 +220,7 @@ __global__ void __launch_bounds__(PdSizes<D, BITS, NT>::THREADS, 1) packed_decod
   const int total = prefix[a.n];
   auto zeros = [&]() {                             // tokens without a key in sight, spread over the blocks
     for (int i = blockIdx.x; i < a.n; i += a.blocks) {
-      const int b = a.seqs ? a.seqs[i] : i;
+      const int b = sequence_of(a, i);
       if (contexts[i] > 0 || b < 0) continue;
       __nv_bfloat162* o = reinterpret_cast<__nv_bfloat162*>(a.out + (size_t)(a.cu_q_lens ? a.cu_q_lens[b] : b) * a.nh * D);
       for (int e = tid; e < a.nh * D / 2; e += Z::THREADS) o[e] = __floats2bfloat162_rn(0.f, 0.f);
@@ -902,7 +907,7 @@ static int pd_launch(const PackedDecode& a, int smem, bool join, cudaStream_t st
   return gg_check_launch("packed_join");
 }
 
-extern "C" int gg_packed_decode_mma(const void* q, long long q_stride, const void* pages, int num_pages, const int* tables, int bt_stride,
+extern "C" int gg_packed_decode_mma(const void* q, long long q_stride, const void* pages, int num_pages, const int* tables, int bt_stride, int B,
                                     const int* cu_q_lens, const int* context_lens, const int* seqs, int n, int max_context, float* scratch,
                                     long long scratch_floats, void* out, int nh, int nkv, int d, int page_size, int bits, int window,
                                     float scale, float softcap, const float* sink, const float* slopes, float temp_coef, float temp_every,
@@ -913,12 +918,14 @@ extern "C" int gg_packed_decode_mma(const void* q, long long q_stride, const voi
              "packed_decode: bad sizes n=%d pages=%d table width=%d window=%d", n, num_pages, bt_stride, window);
   GG_REQUIRE(((size_t)q % 16) == 0 && q_stride % 8 == 0 && ((size_t)out % 16) == 0 && ((size_t)pages % 16) == 0,
              "packed_decode: q, its rows, the output and the pages must start on 16 bytes");
+  GG_REQUIRE(B >= 0 && (seqs || n <= B), "packed_decode: %d tokens of %d sequences", n, B);
+  GG_REQUIRE((long long)n * nh * (((long long)bt_stride * page_size + 15) / 16) < (1LL << 31), "packed_decode: block tables of %d pages for %d tokens are too large for one launch", bt_stride, n);
   if (n == 0) return GG_OK;
   const PdShape s = pd_shape(n, nh, nkv, d, bits, max_context, window);
   GG_REQUIRE(scratch && ((size_t)scratch % 16) == 0 && scratch_floats >= s.part_floats + 4LL * s.blocks, "packed_decode: scratch too small");
   PackedDecode a = {};
   a.q = (const __nv_bfloat16*)q; a.q_stride = q_stride; a.pages = (const unsigned char*)pages; a.num_pages = num_pages;
-  a.tables = tables; a.bt_stride = bt_stride; a.cu_q_lens = cu_q_lens; a.context_lens = context_lens; a.seqs = seqs; a.n = n;
+  a.tables = tables; a.bt_stride = bt_stride; a.cu_q_lens = cu_q_lens; a.context_lens = context_lens; a.seqs = seqs; a.n = n; a.B = B;
   a.out = (__nv_bfloat16*)out; a.nh = nh; a.nkv = nkv; a.group = nh / nkv; a.chunks = s.chunks;
   a.page_log2 = 31 - __builtin_clz(page_size);
   a.page_bytes = PackedRows(bits, d, page_size).page_bytes();

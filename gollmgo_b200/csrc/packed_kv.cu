@@ -159,53 +159,40 @@ __device__ __forceinline__ uint2 codes8(const PackCoder& k, const float* x) {
   return k.pair == 0x7fff7fffu ? make_uint2(0u, 0u) : make_uint2(w[0], w[1]);
 }
 
-// The same for float64 values: the quotient in float32, and near a border the remainder in float64.
+// The same for float64 values: a rotated key's float64 quotient lies on the wrong side of a border once in 10^12, and 1.5 * 2^52
+// leaves the whole number in the low word without a conversion (those between the widths take eight clocks a warp).
 template <int BITS>
 __device__ __forceinline__ uint2 codes8(const PackCoder& k, const double* x) {
-  constexpr float MOST = (1 << BITS) - 1, NEAR = 0.5f - MOST * 0x1p-20f;
-  constexpr float MAGIC = 12582912.f;
-  // (differences of halves stay inside float32's range; a scale whose reciprocal does not is brought up first)
-  const double offset = k.offset, scale = k.scale;
-  const float up = scale < 0x1p-60 ? 0x1p64f : 1.f, inv = scale > 0.0 ? 1.f / ((float)(0.5 * scale) * up) : 0.f;
-  unsigned q[8];
-  float far = 0.f;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const float t = ((float)(0.5 * (x[i] - offset)) * up) * inv, m = t + MAGIC;
-    far = fmaxf(far, fabsf(t - (m - MAGIC)));
-    q[i] = __float_as_uint(m);
-  }
-  if (far >= NEAR) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const double rest = fma(-(double)(__uint_as_float(q[i]) - MAGIC), scale, x[i] - offset), border = 0.5 * scale;
-      const bool odd = q[i] & 1u;
-      q[i] += (rest > border || (rest == border && odd)) ? 1u : (rest < -border || (rest == -border && odd)) ? ~0u : 0u;
-    }
-  }
+  const double inv = k.scale > 0.0 ? 1.0 / k.scale : 0.0, shift = -k.offset * inv;
   unsigned w[2] = {0u, 0u};
 #pragma unroll
-  for (int i = 0; i < 8; ++i) w[i * BITS / 32] |= (q[i] & ((1u << BITS) - 1)) << (i * BITS & 31);
+  for (int i = 0; i < 8; ++i)
+    w[i * BITS / 32] |= ((unsigned)__double2loint(fma(x[i], inv, shift) + 6755399441055744.0) & ((1u << BITS) - 1)) << (i * BITS & 31);
   return k.pair == 0x7fff7fffu ? make_uint2(0u, 0u) : make_uint2(w[0], w[1]);
+}
+// A bfloat16 value (as a float) as float64: the exponent moved over, in integer arithmetic.
+__device__ __forceinline__ double widen(float x) {
+  const unsigned b = __float_as_uint(x), e = b & 0x7f800000u;
+  if (e == 0u || e == 0x7f800000u) return (double)x;                 // zeros, subnormal numbers, infinities and NaN
+  return __hiloint2double((int)((b & 0x80000000u) | (((b & 0x7fffffffu) >> 3) + 0x38000000u)), 0);
 }
 
 // One head of one token, channels p .. p + 7 (a) and D / 2 + p .. (c) in each of the head's lanes: the group's extremes, its pair, the codes.
 __device__ __forceinline__ float least(float a, float b) { return fminf(a, b); }
 __device__ __forceinline__ float most(float a, float b) { return fmaxf(a, b); }
-__device__ __forceinline__ double least(double a, double b) { return fmin(a, b); }
-__device__ __forceinline__ double most(double a, double b) { return fmax(a, b); }
+__device__ __forceinline__ double least(double a, double b) { return a < b ? a : b; }
+__device__ __forceinline__ double most(double a, double b) { return a < b ? b : a; }
 template <int D, int BITS, typename TC>
-__device__ __forceinline__ void store_head(const TC* a, const TC* c, int p, unsigned char* block, const PackedRows& r, int which, int place) {
+__device__ __forceinline__ void store_head(const TC* a, const TC* c, bool nan0, bool nan1, int p, unsigned char* block, const PackedRows& r, int which, int place) {
   constexpr int HALF = D / 2, LANES = D / 16;
-  // (heads of 64: one group)  A NaN shows in the sum of x * 0, an infinity as an extreme.
+  // (heads of 64: one group)
   TC mn[2] = {a[0], c[0]}, mx[2] = {a[0], c[0]};
-  float nan[2] = {0.f, 0.f};
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    mn[0] = least(mn[0], a[j]); mx[0] = most(mx[0], a[j]); nan[0] = fmaf((float)a[j], 0.f, nan[0]);
-    mn[1] = least(mn[1], c[j]); mx[1] = most(mx[1], c[j]); nan[1] = fmaf((float)c[j], 0.f, nan[1]);
+  for (int j = 1; j < 8; ++j) {
+    mn[0] = least(mn[0], a[j]); mx[0] = most(mx[0], a[j]);
+    mn[1] = least(mn[1], c[j]); mx[1] = most(mx[1], c[j]);
   }
-  if (D == 64) { mn[0] = least(mn[0], mn[1]); mx[0] = most(mx[0], mx[1]); nan[0] += nan[1]; }
+  if (D == 64) { mn[0] = least(mn[0], mn[1]); mx[0] = most(mx[0], mx[1]); }
   const unsigned mates = ((1u << LANES) - 1) << ((threadIdx.x & 31) & ~(LANES - 1));
   PackCoder k[2];
 #pragma unroll
@@ -215,7 +202,7 @@ __device__ __forceinline__ void store_head(const TC* a, const TC* c, int p, unsi
       mn[g] = least(mn[g], __shfl_xor_sync(mates, mn[g], o));
       mx[g] = most(mx[g], __shfl_xor_sync(mates, mx[g], o));
     }
-    const bool bad = __any_sync(mates, nan[g] != 0.f) || !(mx[g] - mx[g] == 0) || !(mn[g] - mn[g] == 0);
+    const bool bad = __any_sync(mates, g ? nan1 : nan0) || !(mx[g] - mx[g] == 0) || !(mn[g] - mn[g] == 0);
     k[g].set(mn[g], mx[g], bad, BITS);
   }
   if (D == 64) k[1] = k[0];
@@ -310,17 +297,23 @@ packed_write_vec_kernel(const __nv_bfloat16* __restrict__ qkv, long long row_str
     if (slot < 0 || (slot >> page_log2) >= num_pages) continue;
     const int which = h >= nh + nkv, kvh = h - nh - which * nkv, place = slot & (P - 1);
     unsigned char* block = pages + ((size_t)(slot >> page_log2) * nkv + kvh) * r.page_bytes();
-    if (inv_freq && !which) {
+    // a NaN (or infinity) shows in the sum of x * 0; turned, it is in both halves
+    float bad0 = 0.f, bad1 = 0.f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) { bad0 = fmaf(a[j], 0.f, bad0); bad1 = fmaf(c[j], 0.f, bad1); }
+    const bool turned = inv_freq && !which, one = turned || D == 64;
+    const bool nan0 = bad0 != 0.f || (one && bad1 != 0.f), nan1 = bad1 != 0.f || (one && bad0 != 0.f);
+    if (turned) {
       double x[8], y[8];
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        const double u = a[j], v = c[j], co = cs[n][0][p + j], si = cs[n][1][p + j];
+        const double u = widen(a[j]), v = widen(c[j]), co = cs[n][0][p + j], si = cs[n][1][p + j];
         x[j] = u * co - v * si;
         y[j] = u * si + v * co;
       }
-      store_head<D, BITS, double>(x, y, p, block, r, which, place);
+      store_head<D, BITS, double>(x, y, nan0, nan1, p, block, r, which, place);
     } else {
-      store_head<D, BITS, float>(a, c, p, block, r, which, place);
+      store_head<D, BITS, float>(a, c, nan0, nan1, p, block, r, which, place);
     }
   }
 }
@@ -542,7 +535,8 @@ extern "C" int gg_packed_write(const void* qkv, long long row_stride, int act_dt
                                             stream, (const __nv_bfloat16*)qkv, row_stride, positions, slots, rot ? inv_freq : nullptr, mag, \
                                             (unsigned char*)pages, num_pages, (__nv_bfloat16*)q_out, q_stride, T, nh, nkv, \
                                             31 - __builtin_clz(page_size), early)
-#define WRITE_VEC(D, BITS) do { if (T >= 1024) WRITE_VEC_T(D, BITS, 4); else WRITE_VEC_T(D, BITS, 1); } while (0)
+    // tokens a block: us for 1 / 2 / 4 at 200, 512 and 1024 tokens of 32 + 2 x 8 heads of 128: 4.3 5.0 7.7, 8.4 6.6 8.9, 16.3 11.8 9.6
+#define WRITE_VEC(D, BITS) do { if (T >= 888) WRITE_VEC_T(D, BITS, 4); else if (T >= 296) WRITE_VEC_T(D, BITS, 2); else WRITE_VEC_T(D, BITS, 1); } while (0)
     if (d == 64) { if (bits == 4) WRITE_VEC(64, 4); else WRITE_VEC(64, 8); }
     else { if (bits == 4) WRITE_VEC(128, 4); else WRITE_VEC(128, 8); }
     return gg_check_launch("packed_write");
@@ -627,18 +621,18 @@ static int check_heads(const char* who, int nh, int nkv, int bt_stride, int wind
 
 // Single tokens on the general kernel.  part_o float[n * nh * splits * d], part_ml float[n * nh * splits * 2].
 extern "C" int gg_packed_decode(const void* q, long long q_stride, int act_dtype, const void* pages, int num_pages, const int* tables,
-                                int bt_stride, const int* cu_q_lens, const int* context_lens, const int* seqs, int n, int splits,
+                                int bt_stride, int B, const int* cu_q_lens, const int* context_lens, const int* seqs, int n, int splits,
                                 float* part_o, float* part_ml, void* out, int nh, int nkv, int d, int page_size, int bits, int window,
                                 float scale, float softcap, const float* sink, const float* slopes, float temp_coef, float temp_every,
                                 cudaStream_t stream) {
   int rc = check_packed("packed_decode", pages, num_pages, nkv, d, page_size, bits);
   if (!rc) rc = check_heads("packed_decode", nh, nkv, bt_stride, window);
   if (rc) return rc;
-  GG_REQUIRE(n >= 0 && splits >= 1 && splits <= 65535, "packed_decode: bad n %d or splits %d", n, splits);
+  GG_REQUIRE(n >= 0 && B >= 0 && (seqs || n <= B) && splits >= 1 && splits <= 65535, "packed_decode: bad n %d of %d or splits %d", n, B, splits);
   if (n == 0) return GG_OK;
   AttnArgs a = packed_args(q, q_stride, pages, num_pages, tables, bt_stride, cu_q_lens, context_lens, out, nh, nkv, d, page_size, bits, window,
                            scale, softcap, sink, slopes, temp_coef, temp_every);
-  a.dec_seqs = seqs; a.num_splits = splits; a.part_o = part_o; a.part_ml = part_ml;
+  a.num_seqs = B; a.dec_seqs = seqs; a.num_splits = splits; a.part_o = part_o; a.part_ml = part_ml;
   rc = attn_decode_general(a, act_dtype, n, stream);
   return rc ? rc : attn_merge_launch(a, act_dtype, n, stream);
 }

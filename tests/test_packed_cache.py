@@ -260,9 +260,11 @@ def errors_of(dtype, q, keys, scale):
 
 
 @pytest.mark.parametrize("bits", [4, 8])
-def test_decode_of_listed_sequences(bits):
-    """Tokens of some of a step's sequences: seqs with padding, rows through cu_q_lens, the other rows left as they were."""
-    nh, nkv, d, page = 8, 2, 128, 16
+@pytest.mark.parametrize("page", [16, 8])
+def test_decode_of_listed_sequences(bits, page):
+    """Tokens of some of a step's sequences: seqs with padding, rows through cu_q_lens, the other rows left as they were (pages of 16:
+    on the tensor cores, of 8: the general kernel).  A context longer than its block table is cut there."""
+    nh, nkv, d = 8, 2, 128
     lens = [40, 7, 90, 33]
     pool = Pool(lens, nkv, d, page, bits, seed=1)
     g = torch.Generator().manual_seed(2)
@@ -270,7 +272,7 @@ def test_decode_of_listed_sequences(bits):
     wide = torch.randn(10, (nh + 2 * nkv) * d, generator=g).to(BF16).cuda()
     q = wide[:, :nh * d].unflatten(1, (nh, d))
     out = torch.full((10, nh, d), 3.0, dtype=BF16, device="cuda")
-    seqs = torch.tensor([3, -1, 1], dtype=torch.int32).cuda()
+    seqs = torch.tensor([3, -1, 1, 4], dtype=torch.int32).cuda()           # below 0 and beyond the tables: padding
     pool.kv.decode(q, pool.tables.cuda(), torch.tensor(lens, dtype=torch.int32).cuda(), 90, d ** -0.5, cu_q_lens=cu.cuda(), seqs=seqs, out=out)
     for b in (1, 3):
         row = int(cu[b])
@@ -279,6 +281,10 @@ def test_decode_of_listed_sequences(bits):
         assert ((out[row].cpu().double() - ref).abs() <= bound(ref, [pool.values[b]], BF16, *e)).all()
     others = [r for r in range(10) if r not in (3, 9)]
     assert (out[others] == 3.0).all()
+    held = -(-90 // page) * page                       # sequence 2 with a table of just its pages and a context that says more
+    far = pool.kv.decode(q[4:5], pool.tables[2:3, :held // page].contiguous().cuda(), torch.tensor([10 ** 6], dtype=torch.int32).cuda(), 90, d ** -0.5)
+    same = pool.kv.decode(q[4:5], pool.tables[2:3].cuda(), torch.tensor([held], dtype=torch.int32).cuda(), 90, d ** -0.5)
+    assert torch.equal(far.isnan(), same.isnan()) and torch.equal(far.nan_to_num(), same.nan_to_num())
 
 
 def prompt_errors(dtype, q, keys, scale):
