@@ -1542,7 +1542,7 @@ _PACKED_TYPES = {
     "gg_packed_write": [_P, _L, _I, _P, _P, _P, _F, _P, _I, _P, _L, _I, _I, _I, _I, _I, _I, _I, _I, _I, _P],
     "gg_packed_read": [_P, _I, _P, _I, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _P],
     "gg_packed_decode": [_P, _L, _I, _P, _I, _P, _I, _I, _P, _P, _P, _I, _I, _P, _P, _P, _I, _I, _I, _I, _I, _I, _F, _F, _P, _P, _F, _F, _P],
-    "gg_packed_decode_mma": [_P, _L, _P, _I, _P, _I, _I, _P, _P, _P, _I, _I, _P, _L, _P, _I, _I, _I, _I, _I, _I, _F, _F, _P, _P, _F, _F, _P, _I, _P],
+    "gg_packed_decode_mma": [_P, _L, _P, _I, _P, _I, _I, _P, _P, _P, _I, _I, _P, _L, _P, _I, _I, _I, _I, _I, _I, _F, _F, _P, _P, _F, _F, _I, _P],
     "gg_packed_decode_scratch": [_I, _I, _I, _I, _I, _I, _I],
     "gg_packed_unfold": [_P, _I, _P, _I, _P, _P, _I, _P, _P, _I, _I, _I, _P, _I, _I, _P, _P, _I, _I, _P, _P, _I, _I, _I, _I, _I, _I, _P],
 }
@@ -1681,7 +1681,7 @@ def packed_decode(q: torch.Tensor, pages: torch.Tensor, tables: torch.Tensor, cu
                                        every, stream), 2)
 
 
-PACKED_DECODE_TOKENS = 1024      # tokens that packed_decode_mma takes in one launch
+PACKED_DECODE_TOKENS = 512      # tokens that packed_decode_mma takes in one launch
 
 
 def packed_decode_mma_ok(dtype: torch.dtype, d: int, page_size: int) -> bool:
@@ -1703,7 +1703,6 @@ def packed_decode_mma(q: torch.Tensor, pages: torch.Tensor, tables: torch.Tensor
     """packed_decode on the tensor cores (packed_decode_mma_ok).  ``scratch`` float32 of packed_decode_scratch for the same
     sizes; contexts longer than ``max_context`` are right too, only the work was split for shorter ones.  ``early``: the index
     lists and block tables may be read before the kernel ahead of this one has finished (they are not its output)."""
-    global tc_launched
     stream = _stream_of("packed_decode", q, pages, tables, cu_q_lens, context_lens, seqs, scratch, out, sink, slopes)
     stride = _packed_q("packed_decode", q, out, nh, d)
     if sink is not None or slopes is not None:
@@ -1713,11 +1712,10 @@ def packed_decode_mma(q: torch.Tensor, pages: torch.Tensor, tables: torch.Tensor
     if scratch.dtype != torch.float32 or not scratch.is_contiguous():
         raise KernelError("packed_decode: the scratch is contiguous float32")
     coef, every = temperature or (0.0, 0.0)
-    tc_launched = True
     _check(_packed("gg_packed_decode_mma")(q.data_ptr(), stride, pages.data_ptr(), pages.shape[0], tables.data_ptr(), width, B, _at(cu_q_lens),
                                            context_lens.data_ptr(), _at(seqs), n, max_context, scratch.data_ptr(), scratch.numel(),
                                            out.data_ptr(), nh, nkv, d, page_size, bits, window, scale, softcap, _at(sink), _at(slopes),
-                                           coef, every, tc_status(q.device).data_ptr(), early, stream), 2)
+                                           coef, every, early, stream), 2)
 
 
 @contextlib.contextmanager

@@ -16,21 +16,20 @@
 // channels of four keys for the output, whose pairs (key, key) are put together by byte permutation.  The weights pass from the
 // score layout to the B operand by a register transpose of 8 x 8.
 //
-// Bytes are what bounds it (4.5 or 8.5 bits a channel), closely followed by the masks that make operands of codes.  The work is
-// cut into equal ranges of tiles over all (token, kv head) pairs, a range for each warp.  A warp brings its tiles by bulk copies
-// (one per page and kv head) into a ring of its own, the pages of its next 16 or 32 tiles found by one lane each, and shares
+// Bytes are what bounds it (4.5 or 8.5 bits a channel), closely followed by the instructions that make operands of codes.  The
+// work is cut into equal ranges of tiles over all (token, kv head) pairs, a range for each warp.  A warp brings its tiles into a
+// ring of its own by 16-byte asynchronous copies (bulk copies, one a page, were started by one lane after the other with more
+// instructions than ten copies of all lanes take), the pages of its next 16 or 32 tiles found by one lane each, and shares
 // nothing until it is done: a pair that lies inside its range is written out, parts of pairs are joined inside the block and
 // then, by a second kernel, between blocks.
 #include "attention_common.cuh"
 #include "packed_kv.cuh"
-#include "tc_common.cuh"
 
-#include <atomic>
 #include <cuda_fp16.h>
 
-#define PD_MAX_TOKENS 1024         // tokens of one launch
-#define PD_STATUS 71               // reported where a copy did not arrive
-#define PD_STAGES 8                // most stages of a ring
+#include <atomic>
+
+#define PD_MAX_TOKENS 512          // tokens of one launch
 #define PD_EACH 4                  // tiles of a block below which fewer blocks are launched
 #define PD_ALONE 2                 // tiles a warp up to which a single token's pairs get a block each
 #define PD_SMEM (222 * 1024)       // dynamic shared memory: of 227 KB, with what a block has besides
@@ -59,8 +58,7 @@ struct PackedDecode {
   float* part;                     // parts of pairs, [8 NT * D + 2 * 8 NT] each (outputs, then max and sum of each head): two of every block,
                                    // then one of every warp
   int4* cut;                       // of each block: what the second kernel joins (see there)
-  int blocks, stages, early;       // early: the lists are not the output of the kernel ahead
-  int* status;
+  int blocks, early;       // early: the lists are not the output of the kernel ahead
 };
 
 __device__ __forceinline__ void mma_f16(float* c, unsigned a0, unsigned a1, unsigned a2, unsigned a3, unsigned b0, unsigned b1) {
@@ -75,10 +73,6 @@ __device__ __forceinline__ unsigned transpose8(unsigned x) {
 __device__ __forceinline__ unsigned half_pair(float lo, float hi) {
   const __half2 h = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<const unsigned*>(&h);
-}
-__device__ __forceinline__ void bulk_load(unsigned dst, const void* src, unsigned bytes, unsigned bar) {
-  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
-               ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
 }
 template <typename T> __device__ __forceinline__ T ld(const unsigned char* p) { return *reinterpret_cast<const T*>(p); }
 __device__ __forceinline__ float power_of_two(int e) { return __uint_as_float((unsigned)(e + 127) << 23); }   // -126 <= e <= 127
@@ -180,16 +174,16 @@ template <int TILE> struct TileCursor {
   }
 };
 
-// Shapes of the kernel: warps of a block (16 at 128 registers a thread, or 8), keys of a tile.  Twice the heads take twice the
-// registers, so half the warps; a
-// tile is about the same bytes in 4 and in 8 bits.
+// Shapes of the kernel: warps of a block (16 at 128 registers a thread, or 8), keys of a tile, stages of a ring.  Twice the heads
+// take twice the registers, so half the warps; a tile is about the same bytes in 4 and in 8 bits; as many stages as shared
+// memory holds beside the lists of the most tokens.
 template <int D, int BITS, int NT> struct PdSizes {
   static constexpr int WARPS = NT == 1 ? 16 : 8, TILE = BITS == 4 ? 32 : 16, THREADS = WARPS * 32;
   static constexpr int GR = D / 64, ROW = D * BITS / 8, HEADS = 8 * NT, PART = HEADS * D + 2 * HEADS;      // PART in floats
   static constexpr int STAGE = 2 * TILE * (ROW + 4 * GR);
-  static constexpr int smem(int stages, int n) {
-    return WARPS * stages * (STAGE + 8 + 4) + (2 * n + 1) * 4;
-  }
+  static constexpr int bytes(int stages) { return WARPS * stages * (STAGE + 4) + (2 * PD_MAX_TOKENS + 1) * 4; }
+  static constexpr int most(int stages) { return stages < 8 && bytes(stages + 1) <= PD_SMEM ? most(stages + 1) : stages; }
+  static constexpr int STAGES = most(2), SMEM = bytes(most(2));
 };
 
 template <int D, int BITS, int NT, bool OPT>
@@ -203,17 +197,15 @@ __global__ void __launch_bounds__(PdSizes<D, BITS, NT>::THREADS, 1) packed_decod
   __shared__ int4 part_pair[2 * WARPS];            // tiles and heads of that pair, its first row of the result
   __shared__ float part_top[2 * WARPS][HEADS], part_sum[2 * WARPS][HEADS], part_weight[2 * WARPS][HEADS];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
-  const int pairs = a.nkv * a.chunks, S = a.stages;
-  // shared memory: a ring per warp, its barriers, the chunks of a stage that are there, prefix, contexts
-  unsigned long long* bars = reinterpret_cast<unsigned long long*>(smem + (size_t)WARPS * S * STAGE);
-  unsigned* here = reinterpret_cast<unsigned*>(bars + WARPS * S) + warp * S;
-  int* prefix = reinterpret_cast<int*>(bars + WARPS * S) + WARPS * S;
+  const int pairs = a.nkv * a.chunks;
+  constexpr int S = Z::STAGES;
+  // shared memory: a ring per warp, the chunks of a stage that are there, prefix, contexts
+  unsigned* here = reinterpret_cast<unsigned*>(smem + (size_t)WARPS * S * STAGE) + warp * S;
+  int* prefix = reinterpret_cast<int*>(smem + (size_t)WARPS * S * STAGE) + WARPS * S;
   int* contexts = prefix + a.n + 1;
   float* parts = a.part + ((size_t)2 * a.blocks + (size_t)blockIdx.x * WARPS) * Z::PART;
-  const unsigned ring = tc_smem(smem) + warp * S * STAGE, full = tc_smem(bars + warp * S);
-  if (lane < S) mbar_init(full + 8 * lane, 1);
+  const unsigned ring = smem_u32(smem) + warp * S * STAGE;
   if (tid < 2 * WARPS) part_base[tid] = -1;
-  asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   pdl_trigger();
   if (!a.early) pdl_wait();
   scan_tiles<TILE, Z::THREADS>(a, pairs, prefix, contexts, wsum);
@@ -259,36 +251,47 @@ __global__ void __launch_bounds__(PdSizes<D, BITS, NT>::THREADS, 1) packed_decod
     if (key < ctx) id_next = a.tables[(size_t)b * a.bt_stride + (key >> a.page_log2)];
     spot_next = kv_head(a, mine.pair) << 8 | (key & ((1 << a.page_log2) - 1));
   };
-  auto ask = [&](int stage) {                      // start the copies of tile f_ask
-    if (f_ask >= w_hi) return;
-    if (f_ask == batch + (32 >> two) || f_ask == w_lo) {
-      batch = f_ask;
-      id = id_next;
-      spot = spot_next;
-      there = __ballot_sync(0xffffffffu, id >= 0 && id < a.num_pages);
-    }
-    const int k = f_ask - batch;
-    if (k == PD_STAGES) look_up(batch + (32 >> two));         // not before the first stages are on their way
-    const unsigned mask = (there >> (k << two)) & ((1u << chunks) - 1), bar = full + 8 * stage;
-    if (lane == 0) {
-      here[stage] = mask;
-      mbar_expect_tx(bar, __popc(mask) * chunk_bytes);
-    }
-    __syncwarp();
-    if ((lane >> two) == k && ((there >> lane) & 1)) {
-      const unsigned char* block = a.pages + ((size_t)id * a.nkv + (spot >> 8)) * a.page_bytes;
-      const unsigned dst = ring + stage * STAGE + (lane & (chunks - 1)) * chunk_bytes;
-      if (a.page_log2 == 4) {
-        bulk_load(dst, block, chunk_bytes, bar);
-      } else {
-        const int place = spot & 255, P = 1 << a.page_log2;
-        bulk_load(dst, block + place * ROW, chunk * ROW, bar);
-        bulk_load(dst + chunk * ROW, block + (P + place) * ROW, chunk * ROW, bar);
-        bulk_load(dst + 2 * chunk * ROW, block + 2 * P * ROW + place * GR * 4, chunk * GR * 4, bar);
-        bulk_load(dst + 2 * chunk * ROW + chunk * GR * 4, block + 2 * P * ROW + (P + place) * GR * 4, chunk * GR * 4, bar);
+  auto ask = [&](int stage) {                      // start the copies of tile f_ask; a group of copies whether there is one or not
+    if (f_ask < w_hi) {
+      if (f_ask == batch + (32 >> two) || f_ask == w_lo) {
+        batch = f_ask;
+        id = id_next;
+        spot = spot_next;
+        there = __ballot_sync(0xffffffffu, id >= 0 && id < a.num_pages);
       }
+      const int k = f_ask - batch;
+      if (k == S) look_up(batch + (32 >> two));    // not before the first stages are on their way
+      const unsigned mask = (there >> (k << two)) & ((1u << chunks) - 1);
+      const int spot_k = __shfl_sync(0xffffffffu, spot, k << two);
+      const unsigned char* head = a.pages + (size_t)(spot_k >> 8) * a.page_bytes;
+      const size_t page = (size_t)a.nkv * a.page_bytes;
+      if (lane == 0) here[stage] = mask;
+      const unsigned dst = ring + stage * STAGE + lane * 16;
+      if (a.page_log2 == 4) {                      // a chunk is a whole block
+        constexpr int BYTES = 32 * (ROW + 4 * GR);
+#pragma unroll
+        for (int c = 0; c < TILE / 16; ++c) {
+          const int there_c = (mask >> c) & 1 ? 16 : 0;
+          const int id_c = __shfl_sync(0xffffffffu, id, (k << two) + c);
+          const unsigned char* src = head + (there_c ? id_c * page : 0) + lane * 16;
+#pragma unroll
+          for (int u = 0; u < BYTES; u += 512)
+            if (u + 512 <= BYTES || lane * 16 < BYTES - u) cp_async16(dst + c * BYTES + u, src + u, there_c);
+        }
+      } else {                                     // codes and pairs of TILE tokens, each apart in the block
+        const int place = spot_k & 255, P = 1 << a.page_log2;
+        const unsigned char* block = head + (mask ? __shfl_sync(0xffffffffu, id, k << two) * page : 0);
+        constexpr int CODES = TILE * ROW, PAIRS = TILE * GR * 4;
+        for (int u = lane * 16; u < STAGE; u += 512) {
+          const int from = u < CODES ? place * ROW + u : u < 2 * CODES ? (P + place) * ROW + u - CODES
+                           : u < 2 * CODES + PAIRS ? 2 * P * ROW + place * GR * 4 + u - 2 * CODES
+                                                   : 2 * P * ROW + (P + place) * GR * 4 + u - 2 * CODES - PAIRS;
+          cp_async16(dst + u - lane * 16, block + from, mask ? 16 : 0);
+        }
+      }
+      ++f_ask;
     }
-    ++f_ask;
+    cp_async_commit();
   };
   look_up(w_lo);
   if (a.early) pdl_wait();
@@ -312,8 +315,6 @@ __global__ void __launch_bounds__(PdSizes<D, BITS, NT>::THREADS, 1) packed_decod
   const unsigned off_v = chunk * ROW + t * ROW + g * BITS;                 // its 8 channels of keys t, t + 4, t + 8, t + 12
   const unsigned off_kp = 2 * chunk * ROW + key_g * GR * 4, off_vp = off_kp + chunk * GR * 4;
   int stage = 0, f = w_lo;
-  unsigned phase = 0;
-  bool broken = false;
   while (f < w_hi) {
     now.advance(a, contexts, pairs, f);
     const int seg = f, seg_end = min(now.base + now.tiles, w_hi);
@@ -409,10 +410,9 @@ __global__ void __launch_bounds__(PdSizes<D, BITS, NT>::THREADS, 1) packed_decod
       }
 
       for (; f < seg_end; ++f) {
-        if (!broken) broken = __any_sync(0xffffffffu, !mbar_wait(full + 8 * stage, phase));
-        if (broken) {
-          if (lane == 0 && a.status) *a.status = PD_STATUS;
-        } else {
+        cp_async_wait<S - 1>();
+        __syncwarp();                              // every lane's copies of this stage are there
+        {
           const unsigned char* base = smem + (size_t)(warp * S + stage) * STAGE;
           const int key0 = tile0 + (f - now.base) * TILE;
           const unsigned mask = here[stage];
@@ -637,8 +637,8 @@ __global__ void __launch_bounds__(PdSizes<D, BITS, NT>::THREADS, 1) packed_decod
             }
         }
         __syncwarp();                              // every lane has read the stage
-        if (!broken) ask(stage);
-        if (++stage == S) { stage = 0; phase ^= 1; }
+        ask(stage);
+        if (++stage == S) stage = 0;
       }
     }
 
@@ -702,11 +702,6 @@ __global__ void __launch_bounds__(PdSizes<D, BITS, NT>::THREADS, 1) packed_decod
         }
       }
   }
-  if (broken) {                                    // leave no copy in flight behind
-    if (lane == 0 && a.status) *a.status = PD_STATUS;
-    for (int s = 0; s < S; ++s) mbar_wait(full + 8 * ((stage + s) % S), stage + s >= S ? phase ^ 1 : phase);
-  }
-
   // ---- the parts of one pair become the result, or this block's part of the pair
   __syncthreads();
   const int lane_base = lane < 2 * WARPS ? part_base[lane] : -1;
@@ -847,12 +842,9 @@ static int pd_sms() {
   return n > 0 ? n : 148;
 }
 
-struct PdShape { int nt, chunks, blocks, stages, smem; bool join; long long part_floats; };
+struct PdShape { int nt, chunks, blocks; bool join; long long part_floats; };
 template <int D, int BITS, int NT> static void pd_fill(PdShape* s, int n, int nkv, int max_context, int window) {
   typedef PdSizes<D, BITS, NT> Z;
-  s->stages = PD_STAGES;
-  while (s->stages > 2 && Z::smem(s->stages, n) > PD_SMEM) --s->stages;
-  s->smem = Z::smem(s->stages, n);
   const long long reach = window > 0 && window < max_context ? (long long)window + Z::TILE - 1 : max_context;
   const long long tiles = (long long)n * nkv * s->chunks * ((reach + Z::TILE - 1) / Z::TILE);
   const long long want = (tiles + PD_EACH - 1) / PD_EACH;
@@ -889,13 +881,14 @@ extern "C" long long gg_packed_decode_scratch(int n, int nh, int nkv, int d, int
 }
 
 template <int D, int BITS, int NT, bool OPT>
-static int pd_launch(const PackedDecode& a, int smem, bool join, cudaStream_t stream) {
-  // the most it may ever ask for, once for each device
+static int pd_launch(const PackedDecode& a, bool join, cudaStream_t stream) {
+  constexpr int smem = PdSizes<D, BITS, NT>::SMEM;
+  // once for each device
   static std::atomic<unsigned long long> allowed{0};
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e == cudaSuccess && (dev >= 64 || !((allowed.load(std::memory_order_relaxed) >> dev) & 1))) {
-    e = cudaFuncSetAttribute(packed_decode_kernel<D, BITS, NT, OPT>, cudaFuncAttributeMaxDynamicSharedMemorySize, PD_SMEM);
+    e = cudaFuncSetAttribute(packed_decode_kernel<D, BITS, NT, OPT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e == cudaSuccess && dev < 64) allowed.fetch_or(1ull << dev, std::memory_order_relaxed);
   }
   if (e != cudaSuccess) return gg_fail(GG_ERR_CUDA, "packed_decode: %s", cudaGetErrorString(e));
@@ -911,7 +904,7 @@ extern "C" int gg_packed_decode_mma(const void* q, long long q_stride, const voi
                                     const int* cu_q_lens, const int* context_lens, const int* seqs, int n, int max_context, float* scratch,
                                     long long scratch_floats, void* out, int nh, int nkv, int d, int page_size, int bits, int window,
                                     float scale, float softcap, const float* sink, const float* slopes, float temp_coef, float temp_every,
-                                    int* status, int early, cudaStream_t stream) {
+                                    int early, cudaStream_t stream) {
   GG_REQUIRE(gg_packed_decode_mma_ok(GG_BF16, d, page_size, bits), "packed_decode: head size %d, pages of %d tokens or %d bits are not taken", d, page_size, bits);
   GG_REQUIRE(nkv > 0 && nh > 0 && nh % nkv == 0, "packed_decode: %d heads are not a multiple of %d kv heads", nh, nkv);
   GG_REQUIRE(n >= 0 && n <= PD_MAX_TOKENS && num_pages >= 0 && bt_stride > 0 && window >= 0 && max_context >= 0,
@@ -930,9 +923,9 @@ extern "C" int gg_packed_decode_mma(const void* q, long long q_stride, const voi
   a.page_log2 = 31 - __builtin_clz(page_size);
   a.page_bytes = PackedRows(bits, d, page_size).page_bytes();
   a.window = window; a.scale = scale; a.softcap = softcap; a.sink = sink; a.slopes = slopes; a.temp_coef = temp_coef; a.temp_every = temp_every;
-  a.part = scratch; a.cut = reinterpret_cast<int4*>(scratch + s.part_floats); a.blocks = s.blocks; a.stages = s.stages; a.status = status; a.early = early;
+  a.part = scratch; a.cut = reinterpret_cast<int4*>(scratch + s.part_floats); a.blocks = s.blocks; a.early = early;
   const bool opt = softcap > 0.f || sink || slopes || temp_every > 0.f;
   const int nt = s.nt;
-#define PD_RUN(D, BITS, NT) return opt ? pd_launch<D, BITS, NT, true>(a, s.smem, s.join, stream) : pd_launch<D, BITS, NT, false>(a, s.smem, s.join, stream)
+#define PD_RUN(D, BITS, NT) return opt ? pd_launch<D, BITS, NT, true>(a, s.join, stream) : pd_launch<D, BITS, NT, false>(a, s.join, stream)
   PD_SIZES(PD_RUN);
 }

@@ -55,7 +55,7 @@ def test_the_launchers_refuse_sizes_and_missing_lists():
     refused("bad sizes", _11=-1)
     refused("bad sizes", _13=0)
     g = ops._packed("gg_packed_decode_mma")
-    args = [None, 64, None, 4, None, 8, 4, None, None, None, 1, 64, None, 0, None, 8, 2, 64, 16, 4, 0, 1.0, 0.0, None, None, 0.0, 0.0, None, 0, None]
+    args = [None, 64, None, 4, None, 8, 4, None, None, None, 1, 64, None, 0, None, 8, 2, 64, 16, 4, 0, 1.0, 0.0, None, None, 0.0, 0.0, 0, None]
     for at, v, message in ((17, 96, "not taken"), (18, 8, "not taken"), (19, 5, "not taken"), (15, 7, "multiple"), (10, 2000, "bad sizes"),
                            (20, -1, "bad sizes"), (6, 0, "sequences"), (5, 2 ** 29, "too large"), (1, 4, "16 bytes"), (0, 8, "16 bytes"), (0, None, "scratch")):
         bad = list(args)
