@@ -62,12 +62,18 @@ struct PackedDecode {
 };
 
 __device__ __forceinline__ void mma_f16(float* c, unsigned a0, unsigned a1, unsigned a2, unsigned a3, unsigned b0, unsigned b1) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// (no volatile in these: the order of independent products and exponentials is the compiler's to choose)
+__device__ __forceinline__ float exp2_near(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
 }
 __device__ __forceinline__ unsigned transpose8(unsigned x) {
   unsigned y;
-  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
   return y;
 }
 __device__ __forceinline__ unsigned half_pair(float lo, float hi) {
@@ -542,7 +548,7 @@ __global__ void __launch_bounds__(PdSizes<D, BITS, NT>::THREADS, 1) packed_decod
                 m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
                 m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
                 m = fmaxf(m, ref[nt][j]);
-                const float al = fast_exp2(ref[nt][j] - m);
+                const float al = exp2_near(ref[nt][j] - m);
                 ref[nt][j] = m;
                 l[nt][j] *= al;
 #pragma unroll
@@ -562,7 +568,7 @@ __global__ void __launch_bounds__(PdSizes<D, BITS, NT>::THREADS, 1) packed_decod
               for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
-                  const float p = fast_exp2(s[kb][nt][2 * half + j] - ref[nt][j]);
+                  const float p = exp2_near(s[kb][nt][2 * half + j] - ref[nt][j]);
                   s[kb][nt][2 * half + j] = p;
                   l[nt][j] += p;
 #pragma unroll
@@ -671,8 +677,8 @@ __global__ void __launch_bounds__(PdSizes<D, BITS, NT>::THREADS, 1) packed_decod
           float sum = l[nt][j];
           if (OPT && a.sink && h < heads) {
             const float sk = a.sink[kvh * a.group + head0 + h] * PD_LOG2E, top = fmaxf(ref[nt][j], sk);
-            fac = fast_exp2(ref[nt][j] - top);
-            sum = sum * fac + fast_exp2(sk - top);
+            fac = exp2_near(ref[nt][j] - top);
+            sum = sum * fac + exp2_near(sk - top);
           }
           fac = sum != 0.f ? fac / sum : 0.f;
         } else if (g == 0) {
@@ -722,7 +728,7 @@ __global__ void __launch_bounds__(PdSizes<D, BITS, NT>::THREADS, 1) packed_decod
       if (lane - o >= from) top = fmaxf(top, v);
     }
     const float M = __shfl_sync(0xffffffffu, top, to);
-    float w = real ? fast_exp2(mine - M) : 0.f, L = real ? part_sum[lane][h] * w : 0.f;
+    float w = real ? exp2_near(mine - M) : 0.f, L = real ? part_sum[lane][h] * w : 0.f;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const float v = __shfl_up_sync(0xffffffffu, L, o);
@@ -733,9 +739,9 @@ __global__ void __launch_bounds__(PdSizes<D, BITS, NT>::THREADS, 1) packed_decod
     const int4 pair = part_pair[lane];
     if (lane_base >= b_lo && lane_base + pair.x <= b_hi) {        // the weight in the result
       if (OPT && a.sink && h < pair.y) {
-        const float sk = a.sink[pair.z % a.nh + h] * PD_LOG2E, all = fmaxf(M, sk), u = fast_exp2(M - all);
+        const float sk = a.sink[pair.z % a.nh + h] * PD_LOG2E, all = fmaxf(M, sk), u = exp2_near(M - all);
         w *= u;
-        L = L * u + fast_exp2(sk - all);
+        L = L * u + exp2_near(sk - all);
       }
       w = L != 0.f ? w / L : 0.f;
     } else if (lane == from) {
@@ -803,7 +809,7 @@ __global__ void __launch_bounds__(256) packed_join_kernel(PackedDecode a) {
     const float* p = a.part + (size_t)(2 * c + (c == first ? 1 : 0)) * PART;
     const float2 ml = *reinterpret_cast<const float2*>(p + HEADS * D + 2 * h);
     const float4 v = reinterpret_cast<const float4*>(p + h * D)[e];
-    const float top = fmaxf(M, ml.x), u = fast_exp2(M - top), w = fast_exp2(ml.x - top);
+    const float top = fmaxf(M, ml.x), u = exp2_near(M - top), w = exp2_near(ml.x - top);
     L = L * u + w * ml.y;
     y.x = fmaf(w, v.x, u * y.x); y.y = fmaf(w, v.y, u * y.y); y.z = fmaf(w, v.z, u * y.z); y.w = fmaf(w, v.w, u * y.w);
     M = top;
@@ -816,10 +822,10 @@ __global__ void __launch_bounds__(256) packed_join_kernel(PackedDecode a) {
   const int sets = min(SETS, last - first + 1);
   float top = sk;
   for (int k = 0; k < sets; ++k) top = fmaxf(top, ml_s[k].x);
-  float sum = a.sink ? fast_exp2(sk - top) : 0.f;
+  float sum = a.sink ? exp2_near(sk - top) : 0.f;
   y = make_float4(0.f, 0.f, 0.f, 0.f);
   for (int k = 0; k < sets; ++k) {
-    const float w = fast_exp2(ml_s[k].x - top);
+    const float w = exp2_near(ml_s[k].x - top);
     const float4 v = y_s[k][e];
     sum = fmaf(w, ml_s[k].y, sum);
     y.x = fmaf(w, v.x, y.x); y.y = fmaf(w, v.y, y.y); y.z = fmaf(w, v.z, y.z); y.w = fmaf(w, v.w, y.w);
