@@ -4,11 +4,13 @@
 //   score(j, h) = scale q_h . k_j,  k_j = s_jg code_j + o_jg in group g of 64 channels
 //               = scale sum_g ( s_jg (q_h . code_j)_g + o_jg (sum of q_h over g) )
 //   out_h       = sum_j p_jh v_j / sum_j p_jh = sum_j ( (p_jh s'_jg) code'_j + p_jh o'_jg ) / sum_j p_jh
-// so the matrix products run on the codes themselves, which half precision holds exactly, and scales and offsets are applied to
-// the 16 x 8 results in float32.  A code needs one AND to become a half: its bits in the low end of a half are the subnormal
+// so the matrix products run on the codes themselves, and scales and offsets are applied to the 16 x 8 results in float32.
+//
+// A code needs one AND to become a half, which holds it exactly: its bits in the low end of a half are the subnormal
 // code * 2^-24 (4 bits: every second code stands four bits higher and counts sixteenfold; its q, or its row of the output, is
-// divided by 16).  q is scaled by a power of two into the range of half precision (common to the heads of a kv head); the
-// weights p s' are rounded to half precision under a running power of two.
+// divided by 16).  (Codes as e4m3 numbers, four an AND, are slower: their products become conversions and products of halves, 75
+// us where this takes 56.)  q is brought into the range of half precision by a power of two for each head; the weights p s' are
+// rounded to half precision under a running power of two.
 //
 // The products are transposed, keys (16) x heads (8) and channels (16) x heads (8): with 8 query heads to a kv head or fewer no
 // row of a tensor core instruction is empty.  Both operands' other index may be permuted freely, so codes go from shared memory
@@ -342,67 +344,76 @@ __global__ void __launch_bounds__(PdSizes<D, BITS, NT>::THREADS, 1) packed_decod
 #pragma unroll
       for (int gr = 0; gr < GR; ++gr) r[gr][nt][0] = r[gr][nt][1] = 0.f;
     }
+    float unit[NT][2], one[NT][2];                 // a head's scores and maxima are held in units of `unit`
     int vexp = -120;                               // weights are held times 2^(6 - vexp)
 
     {
       // ---- q of this pair: B operands, and its sums over each group
       unsigned qf[GR][4][NT][2];
-      float qsum[GR][NT][2], qfac;
+      float qsum[GR][NT][2];
       {
         const float temp = OPT && a.temp_every > 0.f ? 1.f + a.temp_coef * logf(floorf(__fdiv_rn((float)ctx, a.temp_every)) + 1.f) : 1.f;
-        const float fac = a.scale * temp * (OPT ? 1.f : PD_LOG2E);
-        float x[GR][NT][16];
-        float big = 0.f;
+        const float fac = a.scale * temp * (OPT ? 1.f : PD_LOG2E), size = fmaxf(fabsf(fac), 1e-30f);
+        constexpr int CODE = 24;                   // a code is an operand times 2^-CODE
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
           const bool mine = nt * 8 + g < heads;
           const __nv_bfloat16* qp = a.q + (size_t)row * a.q_stride + (size_t)(kvh * a.group + head0 + (mine ? nt * 8 + g : 0)) * D + t * 16;
+          float x[GR][16], sum[GR], big = 0.f;
 #pragma unroll
           for (int gr = 0; gr < GR; ++gr) {
-            float sum = 0.f;
 #pragma unroll
             for (int v = 0; v < 2; ++v) {
               const uint4 u = mine ? *reinterpret_cast<const uint4*>(qp + gr * 64 + v * 8) : make_uint4(0, 0, 0, 0);
               const unsigned w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
               for (int i = 0; i < 4; ++i) {
-                x[gr][nt][v * 8 + 2 * i] = __uint_as_float(w[i] << 16);
-                x[gr][nt][v * 8 + 2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+                x[gr][v * 8 + 2 * i] = __uint_as_float(w[i] << 16);
+                x[gr][v * 8 + 2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
               }
             }
+            sum[gr] = 0.f;
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
-              sum += x[gr][nt][i];
-              big = fmaxf(big, fabsf(x[gr][nt][i]));
+              sum[gr] += x[gr][i];
+              big = fmaxf(big, fabsf(x[gr][i]));
             }
-            sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-            sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-            sum *= fac;
-            qsum[gr][nt][0] = __shfl_sync(0xffffffffu, sum, 8 * t);
-            qsum[gr][nt][1] = __shfl_sync(0xffffffffu, sum, 8 * t + 4);
+            sum[gr] += __shfl_xor_sync(0xffffffffu, sum[gr], 1);
+            sum[gr] += __shfl_xor_sync(0xffffffffu, sum[gr], 2);
+            if (!(sum[gr] - sum[gr] == 0.f)) sum[gr] = __int_as_float(0x7fffffff);       // an infinity or NaN in q: NaN scores
           }
-        }
-        big = warp_max(big);
-        const int e = max(-90, min(100, 139 - (int)(__float_as_uint(big) >> 23)));   // big * 2^e lies in [2^12, 2^13)
-        const float up = power_of_two(e);
-        qfac = fac * power_of_two(24 - e);
+          big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
+          big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
+          const int e = max(-90, min(100, 139 - (int)(__float_as_uint(big) >> 23)));   // big * 2^e lies in [2^12, 2^13)
+          const float up = copysignf(power_of_two(e), fac), down = copysignf(power_of_two(e - CODE), fac), mul = fmaxf(size * power_of_two(CODE - e), 1e-37f);
 #pragma unroll
-        for (int gr = 0; gr < GR; ++gr)
+          for (int j = 0; j < 2; ++j) {            // of the heads whose scores this lane will hold
+            unit[nt][j] = __shfl_sync(0xffffffffu, mul, 8 * t + 4 * j);
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
+            for (int gr = 0; gr < GR; ++gr) qsum[gr][nt][j] = __shfl_sync(0xffffffffu, sum[gr] * down, 8 * t + 4 * j);
+          }
 #pragma unroll
-            for (int m = 0; m < 4; ++m) {
-              const float* y = x[gr][nt];
-              if (BITS == 4) {                     // m = 2 * word + (codes four bits up)
+          for (int gr = 0; gr < GR; ++gr) {
+            float* y = x[gr];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) y[i] *= up;
+            if (BITS == 4) {
+#pragma unroll
+              for (int m = 0; m < 4; ++m) {        // m = 2 * word + (codes four bits up)
                 const int c = 8 * (m >> 1) + (m & 1);
-                const float u = m & 1 ? up * 0.0625f : up;
+                const float u = m & 1 ? 0.0625f : 1.f;
                 qf[gr][m][nt][0] = half_pair(y[c] * u, y[c + 4] * u);
                 qf[gr][m][nt][1] = half_pair(y[c + 2] * u, y[c + 6] * u);
-              } else {
-                qf[gr][m][nt][0] = half_pair(y[4 * m] * up, y[4 * m + 2] * up);
-                qf[gr][m][nt][1] = half_pair(y[4 * m + 1] * up, y[4 * m + 3] * up);
+              }
+            } else {
+#pragma unroll
+              for (int m = 0; m < 4; ++m) {
+                qf[gr][m][nt][0] = half_pair(y[4 * m], y[4 * m + 2]);
+                qf[gr][m][nt][1] = half_pair(y[4 * m + 1], y[4 * m + 3]);
               }
             }
+          }
+        }
       }
       float slope[NT][2];
       if (OPT) {
@@ -413,6 +424,14 @@ __global__ void __launch_bounds__(PdSizes<D, BITS, NT>::THREADS, 1) packed_decod
             const int h = nt * 8 + 2 * t + j;
             slope[nt][j] = a.slopes && h < heads ? a.slopes[kvh * a.group + head0 + h] : 0.f;
           }
+      }
+
+      if (OPT) {                                   // options are applied to scores as they are
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) one[nt][0] = one[nt][1] = 1.f;
+      } else {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) { one[nt][0] = unit[nt][0]; one[nt][1] = unit[nt][1]; }
       }
 
       for (; f < seg_end; ++f) {
@@ -470,7 +489,7 @@ __global__ void __launch_bounds__(PdSizes<D, BITS, NT>::THREADS, 1) packed_decod
               }
 #pragma unroll
               for (int half = 0; half < 2; ++half) {
-                const float sc = __uint_as_float(kp[half][gr] << 16) * qfac, of = __uint_as_float(kp[half][gr] & 0xffff0000u);
+                const float sc = __uint_as_float(kp[half][gr] << 16), of = __uint_as_float(kp[half][gr] & 0xffff0000u);
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -486,7 +505,7 @@ __global__ void __launch_bounds__(PdSizes<D, BITS, NT>::THREADS, 1) packed_decod
               for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                  float v = s[kb][nt][i];
+                  float v = s[kb][nt][i] * unit[nt][i & 1];
                   if (a.softcap > 0.f) v = a.softcap * tanhf(v / a.softcap);
                   v -= slope[nt][i & 1] * (float)(ctx - 1 - (key0 + 16 * kb + 8 * (i >> 1) + key_g));
                   s[kb][nt][i] = v * PD_LOG2E;
@@ -536,7 +555,7 @@ __global__ void __launch_bounds__(PdSizes<D, BITS, NT>::THREADS, 1) packed_decod
             for (int j = 0; j < 2; ++j) {
               mx[nt][j] = fmaxf(s[0][nt][j], s[0][nt][2 + j]);
               if (KB == 2) mx[nt][j] = fmaxf(mx[nt][j], fmaxf(s[KB - 1][nt][j], s[KB - 1][nt][2 + j]));
-              over = over || mx[nt][j] > ref[nt][j] + 8.f;
+              over = over || (mx[nt][j] - ref[nt][j]) * one[nt][j] > 8.f;
             }
           if (__any_sync(0xffffffffu, over)) {
 #pragma unroll
@@ -548,7 +567,7 @@ __global__ void __launch_bounds__(PdSizes<D, BITS, NT>::THREADS, 1) packed_decod
                 m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
                 m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
                 m = fmaxf(m, ref[nt][j]);
-                const float al = exp2_near(ref[nt][j] - m);
+                const float al = exp2_near((ref[nt][j] - m) * one[nt][j]);
                 ref[nt][j] = m;
                 l[nt][j] *= al;
 #pragma unroll
@@ -557,7 +576,11 @@ __global__ void __launch_bounds__(PdSizes<D, BITS, NT>::THREADS, 1) packed_decod
                 for (int i = 0; i < GR * 4; ++i) { o[i][nt][j] *= al; o[i][nt][2 + j] *= al; }
               }
           }
-          float smax = 0.f;
+          float smax = 0.f, base2[NT][2];
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) base2[nt][j] = fmaxf(ref[nt][j] * one[nt][j], PD_NO_KEY);
 #pragma unroll
           for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
@@ -568,7 +591,7 @@ __global__ void __launch_bounds__(PdSizes<D, BITS, NT>::THREADS, 1) packed_decod
               for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
-                  const float p = exp2_near(s[kb][nt][2 * half + j] - ref[nt][j]);
+                  const float p = exp2_near(fmaf(s[kb][nt][2 * half + j], one[nt][j], -base2[nt][j]));
                   s[kb][nt][2 * half + j] = p;
                   l[nt][j] += p;
 #pragma unroll
@@ -648,7 +671,11 @@ __global__ void __launch_bounds__(PdSizes<D, BITS, NT>::THREADS, 1) packed_decod
       }
     }
 
-    // ---- the pair's result, or this warp's part of it
+    // ---- the pair's result, or this warp's part of it (maxima as powers of two from here)
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) ref[nt][j] = fmaxf(ref[nt][j] * one[nt][j], PD_NO_KEY);
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll

@@ -510,3 +510,25 @@ def test_prefill_in_several_runs(bits, monkeypatch):
     pool.kv.prefill(*args, least=10, out=mark)
     kept = [r for b in (0, 4) for r in range(cu[b], cu[b + 1])]
     assert (mark[kept] == 9.0).all() and (mark != 9.0).any(-1).any(-1).sum() == cu[-1] - len(kept)
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("scale", [0.09, -0.05, 0.0])
+def test_decode_of_loud_quiet_and_bad_queries(bits, scale):
+    """Heads that share a kv head and differ by 2^60, a head with an infinity, one with a NaN, one of zeros: each its own result."""
+    nh, nkv, d, n = 6, 1, 128, 70
+    pool = Pool([n], nkv, d, 16, bits, seed=1)
+    g = torch.Generator().manual_seed(2)
+    q = torch.randn(1, nh, d, generator=g)
+    q[0, 1] *= 2.0 ** 30 * 1e-10 if scale else 1.0
+    q[0, 2] *= 2.0 ** -60
+    q[0, 3] = 0
+    q[0, 4, 77] = math.inf
+    q[0, 5, 3] = math.nan
+    q = q.to(BF16)
+    out = pool.kv.decode(q.cuda(), pool.tables.cuda(), torch.tensor([n], dtype=torch.int32).cuda(), n, scale).cpu().double()[0]
+    ref = plain.attend(q.double(), pool.keys[0], pool.values[0], n, scale)[0]
+    assert torch.isnan(out[4:]).all()
+    for h in range(4):
+        e = errors_of(BF16, q[0, h:h + 1], pool.keys[0], abs(scale))
+        assert ((out[h] - ref[h]).abs() <= bound(ref[h], [pool.values[0]], BF16, *e)).all(), h
