@@ -156,6 +156,7 @@ class PackedKV:
                   temperature, least):
         """prefill() of sequences lo .. hi, whose portions see ``pages`` pages and make counts[i] tiles of 16, 64 and 128 rows."""
         nh, d, P = q.shape[1], self.head_dim, self.page_size
+        ops.packed_prefill_rows(q, out, self.pages, nh, d, sink, slopes)
         if hi - lo != tables.shape[0]:
             tables, context_lens, cu_q_lens = tables[lo:hi], context_lens[lo:hi], cu_q_lens[lo:hi + 1]
         B, width = tables.shape

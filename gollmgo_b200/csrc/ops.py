@@ -1648,6 +1648,13 @@ def _packed_q(what, q, out, nh, d):
     return stride
 
 
+def packed_prefill_rows(q, out, pages, nh: int, d: int, sink=None, slopes=None) -> None:
+    """Refuses rows of q and out that the prompt kernels behind packed_unfold do not take."""
+    _stream_of("prefill", q, out, pages, sink, slopes)
+    dtype_code(q.dtype)
+    _packed_q("prefill", q, out, nh, d)
+
+
 def _packed_tokens(what, q, cu_q_lens, context_lens, seqs, n, B):
     """The index lists of n single tokens fit each other and q."""
     _ints(what, B, context_lens)

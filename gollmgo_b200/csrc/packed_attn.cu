@@ -32,8 +32,12 @@
 #include <atomic>
 
 #define PD_MAX_TOKENS 512          // tokens of one launch
-#define PD_EACH 4                  // tiles of a block below which fewer blocks are launched
-#define PD_ALONE 2                 // tiles a warp up to which a single token's pairs get a block each
+// Tiles of a block below which fewer blocks are launched (us for 1, 2, 4 and 8: one token of 4000 keys of one kv head 16.0 14.0
+// 12.4 12.6; 2000 keys of eight 12.1 12.1 11.9 11.5, 4000 keys 11.1 11.1 11.1 12.5).
+#define PD_EACH 4
+// Tiles a warp up to which a single token's pairs get a block each (us with and without, eight kv heads of 128 in 4 bits: 200 keys
+// 7.2 9.1, 700 keys 10.1 11.0, 1400 keys 12.7 11.3).
+#define PD_ALONE 2
 #define PD_SMEM (222 * 1024)       // dynamic shared memory: of 227 KB, with what a block has besides
 #define PD_LOG2E 1.4426950408889634f
 #define PD_NO_KEY (-3.0e38f)       // the running maximum before the first key: below every finite score
@@ -60,7 +64,7 @@ struct PackedDecode {
   float* part;                     // parts of pairs, [8 NT * D + 2 * 8 NT] each (outputs, then max and sum of each head): two of every block,
                                    // then one of every warp
   int4* cut;                       // of each block: what the second kernel joins (see there)
-  int blocks, early;       // early: the lists are not the output of the kernel ahead
+  int blocks, early;               // early: the lists are not the output of the kernel ahead
 };
 
 __device__ __forceinline__ void mma_f16(float* c, unsigned a0, unsigned a1, unsigned a2, unsigned a3, unsigned b0, unsigned b1) {

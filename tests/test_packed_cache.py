@@ -479,6 +479,14 @@ def test_calls_that_are_refused():
         kv.read(tables, ctx, pos, 2, out=(torch.zeros(2, 2, 16, 64, device="cuda"), torch.zeros(2, 2, 16, 64, device="cuda", dtype=BF16)))
     with pytest.raises(E):
         kv.read(tables, ctx.long(), pos, 2)
+    two, cu = torch.zeros(2, 4, 64, dtype=BF16, device="cuda"), torch.tensor([0, 2], dtype=torch.int32, device="cuda")
+    for bad in (dict(q=two.half()), dict(q=two.cpu()), dict(q=torch.zeros(4, 2, 64, dtype=BF16, device="cuda").transpose(0, 1)), dict(tables=tables.cpu()),
+                dict(cu_q_lens=cu[:1]), dict(cu_q_lens=cu.long()), dict(context_lens=ctx.cpu()), dict(window=-1), dict(out=torch.zeros(2, 4, 64, device="cuda")),
+                dict(out=torch.zeros(3, 4, 64, dtype=BF16, device="cuda")), dict(sink=torch.zeros(4)), dict(sink=torch.zeros(3, device="cuda")),
+                dict(q_lens=[2, 2]), dict(contexts=[1]), dict(contexts=[10 ** 6])):
+        args = dict(dict(q=two, tables=tables, cu_q_lens=cu, context_lens=ctx, q_lens=[2], contexts=[20], scale=0.1), **bad)
+        with pytest.raises(E):
+            kv.prefill(**args)
     assert kv.decode(q[:0], tables[:0], ctx[:0], 20, 0.1).shape == (0, 4, 64)
     assert kv.write(row[:0], pos[:0], pos[:0], 4).shape == (0, 4, 64)
     assert kv.prefill(q[:0], tables, torch.zeros(2, dtype=torch.int32, device="cuda"), ctx, [0], [20], 0.1).shape == (0, 4, 64)
