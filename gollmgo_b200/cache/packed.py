@@ -70,6 +70,10 @@ class PackedKV:
             raise ops.KernelError(f"{what}: q is [tokens, heads in multiples of {self.kv_heads}, {self.head_dim}], got {tuple(shape)}")
         return q.new_empty(shape) if out is None else out
 
+    def _on_tensor_cores(self, q: torch.Tensor, out: torch.Tensor) -> bool:
+        return ops.packed_decode_mma_ok(q.dtype, self.head_dim, self.page_size) and q.data_ptr() % 16 == 0 \
+            and q.stride(0) * q.element_size() % 16 == 0 and out.data_ptr() % 16 == 0
+
     def decode(self, q: torch.Tensor, tables: torch.Tensor, context_lens: torch.Tensor, max_context: int, scale: float, *,
                window: int = 0, softcap: float = 0.0, sink=None, slopes=None, temperature=None, cu_q_lens=None, seqs=None,
                out: Optional[torch.Tensor] = None, early: bool = False) -> torch.Tensor:
@@ -82,11 +86,10 @@ class PackedKV:
         nh, d = q.shape[1], self.head_dim
         n = seqs.numel() if seqs is not None else q.shape[0]
         more = (window, scale, softcap, sink, slopes, temperature)
-        if ops.packed_decode_mma_ok(q.dtype, d, self.page_size) and q.data_ptr() % 16 == 0 and q.stride(0) % 8 == 0 \
-                and out.data_ptr() % 16 == 0:
+        if self._on_tensor_cores(q, out):
             shape = (nh, self.kv_heads, d, self.page_size, self.bits)
             most = ops.PACKED_DECODE_TOKENS
-            size = ops.packed_decode_scratch(min(n, most), nh, self.kv_heads, d, self.bits, max_context, window)
+            size = ops.packed_decode_scratch(q.dtype, min(n, most), nh, self.kv_heads, d, self.bits, max_context, window)
             scratch = q.new_empty((size,), dtype=torch.float32)
             if n <= most:
                 ops.packed_decode_mma(q, self.pages, tables, cu_q_lens, context_lens, seqs, n, max_context, scratch, out, *shape, *more, early)
@@ -121,12 +124,15 @@ class PackedKV:
 
         The pages of the portions are read back once, in the type of the activations, and the prompt kernels run on them;
         steps of many long portions go in runs of sequences, so that what is read back at a time stays within
-        ``SCRATCH_TOKENS`` (or the longest sequence)."""
+        ``SCRATCH_TOKENS`` (or the longest sequence).  float32 rows that the tensor cores take attend to the codes where they lie, as single
+        tokens do."""
         out = self._out("prefill", q, out)
         B, P = len(q_lens), self.page_size
         if len(contexts) != B or tables.shape[0] < B:
             raise ops.KernelError(f"prefill: {B} portions, {len(contexts)} contexts and block tables of {tables.shape[0]} sequences")
-        lo = pages = most = longest = 0
+        lo = pages = most = longest = items = 0
+        exact = q.dtype == torch.float32 and self._on_tensor_cores(q, out)
+        fold = ops.packed_prompt_fold(q.shape[1], self.kv_heads) if exact else 1
         counts = [0, 0, 0]
 
         def run(hi):
@@ -138,6 +144,10 @@ class PackedKV:
                 continue
             if a > c or c > tables.shape[1] * P:
                 raise ops.KernelError(f"prefill: sequence {b} brings {a} of {c} tokens, its block table holds {tables.shape[1] * P}")
+            if exact:
+                items += -(-a // fold)
+                longest = max(longest, c)
+                continue
             n = -(-c // P)
             seen = n - (max(0, c - a - window + 1) // P if window else 0)
             if pages and ((pages + seen) * P > SCRATCH_TOKENS or b - lo >= MOST_SEQUENCES):
@@ -148,6 +158,14 @@ class PackedKV:
             longest = max(longest, c)
             for i, h in enumerate((16, 64, 128)):
                 counts[i] += -(-a // h)
+        if items:
+            if tables.shape[0] != B:
+                tables, context_lens, cu_q_lens = tables[:B], context_lens[:B], cu_q_lens[:B + 1]
+            size = ops.packed_decode_scratch(q.dtype, min(items, ops.PACKED_DECODE_TOKENS), q.shape[1], self.kv_heads, self.head_dim, self.bits,
+                                             longest, window)
+            ops.packed_prompt_f32(q, self.pages, tables, cu_q_lens, context_lens, least, items, q.new_empty((2 * items,), dtype=torch.int32),
+                                  longest, q.new_empty((size,)), out, q.shape[1], self.kv_heads, self.head_dim, self.page_size, self.bits,
+                                  window, scale, softcap, sink, slopes, temperature)
         if pages:
             run(B if B - lo <= MOST_SEQUENCES else lo + MOST_SEQUENCES)
         return out

@@ -1542,8 +1542,10 @@ _PACKED_TYPES = {
     "gg_packed_write": [_P, _L, _I, _P, _P, _P, _F, _P, _I, _P, _L, _I, _I, _I, _I, _I, _I, _I, _I, _I, _P],
     "gg_packed_read": [_P, _I, _P, _I, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _P],
     "gg_packed_decode": [_P, _L, _I, _P, _I, _P, _I, _I, _P, _P, _P, _I, _I, _P, _P, _P, _I, _I, _I, _I, _I, _I, _F, _F, _P, _P, _F, _F, _P],
-    "gg_packed_decode_mma": [_P, _L, _P, _I, _P, _I, _I, _P, _P, _P, _I, _I, _P, _L, _P, _I, _I, _I, _I, _I, _I, _F, _F, _P, _P, _F, _F, _I, _P],
-    "gg_packed_decode_scratch": [_I, _I, _I, _I, _I, _I, _I],
+    "gg_packed_decode_mma": [_P, _L, _I, _P, _I, _P, _I, _I, _P, _P, _P, _I, _I, _P, _L, _P, _I, _I, _I, _I, _I, _I, _F, _F, _P, _P, _F, _F, _I, _P],
+    "gg_packed_decode_scratch": [_I, _I, _I, _I, _I, _I, _I, _I],
+    "gg_packed_prompt_fold": [_I, _I],
+    "gg_packed_prompt_f32": [_P, _L, _P, _I, _P, _I, _I, _P, _P, _I, _I, _P, _I, _P, _L, _P, _I, _I, _I, _I, _I, _I, _F, _F, _P, _P, _F, _F, _P],
     "gg_packed_unfold": [_P, _I, _P, _I, _P, _P, _I, _P, _P, _I, _I, _I, _P, _I, _I, _P, _P, _I, _I, _P, _P, _I, _I, _I, _I, _I, _I, _P],
 }
 _PACKED = {}
@@ -1692,14 +1694,14 @@ PACKED_DECODE_TOKENS = 512      # tokens that packed_decode_mma takes in one lau
 
 
 def packed_decode_mma_ok(dtype: torch.dtype, d: int, page_size: int) -> bool:
-    """Whether packed_decode_mma takes these sizes: bfloat16, heads of 64 or 128, pages of 16 tokens or more."""
-    return dtype == torch.bfloat16 and d in (64, 128) and page_size >= 16
+    """Whether packed_decode_mma and (float32) packed_prompt_f32 take these sizes: heads of 64 or 128, pages of 16 tokens or more."""
+    return dtype in (torch.bfloat16, torch.float32) and d in (64, 128) and page_size >= 16
 
 
 @functools.lru_cache(maxsize=4096)
-def packed_decode_scratch(n: int, nh: int, nkv: int, d: int, bits: int, max_context: int, window: int) -> int:
+def packed_decode_scratch(dtype: torch.dtype, n: int, nh: int, nkv: int, d: int, bits: int, max_context: int, window: int) -> int:
     """float32 scratch of packed_decode_mma."""
-    return _packed("gg_packed_decode_scratch")(n, nh, nkv, d, bits, max_context, window)
+    return _packed("gg_packed_decode_scratch")(dtype_code(dtype), n, nh, nkv, d, bits, max_context, window)
 
 
 def packed_decode_mma(q: torch.Tensor, pages: torch.Tensor, tables: torch.Tensor, cu_q_lens: Optional[torch.Tensor],
@@ -1719,10 +1721,42 @@ def packed_decode_mma(q: torch.Tensor, pages: torch.Tensor, tables: torch.Tensor
     if scratch.dtype != torch.float32 or not scratch.is_contiguous():
         raise KernelError("packed_decode: the scratch is contiguous float32")
     coef, every = temperature or (0.0, 0.0)
-    _check(_packed("gg_packed_decode_mma")(q.data_ptr(), stride, pages.data_ptr(), pages.shape[0], tables.data_ptr(), width, B, _at(cu_q_lens),
+    _check(_packed("gg_packed_decode_mma")(q.data_ptr(), stride, dtype_code(q.dtype), pages.data_ptr(), pages.shape[0], tables.data_ptr(), width, B, _at(cu_q_lens),
                                            context_lens.data_ptr(), _at(seqs), n, max_context, scratch.data_ptr(), scratch.numel(),
                                            out.data_ptr(), nh, nkv, d, page_size, bits, window, scale, softcap, _at(sink), _at(slopes),
                                            coef, every, early, stream), 2)
+
+
+@functools.lru_cache(maxsize=None)
+def packed_prompt_fold(nh: int, nkv: int) -> int:
+    """Rows of an item of packed_prompt_f32."""
+    return _packed("gg_packed_prompt_fold")(nh, nkv)
+
+
+def packed_prompt_f32(q: torch.Tensor, pages: torch.Tensor, tables: torch.Tensor, cu_q_lens: torch.Tensor, context_lens: torch.Tensor,
+                      least: int, count: int, items: torch.Tensor, max_context: int, scratch: torch.Tensor, out: torch.Tensor, nh: int,
+                      nkv: int, d: int, page_size: int, bits: int, window: int, scale: float, softcap: float = 0.0,
+                      sink: Optional[torch.Tensor] = None, slopes: Optional[torch.Tensor] = None, temperature=None) -> None:
+    """Causal attention of prompt portions (sequences with ``least`` rows or more in cu_q_lens) over a packed cache, float32 and
+    packed_decode_mma_ok: ``count`` items of packed_prompt_fold rows (each portion's last one may have fewer), their lists in ``items`` int32
+    [2 count].  ``scratch`` as for packed_decode_mma of min(count, PACKED_DECODE_TOKENS) tokens."""
+    stream = _stream_of("packed_prompt", q, pages, tables, cu_q_lens, context_lens, items, scratch, out, sink, slopes)
+    stride = _packed_q("packed_prompt", q, out, nh, d)
+    if q.dtype != torch.float32:
+        raise KernelError("packed_prompt: q is float32")
+    if sink is not None or slopes is not None:
+        _attn_extras(nh, None, None, None, sink, slopes)
+    B, width = _tables("packed_prompt", tables)
+    _ints("packed_prompt", B, context_lens)
+    _ints("packed_prompt", B + 1, cu_q_lens)
+    _ints("packed_prompt", 2 * count, items)
+    if scratch.dtype != torch.float32 or not scratch.is_contiguous():
+        raise KernelError("packed_prompt: the scratch is contiguous float32")
+    coef, every = temperature or (0.0, 0.0)
+    _check(_packed("gg_packed_prompt_f32")(q.data_ptr(), stride, pages.data_ptr(), pages.shape[0], tables.data_ptr(), width, B,
+                                           cu_q_lens.data_ptr(), context_lens.data_ptr(), least, count, items.data_ptr(), max_context,
+                                           scratch.data_ptr(), scratch.numel(), out.data_ptr(), nh, nkv, d, page_size, bits, window, scale,
+                                           softcap, _at(sink), _at(slopes), coef, every, stream), 1 + 2 * -(-count // PACKED_DECODE_TOKENS))
 
 
 @contextlib.contextmanager

@@ -321,15 +321,81 @@ def test_prefill(bits, dtype, option, nh, nkv, d, page):
 @pytest.mark.parametrize("bits", [4, 8])
 @pytest.mark.parametrize("nh,nkv", [(2, 2), (3, 1), (7, 1), (9, 1), (24, 1), (17, 1), (32, 1), (66, 2)])
 @pytest.mark.parametrize("d", [64, 128])
-def test_decode_groups_of_any_size(bits, nh, nkv, d):
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_decode_groups_of_any_size(bits, nh, nkv, d, dtype):
     lens = [33, 5, 260]
     pool = Pool(lens, nkv, d, 16, bits, seed=nh)
     g = torch.Generator().manual_seed(nh)
-    q = torch.randn(3, nh, d, generator=g).to(BF16)
+    q = torch.randn(3, nh, d, generator=g).to(dtype)
     out = pool.kv.decode(q.cuda(), pool.tables.cuda(), torch.tensor(lens, dtype=torch.int32).cuda(), 260, d ** -0.5).cpu().double()
     for b, n in enumerate(lens):
         ref = plain.attend(q[b:b + 1].double(), pool.keys[b], pool.values[b], n, d ** -0.5)[0]
-        assert ((out[b] - ref).abs() <= bound(ref, [pool.values[b]], BF16, *errors_of(BF16, q[b], pool.keys[b], d ** -0.5))).all()
+        assert ((out[b] - ref).abs() <= bound(ref, [pool.values[b]], dtype, *errors_of(dtype, q[b], pool.keys[b], d ** -0.5))).all()
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("nh,nkv", [(1, 1), (4, 2), (3, 1), (8, 2), (5, 1), (8, 1), (16, 1), (9, 1)])
+@pytest.mark.parametrize("d,window,option", [(64, 0, 0), (128, 7, 1), (128, 40, 0), (64, 100, 1)])
+def test_prompts_in_float32_of_groups_of_any_size(bits, nh, nkv, d, window, option):
+    """Rows of a portion share the columns of a product where a kv head has few heads: portions that end inside such a group, windows
+    and contexts that end between its rows; the rows of short sequences and behind the last one stay as they were."""
+    q_lens, lens = [13, 1, 0, 64, 3, 7], [13, 50, 9, 200, 65, 300]
+    pool = Pool(lens, nkv, d, 16, bits, seed=nh + window, dtype=F32)
+    o, oc = options_of(dict(softcap=20.0, slopes=True, sink=True, temperature=(0.1, 8.0)) if option else {}, nh, 3)
+    cu = [0]
+    for a in q_lens:
+        cu.append(cu[-1] + a)
+    q = torch.randn(cu[-1] + 2, nh, d, generator=torch.Generator().manual_seed(nh))
+    dev = lambda x: torch.tensor(x, dtype=torch.int32).cuda()
+    out = torch.full((cu[-1] + 2, nh, d), 3.0, device="cuda")
+    pool.kv.prefill(q.cuda(), pool.tables.cuda(), dev(cu), dev(lens), q_lens, lens, d ** -0.5, window=window, least=3, out=out, **oc)
+    out = out.cpu().double()
+    for b, (a, n) in enumerate(zip(q_lens, lens)):
+        x = q[cu[b]:cu[b + 1]]
+        if a < 3:
+            assert (out[cu[b]:cu[b + 1]] == 3.0).all()
+            continue
+        ref = plain.attend(x.double(), pool.keys[b], pool.values[b], n, d ** -0.5, window=window, **o)
+        e = errors_of(F32, x, pool.keys[b], d ** -0.5)
+        e = (e[0] * (1.0 + 0.1 * math.log(1 + n / 8.0) if option else 1.0), e[1])
+        assert ((out[cu[b]:cu[b + 1]] - ref).abs() <= bound(ref, [pool.values[b]], F32, *e)).all(), (b, a, n)
+    assert (out[cu[-1]:] == 3.0).all()
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("nh,nkv", [(2, 2), (8, 2), (10, 1)])
+def test_prompts_in_float32_see_bad_tokens_of_their_own_past_only(bits, nh, nkv):
+    d, n, page = 64, 37, 16
+    g = torch.Generator().manual_seed(nh)
+    x = torch.randn(n, (nh + 2 * nkv) * d, generator=g)
+    x[17, nh * d + 3] = math.nan                              # a key of kv head 0
+    x[6, (nh + 2 * nkv) * d - 1] = math.inf                   # a value of the last kv head
+    kv = PackedKV_of(4, nkv, d, page, bits)
+    tables = torch.tensor([[2, 0, 3]], dtype=torch.int32)
+    t = torch.arange(n)
+    q = kv.write(x.cuda(), None, (tables[0][t // page] * page + t % page).to(torch.int32).cuda(), nh)
+    dev = lambda y: torch.tensor(y, dtype=torch.int32).cuda()
+    out = kv.prefill(q, tables.cuda(), dev([0, n]), dev([n]), [n], [n], 0.125, window=9)
+    for row in range(n):
+        for h in range(nh):
+            kvh = h * nkv // nh
+            past = range(max(0, row - 8), row + 1)
+            bad = (kvh == 0 and 17 in past) or (kvh == nkv - 1 and 6 in past)
+            assert bool(out[row, h].isnan().any()) == bad, (row, h)
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+def test_prompts_in_float32_of_more_items_than_a_launch_takes(bits):
+    PackedKV, ops = kit()
+    nh, nkv, d, page = 8, 1, 64, 16
+    a, n = ops.PACKED_DECODE_TOKENS + 90, ops.PACKED_DECODE_TOKENS + 90
+    pool = Pool([40, n], nkv, d, page, bits, seed=1, dtype=F32)
+    q = torch.randn(3 + a, nh, d, generator=torch.Generator().manual_seed(2))
+    dev = lambda y: torch.tensor(y, dtype=torch.int32).cuda()
+    out = pool.kv.prefill(q.cuda(), pool.tables.cuda(), dev([0, 3, 3 + a]), dev([40, n]), [3, a], [40, n], 0.125).cpu().double()
+    for b, lo, hi, c in ((0, 0, 3, 40), (1, 3, 3 + a, n)):
+        ref = plain.attend(q[lo:hi].double(), pool.keys[b], pool.values[b], c, 0.125)
+        assert ((out[lo:hi] - ref).abs() <= bound(ref, [pool.values[b]], F32, *errors_of(F32, q[lo:hi], pool.keys[b], 0.125))).all()
 
 
 @pytest.mark.parametrize("bits", [4, 8])
@@ -398,6 +464,39 @@ def test_decode_of_bad_values_and_far_scales(bits, dtype):
             size = (p[:, None] * seen.abs()).sum(0).max()          # what the weights' roundings are relative to
             e, wt = errors_of(dtype, q[b, h:h + 1], held[0][n - 90:, kvh:kvh + 1], d ** -0.5)
             assert ((out[b, h] - ref).abs() <= torch.finfo(dtype).eps / 2 * ref.abs() + (2 * e + 2 * wt) * size).all(), (b, h)
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("loud", [2.0 ** 25, 2.0 ** 60])
+def test_loud_values_that_another_head_or_an_earlier_key_attends_to(bits, dtype, d, loud):
+    """Head 0 attends to one loud value, head 1 of the same kv head does not: what it sums is held relative to its own.  Head 2 attends to
+    another loud value in an early tile, but far more to what comes later."""
+    n, page, nh = 400, 16, 3
+    g = torch.Generator().manual_seed(11)
+    x = torch.randn(n, (nh + 2) * d, generator=g)
+    k, v = x[:, nh * d:(nh + 1) * d], x[:, (nh + 1) * d:]
+    k[:, :2] = 0.0
+    k[[150, 5], 0] = torch.tensor([30.0, -30.0])
+    k[300:, 1] = 30.0
+    v[[150, 5]] *= loud
+    x = x.to(dtype)
+    q = torch.randn(1, nh, d, generator=g) * 0.3
+    q[0, 0, :2] = torch.tensor([8.0, 0.0])                     # towards key 150
+    q[0, 1, :2] = torch.tensor([0.0, 50.0])                    # to the keys from 300 on alone
+    q[0, 2, :2] = torch.tensor([-8.0, 60.0])                   # towards key 5, and more to those
+    q = q.to(dtype)
+    kv = PackedKV_of(n // page, 1, d, page, bits)
+    kv.write(x.cuda(), None, torch.arange(n, dtype=torch.int32).cuda(), nh)
+    out = kv.decode(q.cuda(), torch.arange(n // page, dtype=torch.int32).view(1, -1).cuda(), torch.tensor([n], dtype=torch.int32).cuda(), n, 0.5).cpu().double()
+    held = [torch.stack([torch.stack([plain.get(kv.pages.cpu(), t, 0, d, bits, page)[w]]) for t in range(n)]) for w in (0, 1)]
+    for h in range(nh):
+        ref = plain.attend(q[:, h:h + 1].double(), held[0], held[1], n, 0.5)[0, 0]
+        p = torch.softmax(held[0][:, 0] @ q[0, h].double() * 0.5, 0)
+        size = (p[:, None] * held[1][:, 0].abs()).sum(0).max()
+        e, w = errors_of(dtype, q[0, h:h + 1], held[0], 0.5)
+        assert ((out[0, h] - ref).abs() <= torch.finfo(dtype).eps / 2 * ref.abs() + (2 * e + 2 * w) * size).all(), h
 
 
 def PackedKV_of(*a):

@@ -55,13 +55,24 @@ def test_the_launchers_refuse_sizes_and_missing_lists():
     refused("bad sizes", _11=-1)
     refused("bad sizes", _13=0)
     g = ops._packed("gg_packed_decode_mma")
-    args = [None, 64, None, 4, None, 8, 4, None, None, None, 1, 64, None, 0, None, 8, 2, 64, 16, 4, 0, 1.0, 0.0, None, None, 0.0, 0.0, 0, None]
-    for at, v, message in ((17, 96, "not taken"), (18, 8, "not taken"), (19, 5, "not taken"), (15, 7, "multiple"), (10, 2000, "bad sizes"),
-                           (20, -1, "bad sizes"), (6, 0, "sequences"), (5, 2 ** 29, "too large"), (1, 4, "16 bytes"), (0, 8, "16 bytes"), (0, None, "scratch")):
+    args = [None, 64, 1, None, 4, None, 8, 4, None, None, None, 1, 64, None, 0, None, 8, 2, 64, 16, 4, 0, 1.0, 0.0, None, None, 0.0, 0.0, 0, None]
+    for at, v, message in ((18, 96, "not taken"), (19, 8, "not taken"), (20, 5, "not taken"), (16, 7, "multiple"), (11, 2000, "too many"),
+                           (21, -1, "bad sizes"), (7, 0, "sequences"), (6, 2 ** 29, "too large"), (1, 4, "16 bytes"), (0, 8, "16 bytes"), (0, None, "scratch"),
+                           (2, 7, "not taken"), (11, -1, "bad sizes"), (12, -1, "too many")):
         bad = list(args)
         bad[at] = v
         assert g(*bad) != 0
         assert message in ops.lib().gg_last_error().decode(), (at, v)
+    p = ops._packed("gg_packed_prompt_f32")
+    args = [None, 64, None, 4, None, 8, 4, 16, None, 1, 5, 16, 64, None, 0, None, 8, 2, 64, 16, 4, 0, 1.0, 0.0, None, None, 0.0, 0.0, None]
+    for at, v, message in ((18, 96, "not taken"), (19, 8, "not taken"), (20, 5, "not taken"), (16, 7, "multiple"), (10, -1, "bad sizes"), (6, -1, "bad sizes"),
+                           (21, -1, "bad sizes"), (1, 2, "16 bytes"), (0, 4, "16 bytes"), (15, 8, "16 bytes"), (7, None, "lists"), (11, None, "lists"),
+                           (12, -1, "lists"), (5, 2 ** 29, "too large"), (0, None, "scratch")):
+        bad = list(args)
+        bad[at] = v
+        assert p(*bad) != 0
+        assert message in ops.lib().gg_last_error().decode(), (at, v)
+    assert [ops.packed_prompt_fold(h, 1) for h in (1, 2, 3, 4, 5, 8, 16)] == [8, 4, 2, 2, 1, 1, 1]
 
 
 def test_rows_and_lists_that_are_refused():
