@@ -6,7 +6,7 @@
 //   the pairs of the keys    P x groups x (scale, offset) in bfloat16,
 //   the pairs of the values  the same.
 // A group is 64 channels where that divides d, else 32, else 16.  A code c stands for scale * c + offset.  Keys and values of a
-// page and head lie in one block so that one bulk copy brings both (2304 bytes: 16 tokens of 128 channels in 4 bits).
+// page and head lie in one block so that one run of copies brings both (2304 bytes: 16 tokens of 128 channels in 4 bits).
 // The offset is the group's smallest value rounded down to bfloat16 and the scale the smallest bfloat16 that is not below
 // (largest - offset) / (2^bits - 1): every value lies inside the codes' range, so none is clipped, and a value is off by at
 // most half a scale.  A group that holds an infinity or a NaN has NaN for both.
