@@ -130,12 +130,12 @@ class PackedKV:
         B, P = len(q_lens), self.page_size
         if len(contexts) != B or tables.shape[0] < B:
             raise ops.KernelError(f"prefill: {B} portions, {len(contexts)} contexts and block tables of {tables.shape[0]} sequences")
-        lo = pages = most = longest = items = 0
+        lo = hi = pages = most = longest = items = 0           # (a run of sequences: from its first portion to behind its last)
         exact = q.dtype == torch.float32 and self._on_tensor_cores(q, out)
         fold = ops.packed_prompt_fold(q.shape[1], self.kv_heads) if exact else 1
         counts = [0, 0, 0]
 
-        def run(hi):
+        def run():
             self._portions(q, out, tables, cu_q_lens, context_lens, lo, hi, pages, most, counts, longest, scale, window, softcap, sink, slopes,
                            temperature, least)
         for b in range(B):
@@ -151,8 +151,11 @@ class PackedKV:
             n = -(-c // P)
             seen = n - (max(0, c - a - window + 1) // P if window else 0)
             if pages and ((pages + seen) * P > SCRATCH_TOKENS or b - lo >= MOST_SEQUENCES):
-                run(b)
-                lo, pages, most, longest, counts = b, 0, 0, 0, [0, 0, 0]
+                run()
+                pages, most, longest, counts = 0, 0, 0, [0, 0, 0]
+            if not pages:
+                lo = b
+            hi = b + 1
             pages += seen
             most = max(most, n)
             longest = max(longest, c)
@@ -167,7 +170,7 @@ class PackedKV:
                                   longest, q.new_empty((size,)), out, q.shape[1], self.kv_heads, self.head_dim, self.page_size, self.bits,
                                   window, scale, softcap, sink, slopes, temperature)
         if pages:
-            run(B if B - lo <= MOST_SEQUENCES else lo + MOST_SEQUENCES)
+            run()
         return out
 
     def _portions(self, q, out, tables, cu_q_lens, context_lens, lo, hi, pages, most, counts, longest, scale, window, softcap, sink, slopes,
