@@ -130,6 +130,8 @@ class PackedKV:
         B, P = len(q_lens), self.page_size
         if len(contexts) != B or tables.shape[0] < B:
             raise ops.KernelError(f"prefill: {B} portions, {len(contexts)} contexts and block tables of {tables.shape[0]} sequences")
+        if sum(a for a in q_lens if a > 0) > q.shape[0]:
+            raise ops.KernelError(f"prefill: portions of {sum(a for a in q_lens if a > 0)} rows in q of {q.shape[0]}")
         lo = hi = pages = most = longest = items = 0           # (a run of sequences: from its first portion to behind its last)
         exact = q.dtype == torch.float32 and self._on_tensor_cores(q, out)
         fold = ops.packed_prompt_fold(q.shape[1], self.kv_heads) if exact else 1

@@ -128,3 +128,19 @@ def tolerance(q, keys, values, context, scale, dtype, tensor_cores):
             rounds = (half * (2 if tensor_cores else 1) + (p + 8) * 2.0 ** -24) * (w @ v.abs())
             tol[i, h] = 1.05 * (spread + rounds) + torch.finfo(dtype).eps / 2 * mean + 1e-30
     return tol
+
+
+@pytest.mark.parametrize("rows,q_lens", [(3, [4]), (0, [1]), (9, [5, 5]), (9, [1, 9]), (9, [0, 10, -3])])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_portions_of_more_rows_than_q_has_are_refused(rows, q_lens, dtype):
+    class NoDevice(PackedKV):
+        def __init__(self):
+            self.head_dim, self.page_size, self.bits, self.kv_heads, self._sms = 64, 16, 4, 1, 148
+
+        def _portions(self, *a):
+            raise AssertionError("rows behind the end of q")
+    from gollmgo_b200.csrc import ops
+    B = len(q_lens)
+    lists = torch.zeros(B + 1, dtype=torch.int32), torch.zeros(B, dtype=torch.int32)
+    with pytest.raises(ops.KernelError, match="rows in q"):
+        NoDevice().prefill(torch.zeros(rows, 2, 64, dtype=dtype), torch.zeros(B, 4, dtype=torch.int32), *lists, q_lens, [20] * B, 1.0)
