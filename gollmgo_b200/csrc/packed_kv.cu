@@ -160,15 +160,34 @@ __device__ __forceinline__ uint2 codes8(const PackCoder& k, const float* x) {
   return k.pair == 0x7fff7fffu ? make_uint2(0u, 0u) : make_uint2(w[0], w[1]);
 }
 
-// The same for float64 values: a rotated key's float64 quotient lies on the wrong side of a border once in 10^12, and 1.5 * 2^52
-// leaves the whole number in the low word without a conversion (those between the widths take eight clocks a warp).
+// The same for float64 values (rotated keys).  1.5 * 2^28 added leaves a quotient in the low word without a conversion (those between the widths
+// take eight clocks a warp), in steps of 2^-24: the code is its rounded upper byte.  The quotient by the reciprocal is off by far less than a
+// step; where the rest lies within a step of one half (a rotation by nothing, as at position 0, leaves bfloat16 values, which lie on a border
+// often; others one in 2^22), the remainder decides, which is exact there.
 template <int BITS>
 __device__ __forceinline__ uint2 codes8(const PackCoder& k, const double* x) {
-  const double inv = k.scale > 0.0 ? 1.0 / k.scale : 0.0, shift = -k.offset * inv;
+  const double inv = k.scale > 0.0 ? 1.0 / k.scale : 0.0;
+  auto quotient = [&](int i) { return (unsigned)__double2loint(fma(x[i] - k.offset, inv, 402653184.0)); };
   unsigned w[2] = {0u, 0u};
+  bool near = false;
 #pragma unroll
-  for (int i = 0; i < 8; ++i)
-    w[i * BITS / 32] |= ((unsigned)__double2loint(fma(x[i], inv, shift) + 6755399441055744.0) & ((1u << BITS) - 1)) << (i * BITS & 31);
+  for (int i = 0; i < 8; ++i) {
+    const unsigned t = quotient(i);
+    near = near || ((t - 0x7fffffu) & 0xffffffu) <= 2u;
+    w[i * BITS / 32] |= (t + 0x800000u) >> 24 << (i * BITS & 31);
+  }
+  if (near) {
+    const double border = 0.5 * k.scale;
+    w[0] = w[1] = 0u;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const unsigned q = (quotient(i) + 0x800000u) >> 24;
+      const double rest = fma(-(double)(int)q, k.scale, x[i] - k.offset);
+      const bool odd = q & 1u;
+      const unsigned move = (rest > border || (rest == border && odd)) ? 1u : (rest < -border || (rest == -border && odd)) ? ~0u : 0u;
+      w[i * BITS / 32] |= (q + move) << (i * BITS & 31);
+    }
+  }
   return k.pair == 0x7fff7fffu ? make_uint2(0u, 0u) : make_uint2(w[0], w[1]);
 }
 // A bfloat16 value (as a float) as float64: the exponent moved over, in integer arithmetic.

@@ -1,0 +1,69 @@
+"""Codes of the packed cache where a value lies on the border between two of them, or next to one: the bytes of the pages are the
+formula's (tests/plain_packed.py), whichever kernel writes them."""
+import pytest
+import torch
+
+import plain_packed as plain
+
+pytestmark = pytest.mark.gpu
+
+BF16, F32, F64 = torch.bfloat16, torch.float32, torch.float64
+
+
+def page_bytes_of(k, v, bits, page):
+    """Pages uint8 [pages, kv heads, bytes] that hold k, v [T, kv heads, d] (float64, host) in slots 0 .. T - 1; zeros behind them."""
+    T, nkv, d = k.shape
+    row, par = d * bits // 8, 4 * (d // plain.group_of(d))
+    out = torch.zeros(-(-T // page), nkv, plain.page_bytes(bits, d, page), dtype=torch.uint8)
+    pg, pl = torch.arange(T) // page, torch.arange(T) % page
+    for which, x in enumerate((k, v)):
+        code, scale, off = plain.quantise(x, bits)
+        c = code.to(torch.int64)
+        if bits == 4:
+            c = c[..., 0::2] + 16 * c[..., 1::2]
+        pairs = torch.stack([scale, off], -1).flatten(-2).float().to(BF16).contiguous().view(torch.uint8)
+        for h in range(nkv):
+            out[pg[:, None], h, (which * page + pl[:, None]) * row + torch.arange(row)] = c[:, h].to(torch.uint8)
+            out[pg[:, None], h, 2 * page * row + (which * page + pl[:, None]) * par + torch.arange(par)] = pairs[:, h]
+    return out
+
+
+def stored(qkv, nh, nkv, d, bits, page, pos=None, inv=None, magnitude=1.0):
+    from gollmgo_b200.cache import PackedKV
+    T = qkv.shape[0]
+    kv = PackedKV.empty(-(-T // page), nkv, d, page, bits)
+    kv.write(qkv.cuda(), None if pos is None else pos.cuda(), torch.arange(T, dtype=torch.int32).cuda(), nh, None if inv is None else inv.cuda(), False, magnitude)
+    return kv.pages.cpu()
+
+
+def rows_on_borders(T, nkv, d, g):
+    """bfloat16 rows with many values half-way between two codes of 4 and of 8 bits: whole and half numbers, some of other scales and offsets."""
+    x = torch.randint(0, 31, (T, nkv, d), generator=g) * 0.5
+    x[..., 0::16], x[..., 1::16] = 0.0, 15.0
+    wide = torch.randint(0, 511, (T, nkv, d), generator=g) * 0.5
+    wide = torch.where(wide > 128, wide.round(), wide)                # (eight bits of a number)
+    wide[..., 0::16], wide[..., 1::16] = 0.0, 255.0
+    x = torch.where((torch.arange(T) % 2 == 0)[:, None, None], x, wide)
+    scale = 2.0 ** torch.randint(-30, 30, (T, nkv, 1), generator=g)
+    return (x * scale).to(BF16)
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("d", [64, 96, 128])
+@pytest.mark.parametrize("rows", ["normal", "borders"])
+@pytest.mark.parametrize("turn", ["position 0", "frequency 0", "none"])
+def test_values_between_two_codes(bits, d, rows, turn):
+    """A rotation by nothing leaves bfloat16 values, which lie exactly between two codes often: ties go to the even one."""
+    T, nh, nkv, page = 400, 1, 4, 16
+    g = torch.Generator().manual_seed(bits * d)
+    if rows == "normal":
+        qkv = torch.randn(T, (nh + 2 * nkv) * d, generator=g).to(BF16)
+    else:
+        qkv = torch.cat([torch.zeros(T, nh, d, dtype=BF16), rows_on_borders(T, 2 * nkv, d, g)], 1).view(T, -1)
+    inv = 500000.0 ** (-torch.arange(0, d, 2, dtype=F64) / d)
+    pos = torch.zeros(T, dtype=torch.int32)
+    if turn == "frequency 0":
+        inv, pos = torch.zeros_like(inv), torch.arange(T, dtype=torch.int32) + 7
+    got = stored(qkv, nh, nkv, d, bits, page, None if turn == "none" else pos, None if turn == "none" else inv)
+    k, v = qkv.view(T, -1, d)[:, nh:].double().split(nkv, 1)
+    assert torch.equal(got, page_bytes_of(k, v, bits, page))
