@@ -4,9 +4,9 @@
 #include "packed_kv.cuh"
 
 // ---------------------------------------------------------------- write
-// Which code a value gets is decided in exact or float64 arithmetic: a bfloat16 value as it came is decided in float32, where its
-// difference from the offset is exact; a rotated key, and whatever came in float32, in float64, whose last bits lie far below
-// a code's border.
+// Which code a value gets is decided as float64 arithmetic decides, round((x - offset) / scale) with ties to even: for a bfloat16 value as it
+// came in float32, with float64 where it lies on a border (its difference from the offset is a float but for values that lie far apart); for
+// a rotated key, and whatever came in float32, in float64.
 
 __device__ __forceinline__ unsigned short bf16_down(float x) { return __bfloat16_as_ushort(__float2bfloat16_rd(x)); }
 __device__ __forceinline__ unsigned short bf16_up(float x) { return __bfloat16_as_ushort(__float2bfloat16_ru(x)); }
@@ -129,34 +129,39 @@ packed_write_kernel(const TA* __restrict__ qkv, long long row_stride, const int*
 
 // The codes of eight values, 4 or 8 bits each, as one or two words.  A quotient by the reciprocal is off by less than 2^-21
 // of the largest code; where one lies that near to a border (half between two codes: with bfloat16 values and scales many lie
-// on it) the remainder decides, which one multiply-add gives to the last bit.  Halves keep a wide group's differences finite,
-// and a group of tiny values is brought up by 2^64 so that its scale has a reciprocal.
+// on it) the remainder decides, which one multiply-add gives to the last bit of the difference (a difference and a border are whole
+// multiples of the difference's last place there, so what the subtraction rounded away decides on the border alone).  Halves keep a wide
+// group's differences finite, and a group of tiny values is brought up by 2^64 so that its scale has a reciprocal.
 template <int BITS>
 __device__ __forceinline__ uint2 codes8(const PackCoder& k, const float* x) {
   constexpr float MOST = (1 << BITS) - 1, NEAR = 0.5f - MOST * 0x1p-21f;
   constexpr float MAGIC = 12582912.f;                  // 1.5 * 2^23: added, the whole number stands in the low bits
   const float up = k.half_scale < 0x1p-60f ? 0x1p64f : 1.f, scale = k.half_scale * up, offset = k.half_offset * up, half = 0.5f * up;
   const float inv = scale > 0.f ? 1.f / scale : 0.f;
-  unsigned q[8];
+  unsigned w[2] = {0u, 0u};
   float far = 0.f;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const float t = fmaf(half, x[i], -offset) * inv, m = t + MAGIC;
     far = fmaxf(far, fabsf(t - (m - MAGIC)));
-    q[i] = __float_as_uint(m);
+    w[i * BITS / 32] |= (__float_as_uint(m) & ((1u << BITS) - 1)) << (i * BITS & 31);
   }
   if (far >= NEAR) {
     const float border = 0.5f * scale;
+    w[0] = w[1] = 0u;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const float c = __uint_as_float(q[i]) - MAGIC, rest = fmaf(-c, scale, fmaf(half, x[i], -offset));
-      const bool odd = q[i] & 1u;
-      q[i] += (rest > border || (rest == border && odd)) ? 1u : (rest < -border || (rest == -border && odd)) ? ~0u : 0u;
+      const float diff = fmaf(half, x[i], -offset), m = diff * inv + MAGIC, rest = fmaf(-(m - MAGIC), scale, diff);
+      const unsigned q = __float_as_uint(m) & 255u;
+      unsigned above = rest > border, below = rest < -border;
+      if (fabsf(rest) == border) {                     // what the difference lost, in float64 as the formula has it; nothing: the even code
+        const double lost = ((double)half * x[i] - offset) - diff;
+        above = rest > 0.f && (lost > 0.0 || (lost == 0.0 && (q & 1u)));
+        below = rest < 0.f && (lost < 0.0 || (lost == 0.0 && (q & 1u)));
+      }
+      w[i * BITS / 32] |= ((q + above - below) & ((1u << BITS) - 1)) << (i * BITS & 31);
     }
   }
-  unsigned w[2] = {0u, 0u};
-#pragma unroll
-  for (int i = 0; i < 8; ++i) w[i * BITS / 32] |= (q[i] & ((1u << BITS) - 1)) << (i * BITS & 31);
   return k.pair == 0x7fff7fffu ? make_uint2(0u, 0u) : make_uint2(w[0], w[1]);
 }
 
@@ -249,7 +254,7 @@ __device__ __forceinline__ void store_head(const TC* a, const TC* c, bool nan0, 
 // and the chain from a row's extremes to its codes: 2048 tokens of 32 + 2 x 8 heads of 128 in 17.7 us (2.5 TB/s), 8000 in 58 us (3.0 TB/s).
 #define WRITE_THREADS 256
 template <int D, int BITS, int TOK>
-__global__ void __launch_bounds__(WRITE_THREADS)
+__global__ void __launch_bounds__(WRITE_THREADS, 3)
 packed_write_vec_kernel(const __nv_bfloat16* __restrict__ qkv, long long row_stride, const int* __restrict__ positions,
                         const int* __restrict__ slots, const double* __restrict__ inv_freq, float mag, unsigned char* __restrict__ pages,
                         int num_pages, __nv_bfloat16* __restrict__ q_out, long long q_stride, int T, int nh, int nkv, int page_log2, int early) {

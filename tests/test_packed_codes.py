@@ -67,3 +67,28 @@ def test_values_between_two_codes(bits, d, rows, turn):
     got = stored(qkv, nh, nkv, d, bits, page, None if turn == "none" else pos, None if turn == "none" else inv)
     k, v = qkv.view(T, -1, d)[:, nh:].double().split(nkv, 1)
     assert torch.equal(got, page_bytes_of(k, v, bits, page))
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("d", [64, 96, 128])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_tiny_values_beside_a_border(bits, d, dtype):
+    """-9 + 2 x 4.5 is 0: a value of 2^-30 lies above the border and one of -2^-30 below it, though both vanish beside the offset in float32.
+    (-11: the border between 5 and 6.  2^-60 vanishes in float64 too, and counts as the border.)"""
+    nkv, page = 2, 16
+    g = torch.Generator().manual_seed(d)
+    rows = []
+    for off, top in ((-9.0, 21.0 if bits == 4 else 500.0), (-11.0, 19.0 if bits == 4 else 498.0)):
+        for up in (0, -20, 40):
+            x = torch.randint(-4, 10, (2, nkv, d), generator=g).double()
+            x[..., 0::16], x[..., 1::16] = off, top
+            for i, tiny in enumerate((2.0 ** -30, -2.0 ** -30, 0.0, 2.0 ** -60, -2.0 ** -60, 2.0 ** -14, -2.0 ** -14)):
+                x[..., 2 + i::16] = tiny
+            rows.append(x * 2.0 ** up)
+    x = torch.cat(rows)
+    assert torch.equal(x.to(BF16).double(), x)
+    k, v = x[0::2], x[1::2]
+    got = stored(torch.cat([k, v], 1).flatten(1).to(dtype), 0, nkv, d, bits, page)
+    code, scale, off = plain.quantise(k[:1], bits)
+    assert float(scale[0, 0, 0]) == 2.0 and [int(c) for c in code[0, 0, 2:7]] == [5, 4, 4, 4, 4]
+    assert torch.equal(got, page_bytes_of(k, v, bits, page))
