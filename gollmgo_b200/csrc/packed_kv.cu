@@ -131,12 +131,12 @@ packed_write_kernel(const TA* __restrict__ qkv, long long row_stride, const int*
 // of the largest code; where one lies that near to a border (half between two codes: with bfloat16 values and scales many lie
 // on it) the remainder decides, which one multiply-add gives to the last bit of the difference (a difference and a border are whole
 // multiples of the difference's last place there, so what the subtraction rounded away decides on the border alone).  Halves keep a wide
-// group's differences finite, and a group of tiny values is brought up by 2^64 so that its scale has a reciprocal.
+// group's differences finite, and a group of tiny values is brought up by 2^64 so that its scale has a reciprocal (one of equal values has none).
 template <int BITS>
 __device__ __forceinline__ uint2 codes8(const PackCoder& k, const float* x) {
   constexpr float MOST = (1 << BITS) - 1, NEAR = 0.5f - MOST * 0x1p-21f;
   constexpr float MAGIC = 12582912.f;                  // 1.5 * 2^23: added, the whole number stands in the low bits
-  const float up = k.half_scale < 0x1p-60f ? 0x1p64f : 1.f, scale = k.half_scale * up, offset = k.half_offset * up, half = 0.5f * up;
+  const float up = k.half_scale > 0.f && k.half_scale < 0x1p-60f ? 0x1p64f : 1.f, scale = k.half_scale * up, offset = k.half_offset * up, half = 0.5f * up;
   const float inv = scale > 0.f ? 1.f / scale : 0.f;
   unsigned w[2] = {0u, 0u};
   float far = 0.f;

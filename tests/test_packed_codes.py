@@ -92,3 +92,17 @@ def test_tiny_values_beside_a_border(bits, d, dtype):
     code, scale, off = plain.quantise(k[:1], bits)
     assert float(scale[0, 0, 0]) == 2.0 and [int(c) for c in code[0, 0, 2:7]] == [5, 4, 4, 4, 4]
     assert torch.equal(got, page_bytes_of(k, v, bits, page))
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("d", [64, 96, 128])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_equal_values_have_code_0(bits, d, dtype):
+    """A group of equal values has scale 0 and code 0, however large they are."""
+    values = [0.0, 1.0, -3.0, 2.0 ** -100, 2.0 ** 62, -2.0 ** 64, 2.0 ** 65, 2.0 ** 100, -3e38, 3.3e38]
+    x = torch.tensor(values, dtype=F64).to(BF16).double()[:, None, None].expand(-1, 2, d)
+    got = stored(torch.cat([x, -x], 1).flatten(1).to(dtype), 0, 2, d, bits, 16)
+    want = page_bytes_of(x, -x, bits, 16)
+    assert torch.equal(got[0, :, :2 * 16 * (d * bits // 8)], torch.zeros_like(got[0, :, :2 * 16 * (d * bits // 8)]))
+    # (the sign of a zero may be either)
+    assert torch.equal(got[..., 2 * 16 * (d * bits // 8):].contiguous().view(BF16).double(), want[..., 2 * 16 * (d * bits // 8):].contiguous().view(BF16).double())
