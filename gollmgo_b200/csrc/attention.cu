@@ -94,11 +94,13 @@ __device__ __forceinline__ void attn_tile(const AttnArgs& a, int nrows, const TA
         for (int i = 0; i < 8; ++i) s[i] = fmaf(Qs[(rb + 2 * i) * d + c], kv, s[i]);
       }
       const int tok = kb + j;
+      bool here = true;                              // (a page of a packed cache that is not in the pool has no keys)
+      if (PACKED && tok >= lo && tok < hi) here = (unsigned)bt[tok / ps] < (unsigned)a.num_pages;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const int r = rb + 2 * i;
         const int p = pos_s[r];
-        const bool ok = tok >= lo && tok < hi && tok <= p && (a.window <= 0 || tok > p - a.window || tok < a.keep_first) &&
+        const bool ok = here && tok >= lo && tok < hi && tok <= p && (a.window <= 0 || tok > p - a.window || tok < a.keep_first) &&
                         (a.chunk <= 0 || tok >= (p / a.chunk) * a.chunk);
         float sc = s[i] * scale_s[r];
         if (a.softcap > 0.f) sc = a.softcap * tanhf(sc / a.softcap);
