@@ -106,14 +106,29 @@ class PackedKV:
                 part = seqs[lo:lo + most]
                 ops.packed_decode_mma(q, self.pages, tables, cu_q_lens, context_lens, part, part.numel(), max_context, scratch, out, *shape, *more, early)
             return out
-        # the general kernel: slices of the context until every multiprocessor has four blocks
-        reach = min(max_context, window) if window else max_context
-        splits = max(1, min(64, -(-reach // 64), 592 // max(1, n * self.kv_heads)))
+        splits = self._splits(n, self.kv_heads, max_context, window)
         rows = n * nh * splits
         part = torch.empty(rows * (d + 2), dtype=torch.float32, device=q.device)
         ops.packed_decode(q, self.pages, tables, cu_q_lens, context_lens, seqs, n, splits, part[:rows * d], part[rows * d:], out, nh,
                           self.kv_heads, d, self.page_size, self.bits, *more)
         return out
+
+    @staticmethod
+    def _splits(n: int, kv_heads: int, max_context: int, window: int) -> int:
+        """The general kernel: slices of the context until every multiprocessor has four blocks."""
+        reach = min(max_context, window) if window else max_context
+        return max(1, min(64, -(-reach // 64), 592 // max(1, n * kv_heads)))
+
+    @staticmethod
+    def decode_spread(dtype: torch.dtype, n: int, num_heads: int, kv_heads: int, head_dim: int, page_size: int, bits: int, max_context: int,
+                      window: int = 0) -> tuple:
+        """How decode() spreads n tokens: two values of ``max_context`` for which this is the same launch the same (a call captured with one
+        of them serves contexts up to the other as well)."""
+        if not ops.packed_decode_mma_ok(dtype, head_dim, page_size):
+            return (PackedKV._splits(n, kv_heads, max_context, window),)
+        most = ops.PACKED_DECODE_TOKENS
+        sizes = sorted({min(n, most), n % most or min(n, most)})
+        return tuple(ops.packed_decode_blocks(dtype, m, num_heads, kv_heads, head_dim, bits, max_context, window) for m in sizes if m)
 
     def prefill(self, q: torch.Tensor, tables: torch.Tensor, cu_q_lens: torch.Tensor, context_lens: torch.Tensor,
                 q_lens: Sequence[int], contexts: Sequence[int], scale: float, *, window: int = 0, softcap: float = 0.0, sink=None,

@@ -1544,6 +1544,7 @@ _PACKED_TYPES = {
     "gg_packed_decode": [_P, _L, _I, _P, _I, _P, _I, _I, _P, _P, _P, _I, _I, _P, _P, _P, _I, _I, _I, _I, _I, _I, _F, _F, _P, _P, _F, _F, _P],
     "gg_packed_decode_mma": [_P, _L, _I, _P, _I, _P, _I, _I, _P, _P, _P, _I, _I, _P, _L, _P, _I, _I, _I, _I, _I, _I, _F, _F, _P, _P, _F, _F, _I, _P],
     "gg_packed_decode_scratch": [_I, _I, _I, _I, _I, _I, _I, _I],
+    "gg_packed_decode_blocks": [_I, _I, _I, _I, _I, _I, _I, _I],
     "gg_packed_prompt_fold": [_I, _I],
     "gg_packed_prompt_f32": [_P, _L, _P, _I, _P, _I, _I, _P, _P, _I, _I, _P, _I, _P, _L, _P, _I, _I, _I, _I, _I, _I, _F, _F, _P, _P, _F, _F, _P],
     "gg_packed_unfold": [_P, _I, _P, _I, _P, _P, _I, _P, _P, _I, _I, _I, _P, _I, _I, _P, _P, _I, _I, _P, _P, _I, _I, _I, _I, _I, _I, _P],
@@ -1702,6 +1703,12 @@ def packed_decode_mma_ok(dtype: torch.dtype, d: int, page_size: int) -> bool:
 def packed_decode_scratch(dtype: torch.dtype, n: int, nh: int, nkv: int, d: int, bits: int, max_context: int, window: int) -> int:
     """float32 scratch of packed_decode_mma."""
     return _packed("gg_packed_decode_scratch")(dtype_code(dtype), n, nh, nkv, d, bits, max_context, window)
+
+
+@functools.lru_cache(maxsize=4096)
+def packed_decode_blocks(dtype: torch.dtype, n: int, nh: int, nkv: int, d: int, bits: int, max_context: int, window: int) -> int:
+    """Blocks of packed_decode_mma, less than 0 where every (token, kv head) pair has one of its own."""
+    return _packed("gg_packed_decode_blocks")(dtype_code(dtype), n, nh, nkv, d, bits, max_context, window)
 
 
 def packed_decode_mma(q: torch.Tensor, pages: torch.Tensor, tables: torch.Tensor, cu_q_lens: Optional[torch.Tensor],

@@ -1093,6 +1093,12 @@ extern "C" long long gg_packed_decode_scratch(int dtype, int n, int nh, int nkv,
   return s.part_floats + 4LL * s.blocks;
 }
 
+// The blocks of that launch, less than 0 where every pair has one of its own: calls for which this says the same spread their work alike.
+extern "C" int gg_packed_decode_blocks(int dtype, int n, int nh, int nkv, int d, int bits, int max_context, int window) {
+  const PdShape s = pd_shape(n, nh, nkv, d, bits, max_context, window, dtype == GG_F32);
+  return s.join ? s.blocks : -s.blocks;
+}
+
 template <int D, int BITS, int NT, bool OPT, bool EXACT>
 static int pd_launch(const PackedDecode& a, bool join, cudaStream_t stream) {
   typedef PdSizes<D, BITS, NT, EXACT> Z;

@@ -15,7 +15,7 @@ import os
 
 import torch
 
-from ..cache import PagedKVNeed
+from ..cache import PackedKV, PagedKVNeed
 from ..csrc import ops
 from ..weights import WeightSpec
 from .context import QueryTiles
@@ -180,6 +180,7 @@ class Attention:
                 raise ValueError("a cache in 4 or 8 bits takes attention without values of another size or shared, biases on q, k and v, or "
                                  "norms over whole projections: leave cache_bits unset for this model")
             ops.packed_page_bytes(self.packed, self.d, ctx.page_size)          # refuses sizes it does not take
+            self._packed_sizes = (self.nh, self.nkv, self.d, ctx.page_size, self.packed)
         self.qkv_bias = None
         self.o_bias = None
         # the general path on mma.sync: bfloat16, keys and values of 64 or 128
@@ -291,9 +292,9 @@ class Attention:
         """The count of slices this step's decoded tokens would be cut into: a step that is
         captured with one count is replayed only for steps that choose the same."""
         n = facts.num_seqs if facts.decode_only else 0
-        if self.packed:              # the blocks a step is spread over: more contexts change nothing once the device is full
-            tiles = context_tiles(facts.max_context, self.window)
-            return (f"packed_tiles={min(tiles, -(-self.num_sms // max(1, n * self.nkv)))}",) if n else ()
+        if self.packed:              # asked with what _attend_packed gives to decode()
+            spread = PackedKV.decode_spread(self.ctx.act_dtype, n, *self._packed_sizes, context_tiles(facts.max_context) * TILE_KEYS, int(self.window or 0))
+            return (f"packed_spread={spread}",) if n else ()
         if n == 0 or self._flat_step(n):
             return ()
         return (f"kv_slices={self._splits(n, facts.max_context)}",)

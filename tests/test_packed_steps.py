@@ -1,0 +1,44 @@
+"""Captured decode steps over a packed cache: a step is replayed for every context of its tag, so its launches have to be those that the
+context at hand wants."""
+import pytest
+import torch
+
+from gollmgo_b200.csrc import ops
+from gollmgo_b200.parts import BuildContext, PartSpec, StepFacts, build_mixer
+from gollmgo_b200.parts.attention import TILE_KEYS, context_tiles
+
+CONTEXTS = [1, 60, 64, 65, 100, 200, 512, 900, 1024, 1100, 2000, 2048, 3000, 4096, 7000, 8192, 16384, 20000, 32768, 65536, 131072]
+
+
+def layer(nh, nkv, d, page, bits, dtype=torch.bfloat16, window=None):
+    spec = PartSpec("attention", dict(hidden_size=64, num_heads=nh, num_kv_heads=nkv, head_dim=d, window=window, position=PartSpec("none")))
+    return build_mixer(spec, BuildContext(dtype, "cpu", 64, 64, page, cache_bits=bits))
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("nh,nkv,d", [(1, 1, 64), (32, 8, 128), (16, 16, 64), (40, 40, 128), (32, 32, 128), (64, 2, 128)])
+@pytest.mark.parametrize("window", [None, 1000])
+def test_a_captured_step_has_the_blocks_of_every_context_of_its_tag(bits, dtype, nh, nkv, d, window):
+    mixer = layer(nh, nkv, d, 16, bits, dtype, window)
+    for n in (1, 2, 4, 8, 16, 24, 32, 64):
+        first = {}
+        for c in CONTEXTS:
+            first.setdefault(mixer.step_tags(StepFacts(n, n, True, c)), c)
+        assert len(first) <= 11
+        # (scratch is so many floats a block; a step is spread for the context that decode() is given)
+        size = {c: ops.packed_decode_scratch(dtype, n, nh, nkv, d, bits, context_tiles(c) * TILE_KEYS, window or 0) for c in CONTEXTS}
+        for c in CONTEXTS:
+            assert size[first[mixer.step_tags(StepFacts(n, n, True, c))]] == size[c], (n, c)
+
+
+@pytest.mark.parametrize("n,nkv,d,page", [(1, 2, 96, 16), (4, 1, 128, 8), (30, 8, 256, 16)])
+def test_steps_on_the_general_kernel_have_the_slices_of_every_context_of_their_tag(n, nkv, d, page):
+    from gollmgo_b200.cache import PackedKV
+    mixer = layer(2 * nkv, nkv, d, page, 4)
+    first = {}
+    for c in CONTEXTS:
+        first.setdefault(mixer.step_tags(StepFacts(n, n, True, c)), c)
+    longest = max(CONTEXTS)
+    found = first[mixer.step_tags(StepFacts(n, n, True, longest))]
+    assert PackedKV._splits(n, nkv, context_tiles(found) * TILE_KEYS, 0) == PackedKV._splits(n, nkv, longest, 0)
