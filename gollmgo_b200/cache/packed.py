@@ -88,8 +88,8 @@ class PackedKV:
         more = (window, scale, softcap, sink, slopes, temperature)
         if self._on_tensor_cores(q, out):
             shape = (nh, self.kv_heads, d, self.page_size, self.bits)
-            most = ops.PACKED_DECODE_TOKENS
-            size = ops.packed_decode_scratch(q.dtype, min(n, most), nh, self.kv_heads, d, self.bits, max_context, window)
+            most = ops.packed_decode_tokens(nh, tables.shape[-1], self.page_size)
+            size = ops.packed_launches_scratch(q.dtype, n, most, nh, self.kv_heads, d, self.bits, max_context, window)
             scratch = q.new_empty((size,), dtype=torch.float32)
             if n <= most:
                 ops.packed_decode_mma(q, self.pages, tables, cu_q_lens, context_lens, seqs, n, max_context, scratch, out, *shape, *more, early)
@@ -181,8 +181,8 @@ class PackedKV:
         if items:
             if tables.shape[0] != B:
                 tables, context_lens, cu_q_lens = tables[:B], context_lens[:B], cu_q_lens[:B + 1]
-            size = ops.packed_decode_scratch(q.dtype, min(items, ops.PACKED_DECODE_TOKENS), q.shape[1], self.kv_heads, self.head_dim, self.bits,
-                                             longest, window)
+            size = ops.packed_launches_scratch(q.dtype, items, ops.packed_decode_tokens(q.shape[1], tables.shape[1], P), q.shape[1], self.kv_heads,
+                                               self.head_dim, self.bits, longest, window)
             ops.packed_prompt_f32(q, self.pages, tables, cu_q_lens, context_lens, least, items, q.new_empty((2 * items,), dtype=torch.int32),
                                   longest, q.new_empty((size,)), out, q.shape[1], self.kv_heads, self.head_dim, self.page_size, self.bits,
                                   window, scale, softcap, sink, slopes, temperature)

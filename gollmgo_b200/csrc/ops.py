@@ -1545,6 +1545,7 @@ _PACKED_TYPES = {
     "gg_packed_decode_mma": [_P, _L, _I, _P, _I, _P, _I, _I, _P, _P, _P, _I, _I, _P, _L, _P, _I, _I, _I, _I, _I, _I, _F, _F, _P, _P, _F, _F, _I, _P],
     "gg_packed_decode_scratch": [_I, _I, _I, _I, _I, _I, _I, _I],
     "gg_packed_decode_blocks": [_I, _I, _I, _I, _I, _I, _I, _I],
+    "gg_packed_decode_tokens": [_I, _I, _I],
     "gg_packed_prompt_fold": [_I, _I],
     "gg_packed_prompt_f32": [_P, _L, _P, _I, _P, _I, _I, _P, _P, _I, _I, _P, _I, _P, _L, _P, _I, _I, _I, _I, _I, _I, _F, _F, _P, _P, _F, _F, _P],
     "gg_packed_unfold": [_P, _I, _P, _I, _P, _P, _I, _P, _P, _I, _I, _I, _P, _I, _I, _P, _P, _I, _I, _P, _P, _I, _I, _I, _I, _I, _I, _P],
@@ -1691,7 +1692,7 @@ def packed_decode(q: torch.Tensor, pages: torch.Tensor, tables: torch.Tensor, cu
                                        every, stream), 2)
 
 
-PACKED_DECODE_TOKENS = 512      # tokens that packed_decode_mma takes in one launch
+PACKED_DECODE_TOKENS = 512      # tokens that packed_decode_mma takes in one launch (fewer over very wide block tables: packed_decode_tokens)
 
 
 def packed_decode_mma_ok(dtype: torch.dtype, d: int, page_size: int) -> bool:
@@ -1703,6 +1704,18 @@ def packed_decode_mma_ok(dtype: torch.dtype, d: int, page_size: int) -> bool:
 def packed_decode_scratch(dtype: torch.dtype, n: int, nh: int, nkv: int, d: int, bits: int, max_context: int, window: int) -> int:
     """float32 scratch of packed_decode_mma."""
     return _packed("gg_packed_decode_scratch")(dtype_code(dtype), n, nh, nkv, d, bits, max_context, window)
+
+
+@functools.lru_cache(maxsize=256)
+def packed_decode_tokens(nh: int, width: int, page_size: int) -> int:
+    """Tokens that packed_decode_mma takes in one launch over block tables of ``width`` pages; one at least (which it may refuse)."""
+    return max(1, _packed("gg_packed_decode_tokens")(nh, width, page_size))
+
+
+def packed_launches_scratch(dtype: torch.dtype, n: int, most: int, *sizes) -> int:
+    """float32 scratch for launches of ``most`` of n tokens and one of the rest; ``sizes`` as packed_decode_scratch has them."""
+    size = packed_decode_scratch(dtype, min(n, most), *sizes)
+    return max(size, packed_decode_scratch(dtype, n % most, *sizes)) if n > most and n % most else size
 
 
 @functools.lru_cache(maxsize=4096)
@@ -1746,7 +1759,7 @@ def packed_prompt_f32(q: torch.Tensor, pages: torch.Tensor, tables: torch.Tensor
                       sink: Optional[torch.Tensor] = None, slopes: Optional[torch.Tensor] = None, temperature=None) -> None:
     """Causal attention of prompt portions (sequences with ``least`` rows or more in cu_q_lens) over a packed cache, float32 and
     packed_decode_mma_ok: ``count`` items of packed_prompt_fold rows (each portion's last one may have fewer), their lists in ``items`` int32
-    [2 count].  ``scratch`` as for packed_decode_mma of min(count, PACKED_DECODE_TOKENS) tokens."""
+    [2 count].  ``scratch`` of packed_launches_scratch for launches of packed_decode_tokens items."""
     stream = _stream_of("packed_prompt", q, pages, tables, cu_q_lens, context_lens, items, scratch, out, sink, slopes)
     stride = _packed_q("packed_prompt", q, out, nh, d)
     if q.dtype != torch.float32:
@@ -1763,7 +1776,8 @@ def packed_prompt_f32(q: torch.Tensor, pages: torch.Tensor, tables: torch.Tensor
     _check(_packed("gg_packed_prompt_f32")(q.data_ptr(), stride, pages.data_ptr(), pages.shape[0], tables.data_ptr(), width, B,
                                            cu_q_lens.data_ptr(), context_lens.data_ptr(), least, count, items.data_ptr(), max_context,
                                            scratch.data_ptr(), scratch.numel(), out.data_ptr(), nh, nkv, d, page_size, bits, window, scale,
-                                           softcap, _at(sink), _at(slopes), coef, every, stream), 1 + 2 * -(-count // PACKED_DECODE_TOKENS))
+                                           softcap, _at(sink), _at(slopes), coef, every, stream),
+           1 + 2 * -(-count // packed_decode_tokens(nh, width, page_size)))
 
 
 @contextlib.contextmanager

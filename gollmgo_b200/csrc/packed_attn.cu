@@ -1130,8 +1130,14 @@ static int pd_check(const char* who, const PackedDecode& a, int dtype, int d, in
              "%s: q, its rows, the output and the pages must start on 16 bytes", who);
   return GG_OK;
 }
+// Tokens of one launch over such block tables: its tiles are counted in an int (0: one token has more).
+extern "C" int gg_packed_decode_tokens(int nh, int bt_stride, int page_size) {
+  if (nh < 1 || bt_stride < 1 || page_size < 1) return PD_MAX_TOKENS;
+  const long long each = nh * (((long long)bt_stride * page_size + 15) / 16), most = ((1LL << 31) - 1) / each;
+  return (int)(most < PD_MAX_TOKENS ? most : PD_MAX_TOKENS);
+}
 static int pd_fits(const PackedDecode& a, const PdShape& s, int page_size, const float* scratch, long long scratch_floats) {
-  GG_REQUIRE((long long)a.n * a.nh * (((long long)a.bt_stride * page_size + 15) / 16) < (1LL << 31), "packed_decode: block tables of %d pages for %d tokens are too large for one launch", a.bt_stride, a.n);
+  GG_REQUIRE(a.n <= gg_packed_decode_tokens(a.nh, a.bt_stride, page_size), "packed_decode: block tables of %d pages for %d tokens are too large for one launch", a.bt_stride, a.n);
   GG_REQUIRE(scratch && ((size_t)scratch % 16) == 0 && scratch_floats >= s.part_floats + 4LL * s.blocks, "packed_decode: scratch too small");
   return GG_OK;
 }
@@ -1200,7 +1206,7 @@ static int pd_fold(int group) { return group <= 4 ? 8 / group : 1; }
 extern "C" int gg_packed_prompt_fold(int nh, int nkv) { return nkv > 0 && nh >= nkv ? pd_fold(nh / nkv) : 1; }
 
 // Every row of the portions attends as a single token does, in float32: `count` items of gg_packed_prompt_fold rows in all, their lists in
-// `items` [2 count], at most PD_MAX_TOKENS a launch.  scratch as for gg_packed_decode_mma with min(count, PD_MAX_TOKENS) tokens.
+// `items` [2 count], at most gg_packed_decode_tokens a launch.  scratch as for gg_packed_decode_mma with as many tokens as the first launch has.
 extern "C" int gg_packed_prompt_f32(const void* q, long long q_stride, const void* pages, int num_pages, const int* tables, int bt_stride, int B,
                                     const int* cu_q_lens, const int* context_lens, int least, int count, int* items, int max_context, float* scratch,
                                     long long scratch_floats, void* out, int nh, int nkv, int d, int page_size, int bits, int window,
@@ -1216,13 +1222,14 @@ extern "C" int gg_packed_prompt_f32(const void* q, long long q_stride, const voi
   GG_REQUIRE(cu_q_lens && items && max_context >= 0, "packed_prompt: no lists");
   if (count == 0) return GG_OK;
   a.fold = pd_fold(nh / nkv);
-  a.n = count < PD_MAX_TOKENS ? count : PD_MAX_TOKENS;
+  const int tokens = gg_packed_decode_tokens(nh, bt_stride, page_size), most = tokens > 0 ? tokens : 1;        // (1: refused below)
+  a.n = count < most ? count : most;
   rc = pd_fits(a, pd_shape(a.n, nh, nkv, d, bits, max_context, window, true), page_size, scratch, scratch_floats);
   if (rc) return rc;
   gg_launch(packed_items_kernel, dim3(B + 1), dim3(256), 0, stream, cu_q_lens, B, least > 1 ? least : 1, a.fold, items, items + count, count);
   rc = gg_check_launch("packed_items");
-  for (int lo = 0; lo < count && !rc; lo += PD_MAX_TOKENS) {
-    a.n = count - lo < PD_MAX_TOKENS ? count - lo : PD_MAX_TOKENS;
+  for (int lo = 0; lo < count && !rc; lo += most) {
+    a.n = count - lo < most ? count - lo : most;
     a.seqs = items + lo;
     a.q0 = items + count + lo;
     rc = pd_run(a, true, d, page_size, bits, max_context, scratch, scratch_floats, stream);
