@@ -101,7 +101,7 @@ class PackedKV:
                                           out[lo:hi], *shape, *more, early)
                 return out
             if seqs is None:
-                seqs = torch.arange(n, dtype=torch.int32, device=q.device)
+                seqs, early = torch.arange(n, dtype=torch.int32, device=q.device), False       # (a list that the kernel ahead writes)
             for lo in range(0, n, most):
                 part = seqs[lo:lo + most]
                 ops.packed_decode_mma(q, self.pages, tables, cu_q_lens, context_lens, part, part.numel(), max_context, scratch, out, *shape, *more, early)

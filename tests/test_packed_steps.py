@@ -42,3 +42,22 @@ def test_steps_on_the_general_kernel_have_the_slices_of_every_context_of_their_t
     longest = max(CONTEXTS)
     found = first[mixer.step_tags(StepFacts(n, n, True, longest))]
     assert PackedKV._splits(n, nkv, context_tiles(found) * TILE_KEYS, 0) == PackedKV._splits(n, nkv, longest, 0)
+
+
+@pytest.mark.parametrize("given", [True, False])
+def test_a_list_made_by_the_call_itself_is_not_read_early(monkeypatch, given):
+    """Rows through cu_q_lens, more tokens than a launch takes: without seqs the call makes that list on the stream, so the launches wait for it."""
+    from gollmgo_b200.cache import PackedKV
+
+    class NoDevice(PackedKV):
+        def __init__(self):
+            self.head_dim, self.page_size, self.bits, self.kv_heads, self._sms = 64, 16, 4, 1, 148
+            self.pages = None
+    seen = []
+    monkeypatch.setattr(ops, "packed_decode_mma", lambda q, pages, tables, cu, ctx, seqs, n, *more: seen.append((seqs.tolist(), more[-1])))
+    n = ops.PACKED_DECODE_TOKENS + 3
+    lists = torch.arange(n + 1, dtype=torch.int32)
+    NoDevice().decode(torch.zeros(n, 2, 64, dtype=torch.bfloat16), torch.zeros(n, 4, dtype=torch.int32), lists[:n], 40, 0.1, cu_q_lens=lists,
+                      seqs=lists[:n] if given else None, early=True)
+    assert [b for part, _ in seen for b in part] == list(range(n))
+    assert [early for _, early in seen] == [given, given]
