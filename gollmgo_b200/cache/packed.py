@@ -6,15 +6,27 @@ block tables are the cache manager's, as of an unpacked layer.  The reference en
 """
 from __future__ import annotations
 
+import os
 from typing import Optional, Sequence
 
 import torch
 
 from ..csrc import ops
 
-SHORT_PROMPT_KEYS = 256        # as in parts/attention.py
+# as in parts/attention.py, which says what they do and what was measured
+ATTN_POLICY = os.environ.get("GOLLMGO_B200_ATTN", "auto")
+SHORT_PROMPT_KEYS = int(os.environ.get("GOLLMGO_B200_ATTN_SHORT_KEYS", "256"))
 SCRATCH_TOKENS = 65536         # tokens that prefill() reads back at a time (one sequence may be longer)
 MOST_SEQUENCES = 1024          # ... of so many sequences
+
+
+def long_tiles(options: bool, tiles128: int, num_heads: int, window: int, longest: int, num_sms: int) -> bool:
+    """Whether the prompt kernels on tcgen05 take portions that make ``tiles128`` tiles of 128 rows, the longest with ``longest`` keys: the line
+    of the attention layer, for plain scores (Attention._few_short_tiles) and for ones with ``options`` (Attention.long_tiles)."""
+    reach = (window or 1 << 30) if options else 1 << 30
+    if options and (reach < 128 or longest <= 144):
+        return False
+    return tiles128 * ((num_heads + 1) // 2) * 2 > num_sms or min(longest, reach) > SHORT_PROMPT_KEYS
 
 
 class PackedKV:
@@ -198,10 +210,10 @@ class PackedKV:
         if hi - lo != tables.shape[0]:
             tables, context_lens, cu_q_lens = tables[lo:hi], context_lens[lo:hi], cu_q_lens[lo:hi + 1]
         B, width = tables.shape
-        fast = q.dtype == torch.bfloat16 and d in (64, 128) and q.stride(0) % 8 == 0 and q.data_ptr() % 16 == 0
+        options = softcap > 0 or sink is not None or slopes is not None or temperature is not None
+        fast = q.dtype == torch.bfloat16 and d in (64, 128) and q.stride(0) % 8 == 0 and q.data_ptr() % 16 == 0 and ATTN_POLICY != "general"
         lists = [(64, counts[1])] if fast else [(16, counts[0])]
-        # the line between the tcgen05 and the mma.sync prompt kernels is the attention layer's: few tiles of few keys
-        if fast and (counts[2] * ((nh + 1) // 2) * 2 > self._sms or min(longest, window or longest) > SHORT_PROMPT_KEYS):
+        if fast and ATTN_POLICY == "auto" and long_tiles(options, counts[2], nh, window, longest, self._sms):
             lists.append((128, counts[2]))
         k, v = torch.empty(2, pages, self.kv_heads, P, d, dtype=q.dtype, device=q.device).unbind(0)
         ints = torch.empty(B * width + 2 * sum(n for _, n in lists), dtype=torch.int32, device=q.device)
@@ -215,7 +227,7 @@ class PackedKV:
         t16, t64 = ((None, None, 0), (seq0, q00, n0)) if fast else ((seq0, q00, n0), (None, None, 0))
         long = dict(tile128_seq=full[1][2], tile128_q0=full[1][3], num_tiles128=full[1][1]) if len(full) > 1 else {}
         with ops.after_everything():               # the prompt kernels read early what packed_unfold has just written
-            if softcap > 0 or sink is not None or slopes is not None or temperature is not None:
+            if options:
                 ops.attn_prefill_x(q, q.stride(0), k, v, plain, width, cu_q_lens, context_lens, *t16, out, nh, self.kv_heads, d, d, 1, P,
                                    window, scale, softcap, *t64, allow_mma=fast, sink=sink, slopes=slopes, temperature=temperature, **long)
             else:

@@ -144,3 +144,53 @@ def test_portions_of_more_rows_than_q_has_are_refused(rows, q_lens, dtype):
     lists = torch.zeros(B + 1, dtype=torch.int32), torch.zeros(B, dtype=torch.int32)
     with pytest.raises(ops.KernelError, match="rows in q"):
         NoDevice().prefill(torch.zeros(rows, 2, 64, dtype=dtype), torch.zeros(B, 4, dtype=torch.int32), *lists, q_lens, [20] * B, 1.0)
+
+
+# ---------------------------------------------------------------- which prompt kernel
+SHAPES = [([3], [0]), ([40], [0]), ([100], [40]), ([144], [0]), ([145], [0]), ([256], [0]), ([257], [0]), ([64], [193]), ([700], [0]), ([20] * 30, [0] * 30),
+          ([100] * 12, [0] * 12), ([200] * 12, [0] * 12), ([30, 90], [3000, 0]), ([2048], [0])]
+
+
+@pytest.mark.parametrize("nh", [2, 8, 16, 32])
+@pytest.mark.parametrize("window", [None, 64, 127, 128, 200, 256, 1000])
+@pytest.mark.parametrize("options", [False, True])
+def test_the_line_between_the_prompt_kernels_is_the_attention_layers(nh, window, options):
+    from types import SimpleNamespace
+
+    from gollmgo_b200.cache import packed
+    from gollmgo_b200.parts import BuildContext, PartSpec, build_mixer
+    from gollmgo_b200.parts.attention import TILES_TC_X
+    spec = PartSpec("attention", dict(hidden_size=64, num_heads=nh, num_kv_heads=nh // 2, head_dim=64, window=window, position=PartSpec("none"), sink=options))
+    plain_layer = build_mixer(spec, BuildContext(torch.bfloat16, "cpu", 64, 4, 16))
+    for q_lens, q_starts in SHAPES:
+        tiles = sum(-(-a // 128) for a in q_lens)
+        batch = SimpleNamespace(q_lens=q_lens, q_starts=q_starts, tiles={})
+        if options:
+            chosen = TILES_TC_X.chosen(range(len(q_lens)), q_lens, q_starts)
+            batch.tiles[TILES_TC_X] = SimpleNamespace(count=tiles if chosen else 0, seq=None, q0=None)
+            want = bool(plain_layer.long_tiles(batch))
+        else:
+            want = not plain_layer._few_short_tiles(tiles, batch)
+        longest = max(a + s for a, s in zip(q_lens, q_starts))
+        assert packed.long_tiles(options, tiles, nh, window or 0, longest, plain_layer.num_sms) == want, (q_lens, q_starts)
+
+
+@pytest.mark.parametrize("policy,lists,mma", [("auto", [64, 128], True), ("mma", [64], True), ("general", [16], False)])
+@pytest.mark.parametrize("options", [False, True])
+def test_the_switch_of_the_prompt_kernels_holds_for_portions(monkeypatch, policy, lists, mma, options):
+    from gollmgo_b200.cache import packed
+    from gollmgo_b200.csrc import ops
+    seen = {}
+    monkeypatch.setattr(packed, "ATTN_POLICY", policy)
+    monkeypatch.setattr(ops, "packed_prefill_rows", lambda *a: None)
+    monkeypatch.setattr(ops, "packed_unfold", lambda *a, **k: seen.update(lists=[h for h, *_ in a[8]]))
+    monkeypatch.setattr(ops, "attn_prefill", lambda *a, **k: seen.update(kernel=False, **k))
+    monkeypatch.setattr(ops, "attn_prefill_x", lambda *a, **k: seen.update(kernel=True, **k))
+
+    class NoDevice(PackedKV):
+        def __init__(self):
+            self.head_dim, self.page_size, self.bits, self.kv_heads, self._sms = 64, 16, 4, 1, 148
+            self.pages = None
+    NoDevice().prefill(torch.zeros(400, 2, 64, dtype=torch.bfloat16), torch.zeros(1, 25, dtype=torch.int32), torch.tensor([0, 400], dtype=torch.int32),
+                       torch.tensor([400], dtype=torch.int32), [400], [400], 0.1, sink=torch.zeros(2) if options else None)
+    assert seen["lists"] == lists and seen["kernel"] == options and seen["allow_mma"] == mma and ("tile128_seq" in seen) == (128 in lists)
