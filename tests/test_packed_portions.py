@@ -104,30 +104,146 @@ def test_portions_among_many_decoding_sequences(bits, dtype, d, counts):
     assert bool((out[mark] == 9.0).all())
 
 
-def tolerance(q, keys, values, context, scale, dtype, tensor_cores):
-    """How far a row may be from attend(): S(j) = sum over channels of |q k| scale, P = the weights.
+def tolerance(q, keys, values, context, scale, dtype, tensor_cores, window=0, softcap=0.0, sink=None, slopes=None, temperature=None):
+    """How far a row may be from attend(): S(j) = sum over channels of |q k| scale, P = the weights.  A score that moves by m(j) moves the
+    output by sum P m |v - out|.
     float32: products of d terms, d roundings of 2^-24 of S at most, and those of the exponential, of the sum over the context and of the output.
-    bfloat16: a key rounds as it is read back, so a score moves by 2^-8 S (and weights move by
-    as much relative to themselves), a weight and a value round once (2^-8 each, relative to sum P |v|), and the result rounds once.  On the
-    general kernel weights stay float32."""
+    On the tensor cores a key is not one number there but s (c - M) + (o + M s) with the middle code M, two sums that are made apart and may cancel.
+    Of a group whose largest value is G, |o + M s| <= 1.01 G (it lies inside the codes' range, whose end is at most a bfloat16 step of the scale
+    beyond the largest value) and |s (c - M)| <= 1.01 x 8 / 15 x 2 G, so roundings are relative to 2.1 G in the place of |k|, and of |v| alike.
+    bfloat16: a key rounds as it is read back, so a score moves by 2^-8 S, a weight and a value round once (2^-8 each, relative to sum P |v|;
+    on the general kernel weights stay float32), and the result rounds once.  A cap is a tanh of the special-function unit there: 2^-11 of the
+    capped score.  A bias by distance rounds in float32."""
     a, nh, d = q.shape
     group = nh // keys.shape[1]
     tol = torch.zeros(a, nh, d, dtype=torch.float64)
+    fast = dtype == torch.bfloat16 and tensor_cores
     half = 2.0 ** -8 if dtype == torch.bfloat16 else 0.0
-    for i in range(a):
-        p = context - a + i
-        for h in range(nh):
-            k, v = keys[:p + 1, h // group], values[:p + 1, h // group]
-            z = k @ q[i, h].double() * scale
-            size = (k.abs() @ q[i, h].double().abs()) * abs(scale)
-            w = torch.softmax(z, 0)
-            move = size * (half + (d + 4) * 2.0 ** -24)                # of each score
-            mean = (w @ v).abs()
-            # d out = sum_j P_j dz_j (v_j - out): each term apart
-            spread = (w * move) @ (v - (w @ v)).abs()
-            rounds = (half * (2 if tensor_cores else 1) + (p + 8) * 2.0 ** -24) * (w @ v.abs())
-            tol[i, h] = 1.05 * (spread + rounds) + torch.finfo(dtype).eps / 2 * mean + 1e-30
+    at, j = torch.arange(context - a, context)[:, None], torch.arange(context)[None]
+    seen = (j <= at) & ((at - j < window) if window else True)
+    factor = torch.full((a, 1), float(scale), dtype=torch.float64)
+    if temperature:
+        factor = factor * (1.0 + temperature[0] * torch.log(torch.floor((at + 1).double() / temperature[1]) + 1.0))
+    for h in range(nh):
+        k, v, x = keys[:, h // group], values[:, h // group], q[:, h].double()
+        size_k, size_v = k.abs(), v.abs()
+        if dtype == torch.float32 and tensor_cores:
+            size_k, size_v = ((2.1 * y.abs().view(context, d // 64, 64).amax(2, keepdim=True)).expand(-1, -1, 64).reshape(context, d) for y in (k, v))
+        z, move = x @ k.T * factor, x.abs() @ size_k.T * factor.abs() * (half + (d + 8) * 2.0 ** -24)
+        if softcap > 0:
+            z = softcap * torch.tanh(z / softcap)
+            move = move + z.abs() * (1.1 * 2.0 ** -11 if fast else 2.0 ** -21)
+        if slopes is not None:
+            z = z - slopes[h].double() * (at - j)
+            move = move + (z.abs() + slopes[h].double() * (at - j).abs()) * 2.0 ** -22
+        move = move + (z.abs() + 1.0) * 2.0 ** -22                     # the exponential and its argument
+        z = z.masked_fill(~seen, -float("inf"))
+        if sink is not None:
+            z = torch.cat([z, sink[h].double().expand(a, 1)], 1)
+        w = torch.softmax(z, 1)[:, :context]
+        out = w @ v
+        spread = torch.einsum("ij,ijc->ic", w * move.masked_fill(~seen, 0.0), (v[None] - out[:, None]).abs()) + 2.0 ** -21 * out.abs()
+        rounds = (half * (2 if tensor_cores else 1) + (context + 8) * 2.0 ** -24) * (w @ size_v)
+        tol[:, h] = 1.05 * (spread + rounds) + torch.finfo(dtype).eps / 2 * out.abs() + 1e-30
     return tol
+
+
+OPTIONS = [dict(), dict(window=20), dict(softcap=5.0), dict(sink=True), dict(slopes=True, window=33, sink=True, temperature=(0.1, 16)), dict(slopes=True, window=130)]
+
+
+Q_LENS, LENS = [5, 1, 33, 16, 2, 70, 150], [5, 40, 90, 16, 65, 140, 301]
+
+
+def pointed_portions(bits, dtype, option, nh, nkv, d, seed):
+    """Queries, keys and values as they come, what the cache holds of them, and the options.  Every second row attends to one key nearly alone:
+    its own, the first in sight or one between, so that a key that is left out, doubled or taken for another shows."""
+    g = torch.Generator().manual_seed(seed)
+    o = dict(OPTIONS[option])
+    if o.get("sink"):
+        o["sink"] = torch.randn(nh, generator=g)
+    if o.get("slopes"):
+        o["slopes"] = torch.tensor([2.0 ** (-8.0 * (h + 1) / nh) for h in range(nh)])
+    cu = torch.tensor([0] + Q_LENS).cumsum(0).to(torch.int32)
+    q = torch.randn(int(cu[-1]), nh, d, generator=g)
+    rows, held = [], []
+    for b, n in enumerate(LENS):
+        rows.append(torch.randn(n, 2 * nkv * d, generator=g).to(dtype))
+        held.append([plain.through(y.double().view(n, nkv, d), bits) for y in rows[b].chunk(2, 1)])
+        for i in range(0, Q_LENS[b], 2):
+            p = n - Q_LENS[b] + i
+            lo = max(0, p - o["window"] + 1) if o.get("window") else 0
+            to = (p, lo, (p + lo) // 2)[i // 2 % 3]
+            q[cu[b] + i] = held[b][0][to].float().repeat_interleave(nh // nkv, 0) * (200.0 / d) ** 0.5
+    return q.to(dtype), cu, rows, held, o
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("dtype,policy", [(torch.bfloat16, "auto"), (torch.bfloat16, "mma"), (torch.bfloat16, "general"), (torch.float32, "auto")])
+@pytest.mark.parametrize("option", range(len(OPTIONS)))
+@pytest.mark.parametrize("nh,nkv,d,page", [(4, 1, 64, 16), (4, 2, 128, 16), (3, 3, 128, 32), (4, 2, 128, 8), (2, 1, 64, 128), (4, 2, 96, 16), (3, 1, 16, 4)])
+def test_portions_are_as_near_as_their_roundings(monkeypatch, bits, dtype, policy, option, nh, nkv, d, page):
+    from gollmgo_b200.cache import packed
+    monkeypatch.setattr(packed, "ATTN_POLICY", policy)
+    q, cu, rows, held, o = pointed_portions(bits, dtype, option, nh, nkv, d, d + option)
+    counts = [-(-n // page) for n in LENS]
+    tables = torch.full((len(LENS), max(counts) + 1), -1, dtype=torch.int32)
+    order = torch.randperm(sum(counts), generator=torch.Generator().manual_seed(d)).to(torch.int32).split(counts)
+    kv = PackedKV.empty(sum(counts), nkv, d, page, bits)
+    kv.pages.fill_(255)                                                        # (NaN where nothing is written)
+    for b, n in enumerate(LENS):
+        tables[b, :counts[b]] = order[b]
+        t = torch.arange(n)
+        kv.write(rows[b].cuda(), None, (tables[b][t // page].long() * page + t % page).to(torch.int32).cuda(), 0)
+    dev = lambda x: torch.tensor(x, dtype=torch.int32).cuda()  # noqa: E731
+    on_device = {k: v.cuda() if torch.is_tensor(v) else v for k, v in o.items()}
+    out = kv.prefill(q.cuda(), tables.cuda(), cu.cuda(), dev(LENS), Q_LENS, LENS, d ** -0.5, **on_device).cpu().double()
+    for b, n in enumerate(LENS):
+        x = q[cu[b]:cu[b + 1]]
+        ref = plain.attend(x.double(), *held[b], n, d ** -0.5, **o)
+        tol = tolerance(x, *held[b], n, d ** -0.5, dtype, d in (64, 128) and policy != "general", **o)
+        assert ((out[cu[b]:cu[b + 1]] - ref).abs() <= tol).all(), (b, n)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("option", range(len(OPTIONS)))
+@pytest.mark.parametrize("mistake", ["zeros", "scale", "last key", "first key", "next head", "window"])
+def test_the_tolerance_of_portions_tells_mistakes(dtype, option, mistake):
+    """What test_portions_are_as_near_as_their_roundings allows, against attention with a mistake in it: in every portion of some rows it shows."""
+    nh, nkv, d = 2, 2, 64
+    q, cu, _, held, o = pointed_portions(4, dtype, option, nh, nkv, d, 5)
+    if mistake == "window" and not o.get("window"):
+        return
+    for b, n in enumerate(LENS):
+        x, (k, v) = q[cu[b]:cu[b + 1]], held[b]
+        if x.shape[0] < 5 or n > 140:
+            continue
+        ref = plain.attend(x.double(), k, v, n, d ** -0.5, **o)
+        tol = tolerance(x, k, v, n, d ** -0.5, dtype, True, **o)
+        scale, wrong = d ** -0.5, dict(o)
+        if mistake == "scale":
+            scale *= 0.7
+        if mistake == "window":
+            wrong["window"] -= 1
+            if n <= o["window"]:
+                continue
+        if mistake == "next head":
+            k, v = k.flip(1), v.flip(1)
+        got = plain.attend(x.double(), k, v, n, scale, **wrong)
+        if mistake == "zeros":
+            got = torch.zeros_like(ref)
+        if mistake in ("last key", "first key"):        # of each row: as if it stood at its neighbour's place
+            k2, v2 = k.clone(), v.clone()
+            i = x.shape[0] - 1 - (x.shape[0] - 1) % 6 if mistake == "last key" else None
+            if mistake == "last key":                   # a row that points to its own key sees the one before instead
+                at = n - x.shape[0] + i
+            else:                                       # the last row but some that points to the first key in sight
+                i = max(j for j in range(0, x.shape[0], 2) if j // 2 % 3 == 1)
+                at = max(0, n - x.shape[0] + i - o["window"] + 1) if o.get("window") else 0
+            k2[at], v2[at] = k[at + (1 if at + 1 < n else -1)], v[at + (1 if at + 1 < n else -1)]
+            got = plain.attend(x.double(), k2, v2, n, scale, **o)
+        bad = ((got - ref).abs() > tol).any(-1).any(-1)
+        assert bad.any(), (b, n)
 
 
 @pytest.mark.parametrize("rows,q_lens", [(3, [4]), (0, [1]), (9, [5, 5]), (9, [1, 9]), (9, [0, 10, -3])])
