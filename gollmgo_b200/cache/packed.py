@@ -210,7 +210,8 @@ class PackedKV:
         if hi - lo != tables.shape[0]:
             tables, context_lens, cu_q_lens = tables[lo:hi], context_lens[lo:hi], cu_q_lens[lo:hi + 1]
         B, width = tables.shape
-        options = softcap > 0 or sink is not None or slopes is not None or temperature is not None
+        # (the plain tcgen05 kernel takes the largest product for the largest score)
+        options = softcap > 0 or sink is not None or slopes is not None or temperature is not None or not scale > 0
         fast = q.dtype == torch.bfloat16 and d in (64, 128) and q.stride(0) % 8 == 0 and q.data_ptr() % 16 == 0 and ATTN_POLICY != "general"
         lists = [(64, counts[1])] if fast else [(16, counts[0])]
         if fast and ATTN_POLICY == "auto" and long_tiles(options, counts[2], nh, window, longest, self._sms):

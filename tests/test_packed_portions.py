@@ -310,3 +310,31 @@ def test_the_switch_of_the_prompt_kernels_holds_for_portions(monkeypatch, policy
     NoDevice().prefill(torch.zeros(400, 2, 64, dtype=torch.bfloat16), torch.zeros(1, 25, dtype=torch.int32), torch.tensor([0, 400], dtype=torch.int32),
                        torch.tensor([400], dtype=torch.int32), [400], [400], 0.1, sink=torch.zeros(2) if options else None)
     assert seen["lists"] == lists and seen["kernel"] == options and seen["allow_mma"] == mma and ("tile128_seq" in seen) == (128 in lists)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("scale", [-0.3, 0.0])
+@pytest.mark.parametrize("nh,nkv,d", [(4, 2, 64), (4, 1, 128), (3, 3, 128), (2, 1, 96)])
+def test_portions_with_a_scale_that_is_not_positive(bits, dtype, scale, nh, nkv, d):
+    q_lens, lens, page = [5, 40, 290], [5, 90, 300], 16
+    g = torch.Generator().manual_seed(d)
+    counts = [-(-n // page) for n in lens]
+    tables = torch.zeros(len(lens), max(counts), dtype=torch.int32)
+    for b, order in enumerate(torch.randperm(sum(counts), generator=g).to(torch.int32).split(counts)):
+        tables[b, :counts[b]] = order
+    kv = PackedKV.empty(sum(counts), nkv, d, page, bits)
+    cu = torch.tensor([0] + q_lens).cumsum(0).to(torch.int32)
+    q = torch.randn(int(cu[-1]), nh, d, generator=g).to(dtype)
+    held = []
+    for b, n in enumerate(lens):
+        x = torch.randn(n, 2 * nkv * d, generator=g).to(dtype)
+        t = torch.arange(n)
+        kv.write(x.cuda(), None, (tables[b][t // page].long() * page + t % page).to(torch.int32).cuda(), 0)
+        held.append([plain.through(y.double().view(n, nkv, d), bits) for y in x.chunk(2, 1)])
+    out = kv.prefill(q.cuda(), tables.cuda(), cu.cuda(), torch.tensor(lens, dtype=torch.int32).cuda(), q_lens, lens, scale).cpu().double()
+    for b, n in enumerate(lens):
+        x = q[cu[b]:cu[b + 1]]
+        ref = plain.attend(x.double(), *held[b], n, scale)
+        assert ((out[cu[b]:cu[b + 1]] - ref).abs() <= tolerance(x, *held[b], n, scale, dtype, d in (64, 128))).all(), b
