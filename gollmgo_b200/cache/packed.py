@@ -209,14 +209,22 @@ class PackedKV:
         ops.packed_prefill_rows(q, out, self.pages, nh, d, sink, slopes)
         if hi - lo != tables.shape[0]:
             tables, context_lens, cu_q_lens = tables[lo:hi], context_lens[lo:hi], cu_q_lens[lo:hi + 1]
-        B, width = tables.shape
         # (the plain tcgen05 kernel takes the largest product for the largest score)
         options = softcap > 0 or sink is not None or slopes is not None or temperature is not None or not scale > 0
         fast = q.dtype == torch.bfloat16 and d in (64, 128) and q.stride(0) % 8 == 0 and q.data_ptr() % 16 == 0 and ATTN_POLICY != "general"
-        lists = [(64, counts[1])] if fast else [(16, counts[0])]
-        if fast and ATTN_POLICY == "auto" and long_tiles(options, counts[2], nh, window, longest, self._sms):
+        if not fast:                               # on the codes where they lie, in float32 arithmetic
+            n = counts[0]
+            ints = torch.empty(2 * n, dtype=torch.int32, device=q.device)
+            ops.packed_unfold(self.pages, tables, cu_q_lens, context_lens, None, None, 0, None, [(16, n, ints[:n], ints[n:])], self.kv_heads, d, P,
+                              self.bits, window, least)
+            ops.packed_prefill(q, self.pages, tables, cu_q_lens, context_lens, ints[:n], ints[n:], n, out, nh, self.kv_heads, d, P, self.bits,
+                               window, scale, softcap, sink, slopes, temperature)
+            return
+        lists = [(64, counts[1])]
+        if ATTN_POLICY == "auto" and long_tiles(options, counts[2], nh, window, longest, self._sms):
             lists.append((128, counts[2]))
         k, v = torch.empty(2, pages, self.kv_heads, P, d, dtype=q.dtype, device=q.device).unbind(0)
+        B, width = tables.shape
         ints = torch.empty(B * width + 2 * sum(n for _, n in lists), dtype=torch.int32, device=q.device)
         at, full = B * width, []
         for h, n in lists:
@@ -224,16 +232,15 @@ class PackedKV:
             at += 2 * n
         plain = ints[:B * width]
         ops.packed_unfold(self.pages, tables, cu_q_lens, context_lens, k, v, most, plain, full, self.kv_heads, d, P, self.bits, window, least)
-        _, n0, seq0, q00 = full[0]
-        t16, t64 = ((None, None, 0), (seq0, q00, n0)) if fast else ((seq0, q00, n0), (None, None, 0))
+        t64 = (full[0][2], full[0][3], full[0][1])
         long = dict(tile128_seq=full[1][2], tile128_q0=full[1][3], num_tiles128=full[1][1]) if len(full) > 1 else {}
         with ops.after_everything():               # the prompt kernels read early what packed_unfold has just written
             if options:
-                ops.attn_prefill_x(q, q.stride(0), k, v, plain, width, cu_q_lens, context_lens, *t16, out, nh, self.kv_heads, d, d, 1, P,
-                                   window, scale, softcap, *t64, allow_mma=fast, sink=sink, slopes=slopes, temperature=temperature, **long)
+                ops.attn_prefill_x(q, q.stride(0), k, v, plain, width, cu_q_lens, context_lens, None, None, 0, out, nh, self.kv_heads, d, d, 1, P,
+                                   window, scale, softcap, *t64, sink=sink, slopes=slopes, temperature=temperature, **long)
             else:
-                ops.attn_prefill(q, q.stride(0), k, v, plain, width, cu_q_lens, context_lens, *t16, out, nh, self.kv_heads, d, P, window,
-                                 scale, *t64, allow_mma=fast, allow_tc=bool(long), **long)
+                ops.attn_prefill(q, q.stride(0), k, v, plain, width, cu_q_lens, context_lens, None, None, 0, out, nh, self.kv_heads, d, P, window,
+                                 scale, *t64, allow_tc=bool(long), **long)
 
     @staticmethod
     def scratch_bytes(needs, max_context: int, dtype) -> int:

@@ -66,9 +66,29 @@ __device__ __forceinline__ void attn_tile(const AttnArgs& a, int nrows, const TA
         const PackedRows r(a.packed_bits, d, ps);
         const bool there = page >= 0 && page < a.num_pages;
         const unsigned char* block = (const unsigned char*)a.kcache + ((size_t)(there ? page : 0) * a.nkv + kvh) * r.page_bytes();
-        for (int c = lane; c < d; c += 32) {
-          Ks[j * (d + 1) + c] = there ? r.value(block, 0, tok % ps, c) : 0.f;
-          Vs[j * dv + c] = there ? r.value(block, 1, tok % ps, c) : 0.f;
+        const unsigned char *kq = block + r.codes(0, tok % ps), *vq = block + r.codes(1, tok % ps);
+        const unsigned char *kp = block + r.pairs(0, tok % ps), *vp = block + r.pairs(1, tok % ps);
+        // (all of a row's loads before the first is used)
+        constexpr int STEPS = DMAX / 32;
+        unsigned kcode[STEPS], vcode[STEPS], kpair[STEPS], vpair[STEPS];
+#pragma unroll
+        for (int i = 0; i < STEPS; ++i) {
+          const int c = lane + 32 * i, at = a.packed_bits == 4 ? c >> 1 : c, pair = (c / r.group) * 4;
+          const bool in = there && c < d;
+          kcode[i] = in ? kq[at] : 0u;
+          vcode[i] = in ? vq[at] : 0u;
+          kpair[i] = in ? *reinterpret_cast<const unsigned*>(kp + pair) : 0u;
+          vpair[i] = in ? *reinterpret_cast<const unsigned*>(vp + pair) : 0u;
+        }
+        const int shift = a.packed_bits == 4 ? (lane & 1) * 4 : 0;
+        const unsigned mask = a.packed_bits == 4 ? 15u : 255u;
+#pragma unroll
+        for (int i = 0; i < STEPS; ++i) {
+          const int c = lane + 32 * i;
+          if (c < d) {
+            Ks[j * (d + 1) + c] = fmaf(__uint_as_float(kpair[i] << 16), (float)((kcode[i] >> shift) & mask), __uint_as_float(kpair[i] & 0xffff0000u));
+            Vs[j * dv + c] = fmaf(__uint_as_float(vpair[i] << 16), (float)((vcode[i] >> shift) & mask), __uint_as_float(vpair[i] & 0xffff0000u));
+          }
         }
       } else if (page >= 0) {
         const size_t base = (((size_t)page * a.nkv + kvh) * ps + (tok % ps)) * d;
@@ -166,7 +186,7 @@ __device__ __forceinline__ const float* attn_tile_max(const AttnArgs& a, const f
 }
 
 // ---------------------------------------------------------------- prompt portions
-template <typename TA, int DMAX>
+template <typename TA, int DMAX, bool PACKED>
 __global__ void __launch_bounds__(ATT_THREADS) attn_prefill_kernel(AttnArgs a) {
   constexpr int NACC = ATT_BQ * DMAX / ATT_THREADS;
   extern __shared__ float smem[];
@@ -193,7 +213,7 @@ __global__ void __launch_bounds__(ATT_THREADS) attn_prefill_kernel(AttnArgs a) {
   int lo = a.window > 0 ? max(0, first - a.window + 1) : 0;
   if (a.chunk > 0) lo = max(lo, (first / a.chunk) * a.chunk);       // the chunk of the tile's first row starts earliest
   float acc[NACC];
-  attn_tile<TA, DMAX, false>(a, nrows, qptr_s, pos_s, head_s, scale_s, kvh, a.block_tables + (size_t)b * a.bt_stride, lo, last + 1,
+  attn_tile<TA, DMAX, PACKED>(a, nrows, qptr_s, pos_s, head_s, scale_s, kvh, a.block_tables + (size_t)b * a.bt_stride, lo, last + 1,
                       min(a.keep_first, lo), smem, acc);
   pdl_trigger();
   float* m_s = const_cast<float*>(attn_tile_max(a, smem));
@@ -222,8 +242,9 @@ __global__ void __launch_bounds__(ATT_THREADS) attn_prefill_kernel(AttnArgs a) {
       const int r = e / dv, c = e - r * dv;
       if (r < nrows) {
         const size_t at = (size_t)(t0 + q0 + r) * a.nh * dv + (size_t)h * dv + c;
-        if (a.out_f32) ((float*)a.out)[at] = acc[i] / l_s[r];
-        else ((TA*)a.out)[at] = from_f32<TA>(acc[i] / l_s[r]);
+        const float o = PACKED && l_s[r] == 0.f ? 0.f : acc[i] / l_s[r];        // (pages that are not in the pool: no key may be left)
+        if (a.out_f32) ((float*)a.out)[at] = o;
+        else ((TA*)a.out)[at] = from_f32<TA>(o);
       }
     }
   }
@@ -361,7 +382,7 @@ template <typename K> static int set_smem(K kernel, size_t bytes, const char* wh
     if (rc) return rc;                                                                         \
     gg_launch(KERNEL, dim3(grid), dim3(ATT_THREADS), smem, stream, a);                         \
   } while (0)
-// KERNEL<type, largest head size[, PACKED]>
+// KERNEL<type, largest head size, PACKED>
 #define ATT_SIZES(KERNEL, TA, grid, who, ...)                                                  \
   do {                                                                                         \
     const int dvv = a.dv > 0 ? a.dv : a.d;                                                     \
@@ -375,8 +396,10 @@ int attn_prefill_general(const AttnArgs& a, int dtype, int num_tiles, cudaStream
   GG_REQUIRE(num_tiles >= 0 && a.nh <= 65535, "attn_prefill: bad grid %d x %d", num_tiles, a.nh);
   if (num_tiles == 0) return GG_OK;
   dim3 grid(num_tiles, a.nh);
-  if (dtype == GG_F32) ATT_SIZES(attn_prefill_kernel, float, grid, "attn_prefill");
-  else if (dtype == GG_BF16) ATT_SIZES(attn_prefill_kernel, __nv_bfloat16, grid, "attn_prefill");
+  if (dtype == GG_F32 && a.packed_bits) ATT_SIZES(attn_prefill_kernel, float, grid, "attn_prefill", true);
+  else if (dtype == GG_F32) ATT_SIZES(attn_prefill_kernel, float, grid, "attn_prefill", false);
+  else if (dtype == GG_BF16 && a.packed_bits) ATT_SIZES(attn_prefill_kernel, __nv_bfloat16, grid, "attn_prefill", true);
+  else if (dtype == GG_BF16) ATT_SIZES(attn_prefill_kernel, __nv_bfloat16, grid, "attn_prefill", false);
   else return gg_fail(GG_ERR_INVALID, "attn_prefill: unknown dtype %d", dtype);
   return gg_check_launch("attn_prefill");
 }

@@ -46,7 +46,7 @@ struct AttnArgs {
   const float* slopes;      // [nh] or null: slopes[h] * (i - j) is taken off the scaled score (softmax weights)
   float temp_coef;          // the query at position p is multiplied by 1 + temp_coef * ln(floor((p + 1) / temp_every) + 1)
   float temp_every;         // (0: it is not; softmax weights).  Applied to the score's scale, so q is not rounded once more
-  // a packed cache (packed_kv.cuh; the general decode kernel with PACKED): kcache is then its pages, vcache unused
+  // a packed cache (packed_kv.cuh; the general kernels with PACKED): kcache is then its pages, vcache unused
   int packed_bits;          // 4 or 8; 0 = keys and values as they are
   int num_pages;            // pages of a packed cache: an id outside reads as a page that was given back
   int num_seqs;             // rows of its block tables: a dec_seqs entry outside is padding

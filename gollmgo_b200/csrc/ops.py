@@ -1548,6 +1548,7 @@ _PACKED_TYPES = {
     "gg_packed_decode_tokens": [_I, _I, _I],
     "gg_packed_prompt_fold": [_I, _I],
     "gg_packed_prompt_f32": [_P, _L, _P, _I, _P, _I, _I, _P, _P, _I, _I, _P, _I, _P, _L, _P, _I, _I, _I, _I, _I, _I, _F, _F, _P, _P, _F, _F, _P],
+    "gg_packed_prefill": [_P, _L, _I, _P, _I, _P, _I, _P, _P, _P, _P, _I, _P, _I, _I, _I, _I, _I, _I, _F, _F, _P, _P, _F, _F, _P],
     "gg_packed_unfold": [_P, _I, _P, _I, _P, _P, _I, _P, _P, _I, _I, _I, _P, _I, _I, _P, _P, _I, _I, _P, _P, _I, _I, _I, _I, _I, _I, _P],
 }
 _PACKED = {}
@@ -1657,6 +1658,25 @@ def packed_prefill_rows(q, out, pages, nh: int, d: int, sink=None, slopes=None) 
     _stream_of("prefill", q, out, pages, sink, slopes)
     dtype_code(q.dtype)
     _packed_q("prefill", q, out, nh, d)
+
+
+def packed_prefill(q: torch.Tensor, pages: torch.Tensor, tables: torch.Tensor, cu_q_lens: torch.Tensor, context_lens: torch.Tensor,
+                   tile_seq: torch.Tensor, tile_q0: torch.Tensor, tiles: int, out: torch.Tensor, nh: int, nkv: int, d: int, page_size: int,
+                   bits: int, window: int, scale: float, softcap: float = 0.0, sink: Optional[torch.Tensor] = None,
+                   slopes: Optional[torch.Tensor] = None, temperature=None) -> None:
+    """attn_prefill_x over a packed cache on the general kernel (float32 arithmetic on what the codes stand for): tiles of 16 query rows."""
+    stream = _stream_of("packed_prefill", q, pages, tables, cu_q_lens, context_lens, tile_seq, tile_q0, out, sink, slopes)
+    stride = _packed_q("packed_prefill", q, out, nh, d)
+    _attn_extras(nh, None, None, None, sink, slopes)
+    B, width = _tables("packed_prefill", tables)
+    _ints("packed_prefill", B, context_lens)
+    _ints("packed_prefill", B + 1, cu_q_lens)
+    _ints("packed_prefill", tiles, tile_seq, tile_q0)
+    coef, every = temperature or (0.0, 0.0)
+    _check(_packed("gg_packed_prefill")(q.data_ptr(), stride, dtype_code(q.dtype), pages.data_ptr(), pages.shape[0], tables.data_ptr(), width,
+                                        cu_q_lens.data_ptr(), context_lens.data_ptr(), tile_seq.data_ptr(), tile_q0.data_ptr(), tiles,
+                                        out.data_ptr(), nh, nkv, d, page_size, bits, window, scale, softcap, _at(sink), _at(slopes), coef,
+                                        every, stream))
 
 
 def _packed_tokens(what, q, cu_q_lens, context_lens, seqs, n, B):
@@ -1792,17 +1812,19 @@ def after_everything():
         pause(0)
 
 
-def packed_unfold(pages: torch.Tensor, tables: torch.Tensor, cu_q_lens: torch.Tensor, context_lens: torch.Tensor, k_out: torch.Tensor,
-                  v_out: torch.Tensor, most_pages: int, out_tables: torch.Tensor, lists, nkv: int, d: int, page_size: int, bits: int,
+def packed_unfold(pages: torch.Tensor, tables: torch.Tensor, cu_q_lens: torch.Tensor, context_lens: torch.Tensor, k_out: Optional[torch.Tensor],
+                  v_out: Optional[torch.Tensor], most_pages: int, out_tables: Optional[torch.Tensor], lists, nkv: int, d: int, page_size: int, bits: int,
                   window: int, least: int = 1) -> None:
     """What the prompt kernels need of the portions of a step (sequences with ``least`` rows or more in cu_q_lens): their pages as
     plain keys and values behind one another in k_out, v_out [pages, nkv, page_size, d], block tables of those pages in
     ``out_tables`` (shape of ``tables``), and one or two tile lists: ``lists`` of (height, count, seq, q0) with the number of
-    tiles that the portions cut into rows of that height make.  Pages that the window hides are left out."""
+    tiles that the portions cut into rows of that height make.  Pages that the window hides are left out.  Without ``k_out`` and ``v_out`` (and
+    ``most_pages`` 0): the lists alone."""
     stream = _stream_of("packed_unfold", pages, tables, cu_q_lens, context_lens, k_out, v_out, out_tables)
     B, width = _tables("packed_unfold", tables)
     _ints("packed_unfold", B, context_lens)
-    _ints("packed_unfold", B * width, out_tables)
+    if k_out is not None:
+        _ints("packed_unfold", B * width, out_tables)
     _ints("packed_unfold", B + 1, cu_q_lens)
     flat = []
     for height, count, seq, q0 in lists:
@@ -1811,6 +1833,6 @@ def packed_unfold(pages: torch.Tensor, tables: torch.Tensor, cu_q_lens: torch.Te
     if len(lists) == 1:
         flat += [0, 0, None, None]
     _check(_packed("gg_packed_unfold")(pages.data_ptr(), pages.shape[0], tables.data_ptr(), width, cu_q_lens.data_ptr(),
-                                       context_lens.data_ptr(), B, k_out.data_ptr(), v_out.data_ptr(), dtype_code(k_out.dtype),
-                                       k_out.shape[0], most_pages, out_tables.data_ptr(), *flat, least, nkv, d, page_size, bits, window,
+                                       context_lens.data_ptr(), B, _at(k_out), _at(v_out), dtype_code(k_out.dtype) if k_out is not None else 1,
+                                       k_out.shape[0] if k_out is not None else 0, most_pages, _at(out_tables), *flat, least, nkv, d, page_size, bits, window,
                                        stream))

@@ -415,7 +415,8 @@ packed_read_kernel(const unsigned char* __restrict__ pages, int num_pages, const
   unpack_page<TO, BITS>(pages, tables[(size_t)b * bt_stride + j], num_pages, len - j * page_size, k_out + at, v_out + at, nkv, d, page_size);
 }
 
-// What the prompt kernels need of a packed layer's portions (sequences that bring `least` tokens or more), in one launch: their
+// What the prompt kernels need of a packed layer's portions (sequences that bring `least` tokens or more), in one launch (without pages: the
+// tiles alone): their
 // pages as plain keys and values, one sequence behind the other; block tables of those pages; and the portions cut into tiles
 // of query rows, those that attend to most keys first (up to UNFOLD_SORTED tiles; more stay in the order of the sequences).
 // Pages behind the window of a portion's first token are left out (-1 in the table).  4 us for 2048 tokens of 8 heads of 128.
@@ -612,7 +613,7 @@ extern "C" int gg_packed_unfold(const void* pages, int num_pages, const int* tab
                                 int least, int nkv, int d, int page_size, int bits, int window, cudaStream_t stream) {
   int rc = check_packed("packed_unfold", pages, num_pages, nkv, d, page_size, bits);
   if (rc) return rc;
-  GG_REQUIRE(B > 0 && B <= UNFOLD_SEQS && most_pages > 0 && most_pages <= bt_stride && window >= 0 && height0 >= 0 && height1 >= 0,
+  GG_REQUIRE(B > 0 && B <= UNFOLD_SEQS && most_pages >= 0 && most_pages <= bt_stride && window >= 0 && height0 >= 0 && height1 >= 0,
              "packed_unfold: bad sizes B=%d pages=%d of %d window=%d", B, most_pages, bt_stride, window);
   GG_REQUIRE(((size_t)k_out % 16) == 0 && ((size_t)v_out % 16) == 0, "packed_unfold: the outputs must start on 16 bytes");
   GG_REQUIRE(out_dtype == GG_F32 || out_dtype == GG_BF16, "packed_unfold: unknown dtype %d", out_dtype);
@@ -622,7 +623,7 @@ extern "C" int gg_packed_unfold(const void* pages, int num_pages, const int* tab
   a.out_tables = out_tables;
   a.tiles[0] = {height0, count0, seq0, q00};
   a.tiles[1] = {height1, count1, seq1, q01};
-  const dim3 grid(most_pages + 1, B, head_blocks(out_pages, nkv)), block(256);
+  const dim3 grid(most_pages + 1, most_pages ? B : 1, most_pages ? head_blocks(out_pages, nkv) : 1), block(256);
 #define UNFOLD_LAUNCH(TO, BITS) gg_launch(packed_unfold_kernel<TO, BITS>, grid, block, 0, stream, a, (TO*)k_out, (TO*)v_out)
   if (out_dtype == GG_F32) { if (bits == 4) UNFOLD_LAUNCH(float, 4); else UNFOLD_LAUNCH(float, 8); }
   else { if (bits == 4) UNFOLD_LAUNCH(__nv_bfloat16, 4); else UNFOLD_LAUNCH(__nv_bfloat16, 8); }
@@ -662,4 +663,19 @@ extern "C" int gg_packed_decode(const void* q, long long q_stride, int act_dtype
   a.num_seqs = B; a.dec_seqs = seqs; a.num_splits = splits; a.part_o = part_o; a.part_ml = part_ml;
   rc = attn_decode_general(a, act_dtype, n, stream);
   return rc ? rc : attn_merge_launch(a, act_dtype, n, stream);
+}
+
+// Prompt portions on the general kernel: tiles of 16 rows (packed_unfold lists them).
+extern "C" int gg_packed_prefill(const void* q, long long q_stride, int act_dtype, const void* pages, int num_pages, const int* tables,
+                                 int bt_stride, const int* cu_q_lens, const int* context_lens, const int* tile_seq, const int* tile_q0, int tiles,
+                                 void* out, int nh, int nkv, int d, int page_size, int bits, int window, float scale, float softcap,
+                                 const float* sink, const float* slopes, float temp_coef, float temp_every, cudaStream_t stream) {
+  int rc = check_packed("packed_prefill", pages, num_pages, nkv, d, page_size, bits);
+  if (!rc) rc = check_heads("packed_prefill", nh, nkv, bt_stride, window);
+  if (rc) return rc;
+  GG_REQUIRE(tiles >= 0 && cu_q_lens && context_lens && (tiles == 0 || (tile_seq && tile_q0)), "packed_prefill: bad lists of %d tiles", tiles);
+  AttnArgs a = packed_args(q, q_stride, pages, num_pages, tables, bt_stride, cu_q_lens, context_lens, out, nh, nkv, d, page_size, bits, window,
+                           scale, softcap, sink, slopes, temp_coef, temp_every);
+  a.tile_seq = tile_seq; a.tile_q0 = tile_q0;
+  return attn_prefill_general(a, act_dtype, tiles, stream);
 }

@@ -24,13 +24,6 @@ struct PackedRows {
   // offsets inside a block: codes and pairs of token `place`; which = 0 keys, 1 values
   __host__ __device__ int codes(int which, int place) const { return (which * page_size + place) * row(); }
   __host__ __device__ int pairs(int which, int place) const { return 2 * page_size * row() + (which * page_size + place) * groups() * 4; }
-  // what channel c of a token stands for
-  __device__ __forceinline__ float value(const unsigned char* block, int which, int place, int c) const {
-    const unsigned char* q = block + codes(which, place);
-    const unsigned code = bits == 4 ? (q[c >> 1] >> ((c & 1) * 4)) & 15u : q[c];
-    const unsigned pair = *reinterpret_cast<const unsigned*>(block + pairs(which, place) + (c / group) * 4);
-    return fmaf(__uint_as_float(pair << 16), (float)code, __uint_as_float(pair & 0xffff0000u));
-  }
 };
 // pages of a size whose blocks and rows of pairs start on 16 bytes
 __host__ __device__ __forceinline__ bool packed_sizes_ok(int bits, int d, int page_size) {

@@ -111,14 +111,14 @@ def tolerance(q, keys, values, context, scale, dtype, tensor_cores, window=0, so
     On the tensor cores a key is not one number there but s (c - M) + (o + M s) with the middle code M, two sums that are made apart and may cancel.
     Of a group whose largest value is G, |o + M s| <= 1.01 G (it lies inside the codes' range, whose end is at most a bfloat16 step of the scale
     beyond the largest value) and |s (c - M)| <= 1.01 x 8 / 15 x 2 G, so roundings are relative to 2.1 G in the place of |k|, and of |v| alike.
-    bfloat16: a key rounds as it is read back, so a score moves by 2^-8 S, a weight and a value round once (2^-8 each, relative to sum P |v|;
-    on the general kernel weights stay float32), and the result rounds once.  A cap is a tanh of the special-function unit there: 2^-11 of the
-    capped score.  A bias by distance rounds in float32."""
+    bfloat16 on the tensor cores: a key rounds as it is read back, so a score moves by 2^-8 S, and a weight and a value round once (2^-8 each,
+    relative to sum P |v|).  A cap is a tanh of the special-function unit there: 2^-11 of the capped score.  The general kernel computes in
+    float32 whatever the type.  A bias by distance rounds in float32, and the result rounds once."""
     a, nh, d = q.shape
     group = nh // keys.shape[1]
     tol = torch.zeros(a, nh, d, dtype=torch.float64)
     fast = dtype == torch.bfloat16 and tensor_cores
-    half = 2.0 ** -8 if dtype == torch.bfloat16 else 0.0
+    half = 2.0 ** -8 if fast else 0.0
     at, j = torch.arange(context - a, context)[:, None], torch.arange(context)[None]
     seen = (j <= at) & ((at - j < window) if window else True)
     factor = torch.full((a, 1), float(scale), dtype=torch.float64)
@@ -143,7 +143,7 @@ def tolerance(q, keys, values, context, scale, dtype, tensor_cores, window=0, so
         w = torch.softmax(z, 1)[:, :context]
         out = w @ v
         spread = torch.einsum("ij,ijc->ic", w * move.masked_fill(~seen, 0.0), (v[None] - out[:, None]).abs()) + 2.0 ** -21 * out.abs()
-        rounds = (half * (2 if tensor_cores else 1) + (context + 8) * 2.0 ** -24) * (w @ size_v)
+        rounds = (2 * half + (context + 8) * 2.0 ** -24) * (w @ size_v)
         tol[:, h] = 1.05 * (spread + rounds) + torch.finfo(dtype).eps / 2 * out.abs() + 1e-30
     return tol
 
@@ -291,17 +291,18 @@ def test_the_line_between_the_prompt_kernels_is_the_attention_layers(nh, window,
         assert packed.long_tiles(options, tiles, nh, window or 0, longest, plain_layer.num_sms) == want, (q_lens, q_starts)
 
 
-@pytest.mark.parametrize("policy,lists,mma", [("auto", [64, 128], True), ("mma", [64], True), ("general", [16], False)])
+@pytest.mark.parametrize("policy,lists", [("auto", [64, 128]), ("mma", [64]), ("general", [16])])
 @pytest.mark.parametrize("options", [False, True])
-def test_the_switch_of_the_prompt_kernels_holds_for_portions(monkeypatch, policy, lists, mma, options):
+def test_the_switch_of_the_prompt_kernels_holds_for_portions(monkeypatch, policy, lists, options):
     from gollmgo_b200.cache import packed
     from gollmgo_b200.csrc import ops
     seen = {}
     monkeypatch.setattr(packed, "ATTN_POLICY", policy)
     monkeypatch.setattr(ops, "packed_prefill_rows", lambda *a: None)
     monkeypatch.setattr(ops, "packed_unfold", lambda *a, **k: seen.update(lists=[h for h, *_ in a[8]]))
-    monkeypatch.setattr(ops, "attn_prefill", lambda *a, **k: seen.update(kernel=False, **k))
-    monkeypatch.setattr(ops, "attn_prefill_x", lambda *a, **k: seen.update(kernel=True, **k))
+    monkeypatch.setattr(ops, "attn_prefill", lambda *a, **k: seen.update(kernel="plain", **k))
+    monkeypatch.setattr(ops, "attn_prefill_x", lambda *a, **k: seen.update(kernel="options", **k))
+    monkeypatch.setattr(ops, "packed_prefill", lambda *a, **k: seen.update(kernel="general"))
 
     class NoDevice(PackedKV):
         def __init__(self):
@@ -309,7 +310,8 @@ def test_the_switch_of_the_prompt_kernels_holds_for_portions(monkeypatch, policy
             self.pages = None
     NoDevice().prefill(torch.zeros(400, 2, 64, dtype=torch.bfloat16), torch.zeros(1, 25, dtype=torch.int32), torch.tensor([0, 400], dtype=torch.int32),
                        torch.tensor([400], dtype=torch.int32), [400], [400], 0.1, sink=torch.zeros(2) if options else None)
-    assert seen["lists"] == lists and seen["kernel"] == options and seen["allow_mma"] == mma and ("tile128_seq" in seen) == (128 in lists)
+    assert seen["lists"] == lists and seen["kernel"] == ("general" if policy == "general" else "options" if options else "plain")
+    assert ("tile128_seq" in seen) == (128 in lists)
 
 
 @pytest.mark.gpu
@@ -338,3 +340,47 @@ def test_portions_with_a_scale_that_is_not_positive(bits, dtype, scale, nh, nkv,
         x = q[cu[b]:cu[b + 1]]
         ref = plain.attend(x.double(), *held[b], n, scale)
         assert ((out[cu[b]:cu[b + 1]] - ref).abs() <= tolerance(x, *held[b], n, scale, dtype, d in (64, 128))).all(), b
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("d,page", [(96, 16), (128, 8), (16, 4)])
+@pytest.mark.parametrize("sink", [False, True])
+def test_portions_on_the_general_kernel_do_not_attend_to_missing_pages(monkeypatch, bits, dtype, d, page, sink):
+    from gollmgo_b200.cache import packed
+    monkeypatch.setattr(packed, "ATTN_POLICY", "general")
+    nh, nkv, n, a = 2, 1, 70, 30
+    if dtype == torch.float32 and d == 128 and page >= 16:
+        return
+    g = torch.Generator().manual_seed(d)
+    width = -(-n // page)
+    kv = PackedKV.empty(width, nkv, d, page, bits)
+    table = torch.randperm(width, generator=g).to(torch.int32)
+    x = torch.randn(n, 2 * nkv * d, generator=g).to(dtype)
+    t = torch.arange(n)
+    kv.write(x.cuda(), None, (table[t // page].long() * page + t % page).to(torch.int32).cuda(), 0)
+    k, v = (plain.through(y.double().view(n, nkv, d), bits) for y in x.chunk(2, 1))
+    missing = table.clone()
+    missing[0], missing[-1] = -1, width
+    there = ((missing >= 0) & (missing < width))[t // page]
+    q = torch.randn(a, nh, d, generator=g).to(dtype)
+    dev = lambda y: torch.tensor(y, dtype=torch.int32).cuda()  # noqa: E731
+    s = torch.randn(nh, generator=g) if sink else None
+    for gone in (False, True):
+        if gone:
+            missing[:] = -1
+        out = kv.prefill(q.cuda(), missing.view(1, -1).cuda(), dev([0, a]), dev([n]), [a], [n], d ** -0.5, sink=None if s is None else s.cuda()).cpu().double()
+        if gone:
+            assert (out == 0).all()
+            continue
+        for i in range(a):
+            seen = there & (t <= n - a + i)
+            for h in range(nh):
+                z = k[seen, 0] @ q[i, h].double() * d ** -0.5
+                z = torch.cat([z, s[h].double()[None]]) if sink else z
+                w = torch.softmax(z, 0)[:int(seen.sum())]
+                # float32 arithmetic: d products a score (relative to |q| |k|), twice, and a sum over the context; the result's rounding
+                e = float(q[i, h].double().norm() * k.norm(dim=-1).max()) * d ** -0.5 * (d + 8) * 2.0 ** -24 + 2.0 ** -20
+                ref = w @ v[seen, 0]
+                assert ((out[i, h] - ref).abs() <= torch.finfo(dtype).eps / 2 * ref.abs() + (2 * e + (n + 8) * 2.0 ** -24) * (w @ v[seen, 0].abs()).max()).all()
