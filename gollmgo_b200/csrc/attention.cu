@@ -58,6 +58,7 @@ __device__ __forceinline__ void attn_tile(const AttnArgs& a, int nrows, const TA
   const int kstart = (lo / ATT_BK) * ATT_BK;
   for (int kb = kstart; kb < hi; kb += ATT_BK) {
     // ---- stage keys and values of tokens [kb, kb+64)
+    bool bad = false;                              // a packed cache: some value is no number
     for (int j = warp; j < ATT_BK; j += ATT_THREADS / 32) {
       const int tok = kb + j;
       int page = -1;
@@ -88,6 +89,7 @@ __device__ __forceinline__ void attn_tile(const AttnArgs& a, int nrows, const TA
           if (c < d) {
             Ks[j * (d + 1) + c] = fmaf(__uint_as_float(kpair[i] << 16), (float)((kcode[i] >> shift) & mask), __uint_as_float(kpair[i] & 0xffff0000u));
             Vs[j * dv + c] = fmaf(__uint_as_float(vpair[i] << 16), (float)((vcode[i] >> shift) & mask), __uint_as_float(vpair[i] & 0xffff0000u));
+            bad = bad || (vpair[i] & 0x7f80u) == 0x7f80u;        // (the scale of such a group is none either)
           }
         }
       } else if (page >= 0) {
@@ -100,7 +102,8 @@ __device__ __forceinline__ void attn_tile(const AttnArgs& a, int nrows, const TA
         for (int c = lane; c < dv; c += 32) Vs[j * dv + c] = 0.f;
       }
     }
-    __syncthreads();
+    if (PACKED) bad = __syncthreads_or(bad);
+    else __syncthreads();
     // ---- scores: thread (j = tid%64, rows tid/64 + 2i)
     {
       const int j = tid & 63, rb = tid >> 6;
@@ -152,11 +155,29 @@ __device__ __forceinline__ void attn_tile(const AttnArgs& a, int nrows, const TA
         p1 = expf(s1 - m_new);
       }
       const float sum = warp_sum(p0 + p1);
+      if (PACKED) {                                // (a weight that is hidden is -0)
+        if (s0 == -INFINITY) p0 = -0.f;
+        if (s1 == -INFINITY) p1 = -0.f;
+      }
       Ss[r * ATT_BK + lane] = p0;
       Ss[r * ATT_BK + lane + 32] = p1;
       if (lane == 0) { m_s[r] = m_new; l_s[r] = l_s[r] * alpha + sum; al_s[r] = alpha; }
     }
     __syncthreads();
+    if (PACKED && bad) {                           // 0 times a NaN is one: rows that see it have it from here, and it goes
+#pragma unroll
+      for (int i = 0; i < NACC; ++i) {
+        const int e = tid + ATT_THREADS * i, r = e / dv, c = e - r * dv;
+        if (e < ATT_BQ * dv)
+#pragma unroll 1
+          for (int j = 0; j < ATT_BK; ++j)
+            if (__float_as_uint(Ss[r * ATT_BK + j]) != 0x80000000u && !isfinite(Vs[j * dv + c])) acc[i] = __int_as_float(0x7fffffff);
+      }
+      __syncthreads();
+      for (int e = tid; e < ATT_BK * dv; e += ATT_THREADS)
+        if (!isfinite(Vs[e])) Vs[e] = 0.f;
+      __syncthreads();
+    }
     // ---- output: thread owns elements e = tid + 128*i of the [16][d] tile
 #pragma unroll
     for (int i = 0; i < NACC; ++i) {

@@ -384,3 +384,39 @@ def test_portions_on_the_general_kernel_do_not_attend_to_missing_pages(monkeypat
                 e = float(q[i, h].double().norm() * k.norm(dim=-1).max()) * d ** -0.5 * (d + 8) * 2.0 ** -24 + 2.0 ** -20
                 ref = w @ v[seen, 0]
                 assert ((out[i, h] - ref).abs() <= torch.finfo(dtype).eps / 2 * ref.abs() + (2 * e + (n + 8) * 2.0 ** -24) * (w @ v[seen, 0].abs()).max()).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("dtype,d,page", [(torch.bfloat16, 96, 16), (torch.float32, 96, 16), (torch.float32, 128, 8), (torch.float32, 64, 16)])
+@pytest.mark.parametrize("window", [0, 9])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+def test_bad_tokens_reach_the_rows_that_see_them(bits, dtype, d, page, window, bad):
+    """A bad key makes the rows of its kv head from its token on NaN, a bad value its group of channels; rows before it, and behind the
+    window, are as without it."""
+    nh, nkv, n = 4, 2, 200
+    g = torch.Generator().manual_seed(d)
+    x = torch.randn(n, (nh + 2 * nkv) * d, generator=g).to(dtype)
+    width = -(-n // page)
+    table = torch.randperm(width, generator=g).to(torch.int32)
+    t = torch.arange(n)
+    slots = (table[t // page].long() * page + t % page).to(torch.int32).cuda()
+    dev = lambda y: torch.tensor(y, dtype=torch.int32).cuda()  # noqa: E731
+    outs = []
+    key, value = 150, 37
+    for spoilt in (False, True):
+        y = x.clone()
+        if spoilt:
+            y[key, nh * d + 3] = bad                              # a key of kv head 0
+            y[value, (nh + 2 * nkv) * d - 1] = -bad               # the last channel of a value of kv head 1
+        kv = PackedKV.empty(width, nkv, d, page, bits)
+        q = kv.write(y.cuda(), None, slots, nh)
+        outs.append(kv.prefill(q, table.view(1, -1).cuda(), dev([0, n]), dev([n]), [n], [n], d ** -0.5, window=window).cpu())
+    good, got = outs
+    sees = lambda at: (t >= at) & (t < at + window if window else True)  # noqa: E731
+    group = plain.group_of(d)
+    hidden = torch.zeros(n, nh, d, dtype=torch.bool)
+    hidden[sees(key), :2] = True
+    hidden[sees(value), 2:, d - group:] = True
+    assert torch.equal(got.isnan(), hidden)
+    assert torch.equal(got[~hidden], good[~hidden])
