@@ -211,7 +211,8 @@ class PackedKV:
             tables, context_lens, cu_q_lens = tables[lo:hi], context_lens[lo:hi], cu_q_lens[lo:hi + 1]
         # (the plain tcgen05 kernel takes the largest product for the largest score)
         options = softcap > 0 or sink is not None or slopes is not None or temperature is not None or not scale > 0
-        fast = q.dtype == torch.bfloat16 and d in (64, 128) and q.stride(0) % 8 == 0 and q.data_ptr() % 16 == 0 and ATTN_POLICY != "general"
+        fast = q.dtype == torch.bfloat16 and d in (64, 128) and q.stride(0) % 8 == 0 and q.data_ptr() % 16 == 0 and ATTN_POLICY != "general" \
+            and self.kv_heads <= 1024
         if not fast:                               # on the codes where they lie, in float32 arithmetic
             n = counts[0]
             ints = torch.empty(2 * n, dtype=torch.int32, device=q.device)
@@ -223,24 +224,20 @@ class PackedKV:
         lists = [(64, counts[1])]
         if ATTN_POLICY == "auto" and long_tiles(options, counts[2], nh, window, longest, self._sms):
             lists.append((128, counts[2]))
-        k, v = torch.empty(2, pages, self.kv_heads, P, d, dtype=q.dtype, device=q.device).unbind(0)
-        B, width = tables.shape
-        ints = torch.empty(B * width + 2 * sum(n for _, n in lists), dtype=torch.int32, device=q.device)
-        at, full = B * width, []
-        for h, n in lists:
-            full.append((h, n, ints[at:at + n], ints[at + n:at + 2 * n]))
+        (B, width), new, loud = tables.shape, q.new_empty, ops.packed_loud_floats(self.kv_heads)
+        k, v = new((2, pages, self.kv_heads, P, d), dtype=torch.float16).unbind(0)
+        loud, kv_unit = new((loud + 2 * self.kv_heads,), dtype=torch.float32).split([loud, 2 * self.kv_heads])
+        ints = new((B * width + 2 * sum(n for _, n in lists),), dtype=torch.int32)
+        at, tiles = B * width, []
+        for _, n in lists:
+            tiles.append((ints[at:at + n], ints[at + n:at + 2 * n], n))
             at += 2 * n
-        plain = ints[:B * width]
-        ops.packed_unfold(self.pages, tables, cu_q_lens, context_lens, k, v, most, plain, full, self.kv_heads, d, P, self.bits, window, least)
-        t64 = (full[0][2], full[0][3], full[0][1])
-        long = dict(tile128_seq=full[1][2], tile128_q0=full[1][3], num_tiles128=full[1][1]) if len(full) > 1 else {}
-        with ops.after_everything():               # the prompt kernels read early what packed_unfold has just written
-            if options:
-                ops.attn_prefill_x(q, q.stride(0), k, v, plain, width, cu_q_lens, context_lens, None, None, 0, out, nh, self.kv_heads, d, d, 1, P,
-                                   window, scale, softcap, *t64, sink=sink, slopes=slopes, temperature=temperature, **long)
-            else:
-                ops.attn_prefill(q, q.stride(0), k, v, plain, width, cu_q_lens, context_lens, None, None, 0, out, nh, self.kv_heads, d, P, window,
-                                 scale, *t64, allow_tc=bool(long), **long)
+        plain, shape = ints[:B * width], (self.kv_heads, d, P, self.bits, window, least)
+        ops.packed_loud(self.pages, tables, cu_q_lens, context_lens, loud, *shape)
+        ops.packed_unfold(self.pages, tables, cu_q_lens, context_lens, k, v, most, plain, [(h, n, *t[:2]) for (h, n), t in zip(lists, tiles)], *shape,
+                          loud, kv_unit)
+        ops.attn_prefill_half(q, k, v, kv_unit, plain, width, cu_q_lens, context_lens, tiles[0], tiles[1] if len(tiles) > 1 else None, out, nh,
+                              self.kv_heads, d, P, window, scale, options, softcap, sink, slopes, temperature)
 
     @staticmethod
     def scratch_bytes(needs, max_context: int, dtype) -> int:

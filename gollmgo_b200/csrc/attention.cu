@@ -647,6 +647,38 @@ extern "C" int gg_attn_prefill_x(const void* q, long long q_stride, const void* 
   return attn_prefill_general(a, dtype, num_tiles, stream);
 }
 
+// Prompt portions in half precision: q bfloat16, pages [num_pages, nkv, page_size, d] of keys and values as half precision numbers, what each
+// kv head's are multiples of in kv_unit [2, nkv], the result in bfloat16.  `options`: with the options of gg_attn_prefill_x or a scale that is
+// not positive.  Tiles of 128 rows (tcgen05) may be missing.
+extern "C" int gg_attn_prefill_half(const void* q, long long q_stride, const void* kcache, const void* vcache, const float* kv_unit,
+                                    const int* block_tables, int bt_stride, const int* cu_q_lens, const int* context_lens, const int* tile64_seq,
+                                    const int* tile64_q0, int num_tiles64, const int* tile128_seq, const int* tile128_q0, int num_tiles128,
+                                    void* out, int T, int num_pages, int nh, int nkv, int d, int page_size, int window, int options, float scale,
+                                    float softcap, const float* sink, const float* slopes, float temp_coef, float temp_every, int* status,
+                                    cudaStream_t stream) {
+  AttnArgs a = {};
+  a.q = q; a.q_stride = q_stride; a.kcache = kcache; a.vcache = vcache; a.kv_unit = kv_unit;
+  a.block_tables = block_tables; a.bt_stride = bt_stride; a.cu_q_lens = cu_q_lens;
+  a.context_lens = context_lens; a.out = out; a.nh = nh; a.nkv = nkv; a.d = d;
+  a.page_size = page_size; a.window = window; a.scale = scale;
+  a.softcap = softcap; a.sink = sink; a.slopes = slopes; a.temp_coef = temp_coef; a.temp_every = temp_every;
+  int rc = check_common(a, "attn_prefill_half");
+  if (rc) return rc;
+  GG_REQUIRE((d == 64 || d == 128) && (page_size & (page_size - 1)) == 0 && kv_unit && tile64_seq && tile64_q0,
+             "attn_prefill_half: head size %d, pages of %d tokens, or no lists", d, page_size);
+  GG_REQUIRE(q_stride % 8 == 0 && ((size_t)q % 16) == 0, "attn_prefill_half: q rows must be 16-byte aligned");
+  GG_REQUIRE(options || (scale > 0.f && softcap <= 0.f && !sink && !slopes && temp_every <= 0.f), "attn_prefill_half: options without the kernels for them");
+  static const bool wide = !(getenv("GOLLMGO_B200_ATTN_STEP") && atoi(getenv("GOLLMGO_B200_ATTN_STEP")) == 64);
+  if (tile128_seq && status) {
+    a.tile_seq = tile128_seq; a.tile_q0 = tile128_q0;
+    if ((wide || options) && attn_tc3_half_supported(d, page_size, nh, nkv, options != 0))
+      return attn_prefill_tc3(a, num_tiles128, T, num_pages, status, options != 0, stream);
+    if (!options && attn_tc_supported(GG_BF16, d, page_size)) return attn_prefill_tc(a, num_tiles128, T, num_pages, status, stream);
+  }
+  a.tile_seq = tile64_seq; a.tile_q0 = tile64_q0;
+  return options ? attn_prefill_mma_x(a, num_tiles64, stream) : attn_prefill_mma(a, num_tiles64, stream);
+}
+
 extern "C" int gg_attn_decode_x(const void* q, long long q_stride, const void* kcache, const void* vcache,
                                 int dtype, const int* block_tables, int bt_stride, const int* cu_q_lens,
                                 const int* context_lens, const int* dec_seqs, int n_dec, int num_splits,

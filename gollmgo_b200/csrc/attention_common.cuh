@@ -2,6 +2,7 @@
 // the bfloat16 fast path (mma.sync m16n8k16, ldmatrix, cp.async, shared-memory swizzle).
 #pragma once
 #include "common.cuh"
+#include <cuda_fp16.h>
 
 struct AttnArgs {
   const void* q;            // [T, q_stride]: head h of token t at q + t*q_stride + h*d
@@ -50,6 +51,9 @@ struct AttnArgs {
   int packed_bits;          // 4 or 8; 0 = keys and values as they are
   int num_pages;            // pages of a packed cache: an id outside reads as a page that was given back
   int num_seqs;             // rows of its block tables: a dec_seqs entry outside is padding
+  // the prompt kernels with HALF: keys and values are half precision numbers, each kv head's keys and values times a power of two.  What they are
+  // multiples of (q is bfloat16; a row of it becomes such numbers in the kernel)
+  const float* kv_unit;     // [2, nkv]: keys, values; null: bfloat16
 };
 
 // the factor on the query at position p (1 where the layer has none)
@@ -57,6 +61,16 @@ __device__ __forceinline__ float query_temperature(const AttnArgs& a, int p) {
   if (!(a.temp_every > 0.f)) return 1.f;
   return 1.f + a.temp_coef * logf(floorf(__fdiv_rn((float)(p + 1), a.temp_every)) + 1.f);
 }
+
+// HALF: weights are held 2^HALF_WEIGHTS times as large (their sum alike), so that what half precision loses of small ones, 2^-25, is that much less.
+// They stay below 2^15: relative to a maximum that may lag by 2^8, or (mma.sync) to the maximum itself.
+#define HALF_WEIGHTS 7.f
+#define HALF_WEIGHTS_MMA 15.f
+// The exponent of the power of two that brings `big` to [2^12, 2^13), inside half precision's range with room on both sides.
+__device__ __forceinline__ int half_exponent(float big) { return max(-120, min(120, 139 - (int)(__float_as_uint(big) >> 23))); }
+__device__ __forceinline__ float two_to(int e) { return __uint_as_float((unsigned)(e + 127) << 23); }        // -126 <= e <= 127
+// HALF: what the products of a row of q (times 2^q_exponent) and the keys of kv head kvh are to be multiplied by, times `scale`
+__device__ __forceinline__ float half_scale(const AttnArgs& a, float scale, int q_exponent, int kvh) { return scale * two_to(-q_exponent) * a.kv_unit[kvh]; }
 
 // General kernels (attention.cu)
 int attn_prefill_general(const AttnArgs& a, int dtype, int num_tiles, cudaStream_t stream);
@@ -94,6 +108,9 @@ int attn_prefill_tc3(const AttnArgs& a, int num_tiles, int T, int num_pages, int
 // query temperature, a.out_f32): x = true above
 bool attn_tc3_x_supported(int dtype, int d, int dv, int page_size, int nh, int nkv);
 
+// (the prompt kernels attn_prefill_mma, _mma_x, _tc and _tc3 run with HALF where a.kv_unit is given; keys and values are then of one size)
+bool attn_tc3_half_supported(int d, int page_size, int nh, int nkv, bool x);
+
 __device__ __forceinline__ unsigned smem_u32(const void* p) {
   return (unsigned)__cvta_generic_to_shared(p);
 }
@@ -123,6 +140,18 @@ __device__ __forceinline__ float fast_exp2(float x) {
   asm volatile("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
   return y;
 }
+__device__ __forceinline__ void mma_half(float* c, const unsigned* a, unsigned b0, unsigned b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ unsigned pack_half(float lo, float hi) {
+  __half2 v = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<unsigned*>(&v);
+}
+// two bfloat16, and the larger of their sizes
+__device__ __forceinline__ float largest_bf16(unsigned w) { return fmaxf(fabsf(__uint_as_float(w << 16)), fabsf(__uint_as_float(w & 0xffff0000u))); }
+__device__ __forceinline__ unsigned half_of_bf16(unsigned w, float up) { return pack_half(__uint_as_float(w << 16) * up, __uint_as_float(w & 0xffff0000u) * up); }
 __device__ __forceinline__ unsigned pack_bf16(float lo, float hi) {
   __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
   return *reinterpret_cast<unsigned*>(&v);

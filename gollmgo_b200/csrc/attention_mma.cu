@@ -63,7 +63,7 @@ __device__ __forceinline__ void load_kv_tile(const AttnArgs& a, const int* bt, i
 }
 
 // Scores of 16 query rows against NT*8 keys (rows key0.. of the staged tile).
-template <int D, int NT>
+template <int D, int NT, bool HALF = false>
 __device__ __forceinline__ void qk_mma(const unsigned (*qf)[4], unsigned ks, int key0, float (*s)[4]) {
   const int lane = threadIdx.x & 31;
 #pragma unroll
@@ -77,14 +77,19 @@ __device__ __forceinline__ void qk_mma(const unsigned (*qf)[4], unsigned ks, int
       const int row = key0 + (j + (mi >> 1)) * 8 + (lane & 7);
       unsigned b0, b1, b2, b3;
       ldmatrix_x4(b0, b1, b2, b3, ks + tile_off<D>(row, 2 * kk + (mi & 1)));
-      mma_bf16(s[j], qf[kk], b0, b1);
-      mma_bf16(s[j + 1], qf[kk], b2, b3);
+      if (HALF) {
+        mma_half(s[j], qf[kk], b0, b1);
+        mma_half(s[j + 1], qf[kk], b2, b3);
+      } else {
+        mma_bf16(s[j], qf[kk], b0, b1);
+        mma_bf16(s[j + 1], qf[kk], b2, b3);
+      }
     }
   }
 }
 
 // O(16 x D) += P(16 x NT*8) V(NT*8 x D); p holds NT/2 A-operand fragments.
-template <int D, int NT>
+template <int D, int NT, bool HALF = false>
 __device__ __forceinline__ void pv_mma(const unsigned (*p)[4], unsigned vs, int key0, float (*o)[4]) {
   const int lane = threadIdx.x & 31;
 #pragma unroll
@@ -96,15 +101,20 @@ __device__ __forceinline__ void pv_mma(const unsigned (*p)[4], unsigned vs, int 
       const int row = key0 + kk * 16 + (mi & 1) * 8 + (lane & 7);
       unsigned b0, b1, b2, b3;
       ldmatrix_x4_trans(b0, b1, b2, b3, vs + tile_off<D>(row, nt + (mi >> 1)));
-      mma_bf16(o[nt], p[kk], b0, b1);
-      mma_bf16(o[nt + 1], p[kk], b2, b3);
+      if (HALF) {
+        mma_half(o[nt], p[kk], b0, b1);
+        mma_half(o[nt + 1], p[kk], b2, b3);
+      } else {
+        mma_bf16(o[nt], p[kk], b0, b1);
+        mma_bf16(o[nt + 1], p[kk], b2, b3);
+      }
     }
   }
 }
 
 // One online-softmax update of a warp's 16 rows with NT*8 new scores (already scaled
 // to base 2 and masked with -inf).  Thread holds rows g = lane/4 (regs 0,1) and g+8 (2,3).
-template <int D, int NT>
+template <int D, int NT, bool HALF = false>
 __device__ __forceinline__ void softmax_update(float (*s)[4], float* m, float* l, float (*o)[4],
                                                unsigned (*p)[4]) {
   float mx0 = -INFINITY, mx1 = -INFINITY;
@@ -123,12 +133,13 @@ __device__ __forceinline__ void softmax_update(float (*s)[4], float* m, float* l
   m[0] = mn0;
   m[1] = mn1;
   float sum0 = 0.f, sum1 = 0.f;
+  const float from0 = HALF ? ref0 - HALF_WEIGHTS_MMA : ref0, from1 = HALF ? ref1 - HALF_WEIGHTS_MMA : ref1;
 #pragma unroll
   for (int j = 0; j < NT; ++j) {
-    s[j][0] = fast_exp2(s[j][0] - ref0);
-    s[j][1] = fast_exp2(s[j][1] - ref0);
-    s[j][2] = fast_exp2(s[j][2] - ref1);
-    s[j][3] = fast_exp2(s[j][3] - ref1);
+    s[j][0] = fast_exp2(s[j][0] - from0);
+    s[j][1] = fast_exp2(s[j][1] - from0);
+    s[j][2] = fast_exp2(s[j][2] - from1);
+    s[j][3] = fast_exp2(s[j][3] - from1);
     sum0 += s[j][0] + s[j][1];
     sum1 += s[j][2] + s[j][3];
   }
@@ -140,10 +151,10 @@ __device__ __forceinline__ void softmax_update(float (*s)[4], float* m, float* l
   }
 #pragma unroll
   for (int kk = 0; kk < NT / 2; ++kk) {
-    p[kk][0] = pack_bf16(s[2 * kk][0], s[2 * kk][1]);
-    p[kk][1] = pack_bf16(s[2 * kk][2], s[2 * kk][3]);
-    p[kk][2] = pack_bf16(s[2 * kk + 1][0], s[2 * kk + 1][1]);
-    p[kk][3] = pack_bf16(s[2 * kk + 1][2], s[2 * kk + 1][3]);
+    p[kk][0] = HALF ? pack_half(s[2 * kk][0], s[2 * kk][1]) : pack_bf16(s[2 * kk][0], s[2 * kk][1]);
+    p[kk][1] = HALF ? pack_half(s[2 * kk][2], s[2 * kk][3]) : pack_bf16(s[2 * kk][2], s[2 * kk][3]);
+    p[kk][2] = HALF ? pack_half(s[2 * kk + 1][0], s[2 * kk + 1][1]) : pack_bf16(s[2 * kk + 1][0], s[2 * kk + 1][1]);
+    p[kk][3] = HALF ? pack_half(s[2 * kk + 1][2], s[2 * kk + 1][3]) : pack_bf16(s[2 * kk + 1][2], s[2 * kk + 1][3]);
   }
 }
 
@@ -159,6 +170,30 @@ __device__ __forceinline__ void load_q_frags(unsigned (*qf)[4], F qrow) {
     qf[kk][1] = r1 ? *reinterpret_cast<const unsigned*>(r1 + kk * 16 + c) : 0u;
     qf[kk][2] = r0 ? *reinterpret_cast<const unsigned*>(r0 + kk * 16 + c + 8) : 0u;
     qf[kk][3] = r1 ? *reinterpret_cast<const unsigned*>(r1 + kk * 16 + c + 8) : 0u;
+  }
+}
+
+// Fragments of bfloat16 rows as half precision numbers times a power of two for each of the thread's two rows (2^e0, 2^e1).
+template <int D>
+__device__ __forceinline__ void q_halves(unsigned (*qf)[4], int* e0, int* e1) {
+  float big0 = 0.f, big1 = 0.f;
+#pragma unroll
+  for (int kk = 0; kk < D / 16; ++kk) {
+    big0 = fmaxf(big0, fmaxf(largest_bf16(qf[kk][0]), largest_bf16(qf[kk][2])));
+    big1 = fmaxf(big1, fmaxf(largest_bf16(qf[kk][1]), largest_bf16(qf[kk][3])));
+  }
+#pragma unroll
+  for (int o = 1; o < 4; o <<= 1) {
+    big0 = fmaxf(big0, __shfl_xor_sync(0xffffffffu, big0, o));
+    big1 = fmaxf(big1, __shfl_xor_sync(0xffffffffu, big1, o));
+  }
+  *e0 = half_exponent(big0);
+  *e1 = half_exponent(big1);
+  const float up0 = two_to(*e0), up1 = two_to(*e1);
+#pragma unroll
+  for (int kk = 0; kk < D / 16; ++kk) {
+    qf[kk][0] = half_of_bf16(qf[kk][0], up0); qf[kk][2] = half_of_bf16(qf[kk][2], up0);
+    qf[kk][1] = half_of_bf16(qf[kk][1], up1); qf[kk][3] = half_of_bf16(qf[kk][3], up1);
   }
 }
 
@@ -739,14 +774,15 @@ __global__ void __launch_bounds__(128) attn_merge_flat_kernel(AttnArgs a, int n_
 }
 
 // ---------------------------------------------------------------- prompt portions
-template <int D>
+template <int D, bool HALF>
 __global__ void __launch_bounds__(MMA_THREADS) attn_prefill_mma_kernel(AttnArgs a) {
   extern __shared__ __align__(128) unsigned char smem_raw[];
   constexpr int TILE_BYTES = MMA_BK * D * 2;
   constexpr int STAGES = 2;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, c2 = (lane & 3) * 2;
   // the lists that say what this CTA works on were copied in before the step began: they are
-  // read while the kernel ahead (it writes the queries and the newest keys) is still finishing
+  // read while the kernel ahead (it writes the queries and the newest keys) is still finishing (HALF: the kernel ahead makes them)
+  if (HALF) pdl_wait();
   const int ps_log2 = 31 - __clz(a.page_size);
   const int b = a.tile_seq[blockIdx.x], q0 = a.tile_q0[blockIdx.x];
   const int h = blockIdx.y, kvh = h / (a.nh / a.nkv);
@@ -781,7 +817,13 @@ __global__ void __launch_bounds__(MMA_THREADS) attn_prefill_mma_kernel(AttnArgs 
   float o[D / 8][4];
 #pragma unroll
   for (int nt = 0; nt < D / 8; ++nt) { o[nt][0] = o[nt][1] = o[nt][2] = o[nt][3] = 0.f; }
-  const float sc = a.scale * LOG2E;
+  float sc0 = a.scale * LOG2E, sc1 = sc0;             // of the thread's two rows
+  if (HALF) {
+    int e0, e1;
+    q_halves<D>(qf, &e0, &e1);
+    sc0 = half_scale(a, sc0, e0, kvh);
+    sc1 = half_scale(a, sc1, e1, kvh);
+  }
 
   for (int it = 0; it < ntiles; ++it) {
     if (it + 1 < ntiles) {
@@ -796,12 +838,12 @@ __global__ void __launch_bounds__(MMA_THREADS) attn_prefill_mma_kernel(AttnArgs 
     const int kb = kstart + it * MMA_BK;
     if (wrow0 < nrows && kb <= wlast) {
       float s[8][4];
-      qk_mma<D, 8>(qf, ks, 0, s);
+      qk_mma<D, 8, HALF>(qf, ks, 0, s);
       const bool interior = kb >= lo && kb + MMA_BK - 1 <= first + wrow0 &&
                             (a.window <= 0 || kb > wlast - a.window);
       if (interior) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) { s[j][0] *= sc; s[j][1] *= sc; s[j][2] *= sc; s[j][3] *= sc; }
+        for (int j = 0; j < 8; ++j) { s[j][0] *= sc0; s[j][1] *= sc0; s[j][2] *= sc1; s[j][3] *= sc1; }
       } else {
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
@@ -809,13 +851,13 @@ __global__ void __launch_bounds__(MMA_THREADS) attn_prefill_mma_kernel(AttnArgs 
           for (int e = 0; e < 4; ++e) {
             const int tk = kb + j * 8 + c2 + (e & 1), from = (e & 2) ? from1 : from0;
             const unsigned n = (e & 2) ? keys1 : keys0;
-            s[j][e] = (unsigned)(tk - from) < n ? s[j][e] * sc : -INFINITY;
+            s[j][e] = (unsigned)(tk - from) < n ? s[j][e] * ((e & 2) ? sc1 : sc0) : -INFINITY;
           }
         }
       }
       unsigned p[4][4];
-      softmax_update<D, 8>(s, m, l, o, p);
-      pv_mma<D, 8>(p, vs, 0, o);
+      softmax_update<D, 8, HALF>(s, m, l, o, p);
+      pv_mma<D, 8, HALF>(p, vs, 0, o);
     }
     __syncthreads();
   }
@@ -826,6 +868,14 @@ __global__ void __launch_bounds__(MMA_THREADS) attn_prefill_mma_kernel(AttnArgs 
   l[1] += __shfl_xor_sync(0xffffffffu, l[1], 1);
   l[1] += __shfl_xor_sync(0xffffffffu, l[1], 2);
   const float inv0 = l[0] > 0.f ? 1.f / l[0] : 0.f, inv1 = l[1] > 0.f ? 1.f / l[1] : 0.f;
+  if (HALF) {                                      // (divided first: a sum of values times their unit may be more than a float)
+    const float unit = a.kv_unit[a.nkv + kvh];
+#pragma unroll
+    for (int nt = 0; nt < D / 8; ++nt) {
+      o[nt][0] = o[nt][0] * inv0 * unit; o[nt][1] = o[nt][1] * inv0 * unit; o[nt][2] = o[nt][2] * inv1 * unit; o[nt][3] = o[nt][3] * inv1 * unit;
+    }
+  }
+  const float div0 = HALF ? 1.f : inv0, div1 = HALF ? 1.f : inv1;
   __nv_bfloat16* out = (__nv_bfloat16*)a.out;
   const size_t ostride = (size_t)a.nh * D;
 #pragma unroll
@@ -833,10 +883,10 @@ __global__ void __launch_bounds__(MMA_THREADS) attn_prefill_mma_kernel(AttnArgs 
     const int col = nt * 8 + c2;
     if (row0_ok)
       *reinterpret_cast<unsigned*>(out + (size_t)(t0 + q0 + wrow0 + g) * ostride + (size_t)h * D + col) =
-          pack_bf16(o[nt][0] * inv0, o[nt][1] * inv0);
+          pack_bf16(o[nt][0] * div0, o[nt][1] * div0);
     if (row1_ok)
       *reinterpret_cast<unsigned*>(out + (size_t)(t0 + q0 + wrow0 + g + 8) * ostride + (size_t)h * D + col) =
-          pack_bf16(o[nt][2] * inv1, o[nt][3] * inv1);
+          pack_bf16(o[nt][2] * div1, o[nt][3] * div1);
   }
 }
 
@@ -976,21 +1026,20 @@ int attn_decode_mma(const AttnArgs& a, int n_dec, cudaStream_t stream, bool* mer
   return gg_check_launch("attn_decode_mma");
 }
 
+template <int D, bool HALF>
+static int prefill_go(const AttnArgs& a, int num_tiles, cudaStream_t stream) {
+  const size_t smem = (size_t)2 * 2 * MMA_BK * D * 2;                // 64 KB, 32 KB
+  int rc = opt_in_smem(attn_prefill_mma_kernel<D, HALF>, smem, "attn_prefill");
+  if (rc) return rc;
+  gg_launch(attn_prefill_mma_kernel<D, HALF>, dim3(num_tiles, a.nh), dim3(MMA_THREADS), smem, stream, a);
+  return gg_check_launch("attn_prefill_mma");
+}
 int attn_prefill_mma(const AttnArgs& a, int num_tiles, cudaStream_t stream) {
   GG_REQUIRE(power_of_two(a.page_size), "attn_prefill: page size %d is not a power of two", a.page_size);
   GG_REQUIRE(num_tiles >= 0 && a.nh <= 65535, "attn_prefill: bad grid %d x %d", num_tiles, a.nh);
   if (num_tiles == 0) return GG_OK;
-  dim3 grid(num_tiles, a.nh);
-  int rc;
-  if (a.d == 128) {
-    const size_t smem = (size_t)2 * 2 * MMA_BK * 128 * 2;            // 64 KB
-    if ((rc = opt_in_smem(attn_prefill_mma_kernel<128>, smem, "attn_prefill"))) return rc;
-    gg_launch(attn_prefill_mma_kernel<128>, dim3(grid), dim3(MMA_THREADS), smem, stream, a);
-  } else {
-    const size_t smem = (size_t)2 * 2 * MMA_BK * 64 * 2;             // 32 KB
-    gg_launch(attn_prefill_mma_kernel<64>, dim3(grid), dim3(MMA_THREADS), smem, stream, a);
-  }
-  return gg_check_launch("attn_prefill_mma");
+  if (a.kv_unit) return a.d == 128 ? prefill_go<128, true>(a, num_tiles, stream) : prefill_go<64, true>(a, num_tiles, stream);
+  return a.d == 128 ? prefill_go<128, false>(a, num_tiles, stream) : prefill_go<64, false>(a, num_tiles, stream);
 }
 
 // CTAs the flat decode kernel is launched with (its whole grid is resident at once).
@@ -1081,12 +1130,13 @@ __device__ __forceinline__ float sigmoid_weight(float x) {
 // out once per CTA as a table over distances behind the staged tiles; the first keep_first keys
 // stay visible behind the window (their tiles come first); where the values are the keys (one
 // cache tensor, equal sizes) the staged key tile serves as the value tile.
-template <int DK, int DV, bool SIG>
+template <int DK, int DV, bool SIG, bool HALF>
 __global__ void __launch_bounds__(MMA_THREADS) attn_prefill_mma_x_kernel(AttnArgs a) {
   extern __shared__ __align__(128) unsigned char smem_raw[];
   constexpr int K_BYTES = MMA_BK * DK * 2, V_BYTES = MMA_BK * DV * 2, STAGE = K_BYTES + V_BYTES;
   constexpr int STAGES = 2;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, c2 = (lane & 3) * 2;
+  if (HALF) pdl_wait();                            // the kernel ahead makes the lists
   const int ps_log2 = 31 - __clz(a.page_size);
   const int b = a.tile_seq[blockIdx.x], q0 = a.tile_q0[blockIdx.x];
   const int h = blockIdx.y, kvh = h / (a.nh / a.nkv);
@@ -1139,7 +1189,13 @@ __global__ void __launch_bounds__(MMA_THREADS) attn_prefill_mma_x_kernel(AttnArg
   const unsigned keys0 = row0_ok ? max(pos0 + 1 - from0, 0) : 0, keys1 = row1_ok ? max(pos1 + 1 - from1, 0) : 0;
   // this head's slope over the distance (base-2 exponents) and the two rows' scales (a query temperature is part of them)
   const float slope = !SIG && a.slopes ? a.slopes[h] * LOG2E : 0.f;
-  const float scale0 = SIG ? a.scale : a.scale * query_temperature(a, pos0), scale1 = SIG ? a.scale : a.scale * query_temperature(a, pos1);
+  float scale0 = SIG ? a.scale : a.scale * query_temperature(a, pos0), scale1 = SIG ? a.scale : a.scale * query_temperature(a, pos1);
+  if (HALF) {
+    int e0, e1;
+    q_halves<DK>(qf, &e0, &e1);
+    scale0 = half_scale(a, scale0, e0, kvh);
+    scale1 = half_scale(a, scale1, e1, kvh);
+  }
 
   float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
   float o[DV / 8][4];
@@ -1162,7 +1218,7 @@ __global__ void __launch_bounds__(MMA_THREADS) attn_prefill_mma_x_kernel(AttnArg
     const int kb = tile_kb(it), tlo = tile_lo(it), thi = tile_hi(it);
     if (wrow0 < nrows && kb <= wlast && (SIG || kb + MMA_BK > wfirst)) {
       float s[8][4];
-      qk_mma<DK, 8>(qf, ks, 0, s);
+      qk_mma<DK, 8, HALF>(qf, ks, 0, s);
       unsigned p[4][4];
       if (SIG) {
 #pragma unroll
@@ -1209,9 +1265,9 @@ __global__ void __launch_bounds__(MMA_THREADS) attn_prefill_mma_x_kernel(AttnArg
             for (int e = 0; e < 4; ++e) s[j][e] -= slope * (((e & 2) ? away1 : away0) - (float)(j * 8 + (e & 1)));
           }
         }
-        softmax_update<DV, 8>(s, m, l, o, p);
+        softmax_update<DV, 8, HALF>(s, m, l, o, p);
       }
-      pv_mma<DV, 8>(p, vs, 0, o);
+      pv_mma<DV, 8, HALF>(p, vs, 0, o);
     }
     __syncthreads();
   }
@@ -1222,11 +1278,19 @@ __global__ void __launch_bounds__(MMA_THREADS) attn_prefill_mma_x_kernel(AttnArg
   l[1] += __shfl_xor_sync(0xffffffffu, l[1], 1);
   l[1] += __shfl_xor_sync(0xffffffffu, l[1], 2);
   if (!SIG && a.sink) {                          // one more term of the denominator (the maxima are base-2 exponents)
-    const float sk = a.sink[h] * LOG2E;
-    if (m[0] != -INFINITY) l[0] += fast_exp2(fminf(sk - m[0], 120.f));
-    if (m[1] != -INFINITY) l[1] += fast_exp2(fminf(sk - m[1], 120.f));
+    const float sk = a.sink[h] * LOG2E, more = HALF ? HALF_WEIGHTS_MMA : 0.f;
+    if (m[0] != -INFINITY) l[0] += fast_exp2(fminf(sk - m[0] + more, 120.f));
+    if (m[1] != -INFINITY) l[1] += fast_exp2(fminf(sk - m[1] + more, 120.f));
   }
   const float inv0 = SIG ? 1.f : l[0] > 0.f ? 1.f / l[0] : 0.f, inv1 = SIG ? 1.f : l[1] > 0.f ? 1.f / l[1] : 0.f;
+  if (HALF) {                                      // (divided first: a sum of values times their unit may be more than a float)
+    const float unit = a.kv_unit[a.nkv + kvh];
+#pragma unroll
+    for (int nt = 0; nt < DV / 8; ++nt) {
+      o[nt][0] = o[nt][0] * inv0 * unit; o[nt][1] = o[nt][1] * inv0 * unit; o[nt][2] = o[nt][2] * inv1 * unit; o[nt][3] = o[nt][3] * inv1 * unit;
+    }
+  }
+  const float div0 = HALF ? 1.f : inv0, div1 = HALF ? 1.f : inv1;
   const size_t ostride = (size_t)a.nh * DV;
   const size_t at0 = (size_t)(t0 + q0 + wrow0 + g) * ostride + (size_t)h * DV, at1 = at0 + 8 * ostride;
 #pragma unroll
@@ -1234,12 +1298,12 @@ __global__ void __launch_bounds__(MMA_THREADS) attn_prefill_mma_x_kernel(AttnArg
     const int col = nt * 8 + c2;
     if (a.out_f32) {
       float* out = (float*)a.out;
-      if (row0_ok) *reinterpret_cast<float2*>(out + at0 + col) = make_float2(o[nt][0] * inv0, o[nt][1] * inv0);
-      if (row1_ok) *reinterpret_cast<float2*>(out + at1 + col) = make_float2(o[nt][2] * inv1, o[nt][3] * inv1);
+      if (row0_ok) *reinterpret_cast<float2*>(out + at0 + col) = make_float2(o[nt][0] * div0, o[nt][1] * div0);
+      if (row1_ok) *reinterpret_cast<float2*>(out + at1 + col) = make_float2(o[nt][2] * div1, o[nt][3] * div1);
     } else {
       __nv_bfloat16* out = (__nv_bfloat16*)a.out;
-      if (row0_ok) *reinterpret_cast<unsigned*>(out + at0 + col) = pack_bf16(o[nt][0] * inv0, o[nt][1] * inv0);
-      if (row1_ok) *reinterpret_cast<unsigned*>(out + at1 + col) = pack_bf16(o[nt][2] * inv1, o[nt][3] * inv1);
+      if (row0_ok) *reinterpret_cast<unsigned*>(out + at0 + col) = pack_bf16(o[nt][0] * div0, o[nt][1] * div0);
+      if (row1_ok) *reinterpret_cast<unsigned*>(out + at1 + col) = pack_bf16(o[nt][2] * div1, o[nt][3] * div1);
     }
   }
 }
@@ -1430,12 +1494,12 @@ bool attn_mma_x_supported(int dtype, int d, int dv, int page_size) {
   return dtype == GG_BF16 && (d == 64 || d == 128) && (dv == 64 || dv == 128) && power_of_two(page_size);
 }
 
-template <int DK, int DV, bool SIG>
+template <int DK, int DV, bool SIG, bool HALF = false>
 static int prefill_x_go(const AttnArgs& a, int num_tiles, cudaStream_t stream) {
   const size_t smem = (size_t)2 * MMA_BK * (DK + DV) * 2 + (SIG ? (size_t)(a.dist_max + 1) * sizeof(float) : 0);
-  int rc = opt_in_smem(attn_prefill_mma_x_kernel<DK, DV, SIG>, smem, "attn_prefill_x");
+  int rc = opt_in_smem(attn_prefill_mma_x_kernel<DK, DV, SIG, HALF>, smem, "attn_prefill_x");
   if (rc) return rc;
-  gg_launch(attn_prefill_mma_x_kernel<DK, DV, SIG>, dim3(num_tiles, a.nh), dim3(MMA_THREADS), smem, stream, a);
+  gg_launch(attn_prefill_mma_x_kernel<DK, DV, SIG, HALF>, dim3(num_tiles, a.nh), dim3(MMA_THREADS), smem, stream, a);
   return gg_check_launch("attn_prefill_x");
 }
 
@@ -1451,6 +1515,10 @@ int attn_prefill_mma_x(const AttnArgs& a, int num_tiles, cudaStream_t stream) {
   GG_REQUIRE(num_tiles >= 0 && a.nh <= 65535, "attn_prefill_x: bad grid");
   if (num_tiles == 0) return GG_OK;
   const int dv = a.dv > 0 ? a.dv : a.d;
+  if (a.kv_unit) {
+    GG_REQUIRE(dv == a.d && a.weights == 0 && a.v_share <= 1 && !a.keep_first, "attn_prefill_x: not in half precision");
+    return a.d == 128 ? prefill_x_go<128, 128, false, true>(a, num_tiles, stream) : prefill_x_go<64, 64, false, true>(a, num_tiles, stream);
+  }
   if (a.weights == 1) {
     GG_REQUIRE(attn_mma_x_sigmoid_supported(a), "attn_prefill_x: a distance table of %d entries does not fit", a.dist_max + 1);
     if (a.d == 64 && dv == 64) return prefill_x_go<64, 64, true>(a, num_tiles, stream);

@@ -62,7 +62,7 @@ struct AtcArgs {
 };
 
 // A Q, K or V tile is [128 rows x D]: D/64 halves.
-template <int D>
+template <int D, bool HALF>
 __global__ void __launch_bounds__(ATC_THREADS)
 attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                        const __grid_constant__ CUtensorMap map_v, const AtcArgs args) {
@@ -82,7 +82,8 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
                  p_smem = v_smem + 2 * ATC_TILE_BYTES;
   const unsigned q_full = tc_smem(&bars[0]), k_full0 = tc_smem(&bars[1]), k_empty0 = tc_smem(&bars[3]),
                  v_full0 = tc_smem(&bars[5]), v_empty0 = tc_smem(&bars[7]), s_full0 = tc_smem(&bars[9]),
-                 s_empty0 = tc_smem(&bars[11]), p_full = tc_smem(&bars[13]), pv_done = tc_smem(&bars[14]);
+                 s_empty0 = tc_smem(&bars[11]), p_full = tc_smem(&bars[13]), pv_done = tc_smem(&bars[14]),
+                 q_half = tc_smem(&bars[15]);
 
   if (threadIdx.x == 0) {
     mbar_init(q_full, 1);
@@ -93,6 +94,7 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
     }
     mbar_init(p_full, 8);
     mbar_init(pv_done, 1);
+    mbar_init(q_half, 8);
     abort_s = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -106,7 +108,8 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
   const unsigned tmem_base = tmem_base_s;
   pdl_trigger();
 
-  // ---- what this CTA works on (lists copied in before the step began: read before the wait)
+  // ---- what this CTA works on (lists copied in before the step began: read before the wait; HALF: the kernel ahead makes them)
+  if (HALF) pdl_wait();
   // grid (heads, tiles): the heads of one tile are neighbours, and the caller lists the tiles
   // with the most keys first, so the long ones start early and the short ones fill the end
   const int b = a.tile_seq[blockIdx.y], q0 = a.tile_q0[blockIdx.y];
@@ -165,12 +168,13 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
     if (!ok && lane == 0) { atomicExch(args.status, ATC_ERR_PRODUCER); atomicExch(&abort_s, 1); }
   } else if (warp == 1 && lane == 0) {
     // ---------------- MMA issuer
-    // instruction descriptors: f32 accumulate, bf16 inputs, M = 128; scores: N = 128 keys
-    const unsigned idesc_qk = (1u << 4) | (1u << 7) | (1u << 10) | ((128u >> 3) << 17) | ((128u >> 4) << 24);
+    // instruction descriptors: f32 accumulate, bf16 inputs (HALF: f16, format 0), M = 128; scores: N = 128 keys
+    const unsigned types = HALF ? 0u : (1u << 7) | (1u << 10);
+    const unsigned idesc_qk = (1u << 4) | types | ((128u >> 3) << 17) | ((128u >> 4) << 24);
     // O += P V: N = D, B (V) is MN-major
-    const unsigned idesc_pv = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) | (((unsigned)D >> 3) << 17) | ((128u >> 4) << 24);
+    const unsigned idesc_pv = (1u << 4) | types | (1u << 16) | (((unsigned)D >> 3) << 17) | ((128u >> 4) << 24);
     const unsigned tmem_o = tmem_base + 256;
-    bool ok = mbar_wait(q_full, 0);
+    bool ok = mbar_wait(HALF ? q_half : q_full, 0);
     auto issue_qk = [&](int j) -> bool {
       const int s = j & 1;
       const unsigned phase = (j >> 1) & 1;
@@ -223,11 +227,41 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
     const unsigned lane_addr = tmem_base + ((unsigned)(quarter * 32) << 16);
     constexpr int OC = D / 2;                             // O columns of this thread
     const unsigned tmem_o = lane_addr + 256 + sub * OC;
-    const float sc = a.scale * ATC_LOG2E;
+    float sc = a.scale * ATC_LOG2E;
     float m_ref = -INFINITY, l = 0.f;
     const int stale_hi = (hi + ps - 1) / ps * ps;        // end of the last page that is fetched
     bool ok = true;
-    for (int j = 0; j < ntiles; ++j) {
+    if (HALF) {
+      // the Q tile as half precision numbers, each row times a power of two: a thread takes half of a row, in place (16 bytes at a time, in an
+      // order that keeps eight rows on different banks)
+      ok = softmax_all(mbar_wait(q_full, 0) && !*(volatile int*)&abort_s);
+      if (ok) {
+        constexpr int CHUNKS = D / 16;
+        const unsigned row = q_smem + (HALVES == 2 ? sub * ATC_HALF_BYTES : sub * 64) + (unsigned)r * 128;
+        uint4 w[CHUNKS];
+        float big = 0.f;
+#pragma unroll
+        for (int i = 0; i < CHUNKS; ++i) {
+          asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w[i].x), "=r"(w[i].y), "=r"(w[i].z), "=r"(w[i].w)
+                       : "r"(row + (((i + r) & (CHUNKS - 1)) << 4)));
+          big = fmaxf(big, fmaxf(fmaxf(largest_bf16(w[i].x), largest_bf16(w[i].y)), fmaxf(largest_bf16(w[i].z), largest_bf16(w[i].w))));
+        }
+        xsum[sub][r] = big;
+        softmax_sync();
+        const int e = half_exponent(fmaxf(big, xsum[sub ^ 1][r]));
+        const float up = two_to(e);
+#pragma unroll
+        for (int i = 0; i < CHUNKS; ++i)
+          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(row + (((i + r) & (CHUNKS - 1)) << 4)), "r"(half_of_bf16(w[i].x, up)),
+                       "r"(half_of_bf16(w[i].y, up)), "r"(half_of_bf16(w[i].z, up)), "r"(half_of_bf16(w[i].w, up)) : "memory");
+        sc = half_scale(a, sc, e, kvh);
+        fence_async_smem();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(q_half);
+      }
+    }
+    for (int j = 0; j < ntiles && ok; ++j) {
       const int s = j & 1;
       const int kb = kstart + j * ATC_BK + sub * 64;      // first key of this thread's 64
       ok = softmax_all(mbar_wait(s_full0 + 8 * s, (j >> 1) & 1) && !*(volatile int*)&abort_s);
@@ -309,7 +343,7 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
       }
       // p = 2^(s - m_ref), row sum, P to shared memory (bf16, swizzled K-major): this thread's
       // 64 keys are half `sub` of the P tile
-      const float mr = m_ref == -INFINITY ? 0.f : m_ref;
+      const float mr = (m_ref == -INFINITY ? 0.f : m_ref) - (HALF ? HALF_WEIGHTS : 0.f);
       float sum = 0.f;
 #pragma unroll
       for (int c = 0; c < 64; c += 8) {
@@ -318,8 +352,7 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
         for (int i = 0; i < 8; i += 2) {
           const float p0 = fast_exp2(sv[c + i] - mr), p1 = fast_exp2(sv[c + i + 1] - mr);   // 2^-inf = 0
           sum += p0 + p1;
-          __nv_bfloat162 t = __floats2bfloat162_rn(p0, p1);
-          pk[i >> 1] = *reinterpret_cast<unsigned*>(&t);
+          pk[i >> 1] = HALF ? pack_half(p0, p1) : pack_bf16(p0, p1);
         }
         const unsigned addr = p_smem + sub * ATC_HALF_BYTES + (unsigned)r * 128 + (unsigned)(((c >> 3) ^ (r & 7)) << 4);
         asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(pk[0]), "r"(pk[1]), "r"(pk[2]),
@@ -339,20 +372,23 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
     l += xsum[sub ^ 1][r];
     tc_fence_after();
     if (ok && !*(volatile int*)&abort_s) {
-      const float inv = l > 0.f ? 1.f / l : 0.f;
+      const float inv = l > 0.f ? 1.f / l : 0.f, unit = HALF ? a.kv_unit[a.nkv + kvh] : 1.f, div = HALF ? 1.f : inv;
       __nv_bfloat16* o = (__nv_bfloat16*)a.out + (size_t)(t0 + q0 + r) * a.nh * ATC_D + (size_t)h * ATC_D + sub * OC;
 #pragma unroll
       for (int c = 0; c < OC; c += 32) {
         unsigned v[32];
         tc_load32(tmem_o + c, v);
+        if (HALF)                                  // (divided first: a sum of values times their unit may be more than a float)
+#pragma unroll
+          for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * inv * unit);
         if (row_ok) {
 #pragma unroll
           for (int i = 0; i < 32; i += 8) {
             uint4 pk;
-            __nv_bfloat162 t0v = __floats2bfloat162_rn(__uint_as_float(v[i]) * inv, __uint_as_float(v[i + 1]) * inv);
-            __nv_bfloat162 t1v = __floats2bfloat162_rn(__uint_as_float(v[i + 2]) * inv, __uint_as_float(v[i + 3]) * inv);
-            __nv_bfloat162 t2v = __floats2bfloat162_rn(__uint_as_float(v[i + 4]) * inv, __uint_as_float(v[i + 5]) * inv);
-            __nv_bfloat162 t3v = __floats2bfloat162_rn(__uint_as_float(v[i + 6]) * inv, __uint_as_float(v[i + 7]) * inv);
+            __nv_bfloat162 t0v = __floats2bfloat162_rn(__uint_as_float(v[i]) * div, __uint_as_float(v[i + 1]) * div);
+            __nv_bfloat162 t1v = __floats2bfloat162_rn(__uint_as_float(v[i + 2]) * div, __uint_as_float(v[i + 3]) * div);
+            __nv_bfloat162 t2v = __floats2bfloat162_rn(__uint_as_float(v[i + 4]) * div, __uint_as_float(v[i + 5]) * div);
+            __nv_bfloat162 t3v = __floats2bfloat162_rn(__uint_as_float(v[i + 6]) * div, __uint_as_float(v[i + 7]) * div);
             pk.x = *reinterpret_cast<unsigned*>(&t0v); pk.y = *reinterpret_cast<unsigned*>(&t1v);
             pk.z = *reinterpret_cast<unsigned*>(&t2v); pk.w = *reinterpret_cast<unsigned*>(&t3v);
             *reinterpret_cast<uint4*>(o + c + i) = pk;
@@ -386,6 +422,22 @@ static int encode(CUtensorMap* map, const void* ptr, int rank, const cuuint64_t*
   return GG_OK;
 }
 
+template <int D, bool HALF>
+static int tc_launch(const CUtensorMap& map_q, const CUtensorMap& map_k, const CUtensorMap& map_v, const AtcArgs& args, int num_tiles,
+                     cudaStream_t stream) {
+  const size_t smem = 5 * (size_t)(D / 64) * ATC_HALF_BYTES + ATC_P_BYTES + 1024;     // Q, 2 K, 2 V, P
+  static bool set = false;
+  if (!set) {
+    cudaError_t e = cudaFuncSetAttribute(attn_prefill_tc_kernel<D, HALF>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e != cudaSuccess) return gg_fail(GG_ERR_CUDA, "attn_prefill_tc: %s", cudaGetErrorString(e));
+    set = true;
+  }
+  cudaError_t e = gg_launch(attn_prefill_tc_kernel<D, HALF>, dim3(args.a.nh, num_tiles), dim3(ATC_THREADS), smem, stream, map_q, map_k,
+                            map_v, args);
+  if (e != cudaSuccess) return gg_fail(GG_ERR_CUDA, "attn_prefill_tc: launch: %s", cudaGetErrorString(e));
+  return gg_check_launch("attn_prefill_tc");
+}
+
 // a.tile_seq / a.tile_q0 list tiles of 128 query rows.  T = rows of the q buffer.
 int attn_prefill_tc(const AttnArgs& a, int num_tiles, int T, int num_pages, int* status, cudaStream_t stream) {
   GG_REQUIRE(num_tiles >= 0 && num_tiles <= 65535, "attn_prefill_tc: %d tiles in one launch", num_tiles);
@@ -414,28 +466,8 @@ int attn_prefill_tc(const AttnArgs& a, int num_tiles, int T, int num_pages, int*
   args.a = a;
   args.num_pages = num_pages;
   args.status = status;
-  const size_t tile_bytes = (size_t)(a.d / 64) * ATC_HALF_BYTES;
-  const size_t smem = 5 * tile_bytes + ATC_P_BYTES + 1024;     // Q, 2 K, 2 V, P
-  cudaError_t e;
-  if (a.d == 128) {
-    static bool set = false;
-    if (!set) {
-      e = cudaFuncSetAttribute(attn_prefill_tc_kernel<128>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-      if (e != cudaSuccess) return gg_fail(GG_ERR_CUDA, "attn_prefill_tc: %s", cudaGetErrorString(e));
-      set = true;
-    }
-    e = gg_launch(attn_prefill_tc_kernel<128>, dim3(a.nh, num_tiles), dim3(ATC_THREADS), smem, stream, map_q, map_k,
-                  map_v, args);
-  } else {
-    static bool set = false;
-    if (!set) {
-      e = cudaFuncSetAttribute(attn_prefill_tc_kernel<64>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-      if (e != cudaSuccess) return gg_fail(GG_ERR_CUDA, "attn_prefill_tc: %s", cudaGetErrorString(e));
-      set = true;
-    }
-    e = gg_launch(attn_prefill_tc_kernel<64>, dim3(a.nh, num_tiles), dim3(ATC_THREADS), smem, stream, map_q, map_k,
-                  map_v, args);
-  }
-  if (e != cudaSuccess) return gg_fail(GG_ERR_CUDA, "attn_prefill_tc: launch: %s", cudaGetErrorString(e));
-  return gg_check_launch("attn_prefill_tc");
+  if (a.kv_unit) return a.d == 128 ? tc_launch<128, true>(map_q, map_k, map_v, args, num_tiles, stream)
+                                  : tc_launch<64, true>(map_q, map_k, map_v, args, num_tiles, stream);
+  return a.d == 128 ? tc_launch<128, false>(map_q, map_k, map_v, args, num_tiles, stream)
+                    : tc_launch<64, false>(map_q, map_k, map_v, args, num_tiles, stream);
 }

@@ -109,7 +109,7 @@ struct At3Args {
   int* status;
 };
 
-template <int D, int DV, bool X>
+template <int D, int DV, bool X, bool HALF>
 __global__ void __launch_bounds__(AT3_THREADS, 1)
 attn_prefill_tc3_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                         const __grid_constant__ CUtensorMap map_v, const At3Args args) {
@@ -127,13 +127,14 @@ attn_prefill_tc3_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
   const unsigned k_smem = q_smem + 2 * TILE_BYTES;                // [2 stages]
   const unsigned v_smem = k_smem + 2 * TILE_BYTES;                // [2 stages]
   // barriers: 0 q_full; 1,2 k_full; 3,4 k_empty; 5,6 v_full; 7,8 v_empty;
-  // per head t (base 9 + 4 t): +0 s_full, +1 p_full, +2 pv_done, +3 turn
+  // per head t (base 9 + 4 t): +0 s_full, +1 p_full, +2 pv_done, +3 turn; 17 + t: Q as half precision numbers
   const unsigned q_full = tc_smem(&bars[0]), k_full0 = tc_smem(&bars[1]), k_empty0 = tc_smem(&bars[3]),
                  v_full0 = tc_smem(&bars[5]), v_empty0 = tc_smem(&bars[7]);
   auto s_full = [&](int t) { return tc_smem(&bars[9 + 4 * t]); };
   auto p_full = [&](int t) { return tc_smem(&bars[9 + 4 * t + 1]); };
   auto pv_done = [&](int t) { return tc_smem(&bars[9 + 4 * t + 2]); };
   auto turn = [&](int t) { return tc_smem(&bars[9 + 4 * t + 3]); };     // head t may run its exponentials
+  auto q_half = [&](int t) { return tc_smem(&bars[17 + t]); };
 
   if (threadIdx.x == 0) {
     mbar_init(q_full, 1);
@@ -146,6 +147,7 @@ attn_prefill_tc3_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
       mbar_init(p_full(t), 4);
       mbar_init(pv_done(t), 1);
       mbar_init(turn(t), 4);
+      mbar_init(q_half(t), 4);
     }
     abort_s = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -161,7 +163,8 @@ attn_prefill_tc3_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
   pdl_trigger();
 
   // ---- what this CTA works on: grid (head pairs, tiles), the tiles with the most keys first
-  // (the lists were copied in before the step began: read before the wait)
+  // (the lists were copied in before the step began: read before the wait; HALF: the kernel ahead makes them)
+  if (HALF) pdl_wait();
   const int b = a.tile_seq[blockIdx.y], q0 = a.tile_q0[blockIdx.y];
   const int h0 = 2 * blockIdx.x, kvh = h0 / (a.nh / a.nkv);
   const int t0 = a.cu_q_lens[b], qlen = a.cu_q_lens[b + 1] - t0;
@@ -226,10 +229,11 @@ attn_prefill_tc3_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
       // ---------------- MMA issuers: one lane of warp 1 for head 0, one of warp 2 for head 1.
       // A key or value tile is free when both have committed (those barriers count two arrivals).
       const int t = warp - 1;
-      // instruction descriptors: f32 accumulate, bf16 inputs, M = 128; scores: N = 128 keys
-      const unsigned idesc_qk = (1u << 4) | (1u << 7) | (1u << 10) | ((128u >> 3) << 17) | ((128u >> 4) << 24);
+      // instruction descriptors: f32 accumulate, bf16 inputs (HALF: f16, format 0), M = 128; scores: N = 128 keys
+      const unsigned types = HALF ? 0u : (1u << 7) | (1u << 10);
+      const unsigned idesc_qk = (1u << 4) | types | ((128u >> 3) << 17) | ((128u >> 4) << 24);
       // O += P V: N = DV, B (V) is MN-major
-      const unsigned idesc_pv = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) | (((unsigned)DV >> 3) << 17) | ((128u >> 4) << 24);
+      const unsigned idesc_pv = (1u << 4) | types | (1u << 16) | (((unsigned)DV >> 3) << 17) | ((128u >> 4) << 24);
       // the descriptors' upper words never change and a tile's k step only adds to the address
       // field of the lower word
       const unsigned hi_k = 64u | (1u << 14) | (2u << 29);                 // SBO 1024 bytes, version 1, 128-byte swizzle
@@ -243,7 +247,7 @@ attn_prefill_tc3_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
         v_lo[i] = lo_word(v_smem + i * V_BYTES, lbo_v);
       }
       const unsigned tmem_s = tmem_base + t * 256, tmem_o = tmem_s + 128;
-      bool ok = mbar_wait(q_full, 0);
+      bool ok = mbar_wait(HALF ? q_half(t) : q_full, 0);
       auto issue_qk = [&](int j) -> bool {
         const int s = j & 1;
         if (!mbar_wait(k_full0 + 8 * s, (j >> 1) & 1)) return false;
@@ -290,7 +294,37 @@ attn_prefill_tc3_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
     const unsigned tmem_o = lane_addr + 128;
     // X: the row's own scale (a query temperature is part of it), the head's slope in base-2 exponents, the cap, and the
     // first key of the row's chunk
-    const float sc = a.scale * AT3_LOG2E * (X ? query_temperature(a, pos) : 1.f);
+    float sc = a.scale * AT3_LOG2E * (X ? query_temperature(a, pos) : 1.f);
+    bool ok = true;
+    if (HALF) {
+      // the head's Q tile as half precision numbers, each row times a power of two: a thread takes its row, in place (16 bytes at a time, in an
+      // order that keeps eight rows on different banks)
+      ok = mbar_wait(q_full, 0) && !*(volatile int*)&abort_s;
+      ok = __all_sync(0xffffffffu, ok);
+      if (ok) {
+        const unsigned row = q_smem + t * TILE_BYTES + (unsigned)r * 128;
+        uint4 w[HALVES * 8];
+        float big = 0.f;
+#pragma unroll
+        for (int i = 0; i < HALVES * 8; ++i) {
+          asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w[i].x), "=r"(w[i].y), "=r"(w[i].z), "=r"(w[i].w)
+                       : "r"(row + (i >> 3) * AT3_HALF + (((i + r) & 7) << 4)));
+          big = fmaxf(big, fmaxf(fmaxf(largest_bf16(w[i].x), largest_bf16(w[i].y)), fmaxf(largest_bf16(w[i].z), largest_bf16(w[i].w))));
+        }
+        const int e = half_exponent(big);
+        const float up = two_to(e);
+#pragma unroll
+        for (int i = 0; i < HALVES * 8; ++i)
+          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(row + (i >> 3) * AT3_HALF + (((i + r) & 7) << 4)), "r"(half_of_bf16(w[i].x, up)),
+                       "r"(half_of_bf16(w[i].y, up)), "r"(half_of_bf16(w[i].z, up)), "r"(half_of_bf16(w[i].w, up)) : "memory");
+        sc = half_scale(a, sc, e, kvh);
+        if (!X) sc = fminf(fmaxf(sc, 0x1p-126f), 0x1p100f);      // (-infinity times it stays that)
+        fence_async_smem();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(q_half(t));
+      }
+    }
     const float slope = X && a.slopes ? a.slopes[h0 + t] * AT3_LOG2E : 0.f;
     const float cap2 = X ? a.softcap * AT3_LOG2E : 0.f, to_cap = cap2 > 0.f ? sc / cap2 : 0.f;
     const int row_chunk = X && a.chunk > 0 ? (pos / a.chunk) * a.chunk : 0;
@@ -299,8 +333,7 @@ attn_prefill_tc3_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
     const int row_from = max(max(lo, row_chunk), a.window > 0 ? pos - a.window + 1 : 0), row_end = row_ok ? pos + 1 : 0;
     float m_ref = -INFINITY, l = 0.f;
     const int stale_hi = (hi + ps - 1) / ps * ps;        // end of the last page that is fetched
-    bool ok = true;
-    for (int j = 0; j < ntiles; ++j) {
+    for (int j = 0; j < ntiles && ok; ++j) {
       const int s = j & 1;
       const int kb = kstart + j * AT3_BK;
       ok = mbar_wait(s_full(t), j & 1) && !*(volatile int*)&abort_s;
@@ -418,7 +451,7 @@ attn_prefill_tc3_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
       if (!ok) break;
       // p = 2^(s * scale - m_ref), row sum, P into the first 64 columns of the score buffer
       // (column c = keys 2c, 2c + 1 as a pair of bfloat16); the argument and the sum two at a time
-      const float neg_mr = m_ref == -INFINITY ? 0.f : -m_ref;
+      const float neg_mr = (m_ref == -INFINITY ? 0.f : -m_ref) + (HALF ? HALF_WEIGHTS : 0.f);
       float sums[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int c = 0; c < AT3_BK; c += 64) {
@@ -429,8 +462,7 @@ attn_prefill_tc3_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
           at3_fma2(a0, a1, sv[c + i], sv[c + i + 1], X ? 1.f : sc, neg_mr);           // -inf stays -inf
           const float p0 = fast_exp2(a0), p1 = fast_exp2(a1);               // 2^-inf = 0
           at3_add2(sums[i & 2], sums[(i & 2) + 1], p0, p1);
-          __nv_bfloat162 pr = __floats2bfloat162_rn(p0, p1);
-          pk[i >> 1] = *reinterpret_cast<unsigned*>(&pr);
+          pk[i >> 1] = HALF ? pack_half(p0, p1) : pack_bf16(p0, p1);
         }
         tc_store32(lane_addr + (c >> 1), pk);
       }
@@ -447,8 +479,8 @@ attn_prefill_tc3_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
     if (!ok && lane == 0) { atomicExch(args.status, AT3_ERR_SOFTMAX); atomicExch(&abort_s, 1); }
     tc_fence_after();
     if (ok && !*(volatile int*)&abort_s) {
-      if (X && a.sink && m_ref != -INFINITY) l += fast_exp2(fminf(a.sink[h0 + t] * AT3_LOG2E - m_ref, 120.f));
-      const float inv = l > 0.f ? 1.f / l : 0.f;
+      if (X && a.sink && m_ref != -INFINITY) l += fast_exp2(fminf(a.sink[h0 + t] * AT3_LOG2E - m_ref + (HALF ? HALF_WEIGHTS : 0.f), 120.f));
+      const float inv = l > 0.f ? 1.f / l : 0.f, unit = HALF ? a.kv_unit[a.nkv + kvh] : 1.f;
       const size_t at = (size_t)(t0 + q0 + r) * a.nh * DV + (size_t)(h0 + t) * DV;
 #pragma unroll
       for (int c = 0; c < DV; c += 32) {
@@ -457,7 +489,7 @@ attn_prefill_tc3_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
         if (row_ok) {
           float f[32];
 #pragma unroll
-          for (int i = 0; i < 32; ++i) f[i] = __uint_as_float(v[i]) * inv;
+          for (int i = 0; i < 32; ++i) f[i] = HALF ? __uint_as_float(v[i]) * inv * unit : __uint_as_float(v[i]) * inv;
           if (X && a.out_f32) store_row32((float*)a.out + at + c, f, 32);
           else store_row32((__nv_bfloat16*)a.out + at + c, f, 32);
         }
@@ -475,11 +507,11 @@ attn_prefill_tc3_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
 // ---------------------------------------------------------------- host side
 // Registers the kernel is given at launch, times its threads: what the two setmaxnreg numbers
 // must fit into.  0 if the kernel cannot be asked.
-template <int D, int DV, bool X> static int at3_register_pool() {
+template <int D, int DV, bool X, bool HALF = false> static int at3_register_pool() {
   static int pool = -1;
   if (pool < 0) {
     cudaFuncAttributes fa;
-    if (cudaFuncGetAttributes(&fa, attn_prefill_tc3_kernel<D, DV, X>) != cudaSuccess) { (void)cudaGetLastError(); pool = 0; }
+    if (cudaFuncGetAttributes(&fa, attn_prefill_tc3_kernel<D, DV, X, HALF>) != cudaSuccess) { (void)cudaGetLastError(); pool = 0; }
     else pool = fa.numRegs * AT3_THREADS;
   }
   return pool;
@@ -503,6 +535,13 @@ bool attn_tc3_x_supported(int dtype, int d, int dv, int page_size, int nh, int n
   return pool >= AT3_POOL;
 }
 
+bool attn_tc3_half_supported(int d, int page_size, int nh, int nkv, bool x) {
+  if (!at3_shape(GG_BF16, d, page_size, nh, nkv)) return false;
+  const int pool = d == 128 ? (x ? at3_register_pool<128, 128, true, true>() : at3_register_pool<128, 128, false, true>())
+                            : (x ? at3_register_pool<64, 64, true, true>() : at3_register_pool<64, 64, false, true>());
+  return pool >= AT3_POOL;
+}
+
 static int encode3(CUtensorMap* map, const void* ptr, int rank, const cuuint64_t* dims, const cuuint64_t* strides,
                    const cuuint32_t* box) {
   GgEncodeTiledFn fn = gg_encode_tiled();
@@ -515,17 +554,17 @@ static int encode3(CUtensorMap* map, const void* ptr, int rank, const cuuint64_t
   return GG_OK;
 }
 
-template <int D, int DV, bool X>
+template <int D, int DV, bool X, bool HALF = false>
 static int at3_launch(const CUtensorMap& map_q, const CUtensorMap& map_k, const CUtensorMap& map_v, const At3Args& args, int num_tiles,
                       cudaStream_t stream) {
   const size_t smem = (size_t)(4 * (D / 64) + 2 * (DV / 64)) * AT3_HALF + 1024;   // 2 Q, 2 K, 2 V
   static bool set = false;
   if (!set) {
-    cudaError_t e = cudaFuncSetAttribute(attn_prefill_tc3_kernel<D, DV, X>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    cudaError_t e = cudaFuncSetAttribute(attn_prefill_tc3_kernel<D, DV, X, HALF>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) return gg_fail(GG_ERR_CUDA, "attn_prefill_tc3: %s", cudaGetErrorString(e));
     set = true;
   }
-  cudaError_t e = gg_launch(attn_prefill_tc3_kernel<D, DV, X>, dim3(args.a.nh / 2, num_tiles), dim3(AT3_THREADS), smem, stream, map_q,
+  cudaError_t e = gg_launch(attn_prefill_tc3_kernel<D, DV, X, HALF>, dim3(args.a.nh / 2, num_tiles), dim3(AT3_THREADS), smem, stream, map_q,
                             map_k, map_v, args);
   if (e != cudaSuccess) return gg_fail(GG_ERR_CUDA, "attn_prefill_tc3: launch: %s", cudaGetErrorString(e));
   return gg_check_launch("attn_prefill_tc3");
@@ -538,7 +577,8 @@ int attn_prefill_tc3(const AttnArgs& a, int num_tiles, int T, int num_pages, int
   GG_REQUIRE(status != nullptr, "attn_prefill_tc3: no status word given");
   GG_REQUIRE(a.q_stride % 8 == 0 && ((size_t)a.q % 16) == 0, "attn_prefill_tc3: q rows must be 16-byte aligned");
   GG_REQUIRE((a.nh / a.nkv) % 2 == 0, "attn_prefill_tc3: %d heads per kv head; pairs of heads must share a kv head", a.nh / a.nkv);
-  GG_REQUIRE(x ? attn_tc3_x_supported(GG_BF16, a.d, dv, a.page_size, a.nh, a.nkv) : attn_tc3_supported(GG_BF16, a.d, a.page_size, a.nh, a.nkv),
+  GG_REQUIRE(a.kv_unit ? dv == a.d && nv == a.nkv && attn_tc3_half_supported(a.d, a.page_size, a.nh, a.nkv, x)
+             : x ? attn_tc3_x_supported(GG_BF16, a.d, dv, a.page_size, a.nh, a.nkv) : attn_tc3_supported(GG_BF16, a.d, a.page_size, a.nh, a.nkv),
              "attn_prefill_tc3: not for this shape or build");
   if (num_tiles == 0) return GG_OK;
   CUtensorMap map_q, map_k, map_v;
@@ -561,6 +601,12 @@ int attn_prefill_tc3(const AttnArgs& a, int num_tiles, int T, int num_pages, int
   args.a = a;
   args.num_pages = num_pages;
   args.status = status;
+  if (a.kv_unit) {
+    if (a.d == 128) return x ? at3_launch<128, 128, true, true>(map_q, map_k, map_v, args, num_tiles, stream)
+                             : at3_launch<128, 128, false, true>(map_q, map_k, map_v, args, num_tiles, stream);
+    return x ? at3_launch<64, 64, true, true>(map_q, map_k, map_v, args, num_tiles, stream)
+             : at3_launch<64, 64, false, true>(map_q, map_k, map_v, args, num_tiles, stream);
+  }
   if (!x) return a.d == 128 ? at3_launch<128, 128, false>(map_q, map_k, map_v, args, num_tiles, stream)
                             : at3_launch<64, 64, false>(map_q, map_k, map_v, args, num_tiles, stream);
   if (a.d == 128) return dv == 128 ? at3_launch<128, 128, true>(map_q, map_k, map_v, args, num_tiles, stream)

@@ -36,7 +36,7 @@ int gg_check_launch(const char* what);
 __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void pdl_trigger() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
-// True unless GOLLMGO_B200_NO_PDL is set in the environment or the calling thread has paused it (gg_pause_pdl).
+// True unless GOLLMGO_B200_NO_PDL is set in the environment.
 bool gg_pdl_enabled();
 
 template <typename... KArgs, typename... Args>

@@ -6,7 +6,6 @@ launches go to torch's current CUDA stream, so they can be captured in a graph.
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes
 import functools
 from typing import Optional
@@ -1549,7 +1548,10 @@ _PACKED_TYPES = {
     "gg_packed_prompt_fold": [_I, _I],
     "gg_packed_prompt_f32": [_P, _L, _P, _I, _P, _I, _I, _P, _P, _I, _I, _P, _I, _P, _L, _P, _I, _I, _I, _I, _I, _I, _F, _F, _P, _P, _F, _F, _P],
     "gg_packed_prefill": [_P, _L, _I, _P, _I, _P, _I, _P, _P, _P, _P, _I, _P, _I, _I, _I, _I, _I, _I, _F, _F, _P, _P, _F, _F, _P],
-    "gg_packed_unfold": [_P, _I, _P, _I, _P, _P, _I, _P, _P, _I, _I, _I, _P, _I, _I, _P, _P, _I, _I, _P, _P, _I, _I, _I, _I, _I, _I, _P],
+    "gg_packed_loud_floats": [_I],
+    "gg_packed_loud": [_P, _I, _P, _I, _P, _P, _I, _P, _I, _I, _I, _I, _I, _I, _P],
+    "gg_packed_unfold": [_P, _I, _P, _I, _P, _P, _I, _P, _P, _I, _I, _P, _P, _P, _I, _I, _P, _P, _I, _I, _P, _P, _I, _I, _I, _I, _I, _I, _P],
+    "gg_attn_prefill_half": [_P, _L, _P, _P, _P, _P, _I, _P, _P, _P, _P, _I, _P, _P, _I, _P, _I, _I, _I, _I, _I, _I, _I, _I, _F, _F, _P, _P, _F, _F, _P, _P],
 }
 _PACKED = {}
 
@@ -1800,32 +1802,42 @@ def packed_prompt_f32(q: torch.Tensor, pages: torch.Tensor, tables: torch.Tensor
            1 + 2 * -(-count // packed_decode_tokens(nh, width, page_size)))
 
 
-@contextlib.contextmanager
-def after_everything():
-    """Launches in this block start when the kernels ahead of them have completed, also those that read their lists early:
-    for kernels whose tile lists or block tables the kernel directly ahead writes."""
-    pause = lib().gg_pause_pdl
-    pause(1)
-    try:
-        yield
-    finally:
-        pause(0)
+@functools.lru_cache(maxsize=None)
+def packed_loud_floats(nkv: int) -> int:
+    """Floats of ``loud`` of packed_loud and packed_unfold."""
+    return _packed("gg_packed_loud_floats")(nkv)
+
+
+def packed_loud(pages: torch.Tensor, tables: torch.Tensor, cu_q_lens: torch.Tensor, context_lens: torch.Tensor, loud: torch.Tensor, nkv: int, d: int,
+                page_size: int, bits: int, window: int, least: int = 1) -> None:
+    """How large the keys and values in sight of the portions are, for packed_unfold: partial maxima in ``loud``, float32 of packed_loud_floats."""
+    stream = _stream_of("packed_loud", pages, tables, cu_q_lens, context_lens, loud)
+    B, width = _tables("packed_loud", tables)
+    _ints("packed_loud", B, context_lens)
+    _ints("packed_loud", B + 1, cu_q_lens)
+    if loud.numel() < packed_loud_floats(nkv) or loud.dtype != torch.float32 or not loud.is_contiguous():
+        raise KernelError("packed_loud: the maxima are contiguous float32, large enough")
+    _check(_packed("gg_packed_loud")(pages.data_ptr(), pages.shape[0], tables.data_ptr(), width, cu_q_lens.data_ptr(), context_lens.data_ptr(), B,
+                                     loud.data_ptr(), least, nkv, d, page_size, bits, window, stream))
 
 
 def packed_unfold(pages: torch.Tensor, tables: torch.Tensor, cu_q_lens: torch.Tensor, context_lens: torch.Tensor, k_out: Optional[torch.Tensor],
-                  v_out: Optional[torch.Tensor], most_pages: int, out_tables: Optional[torch.Tensor], lists, nkv: int, d: int, page_size: int, bits: int,
-                  window: int, least: int = 1) -> None:
-    """What the prompt kernels need of the portions of a step (sequences with ``least`` rows or more in cu_q_lens): their pages as
-    plain keys and values behind one another in k_out, v_out [pages, nkv, page_size, d], block tables of those pages in
-    ``out_tables`` (shape of ``tables``), and one or two tile lists: ``lists`` of (height, count, seq, q0) with the number of
-    tiles that the portions cut into rows of that height make.  Pages that the window hides are left out.  Without ``k_out`` and ``v_out`` (and
-    ``most_pages`` 0): the lists alone."""
-    stream = _stream_of("packed_unfold", pages, tables, cu_q_lens, context_lens, k_out, v_out, out_tables)
+                  v_out: Optional[torch.Tensor], most_pages: int, out_tables: Optional[torch.Tensor], lists, nkv: int, d: int, page_size: int,
+                  bits: int, window: int, least: int = 1, loud: Optional[torch.Tensor] = None, kv_unit: Optional[torch.Tensor] = None) -> None:
+    """What the prompt kernels need of the portions of a step (sequences with ``least`` rows or more in cu_q_lens): one or two tile lists, ``lists``
+    of (height, count, seq, q0) with the number of tiles that the portions cut into rows of that height make; and, with ``k_out`` and ``v_out``
+    float16 [pages, nkv, page_size, d], their pages as keys and values behind one another there, times ``kv_unit`` float32 [2, nkv] (powers of two,
+    from ``loud`` of packed_loud), and block tables of those pages in ``out_tables`` (shape of ``tables``).  Pages that the window hides are
+    left out."""
+    stream = _stream_of("packed_unfold", pages, tables, cu_q_lens, context_lens, k_out, v_out, out_tables, loud, kv_unit)
     B, width = _tables("packed_unfold", tables)
     _ints("packed_unfold", B, context_lens)
+    _ints("packed_unfold", B + 1, cu_q_lens)
     if k_out is not None:
         _ints("packed_unfold", B * width, out_tables)
-    _ints("packed_unfold", B + 1, cu_q_lens)
+        if k_out.dtype != torch.float16 or v_out.dtype != torch.float16 or not (k_out.is_contiguous() and v_out.is_contiguous()) \
+                or loud.numel() < packed_loud_floats(nkv) or kv_unit.numel() < 2 * nkv:
+            raise KernelError("packed_unfold: keys and values go to contiguous float16, with their maxima and units")
     flat = []
     for height, count, seq, q0 in lists:
         _ints("packed_unfold", count, seq, q0)
@@ -1833,6 +1845,28 @@ def packed_unfold(pages: torch.Tensor, tables: torch.Tensor, cu_q_lens: torch.Te
     if len(lists) == 1:
         flat += [0, 0, None, None]
     _check(_packed("gg_packed_unfold")(pages.data_ptr(), pages.shape[0], tables.data_ptr(), width, cu_q_lens.data_ptr(),
-                                       context_lens.data_ptr(), B, _at(k_out), _at(v_out), dtype_code(k_out.dtype) if k_out is not None else 1,
-                                       k_out.shape[0] if k_out is not None else 0, most_pages, _at(out_tables), *flat, least, nkv, d, page_size, bits, window,
-                                       stream))
+                                       context_lens.data_ptr(), B, _at(k_out), _at(v_out), k_out.shape[0] if k_out is not None else 0, most_pages,
+                                       _at(out_tables), _at(loud), _at(kv_unit), *flat, least, nkv, d, page_size, bits, window, stream))
+
+
+def attn_prefill_half(q: torch.Tensor, kcache: torch.Tensor, vcache: torch.Tensor, kv_unit: torch.Tensor, block_tables: torch.Tensor, bt_stride: int,
+                      cu_q_lens: torch.Tensor, context_lens: torch.Tensor, tile64, tile128, out: torch.Tensor, nh: int, nkv: int, d: int,
+                      page_size: int, window: int, scale: float, options: bool, softcap: float = 0.0, sink: Optional[torch.Tensor] = None,
+                      slopes: Optional[torch.Tensor] = None, temperature=None) -> None:
+    """attn_prefill, or with ``options`` attn_prefill_x, in half precision: q and the result are bfloat16, keys, values and ``kv_unit`` what
+    packed_unfold makes.  ``tile64`` and ``tile128`` (or None): (seq, q0, count) of tiles of so many rows."""
+    global tc_launched
+    stream = _stream_of("attn_prefill_half", q, kcache, vcache, kv_unit, block_tables, cu_q_lens, context_lens, out, sink, slopes)
+    stride = _packed_q("attn_prefill_half", q, out, nh, d)
+    _attn_extras(nh, None, None, None, sink, slopes)
+    if q.dtype != torch.bfloat16 or kcache.dtype != torch.float16 or vcache.dtype != torch.float16:
+        raise KernelError("attn_prefill_half: keys and values are float16, q and the result bfloat16")
+    if tile128 is not None:
+        tc_launched = True
+    seq, q0, n = tile128 if tile128 is not None else (None, None, 0)
+    coef, every = temperature or (0.0, 0.0)
+    _check(_packed("gg_attn_prefill_half")(q.data_ptr(), stride, kcache.data_ptr(), vcache.data_ptr(), kv_unit.data_ptr(), block_tables.data_ptr(),
+                                           bt_stride, cu_q_lens.data_ptr(), context_lens.data_ptr(), tile64[0].data_ptr(), tile64[1].data_ptr(),
+                                           tile64[2], _at(seq), _at(q0), n, out.data_ptr(), q.shape[0], kcache.shape[0], nh, nkv, d, page_size,
+                                           window, options, scale, softcap, _at(sink), _at(slopes), coef, every,
+                                           tc_status(q.device).data_ptr() if tile128 is not None else None, stream))

@@ -347,8 +347,8 @@ packed_write_vec_kernel(const __nv_bfloat16* __restrict__ qkv, long long row_str
 // ---------------------------------------------------------------- read
 // Eight neighbouring channels (of one group) of a token.
 template <int BITS>
-__device__ __forceinline__ void unpack8(const unsigned char* codes, unsigned pair, float* y) {
-  const float s = __uint_as_float(pair << 16), o = __uint_as_float(pair & 0xffff0000u);
+__device__ __forceinline__ void unpack8(const unsigned char* codes, unsigned pair, float up, float* y) {       // times `up`, a power of two
+  const float s = __uint_as_float(pair << 16) * up, o = __uint_as_float(pair & 0xffff0000u) * up;
   if (BITS == 4) {
     const unsigned w = *reinterpret_cast<const unsigned*>(codes);
 #pragma unroll
@@ -369,12 +369,15 @@ __device__ __forceinline__ void store8(float* p, const float* y) {
 __device__ __forceinline__ void store8(__nv_bfloat16* p, const float* y) {
   *reinterpret_cast<uint4*>(p) = make_uint4(pack_bf16(y[0], y[1]), pack_bf16(y[2], y[3]), pack_bf16(y[4], y[5]), pack_bf16(y[6], y[7]));
 }
+__device__ __forceinline__ void store8(__half* p, const float* y) {
+  *reinterpret_cast<uint4*>(p) = make_uint4(pack_half(y[0], y[1]), pack_half(y[2], y[3]), pack_half(y[4], y[5]), pack_half(y[6], y[7]));
+}
 
 // One page of one sequence: the codes of kv heads z, z + nz, ... become keys and values; the tokens from `real` on, and all
-// of a page that was given back, become zeros.
-template <typename TO, int BITS>
+// of a page that was given back, become zeros.  UP: times ups[which * nkv + kv head].
+template <typename TO, int BITS, bool UP>
 __device__ __forceinline__ void unpack_page(const unsigned char* pages, int page, int num_pages, int real, TO* k_out, TO* v_out, int nkv, int d,
-                                            int page_size) {
+                                            int page_size, const float* ups) {
   const PackedRows r(BITS, d, page_size);
   const int per_row = d >> 3, units = 2 * page_size * per_row;
   if (page < 0 || page >= num_pages) { page = 0; real = 0; }
@@ -386,7 +389,7 @@ __device__ __forceinline__ void unpack_page(const unsigned char* pages, int page
 #pragma unroll 4
     for (int h = blockIdx.z; h < nkv; h += gridDim.z) {
       float y[8];
-      unpack8<BITS>(block + codes, *reinterpret_cast<const unsigned*>(block + pair), y);
+      unpack8<BITS>(block + codes, *reinterpret_cast<const unsigned*>(block + pair), UP ? ups[which * nkv + h] : 1.f, y);
       if (place >= real) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) y[i] = 0.f;
@@ -412,16 +415,23 @@ packed_read_kernel(const unsigned char* __restrict__ pages, int num_pages, const
   const int to = first_page[b] + j;
   if (to < 0 || to >= out_pages) return;
   const size_t at = (size_t)to * nkv * page_size * d;
-  unpack_page<TO, BITS>(pages, tables[(size_t)b * bt_stride + j], num_pages, len - j * page_size, k_out + at, v_out + at, nkv, d, page_size);
+  unpack_page<TO, BITS, false>(pages, tables[(size_t)b * bt_stride + j], num_pages, len - j * page_size, k_out + at, v_out + at, nkv, d, page_size, nullptr);
 }
 
 // What the prompt kernels need of a packed layer's portions (sequences that bring `least` tokens or more), in one launch (without pages: the
 // tiles alone): their
-// pages as plain keys and values, one sequence behind the other; block tables of those pages; and the portions cut into tiles
+// pages as keys and values in half precision, one sequence behind the other; block tables of those pages; and the portions cut into tiles
 // of query rows, those that attend to most keys first (up to UNFOLD_SORTED tiles; more stay in the order of the sequences).
-// Pages behind the window of a portion's first token are left out (-1 in the table).  4 us for 2048 tokens of 8 heads of 128.
+// Pages behind the window of a portion's first token are left out (-1 in the table).
+//
+// Half precision has three bits more than bfloat16, so that a portion's result is as near as a single token's (0.17 % of 64 bits, the result's
+// own rounding, where keys, values and weights in bfloat16 leave 0.31 to 0.37), and five bits of exponent fewer: a row of q, and the keys and the
+// values of each kv head, are brought to a largest value of 2^12 to 2^13 by a power of two.  packed_loud_kernel finds how large the portions'
+// keys and values are from their pages' scales and offsets, LOUD_BLOCKS partial maxima each; q's rows are made in the prompt kernels.
 #define UNFOLD_SORTED 1024
 #define UNFOLD_SEQS 1024          // most sequences of a step
+#define UNFOLD_HEADS 1024         // most kv heads
+#define LOUD_BLOCKS 128
 struct UnfoldTiles { int height, count; int *seq, *q0; };
 struct UnfoldArgs {
   const unsigned char* pages;
@@ -430,6 +440,8 @@ struct UnfoldArgs {
   int bt_stride, B, least, nkv, d, page_size, window, out_pages;
   int* out_tables;                 // [B, bt_stride]
   UnfoldTiles tiles[2];            // height 0: none
+  float* loud;                     // [LOUD_BLOCKS, 2, nkv]: the largest keys and values
+  float* kv_unit;                  // [2, nkv]: what the halves are multiples of
 };
 __device__ __forceinline__ int unfold_keys(const UnfoldArgs& a, int b, int* q_len) {
   *q_len = a.cu_q_lens[b + 1] - a.cu_q_lens[b];
@@ -502,18 +514,111 @@ __device__ __noinline__ void list_tiles(const UnfoldArgs& a) {
   }
 }
 
-template <typename TO, int BITS>
-__global__ void __launch_bounds__(256) packed_unfold_kernel(UnfoldArgs a, TO* __restrict__ k_out, TO* __restrict__ v_out) {
+// The exponent of kv head v % nkv's keys (v < nkv) or values, by a warp.
+__device__ __forceinline__ int loud_exponent(const UnfoldArgs& a, int v) {
+  float big = 0.f;
+#pragma unroll
+  for (int i = 0; i < LOUD_BLOCKS / 32; ++i) big = fmaxf(big, a.loud[(size_t)(i * 32 + (threadIdx.x & 31)) * 2 * a.nkv + v]);
+  return half_exponent(warp_max(big));
+}
+
+// grid LOUD_BLOCKS.  The 2 nkv kinds (keys, then values, of each kv head) are cut into chunks of LOUD_KINDS, and a warp looks at one chunk of the pages
+// whose number (page - first page in sight + LOUD_APART times the sequence) it has modulo the warps of that chunk: a page or two each, whose loads are
+// all under way at once.  4 us for 2048 tokens of 8 heads, 5 for four sequences of 2900.
+#define LOUD_KINDS 16
+#define LOUD_APART 267            // (sequences begin at different warps)
+template <int BITS>
+__global__ void __launch_bounds__(256) packed_loud_kernel(UnfoldArgs a) {
+  __shared__ unsigned big_s[2 * UNFOLD_HEADS];       // (sizes, which compare as whole numbers do)
+  pdl_wait();
+  pdl_trigger();                                     // not before: what packed_unfold_kernel reads ahead of its wait is all older than this kernel
+  const int lane = threadIdx.x & 31, w = blockIdx.x * 8 + (threadIdx.x >> 5), kinds = 2 * a.nkv;
+  const int P = a.page_size, groups_log2 = a.d >> 7, entries_log2 = 31 - __clz(P) + groups_log2;     // pairs of a page and kind: a power of two
+  const PackedRows r(BITS, a.d, P);
+  const int page_bytes = r.page_bytes(), values = r.pairs(1, 0) - r.pairs(0, 0);
+  for (int v = threadIdx.x; v < kinds; v += 256) big_s[v] = 0u;
+  __syncthreads();
+  const int chunks = (kinds + LOUD_KINDS - 1) / LOUD_KINDS, slots = LOUD_BLOCKS * 8 / chunks, v0 = w % chunks * LOUD_KINDS, slot = w / chunks;
+  unsigned top[LOUD_KINDS];
+#pragma unroll
+  for (int u = 0; u < LOUD_KINDS; ++u) top[u] = 0u;
+  if (slot < slots) {
+    for (int b0 = 0; b0 < a.B; b0 += 32) {
+      int ctx = 0, j = 0, count = 0;
+      if (b0 + lane < a.B) {
+        int q_len;
+        ctx = unfold_keys(a, b0 + lane, &q_len);
+        count = (ctx + P - 1) / P;
+        j = unfold_skip(a, ctx, q_len) + ((slot - (b0 + lane) * LOUD_APART) % slots + slots) % slots;
+      }
+      for (unsigned m = __ballot_sync(0xffffffffu, j < count); m; m &= m - 1) {
+        const int src = __ffs(m) - 1, held = __shfl_sync(0xffffffffu, ctx, src), end = __shfl_sync(0xffffffffu, count, src);
+        const int* row = a.tables + (size_t)(b0 + src) * a.bt_stride;
+        for (int j0 = __shfl_sync(0xffffffffu, j, src); j0 < end; j0 += 32 * slots) {
+          const int mine = j0 + lane * slots;
+          const int id = mine < end ? row[mine] : -1;
+          const int n = min(32, (end - j0 + slots - 1) / slots) << entries_log2;                     // pairs of those pages
+          for (int x0 = 0; x0 < n; x0 += 32) {
+            const int x = x0 + lane, k = min(x >> entries_log2, 31), e = x & ((1 << entries_log2) - 1);
+            const int page = __shfl_sync(0xffffffffu, id, k);
+            // (places behind the last token hold whatever was there)
+            const bool there = x < n && page >= 0 && page < a.num_pages && (j0 + k * slots) * P + (e >> groups_log2) < held;
+            const unsigned char* p = a.pages + (size_t)(there ? page : 0) * a.nkv * page_bytes + r.pairs(0, 0) + (size_t)e * 4;
+            unsigned pair[LOUD_KINDS];
+#pragma unroll
+            for (int u = 0; u < LOUD_KINDS; ++u) {
+              const int v = v0 + u;
+              pair[u] = there && v < kinds ? *reinterpret_cast<const unsigned*>(p + (v < a.nkv ? (size_t)v * page_bytes : (size_t)(v - a.nkv) * page_bytes + values)) : 0u;
+            }
+#pragma unroll
+            for (int u = 0; u < LOUD_KINDS; ++u) {
+              const float s = __uint_as_float(pair[u] << 16), o = __uint_as_float(pair[u] & 0xffff0000u);
+              const float g = fmaxf(fabsf(o), fabsf(fmaf(s, (float)((1 << BITS) - 1), o)));
+              if (g < INFINITY) top[u] = max(top[u], __float_as_uint(g));
+            }
+          }
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < LOUD_KINDS; ++u) {
+    const unsigned most = __reduce_max_sync(0xffffffffu, top[u]);
+    if (lane == 0 && v0 + u < kinds && slot < slots) atomicMax(&big_s[v0 + u], most);
+  }
+  __syncthreads();
+  for (int v = threadIdx.x; v < kinds; v += 256) a.loud[(size_t)blockIdx.x * kinds + v] = __uint_as_float(big_s[v]);
+}
+
+// Ahead of its wait it reads nothing that packed_loud_kernel writes (with the lists alone it has another kernel ahead, and waits at once).
+template <int BITS>
+__global__ void __launch_bounds__(256) packed_unfold_kernel(UnfoldArgs a, __half* __restrict__ k_out, __half* __restrict__ v_out) {
   __shared__ int red[8];
-  pdl_wait();                                        // (no early start for what follows: it reads tables and lists at once)
+  __shared__ float ups[2 * UNFOLD_HEADS];
+  pdl_trigger();
+  if (!k_out) pdl_wait();
+  const int lane = threadIdx.x & 31;
   if (blockIdx.x == 0) {                             // a block of its own, among the first
-    if (blockIdx.y == 0 && blockIdx.z == 0) list_tiles(a);
+    if (blockIdx.y == 0 && blockIdx.z == 0) {
+      list_tiles(a);
+      pdl_wait();
+      if (k_out)
+        for (int v = threadIdx.x >> 5; v < 2 * a.nkv; v += 8) {
+          const int e = loud_exponent(a, v);
+          if (lane == 0) a.kv_unit[v] = two_to(-e);
+        }
+    }
     return;
   }
-  const int b = blockIdx.y, j = blockIdx.x - 1, lane = threadIdx.x & 31;
+  const int b = blockIdx.y, j = blockIdx.x - 1;
   int q_len;
   const int ctx = unfold_keys(a, b, &q_len);
   const int skip = unfold_skip(a, ctx, q_len), P = a.page_size;
+  if (j * P >= ctx || j < skip) {                    // nothing to read back
+    if (j * P < ctx && threadIdx.x == 0 && blockIdx.z == 0) a.out_tables[(size_t)b * a.bt_stride + j] = -1;
+    return;
+  }
+  const int page = a.tables[(size_t)b * a.bt_stride + j];
   // pages of the sequences before this one
   int before = 0;
   for (int i = threadIdx.x; i < b; i += blockDim.x) {
@@ -524,18 +629,22 @@ __global__ void __launch_bounds__(256) packed_unfold_kernel(UnfoldArgs a, TO* __
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) before += __shfl_xor_sync(0xffffffffu, before, o);
   if (lane == 0) red[threadIdx.x >> 5] = before;
+  pdl_wait();
+  // this block's heads (blockIdx.z, blockIdx.z + gridDim.z, ...), keys and values
+  for (int i = threadIdx.x >> 5; (int)blockIdx.z + (i >> 1) * (int)gridDim.z < a.nkv; i += 8) {
+    const int v = (i & 1) * a.nkv + blockIdx.z + (i >> 1) * gridDim.z, e = loud_exponent(a, v);
+    if (lane == 0) ups[v] = two_to(e);
+  }
   __syncthreads();
   before = 0;
 #pragma unroll
   for (int w = 0; w < 8; ++w) before += red[w];
-  if (j * P < ctx) {
-    const int to = before + j - skip;
-    const bool seen = j >= skip && to < a.out_pages;
-    if (threadIdx.x == 0 && blockIdx.z == 0) a.out_tables[(size_t)b * a.bt_stride + j] = seen ? to : -1;
-    if (seen) {
-      const size_t at = (size_t)to * a.nkv * P * a.d;
-      unpack_page<TO, BITS>(a.pages, a.tables[(size_t)b * a.bt_stride + j], a.num_pages, ctx - j * P, k_out + at, v_out + at, a.nkv, a.d, P);
-    }
+  const int to = before + j - skip;
+  const bool seen = to < a.out_pages;
+  if (threadIdx.x == 0 && blockIdx.z == 0) a.out_tables[(size_t)b * a.bt_stride + j] = seen ? to : -1;
+  if (seen) {
+    const size_t at = (size_t)to * a.nkv * P * a.d;
+    unpack_page<__half, BITS, true>(a.pages, page, a.num_pages, ctx - j * P, k_out + at, v_out + at, a.nkv, a.d, P, ups);
   }
 }
 
@@ -607,26 +716,43 @@ extern "C" int gg_packed_read(const void* pages, int num_pages, const int* table
   return gg_check_launch("packed_read");
 }
 
+// Floats of `loud` of gg_packed_loud and gg_packed_unfold.
+extern "C" int gg_packed_loud_floats(int nkv) { return LOUD_BLOCKS * 2 * nkv; }
+
+// How large the keys and values in sight of a run's portions are: partial maxima for gg_packed_unfold.
+extern "C" int gg_packed_loud(const void* pages, int num_pages, const int* tables, int bt_stride, const int* cu_q_lens, const int* context_lens,
+                              int B, float* loud, int least, int nkv, int d, int page_size, int bits, int window, cudaStream_t stream) {
+  int rc = check_packed("packed_loud", pages, num_pages, nkv, d, page_size, bits);
+  if (rc) return rc;
+  GG_REQUIRE((d == 64 || d == 128) && nkv <= UNFOLD_HEADS && B > 0 && bt_stride > 0 && window >= 0 && loud, "packed_loud: bad sizes d=%d nkv=%d B=%d", d, nkv, B);
+  UnfoldArgs a = {};
+  a.pages = (const unsigned char*)pages; a.num_pages = num_pages; a.tables = tables; a.cu_q_lens = cu_q_lens; a.context_lens = context_lens;
+  a.bt_stride = bt_stride; a.B = B; a.least = least > 1 ? least : 1; a.nkv = nkv; a.d = d; a.page_size = page_size; a.window = window; a.loud = loud;
+  if (bits == 4) gg_launch(packed_loud_kernel<4>, dim3(LOUD_BLOCKS), dim3(256), 0, stream, a);
+  else gg_launch(packed_loud_kernel<8>, dim3(LOUD_BLOCKS), dim3(256), 0, stream, a);
+  return gg_check_launch("packed_loud");
+}
+
+// k_out, v_out (half precision) null: the lists alone.
 extern "C" int gg_packed_unfold(const void* pages, int num_pages, const int* tables, int bt_stride, const int* cu_q_lens,
-                                const int* context_lens, int B, void* k_out, void* v_out, int out_dtype, int out_pages, int most_pages,
-                                int* out_tables, int height0, int count0, int* seq0, int* q00, int height1, int count1, int* seq1, int* q01,
-                                int least, int nkv, int d, int page_size, int bits, int window, cudaStream_t stream) {
+                                const int* context_lens, int B, void* k_out, void* v_out, int out_pages, int most_pages,
+                                int* out_tables, float* loud, float* kv_unit, int height0, int count0, int* seq0, int* q00, int height1, int count1,
+                                int* seq1, int* q01, int least, int nkv, int d, int page_size, int bits, int window, cudaStream_t stream) {
   int rc = check_packed("packed_unfold", pages, num_pages, nkv, d, page_size, bits);
   if (rc) return rc;
   GG_REQUIRE(B > 0 && B <= UNFOLD_SEQS && most_pages >= 0 && most_pages <= bt_stride && window >= 0 && height0 >= 0 && height1 >= 0,
              "packed_unfold: bad sizes B=%d pages=%d of %d window=%d", B, most_pages, bt_stride, window);
   GG_REQUIRE(((size_t)k_out % 16) == 0 && ((size_t)v_out % 16) == 0, "packed_unfold: the outputs must start on 16 bytes");
-  GG_REQUIRE(out_dtype == GG_F32 || out_dtype == GG_BF16, "packed_unfold: unknown dtype %d", out_dtype);
+  GG_REQUIRE(k_out ? v_out && out_tables && loud && kv_unit && nkv <= UNFOLD_HEADS : most_pages == 0, "packed_unfold: missing outputs, or %d kv heads", nkv);
   UnfoldArgs a = {};
   a.pages = (const unsigned char*)pages; a.num_pages = num_pages; a.tables = tables; a.cu_q_lens = cu_q_lens; a.context_lens = context_lens;
   a.bt_stride = bt_stride; a.B = B; a.least = least > 1 ? least : 1; a.nkv = nkv; a.d = d; a.page_size = page_size; a.window = window; a.out_pages = out_pages;
-  a.out_tables = out_tables;
+  a.out_tables = out_tables; a.loud = loud; a.kv_unit = kv_unit;
   a.tiles[0] = {height0, count0, seq0, q00};
   a.tiles[1] = {height1, count1, seq1, q01};
   const dim3 grid(most_pages + 1, most_pages ? B : 1, most_pages ? head_blocks(out_pages, nkv) : 1), block(256);
-#define UNFOLD_LAUNCH(TO, BITS) gg_launch(packed_unfold_kernel<TO, BITS>, grid, block, 0, stream, a, (TO*)k_out, (TO*)v_out)
-  if (out_dtype == GG_F32) { if (bits == 4) UNFOLD_LAUNCH(float, 4); else UNFOLD_LAUNCH(float, 8); }
-  else { if (bits == 4) UNFOLD_LAUNCH(__nv_bfloat16, 4); else UNFOLD_LAUNCH(__nv_bfloat16, 8); }
+  if (bits == 4) gg_launch(packed_unfold_kernel<4>, grid, block, 0, stream, a, (__half*)k_out, (__half*)v_out);
+  else gg_launch(packed_unfold_kernel<8>, grid, block, 0, stream, a, (__half*)k_out, (__half*)v_out);
   return gg_check_launch("packed_unfold");
 }
 

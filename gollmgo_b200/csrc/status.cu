@@ -21,14 +21,7 @@ int gg_check_launch(const char* what) {
   return GG_OK;
 }
 
-static thread_local int g_pdl_paused = 0;
-
-// While paused, this thread's launches start when everything ahead of them in the stream has completed: for a kernel that
-// reads early what the kernel directly ahead of it wrote.
-extern "C" void gg_pause_pdl(int paused) { g_pdl_paused = paused; }
-
 bool gg_pdl_enabled() {
-  if (g_pdl_paused) return false;
   static int on = -1;
   if (on < 0) {
     const char* v = getenv("GOLLMGO_B200_NO_PDL");

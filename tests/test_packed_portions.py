@@ -111,14 +111,16 @@ def tolerance(q, keys, values, context, scale, dtype, tensor_cores, window=0, so
     On the tensor cores a key is not one number there but s (c - M) + (o + M s) with the middle code M, two sums that are made apart and may cancel.
     Of a group whose largest value is G, |o + M s| <= 1.01 G (it lies inside the codes' range, whose end is at most a bfloat16 step of the scale
     beyond the largest value) and |s (c - M)| <= 1.01 x 8 / 15 x 2 G, so roundings are relative to 2.1 G in the place of |k|, and of |v| alike.
-    bfloat16 on the tensor cores: a key rounds as it is read back, so a score moves by 2^-8 S, and a weight and a value round once (2^-8 each,
-    relative to sum P |v|).  A cap is a tanh of the special-function unit there: 2^-11 of the capped score.  The general kernel computes in
-    float32 whatever the type.  A bias by distance rounds in float32, and the result rounds once."""
+    bfloat16 on the tensor cores: a key rounds to half precision as it is read back, so a score moves by 2^-11 S, and a weight and a value round
+    once (2^-11 each, relative to sum P |v|).  A weight is held times 2^7 or 2^15 relative to the row's largest, which is 1 at least, and below 2^-14
+    as held off by 2^-25 at most: of each key 2^-32 of the largest value.  (Keys and values below 2^-26 of their kv head's largest lose bits too, which tests of that
+    allow for.)  A cap is a tanh of the special-function unit there: 2^-11 of the capped score.  The general kernel computes in float32 whatever the type.
+    A bias by distance rounds in float32, and the result rounds once."""
     a, nh, d = q.shape
     group = nh // keys.shape[1]
     tol = torch.zeros(a, nh, d, dtype=torch.float64)
     fast = dtype == torch.bfloat16 and tensor_cores
-    half = 2.0 ** -8 if fast else 0.0
+    half = 2.0 ** -11 if fast else 0.0
     at, j = torch.arange(context - a, context)[:, None], torch.arange(context)[None]
     seen = (j <= at) & ((at - j < window) if window else True)
     factor = torch.full((a, 1), float(scale), dtype=torch.float64)
@@ -144,6 +146,8 @@ def tolerance(q, keys, values, context, scale, dtype, tensor_cores, window=0, so
         out = w @ v
         spread = torch.einsum("ij,ijc->ic", w * move.masked_fill(~seen, 0.0), (v[None] - out[:, None]).abs()) + 2.0 ** -21 * out.abs()
         rounds = (2 * half + (context + 8) * 2.0 ** -24) * (w @ size_v)
+        if fast:
+            rounds = rounds + context * 2.0 ** -32 * v.abs().max()
         tol[:, h] = 1.05 * (spread + rounds) + torch.finfo(dtype).eps / 2 * out.abs() + 1e-30
     return tol
 
@@ -299,9 +303,9 @@ def test_the_switch_of_the_prompt_kernels_holds_for_portions(monkeypatch, policy
     seen = {}
     monkeypatch.setattr(packed, "ATTN_POLICY", policy)
     monkeypatch.setattr(ops, "packed_prefill_rows", lambda *a: None)
-    monkeypatch.setattr(ops, "packed_unfold", lambda *a, **k: seen.update(lists=[h for h, *_ in a[8]]))
-    monkeypatch.setattr(ops, "attn_prefill", lambda *a, **k: seen.update(kernel="plain", **k))
-    monkeypatch.setattr(ops, "attn_prefill_x", lambda *a, **k: seen.update(kernel="options", **k))
+    monkeypatch.setattr(ops, "packed_loud", lambda *a: None)
+    monkeypatch.setattr(ops, "packed_unfold", lambda *a: seen.update(lists=[h for h, *_ in a[8]]))
+    monkeypatch.setattr(ops, "attn_prefill_half", lambda *a: seen.update(kernel="options" if a[17] else "plain", tile128=a[9]))
     monkeypatch.setattr(ops, "packed_prefill", lambda *a, **k: seen.update(kernel="general"))
 
     class NoDevice(PackedKV):
@@ -311,7 +315,7 @@ def test_the_switch_of_the_prompt_kernels_holds_for_portions(monkeypatch, policy
     NoDevice().prefill(torch.zeros(400, 2, 64, dtype=torch.bfloat16), torch.zeros(1, 25, dtype=torch.int32), torch.tensor([0, 400], dtype=torch.int32),
                        torch.tensor([400], dtype=torch.int32), [400], [400], 0.1, sink=torch.zeros(2) if options else None)
     assert seen["lists"] == lists and seen["kernel"] == ("general" if policy == "general" else "options" if options else "plain")
-    assert ("tile128_seq" in seen) == (128 in lists)
+    assert (seen.get("tile128") is not None) == (128 in lists)
 
 
 @pytest.mark.gpu
@@ -391,9 +395,9 @@ def test_portions_on_the_general_kernel_do_not_attend_to_missing_pages(monkeypat
 @pytest.mark.parametrize("dtype,d,page", [(torch.bfloat16, 96, 16), (torch.float32, 96, 16), (torch.float32, 128, 8), (torch.float32, 64, 16)])
 @pytest.mark.parametrize("window", [0, 9])
 @pytest.mark.parametrize("bad", [float("nan"), float("inf")])
-def test_bad_tokens_reach_the_rows_that_see_them(bits, dtype, d, page, window, bad):
-    """A bad key makes the rows of its kv head from its token on NaN, a bad value its group of channels; rows before it, and behind the
-    window, are as without it."""
+def test_bad_tokens_reach_the_rows_that_see_them(bits, dtype, d, page, window, bad, whole=False):
+    """A bad key makes the rows of its kv head from its token on NaN, a bad value its group of channels (``whole``: all of them); rows before it,
+    and behind the window, are as without it."""
     nh, nkv, n = 4, 2, 200
     g = torch.Generator().manual_seed(d)
     x = torch.randn(n, (nh + 2 * nkv) * d, generator=g).to(dtype)
@@ -417,6 +421,92 @@ def test_bad_tokens_reach_the_rows_that_see_them(bits, dtype, d, page, window, b
     group = plain.group_of(d)
     hidden = torch.zeros(n, nh, d, dtype=torch.bool)
     hidden[sees(key), :2] = True
-    hidden[sees(value), 2:, d - group:] = True
+    hidden[sees(value), 2:, 0 if whole else d - group:] = True
     assert torch.equal(got.isnan(), hidden)
     assert torch.equal(got[~hidden], good[~hidden])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("policy", ["auto", "mma", "general"])
+@pytest.mark.parametrize("options", [False, True])
+@pytest.mark.parametrize("nh,nkv,d", [(4, 2, 64), (4, 2, 128), (2, 2, 128)])
+@pytest.mark.parametrize("key,value", [(0, 0), (40, 100), (-40, -100), (100, 60), (-100, 118)])
+def test_portions_of_loud_and_quiet_heads(monkeypatch, bits, policy, options, nh, nkv, d, key, value):
+    """Keys of one kv head times 2^key, its queries times 2^-key, values times 2^value; the other kv head's the other way round; rows of q that differ
+    by 2^20 beside one another, and a value 2^20 times the others that hardly any row attends to."""
+    from gollmgo_b200.cache import packed
+    if policy == "general" and value == 126:
+        return      # its float32 sums are divided at the end: 300 weights of 1 and values of 2^126 make 2^134, a float ends at 2^128
+    monkeypatch.setattr(packed, "ATTN_POLICY", policy)
+    page, q_lens, lens = 16, [40, 290], [90, 300]
+    g = torch.Generator().manual_seed(d + key)
+    counts = [-(-n // page) for n in lens]
+    tables = torch.zeros(len(lens), max(counts), dtype=torch.int32)
+    for b, order in enumerate(torch.randperm(sum(counts), generator=g).to(torch.int32).split(counts)):
+        tables[b, :counts[b]] = order
+    kv = PackedKV.empty(sum(counts), nkv, d, page, bits)
+    kv.pages.fill_(255)
+    cu = torch.tensor([0] + q_lens).cumsum(0).to(torch.int32)
+    sign = torch.tensor([1.0, -1.0])
+    up_k, up_v = 2.0 ** (key * sign)[:, None], 2.0 ** (value * sign)[:, None]
+    q = torch.randn(int(cu[-1]), nkv, nh // nkv, d, generator=g)
+    q[1::2] *= 2.0 ** -20
+    q = (q / up_k[:, None]).view(-1, nh, d).to(torch.bfloat16)
+    held = []
+    for b, n in enumerate(lens):
+        x = torch.randn(n, 2, nkv, d, generator=g)
+        x[:, 0, :, 0] = 0.0
+        x[7, 1] *= 2.0 ** 20 if value < 100 else 1.0
+        x[7, 0, :, 0] = -400.0                                   # (no row attends to it but those whose first channel says so)
+        x[:, 0] *= up_k
+        x[:, 1] *= up_v
+        x = x.flatten(1).to(torch.bfloat16)
+        t = torch.arange(n)
+        kv.write(x.cuda(), None, (tables[b][t // page].long() * page + t % page).to(torch.int32).cuda(), 0)
+        held.append([plain.through(y.double().view(n, nkv, d), bits) for y in x.chunk(2, 1)])
+    q.view(-1, nh, d)[..., 0] = q[..., 0].abs()
+    o = dict(sink=torch.zeros(nh), window=280) if options else {}
+    out = kv.prefill(q.cuda(), tables.cuda(), cu.cuda(), torch.tensor(lens, dtype=torch.int32).cuda(), q_lens, lens, d ** -0.5,
+                     **{k: v.cuda() if torch.is_tensor(v) else v for k, v in o.items()}).cpu().double()
+    for b, n in enumerate(lens):
+        x, (k, v) = q[cu[b]:cu[b + 1]], held[b]
+        ref = plain.attend(x.double(), k, v, n, d ** -0.5, **o)
+        for h in range(nh):
+            one = h * nkv // nh
+            # (keys and values below 2^-26 of their kv head's largest are off by 2^-37 of it)
+            there = v[:, one:one + 1].nan_to_num()                   # (rows that are kept see none of the others)
+            more = dict(o, sink=o["sink"][h:h + 1]) if options else {}
+            tol = tolerance(x[:, h:h + 1], k[:, one:one + 1], there, n, d ** -0.5, torch.bfloat16, policy != "general", **more)
+            got, gone = out[cu[b]:cu[b + 1], h], ref[:, h].isnan()       # (2^126 times what is above 4 is an infinity: rows that see it are NaN)
+            assert got[gone].isnan().all()
+            tol = tol[:, 0] + 2.0 ** -36 * there.abs().max()
+            kept = ~gone.any(-1)
+            assert kept.any() or value == 126
+            assert ((got[kept] - ref[kept, h]).abs() <= tol[kept]).all(), (b, h)
+
+
+def test_the_launchers_of_portions_refuse_sizes_and_missing_lists():
+    from gollmgo_b200.csrc import ops
+    ops.lib()
+
+    def refused(name, args, cases):
+        f = ops._packed(name)
+        for at, v, message in cases:
+            bad = list(args)
+            bad[at] = v
+            assert f(*bad) != 0
+            assert message in ops.lib().gg_last_error().decode(), (name, at, v)
+    one = 16                                          # (any address that is not looked at)
+    refused("gg_packed_loud", [None, 4, one, 8, one, one, 2, one, 1, 2, 64, 16, 4, 0, None],
+            [(10, 96, "bad sizes"), (9, 2000, "bad sizes"), (6, 0, "bad sizes"), (7, None, "bad sizes"), (13, -1, "bad sizes"), (0, 8, "16 bytes"), (12, 5, "packed cache")])
+    refused("gg_packed_unfold", [None, 4, one, 8, one, one, 2, one, one, 3, 2, one, one, one, 64, 1, one, one, 0, 0, None, None, 1, 2, 64, 16, 4, 0, None],
+            [(6, 0, "bad sizes"), (6, 1025, "bad sizes"), (10, 9, "bad sizes"), (27, -1, "bad sizes"), (7, 8, "16 bytes"), (8, None, "missing"), (11, None, "missing"),
+             (12, None, "missing"), (13, None, "missing"), (7, None, "missing"), (23, 1025, "missing")])
+    refused("gg_packed_prefill", [one, 128, 1, None, 4, one, 8, one, one, one, one, 1, one, 4, 2, 64, 16, 4, 0, 1.0, 0.0, None, None, 0.0, 0.0, None],
+            [(2, 7, "dtype"), (13, 3, "multiple"), (14, 0, "bad sizes"), (11, -1, "bad lists"), (9, None, "bad lists"), (7, None, "bad lists"), (18, -1, "window"),
+             (17, 3, "packed cache")])
+    refused("gg_attn_prefill_half", [one, 256, one, one, one, one, 8, one, one, one, one, 1, None, None, 0, one, 3, 4, 4, 2, 64, 16, 0, 0, 1.0, 0.0, None, None, 0.0, 0.0,
+                                     None, None],
+            [(20, 96, "head size"), (21, 24, "pages"), (4, None, "no lists"), (9, None, "no lists"), (0, 8, "aligned"), (1, 100, "aligned"), (24, -1.0, "options"),
+             (25, 3.0, "options"), (26, one, "options"), (27, one, "options"), (29, 2.0, "options"), (18, 3, "multiple")])
