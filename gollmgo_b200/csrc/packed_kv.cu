@@ -401,6 +401,24 @@ __device__ __forceinline__ void unpack_page(const unsigned char* pages, int page
   }
 }
 
+// A value that is no number goes over to its token's key: 0 times it would be a NaN in rows that do not see it, where a key's score is replaced
+// (heads of 64 or 128 channels; all of the head is NaN in rows that do).  Behind unpack_page, by a call of its own (inlined, it takes registers).
+__device__ __forceinline__ bool no_number(unsigned pair) { return (pair & 0x7f80u) == 0x7f80u; }          // the scale: of a group with an infinity or a NaN
+template <int BITS>
+__device__ __noinline__ void bad_values(const unsigned char* pages, int page, int real, __half* k_out, __half* v_out, int nkv, int d, int page_size) {
+  const PackedRows r(BITS, d, page_size);
+  __syncthreads();
+  for (int h = blockIdx.z; h < nkv; h += gridDim.z)
+    for (int u = threadIdx.x; u < min(real, page_size) * (d >> 3); u += blockDim.x) {
+      const int place = u / (d >> 3), c = (u - place * (d >> 3)) << 3;
+      const unsigned* values = reinterpret_cast<const unsigned*>(pages + ((size_t)page * nkv + h) * r.page_bytes() + r.pairs(1, place));
+      if (!no_number(values[0]) && !no_number(values[r.groups() - 1])) continue;
+      const size_t at = ((size_t)h * page_size + place) * d + c;
+      *reinterpret_cast<uint4*>(k_out + at) = make_uint4(0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu);
+      *reinterpret_cast<uint4*>(v_out + at) = make_uint4(0u, 0u, 0u, 0u);
+    }
+}
+
 // grid (pages of the longest sequence, B, nz): page j of sequence b becomes page first_page[b] + j of the results.  Bound by the results' bytes
 // where there are many: 8000 tokens of 8 heads of 128 in 15.5 us from 4 bits (2.7 TB/s), 14.5 from 8 (3.5 TB/s); 2048 in 6.3 us.
 template <typename TO, int BITS>
@@ -440,7 +458,7 @@ struct UnfoldArgs {
   int bt_stride, B, least, nkv, d, page_size, window, out_pages;
   int* out_tables;                 // [B, bt_stride]
   UnfoldTiles tiles[2];            // height 0: none
-  float* loud;                     // [LOUD_BLOCKS, 2, nkv]: the largest keys and values
+  float* loud;                     // [LOUD_BLOCKS, 2, nkv]: the largest keys and values; [LOUD_BLOCKS]: whether some value is no number
   float* kv_unit;                  // [2, nkv]: what the halves are multiples of
 };
 __device__ __forceinline__ int unfold_keys(const UnfoldArgs& a, int b, int* q_len) {
@@ -539,6 +557,7 @@ __global__ void __launch_bounds__(256) packed_loud_kernel(UnfoldArgs a) {
   for (int v = threadIdx.x; v < kinds; v += 256) big_s[v] = 0u;
   __syncthreads();
   const int chunks = (kinds + LOUD_KINDS - 1) / LOUD_KINDS, slots = LOUD_BLOCKS * 8 / chunks, v0 = w % chunks * LOUD_KINDS, slot = w / chunks;
+  bool bad = false;                                  // some value is no number
   unsigned top[LOUD_KINDS];
 #pragma unroll
   for (int u = 0; u < LOUD_KINDS; ++u) top[u] = 0u;
@@ -575,6 +594,7 @@ __global__ void __launch_bounds__(256) packed_loud_kernel(UnfoldArgs a) {
               const float s = __uint_as_float(pair[u] << 16), o = __uint_as_float(pair[u] & 0xffff0000u);
               const float g = fmaxf(fabsf(o), fabsf(fmaf(s, (float)((1 << BITS) - 1), o)));
               if (g < INFINITY) top[u] = max(top[u], __float_as_uint(g));
+              else bad = bad || v0 + u >= a.nkv;
             }
           }
         }
@@ -586,13 +606,14 @@ __global__ void __launch_bounds__(256) packed_loud_kernel(UnfoldArgs a) {
     const unsigned most = __reduce_max_sync(0xffffffffu, top[u]);
     if (lane == 0 && v0 + u < kinds && slot < slots) atomicMax(&big_s[v0 + u], most);
   }
-  __syncthreads();
+  bad = __syncthreads_or(bad);
   for (int v = threadIdx.x; v < kinds; v += 256) a.loud[(size_t)blockIdx.x * kinds + v] = __uint_as_float(big_s[v]);
+  if (threadIdx.x == 0) a.loud[(size_t)LOUD_BLOCKS * kinds + blockIdx.x] = bad ? 1.f : 0.f;
 }
 
 // Ahead of its wait it reads nothing that packed_loud_kernel writes (with the lists alone it has another kernel ahead, and waits at once).
 template <int BITS>
-__global__ void __launch_bounds__(256) packed_unfold_kernel(UnfoldArgs a, __half* __restrict__ k_out, __half* __restrict__ v_out) {
+__global__ void __launch_bounds__(256, 5) packed_unfold_kernel(UnfoldArgs a, __half* __restrict__ k_out, __half* __restrict__ v_out) {
   __shared__ int red[8];
   __shared__ float ups[2 * UNFOLD_HEADS];
   pdl_trigger();
@@ -635,6 +656,10 @@ __global__ void __launch_bounds__(256) packed_unfold_kernel(UnfoldArgs a, __half
     const int v = (i & 1) * a.nkv + blockIdx.z + (i >> 1) * gridDim.z, e = loud_exponent(a, v);
     if (lane == 0) ups[v] = two_to(e);
   }
+  bool bad = false;                                  // some value is no number
+#pragma unroll
+  for (int i = 0; i < LOUD_BLOCKS / 32; ++i) bad = bad || a.loud[(size_t)LOUD_BLOCKS * 2 * a.nkv + i * 32 + lane] != 0.f;
+  bad = __any_sync(0xffffffffu, bad);
   __syncthreads();
   before = 0;
 #pragma unroll
@@ -645,6 +670,7 @@ __global__ void __launch_bounds__(256) packed_unfold_kernel(UnfoldArgs a, __half
   if (seen) {
     const size_t at = (size_t)to * a.nkv * P * a.d;
     unpack_page<__half, BITS, true>(a.pages, page, a.num_pages, ctx - j * P, k_out + at, v_out + at, a.nkv, a.d, P, ups);
+    if (bad && page >= 0 && page < a.num_pages) bad_values<BITS>(a.pages, page, ctx - j * P, k_out + at, v_out + at, a.nkv, a.d, P);
   }
 }
 
@@ -717,7 +743,7 @@ extern "C" int gg_packed_read(const void* pages, int num_pages, const int* table
 }
 
 // Floats of `loud` of gg_packed_loud and gg_packed_unfold.
-extern "C" int gg_packed_loud_floats(int nkv) { return LOUD_BLOCKS * 2 * nkv; }
+extern "C" int gg_packed_loud_floats(int nkv) { return LOUD_BLOCKS * (2 * nkv + 1); }
 
 // How large the keys and values in sight of a run's portions are: partial maxima for gg_packed_unfold.
 extern "C" int gg_packed_loud(const void* pages, int num_pages, const int* tables, int bt_stride, const int* cu_q_lens, const int* context_lens,

@@ -428,10 +428,23 @@ def test_bad_tokens_reach_the_rows_that_see_them(bits, dtype, d, page, window, b
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("policy", ["auto", "mma"])
+@pytest.mark.parametrize("d,page", [(64, 16), (128, 16), (128, 32)])
+@pytest.mark.parametrize("window", [0, 9])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+def test_bad_tokens_of_bfloat16_portions(monkeypatch, bits, policy, d, page, window, bad):
+    from gollmgo_b200.cache import packed
+    monkeypatch.setattr(packed, "ATTN_POLICY", policy)
+    monkeypatch.setattr(packed, "SHORT_PROMPT_KEYS", 100)            # (200 keys: on tcgen05 where it may)
+    test_bad_tokens_reach_the_rows_that_see_them(bits, torch.bfloat16, d, page, window, bad, whole=True)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits", [4, 8])
 @pytest.mark.parametrize("policy", ["auto", "mma", "general"])
 @pytest.mark.parametrize("options", [False, True])
 @pytest.mark.parametrize("nh,nkv,d", [(4, 2, 64), (4, 2, 128), (2, 2, 128)])
-@pytest.mark.parametrize("key,value", [(0, 0), (40, 100), (-40, -100), (100, 60), (-100, 118)])
+@pytest.mark.parametrize("key,value", [(0, 0), (40, 100), (-40, -100), (100, 60), (-100, 126)])
 def test_portions_of_loud_and_quiet_heads(monkeypatch, bits, policy, options, nh, nkv, d, key, value):
     """Keys of one kv head times 2^key, its queries times 2^-key, values times 2^value; the other kv head's the other way round; rows of q that differ
     by 2^20 beside one another, and a value 2^20 times the others that hardly any row attends to."""
