@@ -140,7 +140,7 @@ class PackedKV:
             return (PackedKV._splits(n, kv_heads, max_context, window),)
         most = ops.PACKED_DECODE_TOKENS
         sizes = sorted({min(n, most), n % most or min(n, most)})
-        return tuple(ops.packed_decode_blocks(dtype, m, num_heads, kv_heads, head_dim, bits, max_context, window) for m in sizes if m)
+        return tuple(ops.packed_decode_shape(dtype, m, num_heads, kv_heads, head_dim, bits, max_context, window) for m in sizes if m)
 
     def prefill(self, q: torch.Tensor, tables: torch.Tensor, cu_q_lens: torch.Tensor, context_lens: torch.Tensor,
                 q_lens: Sequence[int], contexts: Sequence[int], scale: float, *, window: int = 0, softcap: float = 0.0, sink=None,

@@ -1543,7 +1543,7 @@ _PACKED_TYPES = {
     "gg_packed_decode": [_P, _L, _I, _P, _I, _P, _I, _I, _P, _P, _P, _I, _I, _P, _P, _P, _I, _I, _I, _I, _I, _I, _F, _F, _P, _P, _F, _F, _P],
     "gg_packed_decode_mma": [_P, _L, _I, _P, _I, _P, _I, _I, _P, _P, _P, _I, _I, _P, _L, _P, _I, _I, _I, _I, _I, _I, _F, _F, _P, _P, _F, _F, _I, _P],
     "gg_packed_decode_scratch": [_I, _I, _I, _I, _I, _I, _I, _I],
-    "gg_packed_decode_blocks": [_I, _I, _I, _I, _I, _I, _I, _I],
+    "gg_packed_decode_shape": [_I, _I, _I, _I, _I, _I, _I, _I],
     "gg_packed_decode_tokens": [_I, _I, _I],
     "gg_packed_prompt_fold": [_I, _I],
     "gg_packed_prompt_f32": [_P, _L, _P, _I, _P, _I, _I, _P, _P, _I, _I, _P, _I, _P, _L, _P, _I, _I, _I, _I, _I, _I, _F, _F, _P, _P, _F, _F, _P],
@@ -1741,9 +1741,9 @@ def packed_launches_scratch(dtype: torch.dtype, n: int, most: int, *sizes) -> in
 
 
 @functools.lru_cache(maxsize=4096)
-def packed_decode_blocks(dtype: torch.dtype, n: int, nh: int, nkv: int, d: int, bits: int, max_context: int, window: int) -> int:
-    """Blocks of packed_decode_mma, less than 0 where every (token, kv head) pair has one of its own."""
-    return _packed("gg_packed_decode_blocks")(dtype_code(dtype), n, nh, nkv, d, bits, max_context, window)
+def packed_decode_shape(dtype: torch.dtype, n: int, nh: int, nkv: int, d: int, bits: int, max_context: int, window: int) -> int:
+    """How packed_decode_mma spreads n tokens, as one number that is the same for the same launch."""
+    return _packed("gg_packed_decode_shape")(dtype_code(dtype), n, nh, nkv, d, bits, max_context, window)
 
 
 def packed_decode_mma(q: torch.Tensor, pages: torch.Tensor, tables: torch.Tensor, cu_q_lens: Optional[torch.Tensor],

@@ -48,8 +48,13 @@
 // 7.2 9.1, 700 keys 10.1 11.0, 1400 keys 12.7 11.3).
 #define PD_ALONE 2
 // Warps of a block for float32 (us with 8 and 12: the portions above 445 419, one of 600 rows of 40 heads 243 189, a context of 20000 of 40 heads 54 53, three
-// of 8000 of four kv heads 15.1 17.1; 16 spill).
+// of 8000 of four kv heads 15.1 17.1; with 16, heads of 128 spill 132 to 296 bytes, with 12 4 to 28).
 #define PD_EXACT_WARPS 12
+// Keys of all (token, kv head) pairs from which more than eight heads of a kv head take sixteen columns at a time (twice the registers, so 8 warps for
+// 16), below which they go eight by eight, each key read as often (us, sixteen and eight, 4 bits: 16 heads on one kv head of 128, one token of 20000
+// keys 19.2 16.3, 24 of up to 4000 18.6 15.7, 64 of 8000 33.6 32.0; 32 on two, 64 of 8000 51.2 54.5; 128 on eight, one of 20000 23.1 22.0, 40 of
+// 600 25.5 21.7, 24 of 4000 43.4 44.3, in 8 bits 52.3 54.7).
+#define PD_WIDE 640000
 #define PD_SMEM (222 * 1024)       // dynamic shared memory: of 227 KB, with what a block has besides
 #define PD_LOG2E 1.4426950408889634f
 #define PD_NO_KEY (-3.0e38f)       // the running maximum before the first key: below every finite score
@@ -245,7 +250,7 @@ template <int TILE, bool EXACT> struct TileCursor {
 };
 
 // Shapes of the kernel: warps of a block (16 at 128 registers a thread, or 8), keys of a tile, stages of a ring.  Twice the heads
-// take twice the registers, so half the warps; a tile is about the same bytes in 4 and in 8 bits; as many stages as shared
+// take twice the registers, so half the warps (PD_WIDE); a tile is about the same bytes in 4 and in 8 bits; as many stages as shared
 // memory holds beside the lists of the most tokens.
 template <int D, int BITS, int NT, bool EXACT> struct PdSizes {
   static constexpr int WARPS = EXACT ? PD_EXACT_WARPS : NT == 1 ? 16 : 8, TILE = BITS == 4 ? 32 : 16, THREADS = WARPS * 32;
@@ -1079,7 +1084,8 @@ template <int D, int BITS, int NT, bool EXACT> static void pd_fill(PdShape* s, i
   } while (0)
 static PdShape pd_shape(int n, int nh, int nkv, int d, int bits, int max_context, int window, bool exact) {
   PdShape s;
-  const int group = nh / nkv, nt = group > 8 && !exact ? 2 : 1;
+  const long long keys = (long long)n * nkv * (window > 0 && window < max_context ? window : max_context);
+  const int group = nh / nkv, nt = group > 8 && !exact && keys >= PD_WIDE ? 2 : 1;
   s.nt = nt;
   s.chunks = (group + 8 * nt - 1) / (8 * nt);
 #define PD_FILL(D, BITS, NT, EXACT) pd_fill<D, BITS, NT, EXACT>(&s, n, nkv, max_context, window)
@@ -1093,10 +1099,10 @@ extern "C" long long gg_packed_decode_scratch(int dtype, int n, int nh, int nkv,
   return s.part_floats + 4LL * s.blocks;
 }
 
-// The blocks of that launch, less than 0 where every pair has one of its own: calls for which this says the same spread their work alike.
-extern "C" int gg_packed_decode_blocks(int dtype, int n, int nh, int nkv, int d, int bits, int max_context, int window) {
+// The shape of that launch as one number: calls for which this says the same spread their work alike.
+extern "C" int gg_packed_decode_shape(int dtype, int n, int nh, int nkv, int d, int bits, int max_context, int window) {
   const PdShape s = pd_shape(n, nh, nkv, d, bits, max_context, window, dtype == GG_F32);
-  return s.join ? s.blocks : -s.blocks;
+  return (s.blocks * 2 + s.join) * 2 + s.nt - 1;
 }
 
 template <int D, int BITS, int NT, bool OPT, bool EXACT>

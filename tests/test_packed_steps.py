@@ -61,3 +61,44 @@ def test_a_list_made_by_the_call_itself_is_not_read_early(monkeypatch, given):
                       seqs=lists[:n] if given else None, early=True)
     assert [b for part, _ in seen for b in part] == list(range(n))
     assert [early for _, early in seen] == [given, given]
+
+
+def test_more_than_eight_heads_of_a_kv_head_are_a_shape_of_their_own():
+    """Sixteen columns at a time from so many keys on: steps of either side have tags of their own, and scratch for what they run."""
+    mixer = layer(32, 2, 128, 16, 4)
+    below, above = (StepFacts(64, 64, True, c) for c in (4096, 8192))            # 64 x 2 x 4096 keys, and twice as many
+    assert mixer.step_tags(below) != mixer.step_tags(above)
+    few, many = (ops.packed_decode_scratch(torch.bfloat16, 64, 32, 2, 128, 4, c, 0) for c in (4096, 8192))
+    assert few == 148 * (18 * (8 * 128 + 16) + 4) and many == 148 * (10 * (16 * 128 + 32) + 4)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("nh,nkv", [(9, 1), (16, 1), (24, 1), (33, 1), (66, 2)])
+@pytest.mark.parametrize("d,option", [(64, 0), (128, 0), (128, 1)])
+def test_many_heads_of_a_kv_head_in_either_shape(bits, nh, nkv, d, option):
+    import plain_packed as plain
+    from gollmgo_b200.cache import PackedKV
+    lens, page = [33, 5, 260, 700], 16
+    g = torch.Generator().manual_seed(nh)
+    counts = [-(-n // page) for n in lens]
+    kv = PackedKV.empty(sum(counts), nkv, d, page, bits)
+    tables = torch.zeros(4, max(counts), dtype=torch.int32)
+    held = []
+    for b, order in enumerate(torch.randperm(sum(counts), generator=g).to(torch.int32).split(counts)):
+        tables[b, :counts[b]] = order
+        x = torch.randn(lens[b], 2 * nkv * d, generator=g).to(torch.bfloat16)
+        t = torch.arange(lens[b])
+        kv.write(x.cuda(), None, (order[t // page].long() * page + t % page).to(torch.int32).cuda(), 0)
+        held.append([plain.through(y.double().view(lens[b], nkv, d), bits) for y in x.chunk(2, 1)])
+    q = torch.randn(4, nh, d, generator=g).to(torch.bfloat16)
+    o = dict(sink=torch.randn(nh, generator=g), slopes=torch.rand(nh, generator=g) * 0.1, window=300) if option else {}
+    more = {k: v.cuda() if torch.is_tensor(v) else v for k, v in o.items()}
+    for said in (700, 10 ** 6):                      # (the work is spread for so long contexts; a window is counted instead)
+        out = kv.decode(q.cuda(), tables.cuda(), torch.tensor(lens, dtype=torch.int32).cuda(), said, d ** -0.5, **more).cpu().double()
+        for b, n in enumerate(lens):
+            k, v = held[b]
+            ref = plain.attend(q[b:b + 1].double(), k, v, n, d ** -0.5, **o)[0]
+            # scores: |q| |k| scale in steps of 2^-20 at most where a tensor core truncates, twice, and a bias of up to 30; weights as halves; the result's rounding
+            e = float(q[b].double().norm(dim=-1).max() * k.norm(dim=-1).max()) * d ** -0.5 * 2.0 ** -20 + 2.0 ** -18
+            assert ((out[b] - ref).abs() <= 2.0 ** -8 * ref.abs() + (2 * e + 2.0 ** -11) * float(v.abs().max())).all(), (said, b)
