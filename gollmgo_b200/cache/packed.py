@@ -56,8 +56,8 @@ class PackedKV:
         """Rows of qkv [T, (num_heads + 2 kv heads) * head size]: q and k are rotated by ``positions`` (``inv_freq`` float64
         [width / 2]; None: they are not), k and v quantised into their pages at ``slots`` (page * page_size + place; below
         0: not stored; none twice; None: nothing is stored).  Returns the rotated q [T, num_heads, head size], in ``q_out``
-        where given (which may be the q columns of qkv).  ``early``: positions, slots and inv_freq are not the output of the kernel
-        ahead on the stream, and may be read while it runs."""
+        where given (which may be the q columns of qkv).  ``early``: no kernel that may still run on the stream writes positions, slots or inv_freq
+        (they came by a copy, or before an event that the stream has waited for), and they may be read while kernels ahead run."""
         if q_out is None:
             q_out = qkv.new_empty((qkv.shape[0], num_heads, self.head_dim))
         ops.packed_write(qkv, positions, slots, inv_freq, magnitude, self.pages, q_out, num_heads, self.kv_heads, self.head_dim,
@@ -92,8 +92,9 @@ class PackedKV:
         """Attention of single tokens, each the last of its sequence's context_lens[b] stored ones: q [n, heads, head size]
         (row i of sequence i; with ``seqs`` token i belongs to sequence seqs[i], none of the tables': padding, and with ``cu_q_lens``
         its row is cu_q_lens[sequence]).  ``max_context``: no context is expected to be longer (the work is spread by it).
-        The options are those of the attention layer; a token with no key in sight gives zeros.  ``early``: block tables
-        and index lists are not the output of the kernel ahead on the stream, and may be read while it runs."""
+        The options are those of the attention layer; a token with no key in sight gives zeros.  ``early``: no kernel that may still run on
+        the stream writes block tables or index lists (they came by a copy, or before an event that the stream has waited for), and they may be
+        read while kernels ahead run."""
         out = self._out("decode", q, out)
         nh, d = q.shape[1], self.head_dim
         n = seqs.numel() if seqs is not None else q.shape[0]
@@ -149,10 +150,10 @@ class PackedKV:
         size], the last q_lens[b] of its context_lens[b] stored tokens.  ``q_lens`` and ``contexts`` say on the host what
         the two device lists hold.  Sequences of fewer than ``least`` rows are left out (their rows of ``out`` stay as they are).
 
-        The pages of the portions are read back once, in the type of the activations, and the prompt kernels run on them;
-        steps of many long portions go in runs of sequences, so that what is read back at a time stays within
-        ``SCRATCH_TOKENS`` (or the longest sequence).  float32 rows that the tensor cores take attend to the codes where they lie, as single
-        tokens do."""
+        bfloat16 rows, heads of 64 or 128: the pages of the portions are read back once, in half precision, and the prompt kernels run on them
+        (0.17 % off 64 bits, as single tokens are); steps of many long portions go in runs of sequences, so that what is read back at a time
+        stays within ``SCRATCH_TOKENS`` (or the longest sequence).  float32 rows that the tensor cores take attend to the codes where they lie, as
+        single tokens do; other rows too, on the general kernel."""
         out = self._out("prefill", q, out)
         B, P = len(q_lens), self.page_size
         if len(contexts) != B or tables.shape[0] < B:

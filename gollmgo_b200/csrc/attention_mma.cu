@@ -16,7 +16,8 @@
 // head, so every key and value is read once per group; the four warps take 16
 // keys each of every 64 and are combined through shared memory at the end.
 // Prompt portions: one CTA per (64 queries of a sequence, head); a warp owns 16
-// query rows.
+// query rows.  HALF: keys, values and weights are half precision numbers, and the
+// fragments of q become such, as in attention_tc3.cu.
 #include "attention_common.cuh"
 #include <cstdlib>
 

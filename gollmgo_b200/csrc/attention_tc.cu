@@ -24,6 +24,7 @@
 //            rescaled through tcgen05.ld/st) when a row's maximum has grown by more than
 //            2^8; P goes to shared memory in the swizzled K-major layout the second
 //            product reads.  At the end O is divided by the row sums and stored.
+// HALF: keys, values and weights are half precision numbers, and Q becomes such in shared memory, as in attention_tc3.cu.
 // Tensor memory: columns [0,128) and [128,256) scores, [256,384) O.
 // All waits are bounded; a wait that runs out sets *status and the CTA winds down.
 #include "attention_common.cuh"

@@ -35,6 +35,9 @@
 // multiply-adds a pair with a bias, a tanh of the special-function unit more with a cap); everything else is the plain
 // kernel.  2048 tokens of 32 heads of 128, window 1024, with a bias, a sink and a temperature: 67 us, on mma.sync 266
 // (the plain kernel without a window: 54).
+// HALF: the portions of a packed cache (packed_kv.cu).  Keys, values and weights are half precision numbers, three bits more than bfloat16 (a result
+// 0.17 % off 64 bits, its own rounding, for 0.31 to 0.37); a softmax thread makes its row of Q such numbers where TMA put it, before the first
+// product (2.4 us of 2048 tokens' 48), and has the row's and the kv head's powers of two in its scale.
 // Tensor memory per head: columns [0, 128) scores / P, [128, 128 + dv) O; head 1 at +256.
 // All waits on barriers are bounded; a wait that runs out sets *status and the CTA winds down.
 #include "attention_common.cuh"

@@ -1611,8 +1611,8 @@ def packed_write(qkv: torch.Tensor, positions: Optional[torch.Tensor], slots: Op
     """Rotate the q heads of qkv [T, (nh + 2 nkv) d] into ``q_out`` [T, nh d] (None: they are left alone; it may be the
     columns of qkv itself), rotate the k heads, and quantise k and v into ``pages`` at slots[t] = page * page_size + place.
     A slot below 0 or outside the pool is not written; no slot may be given twice.  ``inv_freq`` None: no rotation.
-    ``early``: ``positions``, ``slots`` and ``inv_freq`` may be read before the kernel ahead of this one has finished (they are
-    not its output)."""
+    ``early``: ``positions``, ``slots`` and ``inv_freq`` may be read before the kernels ahead of this one have finished (none of
+    those that may still run writes them)."""
     T = qkv.shape[0]
     stream = _stream_of("packed_write", qkv, positions, slots, inv_freq, pages, q_out)
     stride = _rows_of(qkv, (nh + 2 * nkv) * d, "packed_write: qkv")
@@ -1753,7 +1753,7 @@ def packed_decode_mma(q: torch.Tensor, pages: torch.Tensor, tables: torch.Tensor
                       temperature=None, early: bool = False) -> None:
     """packed_decode on the tensor cores (packed_decode_mma_ok).  ``scratch`` float32 of packed_decode_scratch for the same
     sizes; contexts longer than ``max_context`` are right too, only the work was split for shorter ones.  ``early``: the index
-    lists and block tables may be read before the kernel ahead of this one has finished (they are not its output)."""
+    lists and block tables may be read before the kernels ahead of this one have finished (none of those that may still run writes them)."""
     stream = _stream_of("packed_decode", q, pages, tables, cu_q_lens, context_lens, seqs, scratch, out, sink, slopes)
     stride = _packed_q("packed_decode", q, out, nh, d)
     if sink is not None or slopes is not None:
@@ -1828,7 +1828,7 @@ def packed_unfold(pages: torch.Tensor, tables: torch.Tensor, cu_q_lens: torch.Te
     of (height, count, seq, q0) with the number of tiles that the portions cut into rows of that height make; and, with ``k_out`` and ``v_out``
     float16 [pages, nkv, page_size, d], their pages as keys and values behind one another there, times ``kv_unit`` float32 [2, nkv] (powers of two,
     from ``loud`` of packed_loud), and block tables of those pages in ``out_tables`` (shape of ``tables``).  Pages that the window hides are
-    left out."""
+    left out.  With pages it goes directly behind packed_loud (it reads its lists before that has finished)."""
     stream = _stream_of("packed_unfold", pages, tables, cu_q_lens, context_lens, k_out, v_out, out_tables, loud, kv_unit)
     B, width = _tables("packed_unfold", tables)
     _ints("packed_unfold", B, context_lens)

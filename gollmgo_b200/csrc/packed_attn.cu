@@ -18,8 +18,8 @@
 // channels of four keys for the output, whose pairs (key, key) are put together by byte permutation.  The weights pass from the
 // score layout to the B operand by a register transpose of 8 x 8.
 //
-// Bytes are what bounds it (4.5 or 8.5 bits a channel), closely followed by the instructions that make operands of codes.  The
-// work is cut into equal ranges of tiles over all (token, kv head) pairs, a range for each warp.  A warp brings its tiles into a
+// Its floor are the bytes (4.5 or 8.5 bits a channel); what bounds it are warps that wait on their own chains, no unit being busy for more than
+// 60 %, the instructions that make operands of codes most.  The work is cut into equal ranges of tiles over all (token, kv head) pairs, a range for each warp.  A warp brings its tiles into a
 // ring of its own by 16-byte asynchronous copies (bulk copies, one a page, were started by one lane after the other with more
 // instructions than ten copies of all lanes take), the pages of its next 16 or 32 tiles found by one lane each, and shares
 // nothing until it is done: a pair that lies inside its range is written out, parts of pairs are joined inside the block and

@@ -1,5 +1,5 @@
-// The packed cache (format: packed_kv.cuh): rotation and quantisation as keys and values are written, reading them back, and
-// the launchers of attention over it.
+// The packed cache (format: packed_kv.cuh): rotation and quantisation as keys and values are written, reading them back (plain, or in half
+// precision for the prompt kernels), and the launchers of attention over it.
 #include "attention_common.cuh"
 #include "packed_kv.cuh"
 
@@ -250,8 +250,9 @@ __device__ __forceinline__ void store_head(const TC* a, const TC* c, bool nan0, 
 // The common case: bfloat16, heads of 64 or 128, half-split pairs over the whole head or no rotation, rows in 16-byte steps.
 // Blocks of y = 0 take the k and v heads of TOK tokens, blocks of y = 1 their q heads (a tenth of the work a row: apart, so that
 // all warps of a block are busy as long).  A thread takes channels p .. p + 7 and D / 2 + p .. of one head (two 16-byte loads,
-// those of its next row under way while it works), so that a head's extremes are found by 4 or 8 neighbouring lanes.  Bound by issue slots
-// and the chain from a row's extremes to its codes: 2048 tokens of 32 + 2 x 8 heads of 128 in 17.7 us (2.5 TB/s), 8000 in 58 us (3.0 TB/s).
+// those of its next row under way while it works), so that a head's extremes are found by 4 or 8 neighbouring lanes.  Bound by waiting for its
+// rows and the chain from a row's extremes to its codes (issue slots 55 % busy): 2048 tokens of 32 + 2 x 8 heads of 128 in 18.3 us (2.4 TB/s), 8000 in 61 us
+// (2.8 TB/s).  Three blocks a multiprocessor: with the 88 to 92 registers that 128 channels would take it has two, and 8000 tokens take 76 us.
 #define WRITE_THREADS 256
 template <int D, int BITS, int TOK>
 __global__ void __launch_bounds__(WRITE_THREADS, 3)
@@ -612,6 +613,8 @@ __global__ void __launch_bounds__(256) packed_loud_kernel(UnfoldArgs a) {
 }
 
 // Ahead of its wait it reads nothing that packed_loud_kernel writes (with the lists alone it has another kernel ahead, and waits at once).
+// 10 us for 2048 tokens of 8 heads of 128 in 4 bits, 25 for 11600 in 8 (71 MB, 2.8 TB/s); five blocks a multiprocessor, since with the 62 registers it
+// would take otherwise it has four, and those take 27.
 template <int BITS>
 __global__ void __launch_bounds__(256, 5) packed_unfold_kernel(UnfoldArgs a, __half* __restrict__ k_out, __half* __restrict__ v_out) {
   __shared__ int red[8];

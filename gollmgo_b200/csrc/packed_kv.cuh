@@ -9,7 +9,8 @@
 // page and head lie in one block so that one run of copies brings both (2304 bytes: 16 tokens of 128 channels in 4 bits).
 // The offset is the group's smallest value rounded down to bfloat16 and the scale the smallest bfloat16 that is not below
 // (largest - offset) / (2^bits - 1): every value lies inside the codes' range, so none is clipped, and a value is off by at
-// most half a scale.  A group that holds an infinity or a NaN has NaN for both.
+// most half a scale.  A group that holds an infinity or a NaN has NaN for both (one with a value below bfloat16's range an infinity, and
+// reads as NaN).
 #pragma once
 #include "common.cuh"
 
