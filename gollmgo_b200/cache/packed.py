@@ -225,19 +225,18 @@ class PackedKV:
         lists = [(64, counts[1])]
         if ATTN_POLICY == "auto" and long_tiles(options, counts[2], nh, window, longest, self._sms):
             lists.append((128, counts[2]))
-        (B, width), new, loud = tables.shape, q.new_empty, ops.packed_loud_floats(self.kv_heads)
+        (B, width), new = tables.shape, q.new_empty
         k, v = new((2, pages, self.kv_heads, P, d), dtype=torch.float16).unbind(0)
-        loud, kv_unit = new((loud + 2 * self.kv_heads,), dtype=torch.float32).split([loud, 2 * self.kv_heads])
+        floats = new((ops.packed_unfold_floats(self.kv_heads),), dtype=torch.float32)
         ints = new((B * width + 2 * sum(n for _, n in lists),), dtype=torch.int32)
         at, tiles = B * width, []
         for _, n in lists:
             tiles.append((ints[at:at + n], ints[at + n:at + 2 * n], n))
             at += 2 * n
-        plain, shape = ints[:B * width], (self.kv_heads, d, P, self.bits, window, least)
-        ops.packed_loud(self.pages, tables, cu_q_lens, context_lens, loud, *shape)
-        ops.packed_unfold(self.pages, tables, cu_q_lens, context_lens, k, v, most, plain, [(h, n, *t[:2]) for (h, n), t in zip(lists, tiles)], *shape,
-                          loud, kv_unit)
-        ops.attn_prefill_half(q, k, v, kv_unit, plain, width, cu_q_lens, context_lens, tiles[0], tiles[1] if len(tiles) > 1 else None, out, nh,
+        plain = ints[:B * width]
+        ops.packed_unfold(self.pages, tables, cu_q_lens, context_lens, k, v, most, plain, [(h, n, *t[:2]) for (h, n), t in zip(lists, tiles)],
+                          self.kv_heads, d, P, self.bits, window, least, floats)
+        ops.attn_prefill_half(q, k, v, floats, plain, width, cu_q_lens, context_lens, tiles[0], tiles[1] if len(tiles) > 1 else None, out, nh,
                               self.kv_heads, d, P, window, scale, options, softcap, sink, slopes, temperature)
 
     @staticmethod

@@ -1548,9 +1548,8 @@ _PACKED_TYPES = {
     "gg_packed_prompt_fold": [_I, _I],
     "gg_packed_prompt_f32": [_P, _L, _P, _I, _P, _I, _I, _P, _P, _I, _I, _P, _I, _P, _L, _P, _I, _I, _I, _I, _I, _I, _F, _F, _P, _P, _F, _F, _P],
     "gg_packed_prefill": [_P, _L, _I, _P, _I, _P, _I, _P, _P, _P, _P, _I, _P, _I, _I, _I, _I, _I, _I, _F, _F, _P, _P, _F, _F, _P],
-    "gg_packed_loud_floats": [_I],
-    "gg_packed_loud": [_P, _I, _P, _I, _P, _P, _I, _P, _I, _I, _I, _I, _I, _I, _P],
-    "gg_packed_unfold": [_P, _I, _P, _I, _P, _P, _I, _P, _P, _I, _I, _P, _P, _P, _I, _I, _P, _P, _I, _I, _P, _P, _I, _I, _I, _I, _I, _I, _P],
+    "gg_packed_unfold_floats": [_I],
+    "gg_packed_unfold": [_P, _I, _P, _I, _P, _P, _I, _P, _P, _I, _I, _P, _P, _I, _I, _P, _P, _I, _I, _P, _P, _I, _I, _I, _I, _I, _I, _P],
     "gg_attn_prefill_half": [_P, _L, _P, _P, _P, _P, _I, _P, _P, _P, _P, _I, _P, _P, _I, _P, _I, _I, _I, _I, _I, _I, _I, _I, _F, _F, _P, _P, _F, _F, _P, _P],
 }
 _PACKED = {}
@@ -1803,41 +1802,28 @@ def packed_prompt_f32(q: torch.Tensor, pages: torch.Tensor, tables: torch.Tensor
 
 
 @functools.lru_cache(maxsize=None)
-def packed_loud_floats(nkv: int) -> int:
-    """Floats of ``loud`` of packed_loud and packed_unfold."""
-    return _packed("gg_packed_loud_floats")(nkv)
-
-
-def packed_loud(pages: torch.Tensor, tables: torch.Tensor, cu_q_lens: torch.Tensor, context_lens: torch.Tensor, loud: torch.Tensor, nkv: int, d: int,
-                page_size: int, bits: int, window: int, least: int = 1) -> None:
-    """How large the keys and values in sight of the portions are, for packed_unfold: partial maxima in ``loud``, float32 of packed_loud_floats."""
-    stream = _stream_of("packed_loud", pages, tables, cu_q_lens, context_lens, loud)
-    B, width = _tables("packed_loud", tables)
-    _ints("packed_loud", B, context_lens)
-    _ints("packed_loud", B + 1, cu_q_lens)
-    if loud.numel() < packed_loud_floats(nkv) or loud.dtype != torch.float32 or not loud.is_contiguous():
-        raise KernelError("packed_loud: the maxima are contiguous float32, large enough")
-    _check(_packed("gg_packed_loud")(pages.data_ptr(), pages.shape[0], tables.data_ptr(), width, cu_q_lens.data_ptr(), context_lens.data_ptr(), B,
-                                     loud.data_ptr(), least, nkv, d, page_size, bits, window, stream))
+def packed_unfold_floats(nkv: int) -> int:
+    """float32 that packed_unfold works in."""
+    return _packed("gg_packed_unfold_floats")(nkv)
 
 
 def packed_unfold(pages: torch.Tensor, tables: torch.Tensor, cu_q_lens: torch.Tensor, context_lens: torch.Tensor, k_out: Optional[torch.Tensor],
                   v_out: Optional[torch.Tensor], most_pages: int, out_tables: Optional[torch.Tensor], lists, nkv: int, d: int, page_size: int,
-                  bits: int, window: int, least: int = 1, loud: Optional[torch.Tensor] = None, kv_unit: Optional[torch.Tensor] = None) -> None:
+                  bits: int, window: int, least: int = 1, floats: Optional[torch.Tensor] = None) -> None:
     """What the prompt kernels need of the portions of a step (sequences with ``least`` rows or more in cu_q_lens): one or two tile lists, ``lists``
     of (height, count, seq, q0) with the number of tiles that the portions cut into rows of that height make; and, with ``k_out`` and ``v_out``
-    float16 [pages, nkv, page_size, d], their pages as keys and values behind one another there, times ``kv_unit`` float32 [2, nkv] (powers of two,
-    from ``loud`` of packed_loud), and block tables of those pages in ``out_tables`` (shape of ``tables``).  Pages that the window hides are
-    left out.  With pages it goes directly behind packed_loud (it reads its lists before that has finished)."""
-    stream = _stream_of("packed_unfold", pages, tables, cu_q_lens, context_lens, k_out, v_out, out_tables, loud, kv_unit)
+    float16 [pages, nkv, page_size, d], their pages as keys and values behind one another there, block tables of those pages in ``out_tables`` (shape
+    of ``tables``), and what each kv head's keys and values are multiples of (powers of two) in the first [2, nkv] of ``floats``, float32 of
+    packed_unfold_floats.  Pages that the window hides are left out."""
+    stream = _stream_of("packed_unfold", pages, tables, cu_q_lens, context_lens, k_out, v_out, out_tables, floats)
     B, width = _tables("packed_unfold", tables)
     _ints("packed_unfold", B, context_lens)
     _ints("packed_unfold", B + 1, cu_q_lens)
     if k_out is not None:
         _ints("packed_unfold", B * width, out_tables)
         if k_out.dtype != torch.float16 or v_out.dtype != torch.float16 or not (k_out.is_contiguous() and v_out.is_contiguous()) \
-                or loud.numel() < packed_loud_floats(nkv) or kv_unit.numel() < 2 * nkv:
-            raise KernelError("packed_unfold: keys and values go to contiguous float16, with their maxima and units")
+                or floats.dtype != torch.float32 or floats.numel() < packed_unfold_floats(nkv):
+            raise KernelError("packed_unfold: keys and values go to contiguous float16, with float32 to work in")
     flat = []
     for height, count, seq, q0 in lists:
         _ints("packed_unfold", count, seq, q0)
@@ -1846,7 +1832,7 @@ def packed_unfold(pages: torch.Tensor, tables: torch.Tensor, cu_q_lens: torch.Te
         flat += [0, 0, None, None]
     _check(_packed("gg_packed_unfold")(pages.data_ptr(), pages.shape[0], tables.data_ptr(), width, cu_q_lens.data_ptr(),
                                        context_lens.data_ptr(), B, _at(k_out), _at(v_out), k_out.shape[0] if k_out is not None else 0, most_pages,
-                                       _at(out_tables), _at(loud), _at(kv_unit), *flat, least, nkv, d, page_size, bits, window, stream))
+                                       _at(out_tables), _at(floats), *flat, least, nkv, d, page_size, bits, window, stream), 1 if k_out is None else 2)
 
 
 def attn_prefill_half(q: torch.Tensor, kcache: torch.Tensor, vcache: torch.Tensor, kv_unit: torch.Tensor, block_tables: torch.Tensor, bt_stride: int,

@@ -745,40 +745,33 @@ extern "C" int gg_packed_read(const void* pages, int num_pages, const int* table
   return gg_check_launch("packed_read");
 }
 
-// Floats of `loud` of gg_packed_loud and gg_packed_unfold.
-extern "C" int gg_packed_loud_floats(int nkv) { return LOUD_BLOCKS * (2 * nkv + 1); }
+// Floats that gg_packed_unfold works in: what the keys and values are multiples of [2, nkv] first, then its own.
+extern "C" int gg_packed_unfold_floats(int nkv) { return 2 * nkv + LOUD_BLOCKS * (2 * nkv + 1); }
 
-// How large the keys and values in sight of a run's portions are: partial maxima for gg_packed_unfold.
-extern "C" int gg_packed_loud(const void* pages, int num_pages, const int* tables, int bt_stride, const int* cu_q_lens, const int* context_lens,
-                              int B, float* loud, int least, int nkv, int d, int page_size, int bits, int window, cudaStream_t stream) {
-  int rc = check_packed("packed_loud", pages, num_pages, nkv, d, page_size, bits);
-  if (rc) return rc;
-  GG_REQUIRE((d == 64 || d == 128) && nkv <= UNFOLD_HEADS && B > 0 && bt_stride > 0 && window >= 0 && loud, "packed_loud: bad sizes d=%d nkv=%d B=%d", d, nkv, B);
-  UnfoldArgs a = {};
-  a.pages = (const unsigned char*)pages; a.num_pages = num_pages; a.tables = tables; a.cu_q_lens = cu_q_lens; a.context_lens = context_lens;
-  a.bt_stride = bt_stride; a.B = B; a.least = least > 1 ? least : 1; a.nkv = nkv; a.d = d; a.page_size = page_size; a.window = window; a.loud = loud;
-  if (bits == 4) gg_launch(packed_loud_kernel<4>, dim3(LOUD_BLOCKS), dim3(256), 0, stream, a);
-  else gg_launch(packed_loud_kernel<8>, dim3(LOUD_BLOCKS), dim3(256), 0, stream, a);
-  return gg_check_launch("packed_loud");
-}
-
-// k_out, v_out (half precision) null: the lists alone.
+// k_out, v_out (half precision, with `floats`) null: the lists alone.
 extern "C" int gg_packed_unfold(const void* pages, int num_pages, const int* tables, int bt_stride, const int* cu_q_lens,
                                 const int* context_lens, int B, void* k_out, void* v_out, int out_pages, int most_pages,
-                                int* out_tables, float* loud, float* kv_unit, int height0, int count0, int* seq0, int* q00, int height1, int count1,
+                                int* out_tables, float* floats, int height0, int count0, int* seq0, int* q00, int height1, int count1,
                                 int* seq1, int* q01, int least, int nkv, int d, int page_size, int bits, int window, cudaStream_t stream) {
   int rc = check_packed("packed_unfold", pages, num_pages, nkv, d, page_size, bits);
   if (rc) return rc;
   GG_REQUIRE(B > 0 && B <= UNFOLD_SEQS && most_pages >= 0 && most_pages <= bt_stride && window >= 0 && height0 >= 0 && height1 >= 0,
              "packed_unfold: bad sizes B=%d pages=%d of %d window=%d", B, most_pages, bt_stride, window);
   GG_REQUIRE(((size_t)k_out % 16) == 0 && ((size_t)v_out % 16) == 0, "packed_unfold: the outputs must start on 16 bytes");
-  GG_REQUIRE(k_out ? v_out && out_tables && loud && kv_unit && nkv <= UNFOLD_HEADS : most_pages == 0, "packed_unfold: missing outputs, or %d kv heads", nkv);
+  GG_REQUIRE(k_out ? v_out && out_tables && floats && nkv <= UNFOLD_HEADS && (d == 64 || d == 128) : most_pages == 0,
+             "packed_unfold: missing outputs, %d kv heads or head size %d", nkv, d);
   UnfoldArgs a = {};
   a.pages = (const unsigned char*)pages; a.num_pages = num_pages; a.tables = tables; a.cu_q_lens = cu_q_lens; a.context_lens = context_lens;
   a.bt_stride = bt_stride; a.B = B; a.least = least > 1 ? least : 1; a.nkv = nkv; a.d = d; a.page_size = page_size; a.window = window; a.out_pages = out_pages;
-  a.out_tables = out_tables; a.loud = loud; a.kv_unit = kv_unit;
+  a.out_tables = out_tables; a.kv_unit = floats; a.loud = floats + 2 * nkv;
   a.tiles[0] = {height0, count0, seq0, q00};
   a.tiles[1] = {height1, count1, seq1, q01};
+  if (k_out) {                                       // directly ahead: see packed_unfold_kernel
+    if (bits == 4) gg_launch(packed_loud_kernel<4>, dim3(LOUD_BLOCKS), dim3(256), 0, stream, a);
+    else gg_launch(packed_loud_kernel<8>, dim3(LOUD_BLOCKS), dim3(256), 0, stream, a);
+    rc = gg_check_launch("packed_loud");
+    if (rc) return rc;
+  }
   const dim3 grid(most_pages + 1, most_pages ? B : 1, most_pages ? head_blocks(out_pages, nkv) : 1), block(256);
   if (bits == 4) gg_launch(packed_unfold_kernel<4>, grid, block, 0, stream, a, (__half*)k_out, (__half*)v_out);
   else gg_launch(packed_unfold_kernel<8>, grid, block, 0, stream, a, (__half*)k_out, (__half*)v_out);

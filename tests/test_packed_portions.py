@@ -303,7 +303,6 @@ def test_the_switch_of_the_prompt_kernels_holds_for_portions(monkeypatch, policy
     seen = {}
     monkeypatch.setattr(packed, "ATTN_POLICY", policy)
     monkeypatch.setattr(ops, "packed_prefill_rows", lambda *a: None)
-    monkeypatch.setattr(ops, "packed_loud", lambda *a: None)
     monkeypatch.setattr(ops, "packed_unfold", lambda *a: seen.update(lists=[h for h, *_ in a[8]]))
     monkeypatch.setattr(ops, "attn_prefill_half", lambda *a: seen.update(kernel="options" if a[17] else "plain", tile128=a[9]))
     monkeypatch.setattr(ops, "packed_prefill", lambda *a, **k: seen.update(kernel="general"))
@@ -511,11 +510,9 @@ def test_the_launchers_of_portions_refuse_sizes_and_missing_lists():
             assert f(*bad) != 0
             assert message in ops.lib().gg_last_error().decode(), (name, at, v)
     one = 16                                          # (any address that is not looked at)
-    refused("gg_packed_loud", [None, 4, one, 8, one, one, 2, one, 1, 2, 64, 16, 4, 0, None],
-            [(10, 96, "bad sizes"), (9, 2000, "bad sizes"), (6, 0, "bad sizes"), (7, None, "bad sizes"), (13, -1, "bad sizes"), (0, 8, "16 bytes"), (12, 5, "packed cache")])
-    refused("gg_packed_unfold", [None, 4, one, 8, one, one, 2, one, one, 3, 2, one, one, one, 64, 1, one, one, 0, 0, None, None, 1, 2, 64, 16, 4, 0, None],
-            [(6, 0, "bad sizes"), (6, 1025, "bad sizes"), (10, 9, "bad sizes"), (27, -1, "bad sizes"), (7, 8, "16 bytes"), (8, None, "missing"), (11, None, "missing"),
-             (12, None, "missing"), (13, None, "missing"), (7, None, "missing"), (23, 1025, "missing")])
+    refused("gg_packed_unfold", [None, 4, one, 8, one, one, 2, one, one, 3, 2, one, one, 64, 1, one, one, 0, 0, None, None, 1, 2, 64, 16, 4, 0, None],
+            [(6, 0, "bad sizes"), (6, 1025, "bad sizes"), (10, 9, "bad sizes"), (26, -1, "bad sizes"), (7, 8, "16 bytes"), (0, 8, "16 bytes"), (8, None, "missing"),
+             (11, None, "missing"), (12, None, "missing"), (7, None, "missing"), (22, 1025, "missing"), (23, 96, "missing"), (25, 5, "packed cache")])
     refused("gg_packed_prefill", [one, 128, 1, None, 4, one, 8, one, one, one, one, 1, one, 4, 2, 64, 16, 4, 0, 1.0, 0.0, None, None, 0.0, 0.0, None],
             [(2, 7, "dtype"), (13, 3, "multiple"), (14, 0, "bad sizes"), (11, -1, "bad lists"), (9, None, "bad lists"), (7, None, "bad lists"), (18, -1, "window"),
              (17, 3, "packed cache")])
