@@ -185,7 +185,7 @@ def pointed_portions(bits, dtype, option, nh, nkv, d, seed):
 @pytest.mark.parametrize("bits", [4, 8])
 @pytest.mark.parametrize("dtype,policy", [(torch.bfloat16, "auto"), (torch.bfloat16, "mma"), (torch.bfloat16, "general"), (torch.float32, "auto")])
 @pytest.mark.parametrize("option", range(len(OPTIONS)))
-@pytest.mark.parametrize("nh,nkv,d,page", [(4, 1, 64, 16), (4, 2, 128, 16), (3, 3, 128, 32), (4, 2, 128, 8), (2, 1, 64, 128), (4, 2, 96, 16), (3, 1, 16, 4)])
+@pytest.mark.parametrize("nh,nkv,d,page", [(4, 1, 64, 16), (4, 2, 128, 16), (3, 3, 128, 32), (4, 2, 128, 8), (2, 1, 64, 128), (2, 1, 64, 4), (2, 1, 128, 256), (4, 2, 96, 16), (3, 1, 16, 4)])
 def test_portions_are_as_near_as_their_roundings(monkeypatch, bits, dtype, policy, option, nh, nkv, d, page):
     from gollmgo_b200.cache import packed
     monkeypatch.setattr(packed, "ATTN_POLICY", policy)
@@ -520,3 +520,50 @@ def test_the_launchers_of_portions_refuse_sizes_and_missing_lists():
                                      None, None],
             [(20, 96, "head size"), (21, 24, "pages"), (4, None, "no lists"), (9, None, "no lists"), (0, 8, "aligned"), (1, 100, "aligned"), (24, -1.0, "options"),
              (25, 3.0, "options"), (26, one, "options"), (27, one, "options"), (29, 2.0, "options"), (18, 3, "multiple")])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("d", [64, 128, 96])
+def test_portions_on_two_streams_and_in_two_graphs(bits, d):
+    """Two prefills at once, eager and captured, behind writes of their own: each as alone, also with other keys in the pages at a replay."""
+    nh, nkv, page, lens = 4, 2, 16, [300, 70]
+    g = torch.Generator().manual_seed(d)
+    counts = [-(-n // page) for n in lens]
+    table = torch.zeros(2, max(counts), dtype=torch.int32)
+    for b, order in enumerate(torch.randperm(sum(counts), generator=g).to(torch.int32).split(counts)):
+        table[b, :counts[b]] = order
+    rows = [torch.randn(sum(lens), (nh + 2 * nkv) * d, generator=g).to(torch.bfloat16).cuda() for _ in range(3)]
+    slots = torch.cat([table[b][torch.arange(n) // page].long() * page + torch.arange(n) % page for b, n in enumerate(lens)]).to(torch.int32).cuda()
+    cu, ctx, table = torch.tensor([0, 300, 370], dtype=torch.int32).cuda(), torch.tensor(lens, dtype=torch.int32).cuda(), table.cuda()
+
+    def step(kv, x):
+        q = kv.write(x, None, slots, nh)
+        return kv.prefill(q, table, cu, ctx, lens, lens, d ** -0.5)
+    caches = [PackedKV.empty(sum(counts), nkv, d, page, bits) for _ in range(2)]
+    want = [step(caches[0], x).clone() for x in rows]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for _ in range(5):
+        got = []
+        for s, kv, x in zip(streams, caches, rows):
+            with torch.cuda.stream(s):
+                got.append(step(kv, x))
+        torch.cuda.synchronize()
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    live, graphs, outs = [rows[0].clone(), rows[1].clone()], [], []
+    for kv, x in zip(caches, live):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append(step(kv, x))
+        graphs.append(graph)
+    for a, b in ((0, 1), (2, 0), (1, 2)):
+        live[0].copy_(rows[a])
+        live[1].copy_(rows[b])
+        torch.cuda.synchronize()
+        for _ in range(4):
+            for s, graph in zip(streams, graphs):
+                with torch.cuda.stream(s):
+                    graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(outs[0], want[a]) and torch.equal(outs[1], want[b])
