@@ -212,8 +212,8 @@ class PackedKV:
             tables, context_lens, cu_q_lens = tables[lo:hi], context_lens[lo:hi], cu_q_lens[lo:hi + 1]
         # (the plain tcgen05 kernel takes the largest product for the largest score)
         options = softcap > 0 or sink is not None or slopes is not None or temperature is not None or not scale > 0
-        fast = q.dtype == torch.bfloat16 and d in (64, 128) and q.stride(0) % 8 == 0 and q.data_ptr() % 16 == 0 and ATTN_POLICY != "general" \
-            and self.kv_heads <= 1024
+        fast = q.dtype == torch.bfloat16 and d in (64, 128) and q.stride(0) % 8 == 0 and q.data_ptr() % 16 == 0 and out.data_ptr() % 16 == 0 \
+            and ATTN_POLICY != "general" and self.kv_heads <= 1024
         if not fast:                               # on the codes where they lie, in float32 arithmetic
             n = counts[0]
             ints = torch.empty(2 * n, dtype=torch.int32, device=q.device)

@@ -666,7 +666,7 @@ extern "C" int gg_attn_prefill_half(const void* q, long long q_stride, const voi
   if (rc) return rc;
   GG_REQUIRE((d == 64 || d == 128) && (page_size & (page_size - 1)) == 0 && kv_unit && tile64_seq && tile64_q0,
              "attn_prefill_half: head size %d, pages of %d tokens, or no lists", d, page_size);
-  GG_REQUIRE(q_stride % 8 == 0 && ((size_t)q % 16) == 0, "attn_prefill_half: q rows must be 16-byte aligned");
+  GG_REQUIRE(q_stride % 8 == 0 && ((size_t)q % 16) == 0 && ((size_t)out % 16) == 0, "attn_prefill_half: rows of q and of the result must be 16-byte aligned");
   GG_REQUIRE(options || (scale > 0.f && softcap <= 0.f && !sink && !slopes && temp_every <= 0.f), "attn_prefill_half: options without the kernels for them");
   static const bool wide = !(getenv("GOLLMGO_B200_ATTN_STEP") && atoi(getenv("GOLLMGO_B200_ATTN_STEP")) == 64);
   if (tile128_seq && status) {

@@ -518,7 +518,7 @@ def test_the_launchers_of_portions_refuse_sizes_and_missing_lists():
              (17, 3, "packed cache")])
     refused("gg_attn_prefill_half", [one, 256, one, one, one, one, 8, one, one, one, one, 1, None, None, 0, one, 3, 4, 4, 2, 64, 16, 0, 0, 1.0, 0.0, None, None, 0.0, 0.0,
                                      None, None],
-            [(20, 96, "head size"), (21, 24, "pages"), (4, None, "no lists"), (9, None, "no lists"), (0, 8, "aligned"), (1, 100, "aligned"), (24, -1.0, "options"),
+            [(20, 96, "head size"), (21, 24, "pages"), (4, None, "no lists"), (9, None, "no lists"), (0, 8, "aligned"), (1, 100, "aligned"), (15, 18, "aligned"), (24, -1.0, "options"),
              (25, 3.0, "options"), (26, one, "options"), (27, one, "options"), (29, 2.0, "options"), (18, 3, "multiple")])
 
 
@@ -567,3 +567,46 @@ def test_portions_on_two_streams_and_in_two_graphs(bits, d):
                     graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(outs[0], want[a]) and torch.equal(outs[1], want[b])
+
+
+def test_a_result_that_starts_anywhere_takes_the_kernel_that_stores_it(monkeypatch):
+    """The tensor-core kernels store 4 and 16 bytes at a time."""
+    from gollmgo_b200.csrc import ops
+    seen = []
+    monkeypatch.setattr(ops, "packed_prefill_rows", lambda *a: None)
+    monkeypatch.setattr(ops, "packed_unfold", lambda *a: None)
+    monkeypatch.setattr(ops, "attn_prefill_half", lambda *a: seen.append("half"))
+    monkeypatch.setattr(ops, "packed_prefill", lambda *a, **k: seen.append("general"))
+
+    class NoDevice(PackedKV):
+        def __init__(self):
+            self.head_dim, self.page_size, self.bits, self.kv_heads, self._sms = 64, 16, 4, 1, 148
+            self.pages = None
+    room = torch.zeros(40 * 2 * 64 + 16, dtype=torch.bfloat16)
+    first = -room.data_ptr() % 16 // 2
+    for at, want in ((0, "half"), (1, "general"), (2, "general"), (4, "general"), (8, "half")):
+        out = room[first + at:first + at + 40 * 2 * 64].view(40, 2, 64)
+        NoDevice().prefill(torch.zeros(40, 2, 64, dtype=torch.bfloat16), torch.zeros(1, 3, dtype=torch.int32), torch.tensor([0, 40], dtype=torch.int32),
+                           torch.tensor([40], dtype=torch.int32), [40], [40], 0.1, out=out)
+        assert seen.pop() == want, at
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("at", [1, 2, 4, 8])
+@pytest.mark.parametrize("nh,nkv", [(4, 2), (3, 3)])
+def test_results_that_start_anywhere(at, nh, nkv):
+    d, n, page = 64, 300, 16
+    g = torch.Generator().manual_seed(at)
+    kv = PackedKV.empty(20, nkv, d, page, 4)
+    x = torch.randn(n, (nh + 2 * nkv) * d, generator=g).to(torch.bfloat16)
+    q = kv.write(x.cuda(), None, torch.arange(n, dtype=torch.int32).cuda(), nh)
+    table = torch.arange(20, dtype=torch.int32).view(1, -1).cuda()
+    dev = lambda y: torch.tensor(y, dtype=torch.int32).cuda()  # noqa: E731
+    room = torch.full((n * nh * d + 16,), 7.0, dtype=torch.bfloat16, device="cuda")
+    out = room[at:at + n * nh * d].view(n, nh, d)
+    kv.prefill(q, table, dev([0, n]), dev([n]), [n], [n], 0.125, out=out)
+    held = [plain.through(y.double().view(n, nkv, d), 4) for y in x[:, nh * d:].chunk(2, 1)]
+    rows = x[:, :nh * d].view(n, nh, d)
+    ref = plain.attend(rows.double(), *held, n, 0.125)
+    assert ((out.cpu().double() - ref).abs() <= tolerance(rows, *held, n, 0.125, torch.bfloat16, True)).all()
+    assert (room[:at] == 7.0).all() and (room[at + n * nh * d:] == 7.0).all()
